@@ -754,6 +754,126 @@ typedef struct phx_dpp_inputs {
 phx_status phx_dpp_rescore_device(int32_t device, const phx_dpp_config* cfg, const phx_dpp_inputs* in, int32_t* out_index,
                                   double* out_score, int32_t* out_count, void* stream);
 
+/* ---- serving over a cached history ---------------------------------------------------------------------------------
+ * A request's history is projected once: its keys and values stay in a paged cache, and what comes later - a new action,
+ * candidates, the drafted continuations of a sequence of ids - is appended behind them and attends to them.  (The reference
+ * runs history and candidates through the trunk together on every request, phoenix/xrex/models/transformer.py:693-993; the
+ * arithmetic here is that of its layers: merged QKV rows, layers.py:728-736, rotation, layers.py:52-67, capped softmax,
+ * pallas/ranker_attention_v2.py:113-148.)  Forward only, bf16 with fp32 sums.
+ *
+ * phx_cache_batch describes the cache and the new tokens of B requests; all pointers are device pointers.  `pages` is
+ * [num_pages][2 (key, value)][num_kv_heads][page_size][key_size] bf16; key i of request b sits in slot i % page_size of page
+ * block_table[b * table_stride + i / page_size].  The new tokens of request b are rows q_start[b] .. q_start[b + 1] - 1 of the
+ * dense arrays (q_start[0] = 0, ascending, q_start[B] = num_tokens) and keys lengths[b], lengths[b] + 1, ... of the cache.
+ * page_size is a multiple of 16, key_size 32, 64 or 128.
+ *
+ * What the host cannot check is checked on the device, and reads or writes nothing out of range: a token whose page is
+ * outside the pool or behind the table's columns is not stored, a key in such a page is left out (as if it did not exist), a
+ * position outside the rotation tables takes the nearest one inside.  Each raises a bit of status_dev[2]: 1 a page, 2 a
+ * position, 4 offsets that do not ascend or leave the token rows (such a request is left out).  status_dev (int32 [4],
+ * required) starts as zeros; [0] is raised when a bounded wait ran out (as phx_sync reports by PHX_E_TIMEOUT), [1] is the limit of those waits in
+ * microseconds (0 = 2 s).  phx_decode_status waits for `stream`, returns PHX_OK, PHX_E_TIMEOUT, or PHX_E_ARG with the
+ * bits in *bits_out, and puts [0] and [2] back to zero. */
+typedef struct phx_cache_batch {
+  uint16_t* pages;
+  int64_t num_pages;
+  const int32_t* q_start;      /* [batch + 1] */
+  const int32_t* lengths;      /* [batch] keys cached before the new tokens */
+  const int32_t* block_table;  /* [batch][table_cols], rows table_stride apart */
+  int64_t table_stride;
+  int32_t* status_dev;         /* [4] */
+  int32_t table_cols;
+  int32_t page_size;
+  int32_t num_kv_heads;
+  int32_t key_size;
+  int32_t batch;
+  int32_t num_tokens;
+} phx_cache_batch;
+phx_status phx_decode_status(int32_t device, int32_t* status_dev, void* stream, int32_t* bits_out);
+
+/* New rows enter the cache.  qkv [num_tokens] rows of (num_q_heads + 2 num_kv_heads) * key_size, qkv_stride elements apart,
+ * in the merged order [kv head][q_0 .. q_{g-1}, k, v]; every query and key head is divided by its root mean square and
+ * multiplied by the gain (q_gain, k_gain fp32 [key_size]; both NULL: no norm), rotated by its token's position (halves (a, b) -> (a cos - b
+ * sin, b cos + a sin); cos_tab, sin_tab fp32 [num_positions][key_size / 2]; both NULL: no rotation), in fp32 with one
+ * rounding; keys and values go to the cache, queries to q_out [num_tokens][num_q_heads][key_size].  One launch,
+ * asynchronous on `stream` (a cudaStream_t, NULL = default stream). */
+typedef struct phx_append_args {
+  const uint16_t* qkv;
+  int64_t qkv_stride;
+  const int32_t* positions;    /* [num_tokens] */
+  const float* cos_tab;
+  const float* sin_tab;
+  const float* q_gain;
+  const float* k_gain;
+  uint16_t* q_out;
+  int32_t num_q_heads;
+  int32_t num_positions;
+  float eps;
+  int32_t _pad;
+} phx_append_args;
+phx_status phx_history_append_device(int32_t device, const phx_cache_batch* cache, const phx_append_args* args, void* stream);
+
+/* Attention of the new tokens over the cache, theirs included (append them first).  Token i of a request sees all its
+ * lengths[b] older keys, and of the new ones those j with pre[j] <= pre[i] < end[j], spans[token] = (pre, end): with pre the
+ * place of a token in a depth-first walk of a tree of tokens and end the place behind its last descendant, that is j = i or
+ * j an ancestor of i (phx_tree_spans makes them from parents, in any order of the tokens); (0, 1) everywhere lets all see
+ * all, as a history does, (i, i + 1) only themselves, as candidates do.  spans NULL: a chain, j <= i.  pre = -1 (end <= 0):
+ * a padding token, seen by none, output zeros; so is the output of a token that sees no key.  A key that a token does not see leaves no trace in its
+ * output, whatever the key's value rows hold (infinities, NaN).  cap > 0: logits go through cap_method (1 soft sign, 2 tanh).
+ * max_tokens and max_keys (cached + new) say how large a request may be; they choose kernels and splits only: larger
+ * requests are computed all the same.  workspace: phx_tree_workspace_bytes of device memory, not shared by calls that may
+ * overlap; nothing in it has to be kept or cleared between calls.  The order of every sum follows from the sizes alone: equal calls
+ * give equal bits.  Asynchronous on `stream`. */
+typedef struct phx_tree_args {
+  const uint16_t* q;           /* [num_tokens][num_q_heads][key_size], rows q_stride apart */
+  int64_t q_stride;
+  const int32_t* spans;        /* [num_tokens][2] or NULL */
+  uint16_t* out;               /* [num_tokens][num_q_heads][key_size] */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t max_keys;
+  int32_t max_tokens;
+  int32_t num_q_heads;
+  float sm_scale;
+  float cap;
+  int32_t cap_method;
+  int32_t _pad;
+} phx_tree_args;
+phx_status phx_tree_workspace_bytes(int32_t device, int64_t* bytes_out);
+phx_status phx_tree_attention_device(int32_t device, const phx_cache_batch* cache, const phx_tree_args* args, void* stream);
+/* Spans of one request's tokens from their parents (host arrays; parent -1: hangs on the cached history, -2: padding;
+ * any order, cycles and parents out of range are refused with PHX_E_ARG).  Host code only. */
+phx_status phx_tree_spans(const int32_t* parents, int32_t n, int32_t* spans_out);
+
+/* What a model answers with, from its logits [rows][vocab] (fp32, or bf16 bit patterns with is_bf16; rows `stride` elements
+ * apart): y = cap tanh(x / cap) / temperature (cap <= 0: x / temperature; -inf stays -inf: an id that is not allowed),
+ *   given_out [rows][num_given]  y[given] - log sum exp y    (an id outside [0, vocab) stands for none: 0)
+ *   entropy_out [rows]           - sum p log p
+ *   top_ids_out, top_out [rows][top_k]   the ids of the largest x, ties lowest id first (NaN counts as largest), and their log probabilities
+ * all fp32, ids int64.  -inf has log probability -inf; a row without an allowed id has entropy 0; a row with NaN, or
+ * without a cap with +inf, has NaN for its finite logits and its entropy.  Any output may be NULL.  top_k at most PHX_LOGPROBS_MAX_TOP and vocab.
+ * One launch that reads the logits once from memory, no workspace, asynchronous on `stream`.  The reference
+ * answers with per-action sigmoids only (model_runner.py:4474); this is the counterpart for heads over a table of ids. */
+#define PHX_LOGPROBS_MAX_TOP 128
+typedef struct phx_logprobs_args {
+  const void* logits;
+  int64_t stride;
+  const int64_t* given;        /* [rows][num_given] */
+  float* given_out;
+  float* entropy_out;
+  float* top_out;
+  int64_t* top_ids_out;
+  int32_t rows;
+  int32_t vocab;
+  int32_t num_given;
+  int32_t top_k;
+  int32_t is_bf16;
+  float cap;
+  float temperature;
+  int32_t _pad;
+} phx_logprobs_args;
+phx_status phx_token_logprobs_device(int32_t device, const phx_logprobs_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -97,6 +97,30 @@ class AdmissionConfig(C.Structure):   # phx_admission_config
                 ("ewma_alpha", C.c_double)]
 
 
+class CacheBatch(C.Structure):   # phx_cache_batch
+    _fields_ = [("pages", C.c_void_p), ("num_pages", C.c_int64), ("q_start", C.c_void_p), ("lengths", C.c_void_p),
+                ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("status_dev", C.c_void_p)] + [(n, C.c_int32) for n in (
+        "table_cols", "page_size", "num_kv_heads", "key_size", "batch", "num_tokens")]
+
+
+class AppendArgs(C.Structure):   # phx_append_args
+    _fields_ = [("qkv", C.c_void_p), ("qkv_stride", C.c_int64)] + [(n, C.c_void_p) for n in (
+        "positions", "cos_tab", "sin_tab", "q_gain", "k_gain", "q_out")] + [
+        ("num_q_heads", C.c_int32), ("num_positions", C.c_int32), ("eps", C.c_float), ("_pad", C.c_int32)]
+
+
+class TreeArgs(C.Structure):   # phx_tree_args
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("spans", C.c_void_p), ("out", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64), ("max_keys", C.c_int64), ("max_tokens", C.c_int32), ("num_q_heads", C.c_int32),
+                ("sm_scale", C.c_float), ("cap", C.c_float), ("cap_method", C.c_int32), ("_pad", C.c_int32)]
+
+
+class LogprobsArgs(C.Structure):   # phx_logprobs_args
+    _fields_ = [("logits", C.c_void_p), ("stride", C.c_int64)] + [(n, C.c_void_p) for n in (
+        "given", "given_out", "entropy_out", "top_out", "top_ids_out")] + [(n, C.c_int32) for n in (
+        "rows", "vocab", "num_given", "top_k", "is_bf16")] + [("cap", C.c_float), ("temperature", C.c_float), ("_pad", C.c_int32)]
+
+
 # every symbol include/phoenix_b200.h declares: name -> (restype, argtypes)
 _P = C.c_void_p
 SIGNATURES = {
@@ -204,6 +228,12 @@ SIGNATURES = {
     "phx_admission_should_reject": (C.c_int32, [_P, C.c_int64, C.c_int64]),
     "phx_admission_estimates": (C.c_int32, [_P, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
     "phx_dpp_rescore_device": (C.c_int32, [C.c_int32, C.POINTER(DppConfig), C.POINTER(DppInputs), _P, _P, _P, _P]),
+    "phx_decode_status": (C.c_int32, [C.c_int32, _P, _P, C.POINTER(C.c_int32)]),
+    "phx_history_append_device": (C.c_int32, [C.c_int32, C.POINTER(CacheBatch), C.POINTER(AppendArgs), _P]),
+    "phx_tree_workspace_bytes": (C.c_int32, [C.c_int32, C.POINTER(C.c_int64)]),
+    "phx_tree_attention_device": (C.c_int32, [C.c_int32, C.POINTER(CacheBatch), C.POINTER(TreeArgs), _P]),
+    "phx_tree_spans": (C.c_int32, [_P, C.c_int32, _P]),
+    "phx_token_logprobs_device": (C.c_int32, [C.c_int32, C.POINTER(LogprobsArgs), _P]),
     "phx_corpus_sync": (C.c_int32, [_P]),
     "phx_corpus_finish": (C.c_int32, [_P, C.POINTER(C.c_int32)]),
     "phx_corpus_set_exact": (C.c_int32, [_P, C.c_int32]),

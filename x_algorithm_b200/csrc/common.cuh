@@ -53,7 +53,10 @@ enum DispatchKind {
   DK_FORM_GEMM_DEEP = 18,   // ... of 128 rows with the deep ring
   DK_FORM_GEMM_KV = 19,     // QKV projection without the query tiles that nobody reads
   DK_FORM_SCAN_SPLIT = 20,  // tcgen05 corpus scan, collect pass with the tiles shared between two sets of warps
-  DK_COUNT = 21
+  DK_HISTORY_APPEND = 21,
+  DK_TREE_MMA = 22,         // attention over a paged cache, mma.sync
+  DK_TOKEN_LOGPROBS = 23,
+  DK_COUNT = 24
 };
 void dispatch_note(int kind);
 
