@@ -1,15 +1,24 @@
 // Log probabilities of given ids, entropy and best alternatives from a row of logits (phx_token_logprobs_device):
 //
-//   c = cap tanh(x / cap),  d = (c - max c) / temperature,  Z = sum e^d
-//   log p = d - ln Z,   entropy = ln Z - sum e^d d / Z
+//   c = cap tanh(x / cap),  d = c - max c,  t = d / temperature,  Z = sum e^t
+//   log p = t - ln Z,   entropy = ln Z - sum e^t t / Z
 //
 // The maximum is taken off before anything else, so that neither rows of a type's lowest value nor large logits overflow or cancel.
 //
-// One block per row.  The first pass keeps, per thread, a running maximum with its two sums and the largest (logit, id) key.  The top_k-th largest of the threads' keys is a lower bound of the row's top_k-th
-// largest key, so the second pass, which finds the row in L2, collects the few keys at or above it.  Rows whose order defeats that
-// bound (more keys than the buffer holds) take the exact bound from a radix select over the keys, a byte a pass.  Keys are distinct - the logit's order-preserving image,
-// then the id, lowest first - so ties need no care and the result does not depend on the order of the atomics.
+// One pass over the logits, bound by memory.  A row belongs to a warp, to a block, or to a cluster of blocks that each take a
+// stretch of it.  A thread fetches its own 16-byte words, cp.async into a ring of its own in shared memory (no barriers), takes a few
+// of them at a time, and keeps a reference, the sum of e^t and the sum of e^t t against it.  The reference is the maximum of the warp's first batch and moves only
+// when the exponentials could outgrow fp32: a running maximum moved in some lane of a warp at almost every batch, a third of the instructions.
+//
+// The best ids are found by words first: a word's key is its largest logit's order-preserving image, then its place, first come first.
+// The top_k-th largest key of any set of words bounds what the row's best ids can be in - a word below it holds nothing that is not
+// beaten by a logit in each of top_k other words - so after the first batch the threads' best words give a bound, and from then on the words at
+// or above it, few, are noted in shared memory.  After 2, 4, 8, ... batches the bound is taken anew from the notes, if they have grown, and the rest is dropped.  At the end the notes' words are
+// read again, their (logit, id) keys bounded in the same way, and the survivors ranked by counting.  Rows whose order defeats the
+// bounds (sorted ones: more words than the notes hold) take the exact bound from a radix select over the keys, a byte a pass.  Keys are
+// distinct, so ties need no care and the result does not depend on the order of the atomics.
 #include <math.h>
+#include <string.h>
 
 #include <string>
 
@@ -18,13 +27,20 @@
 namespace phx {
 namespace {
 
-constexpr int LP_THREADS = 256;
-constexpr int LP_KEEP = 2048;     // keys that the second pass may collect
+constexpr int WARP_ROWS = 4;        // rows of a block whose warps take one each
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float FLOOR = -1e38f, DEEP = -1e37f;
+constexpr float ROOM = 16.0f;       // powers of two that the exponentials may grow to before the reference moves
+typedef unsigned long long u64;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
 // order-preserving: larger logit, larger image; the two zeros are equal, NaN is largest
@@ -33,111 +49,468 @@ __device__ __forceinline__ uint32_t image(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ unsigned long long key_of(float x, int id) { return ((unsigned long long)image(x) << 32) | (uint32_t)~id; }
+__device__ __forceinline__ u64 key_of(float x, int id) { return ((u64)image(x) << 32) | (uint32_t)~id; }
+__device__ __forceinline__ float value_of(u64 key) {           // the logit of a key
+  const uint32_t u = (uint32_t)(key >> 32);
+  return u == 0xFFFFFFFFu ? NAN : __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+}
 
-template <typename T> __device__ __forceinline__ float load_logit(const T* row, int i);
-template <> __device__ __forceinline__ float load_logit<float>(const float* row, int i) { return row[i]; }
-template <> __device__ __forceinline__ float load_logit<bf16>(const bf16* row, int i) { return bf2f(row[i]); }
+template <typename T> struct Words;   // elements of a 16-byte word
+template <> struct Words<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
+    x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ float at(const float* row, long long i) { return row[i]; }
+};
+template <> struct Words<bf16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+  }
+  static __device__ __forceinline__ float at(const bf16* row, long long i) { return bf2f(row[i]); }
+};
 
-// m = max c, z = sum of e^d, s = sum of e^d d
+// m the reference, d = c - m: z = sum of e^t, s = sum of e^t d
 struct Stat { float m, z, s; };
-__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float temperature) {
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float scale) {
   Stat r;
-  r.m = fmaxf(a.m, b.m);
-  if (a.m != a.m || b.m != b.m) r.m = NAN;
+  r.m = max_nan(a.m, b.m);
   const float base = r.m == -INFINITY ? 0.f : r.m;
-  const float da = (a.m - base) / temperature, db = (b.m - base) / temperature, fa = ex2(da * LOG2E), fb = ex2(db * LOG2E);
+  const float da = a.m - base, db = b.m - base, fa = ex2(da * scale), fb = ex2(db * scale);
   r.z = a.z * fa + b.z * fb;
-  r.s = (fa > 0.f ? fa * (a.s + a.z * da) : 0.f) + (fb > 0.f ? fb * (b.s + b.z * db) : 0.f);   // e^d d is 0 where e^d is
+  r.s = (fa == 0.f ? 0.f : fa * (a.s + a.z * da)) + (fb == 0.f ? 0.f : fb * (b.s + b.z * db));   // e^t d is 0 where e^t is
   return r;
 }
 __device__ __forceinline__ float capped(float x, float cap) { return cap > 0.f && x != -INFINITY ? cap * tanhf(x / cap) : x; }
+// The same for the sums, to about 1e-7 of the cap: 1 - 2 / (e^(2 x / cap) + 1).  -inf stays -inf.
+__device__ __forceinline__ float capped_fast(float x, float cap, float two_log2e_by_cap) {
+  const float e = ex2(x * two_log2e_by_cap);
+  const float y = cap - __fdividef(2.0f * cap, e + 1.0f);
+  return x == -INFINITY ? x : y;
+}
 
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const phx_logprobs_args a) {
-  __shared__ unsigned long long keep[LP_KEEP];
-  __shared__ Stat part[LP_THREADS / 32];
-  __shared__ unsigned long long bound;
-  __shared__ int count;
-  __shared__ int hist[256];
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const T* row = static_cast<const T*>(a.logits) + (long long)r * a.stride;
+// the threads that share a stretch of a row
+template <int NT> struct Team {
+  static __device__ __forceinline__ int tid() { return NT == 32 ? threadIdx.x & 31 : threadIdx.x; }
+  static __device__ __forceinline__ void sync() { if (NT == 32) __syncwarp(); else __syncthreads(); }
+};
+
+template <int NT, int KEEP, int WORDS> struct TeamMemory {
+  uint4 word[WORDS][NT];     // the rings; at the end, keys of single logits
+  u64 keep[KEEP];                   // keys of words
+  u64 group[NT], bounds[32];
+  Stat part[NT / 32];
+  int hist[256];
+  int count;
+  // what a block of a cluster hands to the first
+  Stat stat;
+  u64 best[PHX_LOGPROBS_MAX_TOP];
+};
+
+// A lower bound of the k-th largest of all keys that the team has, from each thread's largest (0: it has none).  k of 24 or fewer: the
+// k-th largest of the maxima of 32 groups of threads; about 32 ln(32 / (32 - k)) keys of a random order lie at or above it.  More: with r the rank
+// that three quarters of the warps need for k keys, the r-th largest of each warp's threads, and of these the one that leaves k.  Ranks by counting
+// over 32 keys: over all the threads' it took longer than the logits.  Every call is followed by a barrier before the next.
+template <int NT, typename M>
+__device__ __forceinline__ u64 bound_of(u64 mine, int k, M& mem) {
+  typedef Team<NT> G;
+  constexpr int W = NT / 32;
+  const int lane = threadIdx.x & 31, tid = G::tid();
+  const bool few = W == 1 || k <= 24;
+  if (few) {
+#pragma unroll
+    for (int o = 1; o < W; o <<= 1) { const u64 other = __shfl_xor_sync(0xffffffffu, mine, o); mine = other > mine ? other : mine; }
+    if ((lane & (W - 1)) == 0) mem.group[tid / W] = mine;
+    G::sync();
+    if (tid >= 32) { G::sync(); return mem.bounds[0]; }
+    mine = mem.group[lane];
+  } else {
+    mem.group[tid] = mine;
+    __syncwarp();
+  }
+  const u64* const rivals = mem.group + (few ? 0 : tid & ~31);
+  const int r = few ? k : (k + W * 3 / 4 - 1) / (W * 3 / 4);
+  int above = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) above += rivals[j] > mine;
+  const unsigned who = __ballot_sync(0xffffffffu, above == r - 1 && mine != 0);
+  u64 bound = who == 0 ? 0 : __shfl_sync(0xffffffffu, mine, __ffs(who) - 1);
+  if (few) {
+    if (W > 1) {
+      if (lane == 0) mem.bounds[0] = bound;
+      G::sync();
+    }
+    return bound;
+  }
+  if (lane == 0) mem.bounds[tid >> 5] = bound;
+  G::sync();
+  const int q = (k + r - 1) / r;                 // warps that give k keys together
+  bound = lane < W ? mem.bounds[lane] : 0;
+  above = 0;
+  for (int j = 0; j < W; ++j) above += mem.bounds[j] > bound || (mem.bounds[j] == bound && j < lane);
+  const unsigned which = __ballot_sync(0xffffffffu, lane < W && above == q - 1);
+  return __shfl_sync(0xffffffffu, bound, __ffs(which) - 1);
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory"); }
+template <typename V>
+__device__ __forceinline__ V* in_block(V* p, uint32_t rank) {   // the same place in another block of the cluster
+  u64 out;
+  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(out) : "l"((u64)(uintptr_t)p), "r"(rank));
+  return reinterpret_cast<V*>((uintptr_t)out);
+}
+
+// shape of a team: words it notes (all of a warp's row), words that a thread takes at a time, such batches in its ring, blocks that share an SM
+template <int NT> struct Shape {
+  static constexpr int KEEP = NT == 32 ? 320 : 1024, BATCH = NT == 256 ? 4 : 2, RING = NT == 32 ? 3 : 2, RESIDENT = NT == 1024 ? 1 : 4;
+  typedef TeamMemory<NT, KEEP, RING * BATCH> Memory;
+};
+
+template <typename T, int NT, bool CAP>
+__global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RESIDENT) logprobs_kernel(const phx_logprobs_args a, int blocks) {
+  constexpr int N = Words<T>::N, KEEP = Shape<NT>::KEEP, RING = Shape<NT>::RING, BATCH = Shape<NT>::BATCH;
+  constexpr int SINGLE = RING * BATCH * NT * 2;             // keys of single logits that the rings' memory holds
+  typedef Team<NT> G;
+  typedef typename Shape<NT>::Memory Memory;
+  extern __shared__ __align__(16) uint8_t smem_bytes[];
+  Memory& mem = reinterpret_cast<Memory*>(smem_bytes)[NT == 32 ? threadIdx.x >> 5 : 0];
+  const int r = NT == 32 ? blockIdx.x * WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x / blocks;
+  if (r >= a.rows) return;                                  // whole warps only
+  const uint32_t rank = NT == 32 || blocks == 1 ? 0 : cluster_rank();
+  const int tid = G::tid(), lane = threadIdx.x & 31, warp = tid >> 5;
+  const T* const row = static_cast<const T*>(a.logits) + (long long)r * a.stride;
+  const float scale = LOG2E / a.temperature, cap2 = CAP ? 2.0f * LOG2E / a.cap : 0.f;
+
+  // 16-byte words of the row, the first and last of them perhaps in part
+  const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+  const T* const base = row - off;
+  const int words = (int)(((long long)off + a.vocab + N - 1) / N), share = (words + blocks - 1) / blocks;
+  const int w_begin = min((int)rank * share, words), w_end = min(w_begin + share, words);
+  const int whole_begin = off > 0 ? 1 : 0, whole_end = (int)(((long long)off + a.vocab) / N);   // words that lie in the row with all their elements
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(&mem.word[0][tid]);
+  // batch `it` of this thread - words w_begin + (it * BATCH + i) * NT + tid - on its way into the ring; what is not of the row is -inf
+  auto fetch = [&](int it) {
+    const int slot = (it % RING) * BATCH;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int w = w_begin + (it * BATCH + i) * NT + tid;
+      const uint32_t dst = ring + (uint32_t)((slot + i) * NT) * 16u;
+      if (w >= whole_begin && w < min(whole_end, w_end)) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<const uint4*>(base) + w) : "memory");
+      } else {
+        const uint32_t none = N == 8 ? 0xFF80FF80u : 0xFF800000u;
+        uint4* const slow = &mem.word[slot + i][tid];
+        *slow = make_uint4(none, none, none, none);
+        if (w < w_end)
+#pragma unroll 1
+          for (int k = 0; k < N; ++k)
+            if (w * N - off + k >= 0 && w * N - off + k < a.vocab) reinterpret_cast<T*>(slow)[k] = row[w * N - off + k];
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 
   Stat st = {-INFINITY, 0.f, 0.f};
-  unsigned long long best = 0;
-  for (int i = tid; i < a.vocab; i += LP_THREADS) {
-    const float x = load_logit<T>(row, i);
-    const unsigned long long key = key_of(x, i);
-    best = key > best ? key : best;
-    if (x != -INFINITY) { const Stat one = {capped(x, a.cap), 1.f, 0.f}; st = join(st, one, a.temperature); }
+  const bool want_top = a.top_k > 0 && (a.top_out || a.top_ids_out);
+  u64 bound = ~0ull;              // of words
+  float bound_x = INFINITY;       // its logit
+  bool lost = false;              // more words than the notes hold
+  if (tid == 0) mem.count = 0;
+  G::sync();
+  // a place behind what has been counted for each lane of a whole warp that wants one
+  auto place_for = [&](bool want) {
+    const unsigned who = __ballot_sync(0xffffffffu, want);
+    int at = 0;
+    if (lane == 0 && who != 0) at = atomicAdd(&mem.count, __popc(who));
+    return __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
+  };
+  // keeps those of the keys `list` [n] that reach a bound taken from them, and the bound; between barriers
+  auto tighten = [&](u64* list, int n) {
+    u64 most = 0;
+    for (int i = tid; i < n; i += NT) most = list[i] > most ? list[i] : most;
+    u64 least = bound_of<NT>(most, a.top_k, mem);
+    G::sync();
+    if (tid == 0) mem.count = 0;
+    G::sync();
+    for (int i0 = 0; i0 < n; i0 += NT) {                         // in place: a key never moves up
+      const u64 key = i0 + tid < n ? list[i0 + tid] : 0;
+      G::sync();
+      const bool stays = key != 0 && key >= least;
+      const int at = place_for(stays);
+      if (stays) list[at] = key;
+      G::sync();
+    }
+    return least;
+  };
+
+  const int batches = (w_end - w_begin + BATCH * NT - 1) / (BATCH * NT);
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i) fetch(i);
+  int again = 2;
+#pragma unroll 1
+  for (int it = 0; it < batches; ++it) {
+    fetch(it + RING - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+    const int slot = (it % RING) * BATCH, w0 = w_begin + it * BATCH * NT + tid;
+    uint4 cur[BATCH];
+    float tops[BATCH], top = -INFINITY;     // of each word, of the batch; NaN if there is one
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(cur[i].x), "=r"(cur[i].y), "=r"(cur[i].z), "=r"(cur[i].w) : "r"(ring + (uint32_t)((slot + i) * NT) * 16u) : "memory");
+      if (N == 8) {
+        const uint32_t v[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
+        auto two = [&](int k) { return *reinterpret_cast<const __nv_bfloat162*>(&v[k]); };
+        const __nv_bfloat162 m2 = __hmax2_nan(__hmax2_nan(two(0), two(1)), __hmax2_nan(two(2), two(3)));
+        tops[i] = max_nan(__low2float(m2), __high2float(m2));
+      } else {
+        float x[N];
+        Words<T>::unpack(cur[i], x);
+        tops[i] = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
+      }
+      top = max_nan(top, tops[i]);
+    }
+
+    if (want_top) {
+      if (it == 0) {              // the first bound
+        u64 best = 0;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          const u64 key = key_of(tops[i], w0 + i * NT);
+          if (w0 + i * NT < w_end && key > best) best = key;
+        }
+        bound = bound_of<NT>(best, a.top_k, mem);
+        bound_x = bound == 0 ? -INFINITY : value_of(bound);
+      }
+      if (!(top < bound_x)) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          if (tops[i] < bound_x || w0 + i * NT >= w_end) continue;
+          const u64 key = key_of(tops[i], w0 + i * NT);
+          if (key >= bound) { const int at = atomicAdd(&mem.count, 1); if (at < KEEP) mem.keep[at] = key; }
+        }
+      }
+      if (NT > 32 && it + 1 == again && it + 1 < batches) {          // a closer bound from what is there
+        again *= 2;
+        G::sync();
+        const int n = mem.count;
+        G::sync();
+        if (n > KEEP) { lost = true; bound = ~0ull; bound_x = INFINITY; }   // not worth noting any more
+        else if (n > 3 * a.top_k) {
+          const u64 closer = tighten(mem.keep, n);
+          if (closer > bound) { bound = closer; bound_x = value_of(bound); }
+        }
+      }
+    }
+
+    if (it == 0) {
+      float first = CAP ? capped_fast(top, a.cap, cap2) : top;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) first = max_nan(first, __shfl_xor_sync(0xffffffffu, first, o));
+      st.m = first;
+    }
+    const float ctop = CAP ? capped_fast(top, a.cap, cap2) : top;
+    if (top != -INFINITY) {
+      if (!((ctop - st.m) * scale <= ROOM)) {   // grown too far, the first that is allowed, or NaN
+        const Stat none = {ctop, 0.f, 0.f};
+        st = join(st, none, scale);
+      }
+      if (st.m > DEEP) {
+        // what lies below FLOOR weighs nothing; raised to it, it has a finite distance from the reference
+        float2 z2 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);
+        const float2 m2 = make_float2(-st.m, -st.m), c2 = make_float2(scale, scale);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          float x[N];
+          Words<T>::unpack(cur[i], x);
+#pragma unroll
+          for (int k = 0; k < N; k += 2) {
+            float y0 = CAP ? capped_fast(x[k], a.cap, cap2) : x[k], y1 = CAP ? capped_fast(x[k + 1], a.cap, cap2) : x[k + 1];
+            const float2 d = __fadd2_rn(make_float2(max_nan(y0, FLOOR), max_nan(y1, FLOOR)), m2);
+            const float2 t = __fmul2_rn(d, c2);
+            const float2 e = make_float2(ex2(t.x), ex2(t.y));
+            z2 = __fadd2_rn(z2, e);
+            s2 = __ffma2_rn(e, d, s2);
+          }
+        }
+        st.z += z2.x + z2.y;
+        st.s += s2.x + s2.y;
+      } else {                    // all logits so far are at a type's lowest values, or NaN
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          float x[N];
+          Words<T>::unpack(cur[i], x);
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const float y = CAP ? capped_fast(x[k], a.cap, cap2) : x[k], d = y - st.m, e = ex2(d * scale);
+            if (y != -INFINITY) { st.z += e; st.s += e == 0.f ? 0.f : e * d; }
+          }
+        }
+      }
+    }
   }
-  for (int o = 16; o > 0; o >>= 1) {
-    Stat other;
-    other.m = __shfl_xor_sync(0xffffffffu, st.m, o); other.z = __shfl_xor_sync(0xffffffffu, st.z, o); other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    st = lane & o ? join(other, st, a.temperature) : join(st, other, a.temperature);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+  // the team's sums, in a fixed order
+  auto fold = [&]() {
+    Stat all = {st.m, 0.f, 0.f};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all.m = max_nan(all.m, __shfl_xor_sync(0xffffffffu, all.m, o));
+    st = join(st, all, scale);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { st.z += __shfl_xor_sync(0xffffffffu, st.z, o); st.s += __shfl_xor_sync(0xffffffffu, st.s, o); }
+  };
+  const Stat none = {-INFINITY, 0.f, 0.f};
+  fold();
+  if (NT > 32) {
+    if (lane == 0) mem.part[warp] = st;
+    G::sync();
+    st = lane < NT / 32 ? mem.part[lane] : none;
+    fold();
   }
-  if (lane == 0) part[warp] = st;
-  keep[tid] = best;
-  if (tid == 0) { bound = 0; count = 0; }
-  __syncthreads();
-  st = part[0];
-  for (int w = 1; w < LP_THREADS / 32; ++w) st = join(st, part[w], a.temperature);
+
+  // the team's best keys, of single logits, over the rings
+  u64* const single = reinterpret_cast<u64*>(&mem.word[0][0]);
+  int n = 0;
+  if (want_top) {
+    G::sync();
+    int notes = mem.count;
+    G::sync();
+    lost |= notes > KEEP;
+    if (!lost && notes > 2 * a.top_k) {
+      const u64 closer = tighten(mem.keep, notes);
+      bound = closer > bound ? closer : bound;
+      notes = mem.count;
+    }
+    lost |= notes * N > SINGLE;
+    const int e_begin = max(0, w_begin * N - off), e_end = (int)min((long long)a.vocab, (long long)w_end * N - off);
+    G::sync();
+    if (tid == 0) mem.count = 0;
+    G::sync();
+    if (!lost) {
+      for (int i0 = 0; i0 < notes * N; i0 += NT) {
+        const int i = i0 + tid;
+        u64 key = 0;
+        if (i < notes * N) {
+          const uint32_t word = (uint32_t)mem.keep[i / N];       // ~place
+          const int id = (int)~word * N - off + i % N;
+          if (id >= 0 && id < a.vocab) {
+            key = key_of(Words<T>::at(row, id), id);
+            if (((key >> 32) << 32 | word) < bound) key = 0;
+          }
+        }
+        const int at = place_for(key != 0);
+        if (key != 0) single[at] = key;
+      }
+    } else {
+      u64 prefix = 0;
+      int left = min(a.top_k, e_end - e_begin);
+      for (int shift = 56; shift >= 0; shift -= 8) {
+        for (int i = tid; i < 256; i += NT) mem.hist[i] = 0;
+        G::sync();
+        for (int i = e_begin + tid; i < e_end; i += NT) {
+          const u64 key = key_of(Words<T>::at(row, i), i);
+          if (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&mem.hist[(key >> shift) & 255], 1);
+        }
+        G::sync();
+        int digit = 255;
+        for (; digit > 0 && mem.hist[digit] < left; --digit) left -= mem.hist[digit];
+        prefix |= (u64)digit << shift;
+        G::sync();
+      }
+      for (int i = e_begin + tid; i < e_end; i += NT) {
+        const u64 key = key_of(Words<T>::at(row, i), i);
+        if (key >= prefix) single[atomicAdd(&mem.count, 1)] = key;
+      }
+    }
+    G::sync();
+    n = mem.count;
+    G::sync();
+    if (n > a.top_k + a.top_k / 2) {
+      tighten(single, n);
+      n = mem.count;
+    }
+  }
+  // a key's place is the number of larger ones
+  auto place = [&](u64 key) {
+    int above = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) above += single[j] > key;
+    return above;
+  };
+
+  if (NT > 32 && blocks > 1) {    // the first block takes the others' sums and keys
+    if (tid == 0) mem.stat = st;
+    for (int i = tid; i < a.top_k; i += NT) mem.best[i] = 0;
+    G::sync();
+    for (int i = tid; i < n; i += NT) {
+      const u64 key = single[i];
+      const int above = place(key);
+      if (above < a.top_k) mem.best[above] = key;
+    }
+    cluster_sync();
+    if (rank == 0) {
+      st = lane < blocks ? *in_block(&mem.stat, min(lane, blocks - 1)) : none;
+      fold();
+      n = want_top ? blocks * a.top_k : 0;
+      for (int i = tid; i < n; i += NT) single[i] = in_block(&mem.best[0], i / a.top_k)[i % a.top_k];
+    }
+    cluster_sync();               // nobody leaves before it has been read
+    if (rank != 0) return;
+  }
+  if (NT > 32) G::sync();
+
   const float logz = logf(st.z);
   auto logp = [&](float x) {
     if (x == -INFINITY) return -INFINITY;
     return (capped(x, a.cap) - st.m) / a.temperature - logz;
   };
-  if (a.entropy_out && tid == 0) a.entropy_out[r] = st.z == 0.f ? 0.f : logz - st.s / st.z;
+  if (a.entropy_out && tid == 0) a.entropy_out[r] = st.z == 0.f ? 0.f : logz - st.s / st.z / a.temperature;
   if (a.given_out)
-    for (int i = tid; i < a.num_given; i += LP_THREADS) {
+    for (int i = tid; i < a.num_given; i += NT) {
       const long long id = a.given[(long long)r * a.num_given + i];
-      a.given_out[(long long)r * a.num_given + i] = id < 0 || id >= a.vocab ? 0.f : logp(load_logit<T>(row, (int)id));
+      a.given_out[(long long)r * a.num_given + i] = id < 0 || id >= a.vocab ? 0.f : logp(Words<T>::at(row, id));
     }
-  if (a.top_k == 0 || (!a.top_out && !a.top_ids_out)) return;
+  for (int i = tid; i < n; i += NT) {
+    const u64 key = single[i];
+    const int above = key == 0 ? a.top_k : place(key);
+    if (above >= a.top_k) continue;
+    if (a.top_ids_out) a.top_ids_out[(long long)r * a.top_k + above] = (int)~(uint32_t)key;
+    if (a.top_out) a.top_out[(long long)r * a.top_k + above] = logp(value_of(key));
+  }
+}
 
-  int above = 0;
-  for (int i = 0; i < LP_THREADS; ++i) above += keep[i] > best;
-  if (best != 0 && above == a.top_k - 1) bound = best;
-  __syncthreads();
-  auto collect = [&]() {
-    const unsigned long long least = bound;
-    for (int i = tid; i < a.vocab; i += LP_THREADS) {
-      const unsigned long long key = key_of(load_logit<T>(row, i), i);
-      if (key >= least) { const int at = atomicAdd(&count, 1); if (at < LP_KEEP) keep[at] = key; }
-    }
-    __syncthreads();
-  };
-  collect();
-  if (count > LP_KEEP) {
-    unsigned long long prefix = 0;
-    int left = a.top_k;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      hist[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < a.vocab; i += LP_THREADS) {
-        const unsigned long long key = key_of(load_logit<T>(row, i), i);
-        if (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
-      }
-      __syncthreads();
-      int digit = 255;
-      for (; digit > 0 && hist[digit] < left; --digit) left -= hist[digit];
-      prefix |= (unsigned long long)digit << shift;
-      __syncthreads();
-    }
-    if (tid == 0) { bound = prefix; count = 0; }
-    __syncthreads();
-    collect();
-  }
-  const int n = min(count, LP_KEEP);
-  for (int i = tid; i < n; i += LP_THREADS) {
-    const unsigned long long key = keep[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += keep[j] > key;
-    if (rank >= a.top_k) continue;
-    const int id = (int)~(uint32_t)key;
-    if (a.top_ids_out) a.top_ids_out[(long long)r * a.top_k + rank] = id;
-    if (a.top_out) a.top_out[(long long)r * a.top_k + rank] = logp(load_logit<T>(row, id));
-  }
+template <typename T, int NT, bool CAP>
+cudaError_t logprobs_launch(const phx_logprobs_args& a, int blocks, cudaStream_t stream) {
+  constexpr int smem = (NT == 32 ? WARP_ROWS : 1) * (int)sizeof(typename Shape<NT>::Memory);
+  static SmemLimit limit;
+  const cudaError_t e = smem > 48 * 1024 ? limit.raise(logprobs_kernel<T, NT, CAP>, smem) : cudaSuccess;
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t lc;
+  memset(&lc, 0, sizeof(lc));
+  lc.gridDim = dim3((unsigned)(NT == 32 ? (a.rows + WARP_ROWS - 1) / WARP_ROWS : a.rows * blocks));
+  lc.blockDim = dim3(NT == 32 ? 32 * WARP_ROWS : NT);
+  lc.dynamicSmemBytes = smem; lc.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)blocks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  lc.attrs = at; lc.numAttrs = 1;
+  return cudaLaunchKernelEx(&lc, logprobs_kernel<T, NT, CAP>, a, blocks);
+}
+// Threads of a row: enough for its words in one batch, as far as the device has room for all rows at once (148 SMs of 1024 threads at
+// this kernel's registers); a warp for rows it can hold (and ids it can bound by its lanes), else a block, else a cluster of up to eight.
+template <typename T, bool CAP>
+cudaError_t logprobs_dispatch(const phx_logprobs_args& a, cudaStream_t stream) {
+  const long long need = (a.vocab + 2ll * Words<T>::N) / (Words<T>::N * 4) + 1;
+  const long long room = (long long)device_sms() * 1024 / a.rows;
+  const long long threads = need < room ? need : room;
+  if (a.vocab <= 1024 && a.top_k <= 24) return logprobs_launch<T, 32, CAP>(a, 1, stream);
+  if (threads <= 512 || a.rows > 1 << 27) return logprobs_launch<T, 256, CAP>(a, 1, stream);
+  const int blocks = threads <= 1024 ? 1 : threads <= 2048 ? 2 : threads <= 4096 ? 4 : 8;
+  return logprobs_launch<T, 1024, CAP>(a, blocks, stream);
 }
 
 }  // namespace
@@ -150,6 +523,7 @@ extern "C" phx_status phx_token_logprobs_device(int32_t device, const phx_logpro
   if (!args) return bad("null argument");
   const phx_logprobs_args& a = *args;
   if (a.rows < 0 || a.vocab < 1 || a.num_given < 0) return bad("rows and num_given must not be negative, vocab positive");
+  if (a.vocab > 1 << 28) return bad("vocab must be at most 2^28");
   if (a.top_k < 0 || a.top_k > PHX_LOGPROBS_MAX_TOP || a.top_k > a.vocab) return bad("top_k must be at most 128 and at most vocab");
   if (!(a.temperature > 0.f) || isinf(a.temperature)) return bad("temperature must be positive");
   if (!(a.cap == a.cap) || isinf(a.cap)) return bad("cap must be finite");
@@ -160,9 +534,9 @@ extern "C" phx_status phx_token_logprobs_device(int32_t device, const phx_logpro
   if (a.num_given > 0 && a.given_out && !a.given) return bad("given is required with given_out");
   DeviceScope scope(device);
   if (!scope.ok()) { set_global_error("phx_token_logprobs_device: cudaSetDevice failed"); return PHX_E_CUDA; }
-  if (a.is_bf16) logprobs_kernel<bf16><<<a.rows, LP_THREADS, 0, (cudaStream_t)stream>>>(a);
-  else logprobs_kernel<float><<<a.rows, LP_THREADS, 0, (cudaStream_t)stream>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  cudaStream_t st = (cudaStream_t)stream;
+  const cudaError_t e = a.is_bf16 ? (a.cap > 0.f ? logprobs_dispatch<bf16, true>(a, st) : logprobs_dispatch<bf16, false>(a, st))
+                                  : (a.cap > 0.f ? logprobs_dispatch<float, true>(a, st) : logprobs_dispatch<float, false>(a, st));
   if (e != cudaSuccess) { set_global_error(std::string("phx_token_logprobs_device: ") + cudaGetErrorString(e)); return PHX_E_CUDA; }
   dispatch_note(DK_TOKEN_LOGPROBS);
   return PHX_OK;
