@@ -85,7 +85,7 @@ def test_entry_points_refuse_wrong_arguments():
         assert _lib.lib.phx_history_append_device(0, C.byref(c), C.byref(a), None) == 1, wrong
     tree = dict(q=16, q_stride=256, out=16, workspace=256, workspace_bytes=1 << 40, max_keys=64, max_tokens=1, num_q_heads=4, sm_scale=0.1)
     for wrong in (dict(q=None), dict(q=2), dict(out=None), dict(out=8), dict(q_stride=248), dict(q_stride=260), dict(num_q_heads=5), dict(cap_method=3),
-                  dict(sm_scale=float("nan")), dict(cap=float("nan")), dict(spans=4), dict(max_tokens=-1), dict(max_keys=-1)):
+                  dict(sm_scale=float("nan")), dict(cap=float("nan")), dict(workspace=None), dict(workspace=8), dict(spans=4), dict(max_tokens=-1), dict(max_keys=-1)):
         a = _lib.TreeArgs(**{**tree, **wrong})
         assert _lib.lib.phx_tree_attention_device(0, C.byref(c), C.byref(a), None) == 1, wrong
     logp = dict(logits=16, stride=100, given=16, given_out=16, entropy_out=16, top_out=16, top_ids_out=16, rows=1, vocab=100, num_given=1, top_k=5, temperature=1.0)

@@ -6,23 +6,27 @@
 // a key head are rows of one product: row r of a request and key head is token r / g, head r % g of the group, so K and V are read
 // once for all of them.
 //
-// The mma.sync kernel: a CTA's four warps share 16 such rows and take 32 keys each in turn, every warp with its own ring of key and value
-// tiles (cp.async, 16 bytes a piece, no barrier between the warps), running maximum, sum and output; they are joined once at the end.  Masked logits
+// The mma.sync kernel, for requests of up to 16 such rows: a block's four warps share the rows and take 16 keys each in turn, every warp with
+// its own ring of key and value tiles (copied by TMA, which swizzles them for ldmatrix; no barrier between the warps), running maximum, sum and
+// output; they are joined once at the end.  Masked logits
 // become -inf before the maximum; a value row that some of the tile's rows do not see must not reach them as 0 * NaN either, so tiles that are
 // not seen whole are searched for infinities and NaN, which are then added to the rows that do see them, one by one.
+#include <math.h>
+
 #include <string>
 #include <vector>
 
-#include "cache_batch.cuh"
+#include "sm100_ptx.cuh"
+#include "tree_attention.cuh"
 
 namespace phx {
 namespace {
 
 constexpr int TREE_WARPS = 4;
 constexpr int ROWS = 16;         // query rows of a tile
-constexpr int KEYS = 32;         // keys of a warp's tile
+constexpr int KEYS = 16;         // keys of a warp's tile; a page holds whole tiles
 constexpr int STAGES = 3;
-constexpr float LOG2E = 1.4426950408889634f;
+using namespace sm100;
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -36,148 +40,114 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {   // not there: 16 zero bytes
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ bool odd_value(uint16_t v) { return (v & 0x7F80u) == 0x7F80u; }   // infinity or NaN
-__device__ __forceinline__ bool odd_pair(uint32_t v) { return (v & 0x7F80u) == 0x7F80u || (v & 0x7F800000u) == 0x7F800000u; }
-
-// byte of 16-byte piece `piece` of row `row` in a tile: rows of DH * 2 bytes, pieces exchanged so that the eight rows of an ldmatrix
-// block fall on different banks
+// byte of 16-byte piece `piece` of row `row` in a tile as TMA leaves it: 64 columns at a time, rows of 128 (64) bytes with their pieces exchanged
 template <int DH>
 __device__ __forceinline__ uint32_t tile_at(int row, int piece) {
-  constexpr int PIECES = DH / 8;
-  const int sw = PIECES >= 8 ? (row & 7) : ((row >> 1) & 3);
-  return (uint32_t)(row * DH * 2 + ((piece ^ sw) << 4));
-}
-
-struct TreeView {
-  phx_cache_batch c;
-  phx_tree_args a;
-  float csc;           // scale into the log2 domain (no cap)
-};
-
-// The keys of one request and key head, as the kernels meet them
-struct KeyRange {
-  CacheRequest rq;
-  int keys;             // cached + new, as far as the table has columns
-  const int* table;     // the request's row of the table
-};
-__device__ __forceinline__ KeyRange key_range(const phx_cache_batch& c, int b) {
-  KeyRange k;
-  k.rq = cache_request(c, b);
-  k.keys = (int)min((long long)k.rq.cached + k.rq.tokens, cache_columns(c));
-  k.table = c.block_table + (long long)b * c.table_stride;
-  return k;
-}
-// (pre, end) of new token j of a request
-__device__ __forceinline__ int2 span_of(const TreeView& t, const CacheRequest& rq, int j) {
-  return t.a.spans ? reinterpret_cast<const int2*>(t.a.spans)[rq.row0 + j] : make_int2(j, rq.tokens);
+  if (DH == 32) return (uint32_t)(row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+  return (uint32_t)(((piece >> 3) * KEYS + row) * 128 + (((piece & 7) ^ (row & 7)) << 4));
 }
 
 template <int DH>
 struct TreeSmem {
   uint8_t kv[TREE_WARPS][STAGES][2][KEYS * DH * 2];
-  int tile[TREE_WARPS][STAGES];
-  int there[TREE_WARPS][STAGES];   // bit i: keys 16 i .. 16 i + 15 of the tile sit in a page of the pool
+  uint64_t full[TREE_WARPS][STAGES];
+  int tile[TREE_WARPS][STAGES];    // -1: no more
+  int there[TREE_WARPS][STAGES];   // its keys sit in a page of the pool
   float m[TREE_WARPS][ROWS], l[TREE_WARPS][ROWS];
+  TreePlan<32 * TREE_WARPS> plan;
 };
 
 template <int DH, int CAP>
-__global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeView t) {
-  extern __shared__ __align__(128) uint8_t smem_bytes[];
-  TreeSmem<DH>& sm = *reinterpret_cast<TreeSmem<DH>*>(smem_bytes);
+__device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensorMap& map, TreeSmem<DH>& sm, const TreePiece& pc, int& seq) {
   constexpr int PIECES = DH / 8, KSTEPS = DH / 16, NT = DH / 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y, b = blockIdx.z;
+  const int h = pc.h, b = pc.b, group = t.group;
   const KeyRange kr = key_range(t.c, b);
   const CacheRequest& rq = kr.rq;
-  const int group = t.a.num_q_heads / t.c.num_kv_heads;
-  const long long rows = (long long)rq.tokens * group;
-  const int n_tiles = (kr.keys + KEYS - 1) / KEYS;
-  if (threadIdx.x == 0 && (!rq.ok || kr.keys < (long long)rq.cached + rq.tokens)) cache_report(t.c, rq.ok ? CACHE_BAD_PAGE : CACHE_BAD_OFFSETS);
-  const long long v_off = (long long)t.c.num_kv_heads * t.c.page_size * DH;   // from a key to its value
+  const long long rows = (long long)rq.tokens * group, r0 = (long long)pc.row_tile * ROWS;
+  const int n_tiles = min((kr.keys + KEYS - 1) / KEYS, pc.end * TREE_WARPS);
+  if (threadIdx.x == 0 && kr.keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
+  const int v_off = t.c.num_kv_heads * t.c.page_size;                         // rows of the pool from a key to its value
+  const int no_row = (int)(2 * t.c.num_pages * v_off);                        // behind the pool: zeros
   const uint32_t kv_smem = (uint32_t)__cvta_generic_to_shared(sm.kv[warp]);
+  const TreeCap cap(t);
 
-  for (long long r0 = (long long)blockIdx.x * ROWS; r0 < rows; r0 += (long long)gridDim.x * ROWS) {
+  {
     // rows lane / 4 and lane / 4 + 8 of the tile: token, its place in the walk, A fragments of the query
-    int tok[2], pre[2];
+    int pre[2];
     const uint16_t* qrow[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const long long r = min(r0 + lane / 4 + 8 * i, rows - 1);
-      tok[i] = (int)(r / group);
-      const int head = h * group + (int)(r - (long long)tok[i] * group);
-      pre[i] = span_of(t, rq, tok[i]).x;
-      qrow[i] = t.a.q + (long long)(rq.row0 + tok[i]) * t.a.q_stride + head * DH;
+      const int tok = (int)(r / group), head = h * group + (int)(r - (long long)tok * group);
+      pre[i] = span_of(t, rq, tok).x;
+      qrow[i] = t.a.q + (long long)(rq.row0 + tok) * t.a.q_stride + head * DH;
     }
+    int lo = 0, hi = -2;                               // the places that the tile's rows take in the walk, once they are asked for
+    int next = pc.begin * TREE_WARPS + warp;           // the next tile of this warp that may be needed
+    int ahead = -1, ahead_page = 0;                    // a tile whose page has been looked up
+    auto page_of = [&](int tile) { return kr.table[tile * KEYS / t.c.page_size]; };
+    auto load = [&](int at) {                          // the copy of the next tile that is needed into stage `at`, or a note that there is none
+      int tile = -1;
+      for (; next < n_tiles; next += TREE_WARPS) {
+        if ((next + 1) * KEYS <= rq.cached) { tile = next; break; }
+        if (hi == -2) {
+          lo = min(pre[0] < 0 ? 0x7fffffff : pre[0], pre[1] < 0 ? 0x7fffffff : pre[1]);
+          hi = max(pre[0], pre[1]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) { lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o)); }
+        }
+        const int key = next * KEYS + (lane & (KEYS - 1)), j = key - rq.cached;   // this lane's key, among the new ones if j >= 0
+        bool seen = key < kr.keys && hi >= 0;
+        if (seen && j >= 0) { const int2 s = span_of(t, rq, j); seen = s.x <= hi && s.y > lo; }
+        if (__any_sync(0xffffffffu, seen)) { tile = next; break; }
+      }
+      if (tile >= 0) {
+        const int key = tile * KEYS, page = tile == ahead ? ahead_page : page_of(tile);
+        const bool ok = page >= 0 && page < t.c.num_pages;
+        const int row = ok ? (page * 2 * t.c.num_kv_heads + h) * t.c.page_size + key % t.c.page_size : no_row;
+        __syncwarp();                                  // the stage's last reads are done
+        if (elect_one()) {
+          const uint32_t bar = smem_u32(&sm.full[warp][at]), dst = kv_smem + at * (2 * KEYS * DH * 2);
+          mbar_expect_tx(bar, 2 * KEYS * DH * 2);
+#pragma unroll
+          for (int c = 0; c < (DH + 63) / 64; ++c) {
+            tma_load_2d(dst + c * KEYS * 128, &map, bar, c * 64, row);
+            tma_load_2d(dst + KEYS * DH * 2 + c * KEYS * 128, &map, bar, c * 64, ok ? row + v_off : no_row);
+          }
+        }
+        if (lane == 0) {
+          sm.there[warp][at] = ok;
+          if (!ok) cache_report(t.c, CACHE_BAD_PAGE);
+        }
+        next += TREE_WARPS;
+        ahead = next;
+        if (ahead < n_tiles) ahead_page = page_of(ahead);
+      }
+      if (lane == 0) sm.tile[warp][at] = tile;
+    };
+    const int seq0 = seq;                              // tiles that this warp has taken so far, over all pieces: stage and parity of the next
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) load((seq0 + s) % STAGES);
     uint32_t q[KSTEPS][4];
 #pragma unroll
     for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         q[k][i] = *reinterpret_cast<const uint32_t*>(qrow[i & 1] + k * 16 + (i >> 1) * 8 + (lane & 3) * 2);
-    // the places that the tile's rows take in the walk: a tile of new keys that none of them sees is not loaded
-    int lo = min(pre[0] < 0 ? 0x7fffffff : pre[0], pre[1] < 0 ? 0x7fffffff : pre[1]), hi = max(pre[0], pre[1]);
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) { lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o)); }
 
     float acc[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    int next = warp;                                   // the next tile of this warp that may be needed
-    auto load = [&](int stage) {                       // its copy into `stage`, or a note that there is none
-      int tile = -1;
-      for (; next < n_tiles; next += TREE_WARPS) {
-        const int j = next * KEYS + lane - rq.cached;  // this lane's key among the new ones
-        bool seen = next * KEYS + lane < kr.keys;
-        if (seen && j >= 0) { const int2 s = span_of(t, rq, j); seen = s.x <= hi && s.y > lo; }
-        if (__any_sync(0xffffffffu, seen && hi >= 0)) { tile = next; next += TREE_WARPS; break; }
-      }
-      if (tile >= 0) {
-        int there = 0;
-        long long at[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {                  // 16 keys never cross a page
-          const int key = tile * KEYS + 16 * i, col = key / t.c.page_size;
-          const int page = key < kr.keys ? kr.table[col] : 0;
-          const bool ok = key < kr.keys && page >= 0 && page < t.c.num_pages;
-          if (key < kr.keys && !ok && lane == 0) cache_report(t.c, CACHE_BAD_PAGE);
-          there |= ok ? 1 << i : 0;
-          at[i] = ok ? cache_row0(t.c, page, 0, h) + (long long)(key - col * t.c.page_size) * DH : 0;
-        }
-        const uint32_t dst = kv_smem + stage * (2 * KEYS * DH * 2);
-#pragma unroll
-        for (int i = 0; i < KEYS * PIECES / 32; ++i) {
-          const int row = (i * 32 + lane) / PIECES, piece = (i * 32 + lane) % PIECES;
-          const bool ok = ((there >> (row >> 4)) & 1) && tile * KEYS + row < kr.keys;
-          const uint16_t* src = t.c.pages + (ok ? at[row >> 4] + (row & 15) * DH + piece * 8 : 0);
-          cp16(dst + tile_at<DH>(row, piece), src, ok);
-          cp16(dst + KEYS * DH * 2 + tile_at<DH>(row, piece), src + (ok ? v_off : 0), ok);
-        }
-        if (lane == 0) sm.there[warp][stage] = there;
-      }
-      if (lane == 0) sm.tile[warp][stage] = tile;
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) load(s);
-    for (int it = 0;; ++it) {
-      const int stage = it % STAGES;
-      load((it + STAGES - 1) % STAGES);
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    for (;; ++seq) {
+      const int stage = seq % STAGES;
+      load((seq + STAGES - 1) % STAGES);
       __syncwarp();
-      const int tile = sm.tile[warp][stage];
+      const int tile = sm.tile[warp][stage], there = sm.there[warp][stage];
       if (tile < 0) break;
-      const int there = sm.there[warp][stage];
+      mbar_wait(smem_u32(&sm.full[warp][stage]), (uint32_t)((seq / STAGES) & 1), t.c.status_dev);
       const uint32_t sk = kv_smem + stage * (2 * KEYS * DH * 2), sv = sk + KEYS * DH * 2;
 
       float s[KEYS / 8][4];
@@ -195,17 +165,14 @@ __global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeVie
 
       // seen by every row: cached keys in pages of the pool
       const int key0 = tile * KEYS;
-      const bool whole = key0 + KEYS <= min(rq.cached, kr.keys) && there == 3;
+      const bool whole = key0 + KEYS <= min(rq.cached, kr.keys) && there;
       uint32_t seen[2] = {0xffu, 0xffu};               // bit 2 n + c: key 8 n + (lane & 3) * 2 + c, for either row
 #pragma unroll
       for (int n = 0; n < KEYS / 8; ++n)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float v = s[n][c];
-          if (CAP == 0) v *= t.csc;
-          else if (CAP == 1) { v *= t.a.sm_scale; v = v / (1.0f + fabsf(v) / t.a.cap) * LOG2E; }
-          else { v *= t.a.sm_scale; v = t.a.cap * tanhf(v / t.a.cap) * LOG2E; }
-          s[n][c] = v;
+          const float v = s[n][c];
+          s[n][c] = CAP == 0 ? v * t.csc : cap.of<CAP>(v);
         }
       if (!whole) {
         seen[0] = seen[1] = 0;
@@ -214,7 +181,7 @@ __global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeVie
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const int in = n * 8 + (lane & 3) * 2 + c, key = key0 + in;
-            const bool ok = key < kr.keys && ((there >> (in >> 4)) & 1);
+            const bool ok = key < kr.keys && there;
             int2 span = make_int2(0, 0x7fffffff);      // cached: seen by all
             if (ok && key >= rq.cached) span = span_of(t, rq, key - rq.cached);
 #pragma unroll
@@ -235,12 +202,12 @@ __global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeVie
         for (int n = 0; n < KEYS / 8; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn, alpha = ex2(m[i] - base);
+        const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn, alpha = tree_ex2(m[i] - base);
         m[i] = mn;
         float sum = 0.f;
 #pragma unroll
         for (int n = 0; n < KEYS / 8; ++n) {
-          const float e0 = ex2(s[n][2 * i] - base), e1 = ex2(s[n][2 * i + 1] - base);
+          const float e0 = tree_ex2(s[n][2 * i] - base), e1 = tree_ex2(s[n][2 * i + 1] - base);
           sum += e0 + e1;
           p[n >> 1][(n & 1) * 2 + i] = pack_bf2(e0, e1);   // rounded to bf16 for the product; the sum keeps fp32
         }
@@ -289,8 +256,8 @@ __global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeVie
             uint32_t v[4];
             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
             for (int k = 0; k < 4; ++k) {
-              if (odd_value((uint16_t)v[k])) v[k] &= 0xffff0000u;
-              if (odd_value((uint16_t)(v[k] >> 16))) v[k] &= 0xffffu;
+              if (odd_value(v[k])) v[k] &= 0xffff0000u;
+              if (odd_value(v[k] >> 16)) v[k] &= 0xffffu;
             }
             asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
           }
@@ -308,7 +275,6 @@ __global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeVie
         }
       __syncwarp();
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
 
     // the warps' parts, joined: rows of DH floats over the tiles' memory
 #pragma unroll
@@ -335,7 +301,7 @@ __global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeVie
       float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < TREE_WARPS; ++w) {
-        const float f = ex2(sm.m[w][row] - base);
+        const float f = tree_ex2(sm.m[w][row] - base);
         if (sm.l[w][row] == 0.f) continue;                         // a part that saw no key
         sum += sm.l[w][row] * f;
         const float* src = part + (w * ROWS + row) * DH + piece * 8;
@@ -344,41 +310,160 @@ __global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeVie
       }
       const long long r = r0 + row;
       const int tk = (int)(r / group), head = h * group + (int)(r % group);
-      const bool none = sum == 0.f || span_of(t, rq, tk).x < 0;    // no key seen, or a padding token
+      const bool padding = span_of(t, rq, tk).x < 0;
+      if (!pc.whole()) {                                           // the rest of the row's keys is another block's
+        const long long at = (long long)(2 * blockIdx.x + pc.part()) * ROWS + row;
+        *reinterpret_cast<float4*>(t.part_o + at * DH + piece * 8) = make_float4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<float4*>(t.part_o + at * DH + piece * 8 + 4) = make_float4(o[4], o[5], o[6], o[7]);
+        if (piece == 0) t.part_ml[at] = padding ? make_float2(-INFINITY, 0.f) : make_float2(top, sum);
+        continue;
+      }
+      const bool none = sum == 0.f || padding;                     // no key seen, or a padding token
       const float inv = none ? 0.f : 1.0f / sum;
 #pragma unroll
       for (int k = 0; k < 8; ++k) o[k] = none ? 0.f : o[k] * inv;
       const uint4 v = make_uint4(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]), pack_bf2(o[4], o[5]), pack_bf2(o[6], o[7]));
       *reinterpret_cast<uint4*>(t.a.out + ((long long)(rq.row0 + tk) * t.a.num_q_heads + head) * DH + piece * 8) = v;
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next piece's tiles are copied over this
     __syncthreads();
   }
 }
 
 template <int DH, int CAP>
-cudaError_t tree_mma_launch(const TreeView& t, cudaStream_t stream) {
-  static SmemLimit limit;
-  cudaError_t e = limit.raise(tree_mma_kernel<DH, CAP>, (int)sizeof(TreeSmem<DH>));
-  if (e != cudaSuccess) return e;
-  const long long rows = (long long)t.a.max_tokens * (t.a.num_q_heads / t.c.num_kv_heads);
-  const unsigned tiles = (unsigned)((rows + ROWS - 1) / ROWS < 65535 ? (rows + ROWS - 1) / ROWS : 65535);
-  tree_mma_kernel<DH, CAP><<<dim3(tiles, t.c.num_kv_heads, t.c.batch), 32 * TREE_WARPS, sizeof(TreeSmem<DH>), stream>>>(t);
-  return cudaGetLastError();
-}
-template <int DH>
-cudaError_t tree_mma_launch(const TreeView& t, cudaStream_t stream) {
-  return t.a.cap_method == 0 ? tree_mma_launch<DH, 0>(t, stream) : t.a.cap_method == 1 ? tree_mma_launch<DH, 1>(t, stream) : tree_mma_launch<DH, 2>(t, stream);
+__global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeView t, const __grid_constant__ CUtensorMap map) {
+  extern __shared__ uint8_t smem_bytes[];
+  TreeSmem<DH>& sm = *reinterpret_cast<TreeSmem<DH>*>(smem_bytes + ((1024u - (smem_u32(smem_bytes) & 1023u)) & 1023u));
+  if (threadIdx.x == 0) {
+    *gave_up() = 0;
+    for (int w = 0; w < TREE_WARPS; ++w)
+      for (int i = 0; i < STAGES; ++i) mbar_init(smem_u32(&sm.full[w][i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  int seq = 0;
+  if (t.split == 0) {
+    const int b = blockIdx.z;
+    const KeyRange kr = key_range(t.c, b);
+    if (!kr.rq.ok && threadIdx.x == 0) cache_report(t.c, CACHE_BAD_OFFSETS);
+    const int row_tiles = tree_row_tiles(t, kr.rq.tokens), tiles = tree_key_tiles(t, kr.keys);
+    for (int rt = blockIdx.x; rt < row_tiles; rt += gridDim.x) tree_mma_piece<DH, CAP>(t, map, sm, TreePiece{b, (int)blockIdx.y, rt, 0, tiles, tiles}, seq);
+  } else {
+    sm.plan.make(t);
+    if (blockIdx.x == 0)
+      for (int b = threadIdx.x; b < t.c.batch; b += 32 * TREE_WARPS)
+        if (!cache_request(t.c, b).ok) cache_report(t.c, CACHE_BAD_OFFSETS);
+    const long long end = sm.plan.bound(t, blockIdx.x + 1);
+    for (long long pos = sm.plan.bound(t, blockIdx.x); pos < end;) {
+      const TreePiece pc = sm.plan.piece(t, pos, end);
+      tree_mma_piece<DH, CAP>(t, map, sm, pc, seq);
+      pos += pc.end - pc.begin;
+    }
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (*gave_up()) __nanosleep(1000000);                  // copies may still be on their way into this block's memory
 }
 
+// The parts of a unit that blocks x - 1, x, ... left, joined where x - 1 began it; a warp takes a row
+constexpr int JOIN_THREADS = 128;
+template <int DH>
+__global__ void __launch_bounds__(JOIN_THREADS) tree_join_kernel(const TreeView t) {
+  __shared__ TreePlan<JOIN_THREADS> plan;
+  plan.make(t);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int x = blockIdx.x + 1, lane = threadIdx.x & 31;
+  const long long pos = plan.bound(t, x);
+  if (pos >= plan.all(t)) return;
+  const TreePiece pc = plan.piece(t, pos, pos + 1);
+  const long long unit = pos - pc.begin, last = unit + pc.tiles;
+  if (pc.begin == 0 || plan.bound(t, x - 1) > unit) return;
+  const KeyRange kr = key_range(t.c, pc.b);
+  const long long r0 = (long long)pc.row_tile * t.rows;
+  const int rows = (int)min((long long)t.rows, (long long)kr.rq.tokens * t.group - r0);
+  int to = x;                                            // blocks x .. to - 1 have the parts behind the first
+  while (to < t.split && plan.bound(t, to) < last) ++to;
+  constexpr int PER = DH / 32;
+  for (int row = blockIdx.y * (JOIN_THREADS / 32) + (threadIdx.x >> 5); row < rows; row += gridDim.y * (JOIN_THREADS / 32)) {
+    auto slot = [&](int block) { return (long long)(2 * block + (block == x - 1 ? 1 : 0)) * t.rows + row; };
+    float top = -INFINITY;
+    for (int k = x - 1 + lane; k < to; k += 32)
+      if (plan.bound(t, k) < plan.bound(t, k + 1)) top = fmaxf(top, t.part_ml[slot(k)].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll 4
+    for (int k = x - 1; k < to; ++k) {
+      if (plan.bound(t, k) == plan.bound(t, k + 1)) continue;
+      const float2 ml = t.part_ml[slot(k)];
+      const float f = tree_ex2(ml.x - base);
+      if (ml.y == 0.f) continue;                         // saw no key
+      sum += ml.y * f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] += t.part_o[slot(k) * DH + i * 32 + lane] * f;
+    }
+    const long long r = r0 + row;
+    const int tk = (int)(r / t.group), head = pc.h * t.group + (int)(r % t.group);
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    uint16_t* const out = t.a.out + ((long long)(kr.rq.row0 + tk) * t.a.num_q_heads + head) * DH;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bf16 v = f2bf(sum == 0.f ? 0.f : acc[i] * inv);
+      out[i * 32 + lane] = *reinterpret_cast<const uint16_t*>(&v);
+    }
+  }
+}
+
+template <int DH, int CAP>
+phx_status tree_mma_launch(const TreeView& t, cudaStream_t stream, std::string& err) {
+  constexpr int smem = (int)sizeof(TreeSmem<DH>) + 1024;
+  static SmemLimit limit;
+  PHX_CUDA_TRY(limit.raise(tree_mma_kernel<DH, CAP>, smem), err);
+  CUtensorMap map;
+  const phx_status st = tree_pool_map(&map, t, KEYS, err);
+  if (st != PHX_OK) return st;
+  const long long rows = (long long)t.a.max_tokens * t.group;
+  const unsigned tiles = (unsigned)((rows + ROWS - 1) / ROWS < 65535 ? (rows + ROWS - 1) / ROWS : 65535);
+  const dim3 grid = t.split ? dim3(t.split) : dim3(tiles, t.c.num_kv_heads, t.c.batch);
+  tree_mma_kernel<DH, CAP><<<grid, 32 * TREE_WARPS, smem, stream>>>(t, map);
+  PHX_CUDA_TRY(cudaGetLastError(), err);
+  dispatch_note(DK_TREE_MMA);
+  return PHX_OK;
+}
+template <int DH>
+phx_status tree_mma_launch(const TreeView& t, cudaStream_t stream, std::string& err) {
+  return t.a.cap_method == 0 ? tree_mma_launch<DH, 0>(t, stream, err) : t.a.cap_method == 1 ? tree_mma_launch<DH, 1>(t, stream, err) : tree_mma_launch<DH, 2>(t, stream, err);
+}
+
+long long part_bytes(int split, int rows, int dh) { return 2ll * split * rows * (dh * 4 + 8); }
+
 }  // namespace
+
+// The pool as rows of key_size; a box is 64 (32) columns of `box_rows` rows, swizzled; rows behind the pool read as zeros
+phx_status tree_pool_map(CUtensorMap* map, const TreeView& t, int box_rows, std::string& err) {
+  EncodeTiledFn fn = get_encode_fn(err);
+  if (!fn) return PHX_E_CUDA;
+  const int dh = t.c.key_size;
+  cuuint64_t dims[2] = {(cuuint64_t)dh, (cuuint64_t)(2 * t.c.num_pages * t.c.num_kv_heads * t.c.page_size)};
+  cuuint64_t strides[1] = {(cuuint64_t)dh * 2};
+  cuuint32_t box[2] = {(cuuint32_t)(dh < 64 ? dh : 64), (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, t.c.pages, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        dh < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { err = "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r); return PHX_E_CUDA; }
+  return PHX_OK;
+}
+
 }  // namespace phx
 
 using namespace phx;
 
 extern "C" phx_status phx_tree_workspace_bytes(int32_t device, int64_t* bytes_out) {
   if (!bytes_out) { set_global_error("phx_tree_workspace_bytes: null argument"); return PHX_E_ARG; }
-  (void)device;
-  *bytes_out = 0;
+  DeviceScope scope(device);
+  if (!scope.ok()) { set_global_error("phx_tree_workspace_bytes: cudaSetDevice failed"); return PHX_E_CUDA; }
+  *bytes_out = part_bytes(2 * device_sms(), 128, 128);   // the largest that a call may take
   return PHX_OK;
 }
 
@@ -391,23 +476,45 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   t.c = *cache; t.a = *args;
   if (t.a.num_q_heads < 1 || t.a.num_q_heads > 4096 || t.a.num_q_heads % t.c.num_kv_heads != 0) return bad("num_q_heads must be a multiple of num_kv_heads, at most 4096");
   if (t.a.cap_method < 0 || t.a.cap_method > 2) return bad("cap_method must be 0, 1 or 2");
-  if (!(t.a.sm_scale == t.a.sm_scale) || !(t.a.cap == t.a.cap)) return bad("sm_scale and cap must be numbers");
+  if (!isfinite(t.a.sm_scale) || !isfinite(t.a.cap)) return bad("sm_scale and cap must be finite");
   if (t.a.cap_method != 0 && !(t.a.cap > 0.f)) t.a.cap_method = 0;
   if (t.c.batch > 65535) return bad("at most 65535 requests");
   if (t.a.q_stride < (long long)t.a.num_q_heads * t.c.key_size || t.a.q_stride % 8 != 0) return bad("q_stride must be a multiple of 8 and cover a token's heads");
   if (t.a.max_tokens < 0 || t.a.max_keys < 0) return bad("negative size");
   if (t.c.batch == 0 || t.c.num_tokens == 0) return PHX_OK;
   if (t.a.max_tokens < 1) t.a.max_tokens = 1;
+  if (t.a.max_tokens > t.c.num_tokens) t.a.max_tokens = t.c.num_tokens;
   if (!t.a.q || !t.a.out || !aligned16(t.a.q) || !aligned16(t.a.out)) return bad("q and out must be 16-byte aligned buffers");
   if ((reinterpret_cast<uintptr_t>(t.a.spans) & 7) != 0) return bad("spans must be 8-byte aligned");
-  t.csc = t.a.sm_scale * LOG2E;
+  if (!t.a.workspace || !aligned16(t.a.workspace)) return bad("workspace must be a 16-byte aligned buffer");
+  t.csc = t.a.sm_scale * TREE_LOG2E;
+  t.group = t.a.num_q_heads / t.c.num_kv_heads;
   DeviceScope scope(device);
   if (!scope.ok()) { set_global_error("phx_tree_attention_device: cudaSetDevice failed"); return PHX_E_CUDA; }
   cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = t.c.key_size == 32 ? tree_mma_launch<32>(t, st) : t.c.key_size == 64 ? tree_mma_launch<64>(t, st) : tree_mma_launch<128>(t, st);
-  if (e != cudaSuccess) { set_global_error(std::string("phx_tree_attention_device: ") + cudaGetErrorString(e)); return PHX_E_CUDA; }
-  dispatch_note(DK_TREE_MMA);
-  return PHX_OK;
+  std::string err;
+
+  t.rows = ROWS; t.keys = KEYS * TREE_WARPS;
+  const int per_sm = t.c.key_size == 128 ? 2 : 4;   // by shared memory
+  // Blocks share the tiles of all units where there are few units for them and long ones among them.
+  const long long units = (long long)t.c.batch * t.c.num_kv_heads * (((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows);
+  const long long tiles = (t.a.max_keys + t.keys - 1) / t.keys;
+  int blocks = per_sm * device_sms();
+  t.split = tiles >= 4 && units < 8ll * blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? blocks : 0;
+  if (part_bytes(t.split, t.rows, t.c.key_size) > t.a.workspace_bytes) return bad("workspace is smaller than phx_tree_workspace_bytes");
+  t.part_o = static_cast<float*>(t.a.workspace);
+  t.part_ml = reinterpret_cast<float2*>(t.part_o + 2ll * t.split * t.rows * t.c.key_size);
+  if (t.c.num_pages == 0) return bad("an empty pool has no keys to attend to");
+  phx_status s = t.c.key_size == 32 ? tree_mma_launch<32>(t, st, err) : t.c.key_size == 64 ? tree_mma_launch<64>(t, st, err) : tree_mma_launch<128>(t, st, err);
+  if (s == PHX_OK && t.split) {
+    const dim3 grid(t.split - 1, 4);
+    const cudaError_t e = t.c.key_size == 32 ? launch_programmatic(tree_join_kernel<32>, grid, dim3(JOIN_THREADS), 0, st, t)
+                          : t.c.key_size == 64 ? launch_programmatic(tree_join_kernel<64>, grid, dim3(JOIN_THREADS), 0, st, t)
+                                               : launch_programmatic(tree_join_kernel<128>, grid, dim3(JOIN_THREADS), 0, st, t);
+    if (e != cudaSuccess) { err = cudaGetErrorString(e); s = PHX_E_CUDA; }
+  }
+  if (s != PHX_OK) set_global_error("phx_tree_attention_device: " + err);
+  return s;
 }
 
 // Depth-first places of a forest given by parents, without recursion: tokens below each token are counted from the leaves up

@@ -1,0 +1,132 @@
+// What the kernels of the attention over a paged cache share: the request as they meet it, the caps, and how the work is cut.
+//
+// A unit is one request, key head and tile of query rows; row r of a request and key head is token r / group, head r % group of the
+// head's queries.  Where units are few, the device's blocks share the tiles of keys of all units evenly instead (TreePlan):
+// block c of G takes the tiles at c W / G .. (c + 1) W / G of W in all, units one after the other.  A unit that crosses such a bound is left in
+// parts - rows of fp32 output that are not normalised, with their reference and sum - in the workspace, at most two a block, and tree_join_kernel joins
+// them, in the order of the keys.
+#pragma once
+
+#include "cache_batch.cuh"
+
+namespace phx {
+
+constexpr float TREE_LOG2E = 1.4426950408889634f;
+constexpr int TREE_MAX_SPLIT_BATCH = 1024;      // requests whose tiles the blocks may share
+
+struct TreeView {
+  phx_cache_batch c;
+  phx_tree_args a;
+  float csc;             // scale into the log2 domain (no cap)
+  int group;             // query heads of a key head
+  int rows, keys;        // of a tile
+  int split;             // blocks that share the tiles; 0: a block takes whole units
+  float* part_o;         // [2 split][rows][key_size]
+  float2* part_ml;       // [2 split][rows]: reference (log2 domain), sum
+};
+
+__device__ __forceinline__ float tree_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// cap(s * scale) in the log2 domain: method 1 s / (1 + |s| / cap), 2 cap tanh(s / cap) as cap (1 - 2 / (e^(2 s / cap) + 1)), good to 1e-7 of the cap
+struct TreeCap {
+  float scale, a, b;
+  __device__ __forceinline__ TreeCap(const TreeView& t) {
+    const float cap = t.a.cap;
+    scale = t.a.cap_method == 1 ? t.a.sm_scale : t.a.sm_scale * 2.0f * TREE_LOG2E / cap;
+    a = t.a.cap_method == 1 ? 1.0f / cap : -2.0f * cap * TREE_LOG2E;
+    b = cap * TREE_LOG2E;
+  }
+  template <int METHOD> __device__ __forceinline__ float of(float s) const {
+    const float v = s * scale;
+    if (METHOD == 1) return __fdividef(v, 1.0f + fabsf(v) * a) * TREE_LOG2E;
+    return b + __fdividef(a, tree_ex2(v) + 1.0f);
+  }
+};
+
+// The keys of one request and key head, as the kernels meet them
+struct KeyRange {
+  CacheRequest rq;
+  int keys;             // cached + new, as far as the table has columns
+  const int* table;     // the request's row of the table
+};
+__device__ __forceinline__ KeyRange key_range(const phx_cache_batch& c, int b) {
+  KeyRange k;
+  k.rq = cache_request(c, b);
+  k.keys = (int)min((long long)k.rq.cached + k.rq.tokens, cache_columns(c));
+  k.table = c.block_table + (long long)b * c.table_stride;
+  return k;
+}
+// (pre, end) of new token j of a request
+__device__ __forceinline__ int2 span_of(const TreeView& t, const CacheRequest& rq, int j) {
+  return t.a.spans ? reinterpret_cast<const int2*>(t.a.spans)[rq.row0 + j] : make_int2(j, rq.tokens);
+}
+__device__ __forceinline__ bool odd_value(uint32_t v) { return (v & 0x7F80u) == 0x7F80u; }   // infinity or NaN in the low half
+__device__ __forceinline__ bool odd_pair(uint32_t v) { return odd_value(v) || (v & 0x7F800000u) == 0x7F800000u; }
+
+// A stretch of a unit's tiles of keys
+struct TreePiece {
+  int b, h, row_tile;
+  int begin, end, tiles;        // of `tiles` in all
+  __device__ __forceinline__ bool whole() const { return begin == 0 && end == tiles; }
+  // which of its block's two parts: the one that another block began, or the one that another ends
+  __device__ __forceinline__ int part() const { return begin > 0 ? 0 : 1; }
+};
+
+__device__ __forceinline__ int tree_row_tiles(const TreeView& t, int tokens) { return (int)(((long long)tokens * t.group + t.rows - 1) / t.rows); }
+__device__ __forceinline__ int tree_key_tiles(const TreeView& t, int keys) { return keys > 0 ? (keys - 1) / t.keys + 1 : 1; }
+
+// Tiles in front of each request, in shared memory
+template <int THREADS> struct TreePlan {
+  long long before[TREE_MAX_SPLIT_BATCH + 1];
+  long long warp_sum[THREADS / 32];
+
+  // by all threads of the block; ends with a barrier
+  __device__ void make(const TreeView& t) {
+    const int tid = threadIdx.x, lane = tid & 31, per = (t.c.batch + THREADS - 1) / THREADS, b0 = min(tid * per, t.c.batch), b1 = min(b0 + per, t.c.batch);
+    auto tiles_of = [&](int b) {
+      const KeyRange k = key_range(t.c, b);
+      return (long long)t.c.num_kv_heads * tree_row_tiles(t, k.rq.tokens) * tree_key_tiles(t, k.keys);
+    };
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += tiles_of(b);
+    long long sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, sum, o); sum += lane >= o ? x : 0; }
+    if (lane == 31) warp_sum[tid >> 5] = sum;
+    __syncthreads();
+    long long at = sum - mine;
+    for (int w = 0; w < (tid >> 5); ++w) at += warp_sum[w];
+    for (int b = b0; b < b1; ++b) { before[b] = at; at += per == 1 ? mine : tiles_of(b); }
+    if (tid == THREADS - 1) before[t.c.batch] = at;      // the last thread ends behind all
+    __syncthreads();
+  }
+  __device__ __forceinline__ long long all(const TreeView& t) const { return before[t.c.batch]; }
+  __device__ __forceinline__ long long bound(const TreeView& t, int block) const { return all(t) * block / t.split; }
+  // the piece from position `pos` on, at most to `end`
+  __device__ __forceinline__ TreePiece piece(const TreeView& t, long long pos, long long end) const {
+    int lo = 0, hi = t.c.batch;                          // before[lo] <= pos < before[hi]
+    while (hi - lo > 1) { const int mid = (lo + hi) / 2; if (before[mid] <= pos) lo = mid; else hi = mid; }
+    const KeyRange k = key_range(t.c, lo);
+    TreePiece p;
+    p.b = lo;
+    p.tiles = tree_key_tiles(t, k.keys);
+    const long long in = pos - before[lo], unit = in / p.tiles;
+    const int row_tiles = tree_row_tiles(t, k.rq.tokens);
+    p.h = (int)(unit / row_tiles); p.row_tile = (int)(unit - (long long)p.h * row_tiles);
+    p.begin = (int)(in - unit * p.tiles);
+    p.end = (int)min((long long)p.tiles, p.begin + (end - pos));
+    return p;
+  }
+};
+
+phx_status tree_pool_map(CUtensorMap* map, const TreeView& t, int box_rows, std::string& err);
+// tcgen05 kernel (tree_attention_sm100.cu): whether it takes the call, its tile shape, its launch
+bool tree_tc_supported(const TreeView& t);
+void tree_tc_shape(TreeView& t);                 // rows and keys of a tile
+int tree_tc_blocks_per_sm();
+phx_status tree_tc_launch(const TreeView& t, cudaStream_t stream, std::string& err);
+
+}  // namespace phx
