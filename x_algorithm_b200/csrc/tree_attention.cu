@@ -25,7 +25,7 @@ namespace {
 constexpr int TREE_WARPS = 4;
 constexpr int ROWS = 16;         // query rows of a tile
 constexpr int KEYS = 16;         // keys of a warp's tile; a page holds whole tiles
-constexpr int STAGES = 3;
+constexpr int STAGES = 2;
 using namespace sm100;
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -330,8 +330,11 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
   }
 }
 
+// blocks that share an SM: by shared memory (72 KB of tiles at key_size 128), and as many registers
+template <int DH> constexpr int mma_blocks() { return DH == 128 ? 3 : 4; }
+
 template <int DH, int CAP>
-__global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeView t, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(32 * TREE_WARPS, mma_blocks<DH>()) tree_mma_kernel(const TreeView t, const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t smem_bytes[];
   TreeSmem<DH>& sm = *reinterpret_cast<TreeSmem<DH>*>(smem_bytes + ((1024u - (smem_u32(smem_bytes) & 1023u)) & 1023u));
   if (threadIdx.x == 0) {
@@ -350,44 +353,39 @@ __global__ void __launch_bounds__(32 * TREE_WARPS) tree_mma_kernel(const TreeVie
     for (int rt = blockIdx.x; rt < row_tiles; rt += gridDim.x) tree_mma_piece<DH, CAP>(t, map, sm, TreePiece{b, (int)blockIdx.y, rt, 0, tiles, tiles}, seq);
   } else {
     sm.plan.make(t);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join's blocks may make their plan beside this
     if (blockIdx.x == 0)
       for (int b = threadIdx.x; b < t.c.batch; b += 32 * TREE_WARPS)
         if (!cache_request(t.c, b).ok) cache_report(t.c, CACHE_BAD_OFFSETS);
-    const long long end = sm.plan.bound(t, blockIdx.x + 1);
-    for (long long pos = sm.plan.bound(t, blockIdx.x); pos < end;) {
-      const TreePiece pc = sm.plan.piece(t, pos, end);
-      tree_mma_piece<DH, CAP>(t, map, sm, pc, seq);
-      pos += pc.end - pc.begin;
+    const long long end = sm.plan.bound(blockIdx.x + 1);
+    const long long start = sm.plan.bound(blockIdx.x);
+    if (threadIdx.x == 0) t.join[blockIdx.x].rows = 0;
+    for (long long pos = start; pos < end;) {
+      const bool first = pos == start;
+      long long unit_end;
+      const TreePiece pc = sm.plan.piece(t, pos, end, &pos, &unit_end);
+      if (first && threadIdx.x == 0) sm.plan.note_join(t, blockIdx.x, pc, unit_end);
+      if (pc.begin < pc.end) tree_mma_piece<DH, CAP>(t, map, sm, pc, seq);
     }
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (*gave_up()) __nanosleep(1000000);                  // copies may still be on their way into this block's memory
 }
 
-// The parts of a unit that blocks x - 1, x, ... left, joined where x - 1 began it; a warp takes a row
-constexpr int JOIN_THREADS = 128;
+// The parts of a unit that blocks x - 1, x, ... left, joined in the order of the keys: a block takes a row at a time, its warps every fourth part
+constexpr int JOIN_WARPS = 4;
 template <int DH>
-__global__ void __launch_bounds__(JOIN_THREADS) tree_join_kernel(const TreeView t) {
-  __shared__ TreePlan<JOIN_THREADS> plan;
-  plan.make(t);
+__global__ void __launch_bounds__(32 * JOIN_WARPS) tree_join_kernel(const TreeView t) {
+  __shared__ float acc_of[JOIN_WARPS][DH];
+  __shared__ float sum_of[JOIN_WARPS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int x = blockIdx.x + 1, lane = threadIdx.x & 31;
-  const long long pos = plan.bound(t, x);
-  if (pos >= plan.all(t)) return;
-  const TreePiece pc = plan.piece(t, pos, pos + 1);
-  const long long unit = pos - pc.begin, last = unit + pc.tiles;
-  if (pc.begin == 0 || plan.bound(t, x - 1) > unit) return;
-  const KeyRange kr = key_range(t.c, pc.b);
-  const long long r0 = (long long)pc.row_tile * t.rows;
-  const int rows = (int)min((long long)t.rows, (long long)kr.rq.tokens * t.group - r0);
-  int to = x;                                            // blocks x .. to - 1 have the parts behind the first
-  while (to < t.split && plan.bound(t, to) < last) ++to;
+  const int x = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const TreeJoin j = t.join[x];
   constexpr int PER = DH / 32;
-  for (int row = blockIdx.y * (JOIN_THREADS / 32) + (threadIdx.x >> 5); row < rows; row += gridDim.y * (JOIN_THREADS / 32)) {
-    auto slot = [&](int block) { return (long long)(2 * block + (block == x - 1 ? 1 : 0)) * t.rows + row; };
+  for (int row = blockIdx.y; row < j.rows; row += gridDim.y) {
+    const int parts = j.to - x + 1;
+    auto slot = [&](int k) { return ((long long)2 * (x - 1 + k) + (k == 0 ? 1 : 0)) * t.rows + row; };   // of part k
     float top = -INFINITY;
-    for (int k = x - 1 + lane; k < to; k += 32)
-      if (plan.bound(t, k) < plan.bound(t, k + 1)) top = fmaxf(top, t.part_ml[slot(k)].x);
+    for (int k = lane; k < parts; k += 32) top = fmaxf(top, t.part_ml[slot(k)].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float base = top == -INFINITY ? 0.f : top;
@@ -395,23 +393,27 @@ __global__ void __launch_bounds__(JOIN_THREADS) tree_join_kernel(const TreeView 
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
 #pragma unroll 4
-    for (int k = x - 1; k < to; ++k) {
-      if (plan.bound(t, k) == plan.bound(t, k + 1)) continue;
+    for (int k = warp; k < parts; k += JOIN_WARPS) {
       const float2 ml = t.part_ml[slot(k)];
+      const float* o = t.part_o + slot(k) * DH + lane * PER;
       const float f = tree_ex2(ml.x - base);
-      if (ml.y == 0.f) continue;                         // saw no key
-      sum += ml.y * f;
+      sum += ml.y == 0.f ? 0.f : ml.y * f;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) acc[i] += t.part_o[slot(k) * DH + i * 32 + lane] * f;
+      for (int i = 0; i < PER; ++i) { const float v = o[i]; acc[i] += ml.y == 0.f ? 0.f : v * f; }   // a part that saw no key may hold anything
     }
-    const long long r = r0 + row;
-    const int tk = (int)(r / t.group), head = pc.h * t.group + (int)(r % t.group);
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    uint16_t* const out = t.a.out + ((long long)(kr.rq.row0 + tk) * t.a.num_q_heads + head) * DH;
+    if (row >= (int)gridDim.y) __syncthreads();
+    if (lane == 0) sum_of[warp] = sum;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const bf16 v = f2bf(sum == 0.f ? 0.f : acc[i] * inv);
-      out[i * 32 + lane] = *reinterpret_cast<const uint16_t*>(&v);
+    for (int i = 0; i < PER; ++i) acc_of[warp][lane * PER + i] = acc[i];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < DH) {
+      float s = 0.f, v = 0.f;
+#pragma unroll
+      for (int w = 0; w < JOIN_WARPS; ++w) { s += sum_of[w]; v += acc_of[w][d]; }
+      const int r = j.row0 + row, tk = r / t.group, head = j.h * t.group + r % t.group;
+      const bf16 y = f2bf(s == 0.f ? 0.f : v / s);
+      t.a.out[((long long)(j.token0 + tk) * t.a.num_q_heads + head) * DH + d] = *reinterpret_cast<const uint16_t*>(&y);
     }
   }
 }
@@ -437,7 +439,7 @@ phx_status tree_mma_launch(const TreeView& t, cudaStream_t stream, std::string& 
   return t.a.cap_method == 0 ? tree_mma_launch<DH, 0>(t, stream, err) : t.a.cap_method == 1 ? tree_mma_launch<DH, 1>(t, stream, err) : tree_mma_launch<DH, 2>(t, stream, err);
 }
 
-long long part_bytes(int split, int rows, int dh) { return 2ll * split * rows * (dh * 4 + 8); }
+long long part_bytes(int split, int rows, int dh) { return 2ll * split * rows * (dh * 4 + 8) + split * (long long)sizeof(TreeJoin); }
 
 }  // namespace
 
@@ -463,7 +465,7 @@ extern "C" phx_status phx_tree_workspace_bytes(int32_t device, int64_t* bytes_ou
   if (!bytes_out) { set_global_error("phx_tree_workspace_bytes: null argument"); return PHX_E_ARG; }
   DeviceScope scope(device);
   if (!scope.ok()) { set_global_error("phx_tree_workspace_bytes: cudaSetDevice failed"); return PHX_E_CUDA; }
-  *bytes_out = part_bytes(2 * device_sms(), 128, 128);   // the largest that a call may take
+  *bytes_out = part_bytes(3 * device_sms(), 128, 128);   // the largest that a call may take
   return PHX_OK;
 }
 
@@ -495,22 +497,24 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   std::string err;
 
   t.rows = ROWS; t.keys = KEYS * TREE_WARPS;
-  const int per_sm = t.c.key_size == 128 ? 2 : 4;   // by shared memory
+  const int per_sm = t.c.key_size == 128 ? mma_blocks<128>() : mma_blocks<64>();
   // Blocks share the tiles of all units where there are few units for them and long ones among them.
   const long long units = (long long)t.c.batch * t.c.num_kv_heads * (((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows);
   const long long tiles = (t.a.max_keys + t.keys - 1) / t.keys;
-  int blocks = per_sm * device_sms();
-  t.split = tiles >= 4 && units < 8ll * blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? blocks : 0;
+  const long long blocks = per_sm * device_sms(), fed = units * (tiles + TREE_SETUP) / 4;   // no block for less than four places
+  t.split = tiles >= 4 && units < 8 * blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)(fed < blocks ? fed : blocks) : 0;
   if (part_bytes(t.split, t.rows, t.c.key_size) > t.a.workspace_bytes) return bad("workspace is smaller than phx_tree_workspace_bytes");
   t.part_o = static_cast<float*>(t.a.workspace);
   t.part_ml = reinterpret_cast<float2*>(t.part_o + 2ll * t.split * t.rows * t.c.key_size);
+  t.join = reinterpret_cast<TreeJoin*>(t.part_ml + 2ll * t.split * t.rows);
   if (t.c.num_pages == 0) return bad("an empty pool has no keys to attend to");
   phx_status s = t.c.key_size == 32 ? tree_mma_launch<32>(t, st, err) : t.c.key_size == 64 ? tree_mma_launch<64>(t, st, err) : tree_mma_launch<128>(t, st, err);
   if (s == PHX_OK && t.split) {
-    const dim3 grid(t.split - 1, 4);
-    const cudaError_t e = t.c.key_size == 32 ? launch_programmatic(tree_join_kernel<32>, grid, dim3(JOIN_THREADS), 0, st, t)
-                          : t.c.key_size == 64 ? launch_programmatic(tree_join_kernel<64>, grid, dim3(JOIN_THREADS), 0, st, t)
-                                               : launch_programmatic(tree_join_kernel<128>, grid, dim3(JOIN_THREADS), 0, st, t);
+    const long long rows = (long long)t.a.max_tokens * t.group;
+    const dim3 grid(t.split - 1, (unsigned)(rows < t.rows ? rows : t.rows)), block(32 * JOIN_WARPS);
+    const cudaError_t e = t.c.key_size == 32 ? launch_programmatic(tree_join_kernel<32>, grid, block, 0, st, t)
+                          : t.c.key_size == 64 ? launch_programmatic(tree_join_kernel<64>, grid, block, 0, st, t)
+                                               : launch_programmatic(tree_join_kernel<128>, grid, block, 0, st, t);
     if (e != cudaSuccess) { err = cudaGetErrorString(e); s = PHX_E_CUDA; }
   }
   if (s != PHX_OK) set_global_error("phx_tree_attention_device: " + err);

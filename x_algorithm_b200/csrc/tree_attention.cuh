@@ -1,10 +1,12 @@
 // What the kernels of the attention over a paged cache share: the request as they meet it, the caps, and how the work is cut.
 //
 // A unit is one request, key head and tile of query rows; row r of a request and key head is token r / group, head r % group of the
-// head's queries.  Where units are few, the device's blocks share the tiles of keys of all units evenly instead (TreePlan):
-// block c of G takes the tiles at c W / G .. (c + 1) W / G of W in all, units one after the other.  A unit that crosses such a bound is left in
+// head's queries.  Where units are few, the device's blocks share the tiles of keys of all units evenly instead (TreePlan): the units are laid
+// out one after the other, each as its tiles behind TREE_SETUP places for what beginning one costs (a round trip for the offsets and pages, one for the
+// keys, the join of the warps: as long as two tiles; a block with many short units was the last to finish), and every block takes an equal stretch.  A unit that crosses such a bound is left in
 // parts - rows of fp32 output that are not normalised, with their reference and sum - in the workspace, at most two a block, and tree_join_kernel joins
-// them, in the order of the keys.
+// them, in the order of the keys.  (Its blocks find what is to be joined in notes that the others leave: with a plan of its own and one warp for all parts of a row it took
+// 30-60 us.)
 #pragma once
 
 #include "cache_batch.cuh"
@@ -13,6 +15,7 @@ namespace phx {
 
 constexpr float TREE_LOG2E = 1.4426950408889634f;
 constexpr int TREE_MAX_SPLIT_BATCH = 1024;      // requests whose tiles the blocks may share
+constexpr int TREE_SETUP = 2;
 
 struct TreeView {
   phx_cache_batch c;
@@ -23,6 +26,14 @@ struct TreeView {
   int split;             // blocks that share the tiles; 0: a block takes whole units
   float* part_o;         // [2 split][rows][key_size]
   float2* part_ml;       // [2 split][rows]: reference (log2 domain), sum
+  struct TreeJoin* join; // [split]: what block x's bound in front leaves to be joined
+};
+// A unit cut by the bound between blocks x - 1 and x, the first that cuts it: block x - 1 has its first tiles, blocks x .. to - 1 the others
+struct TreeJoin {
+  int rows;              // 0: nothing to join here
+  int to;
+  int token0, row0, h;   // the request's first token row; the tile's first row of query; its key head
+  int pad[3];
 };
 
 __device__ __forceinline__ float tree_ex2(float x) {
@@ -69,7 +80,7 @@ __device__ __forceinline__ bool odd_pair(uint32_t v) { return odd_value(v) || (v
 // A stretch of a unit's tiles of keys
 struct TreePiece {
   int b, h, row_tile;
-  int begin, end, tiles;        // of `tiles` in all
+  int begin, end, tiles;        // of `tiles` in all; none where the stretch ends in front of them
   __device__ __forceinline__ bool whole() const { return begin == 0 && end == tiles; }
   // which of its block's two parts: the one that another block began, or the one that another ends
   __device__ __forceinline__ int part() const { return begin > 0 ? 0 : 1; }
@@ -82,13 +93,14 @@ __device__ __forceinline__ int tree_key_tiles(const TreeView& t, int keys) { ret
 template <int THREADS> struct TreePlan {
   long long before[TREE_MAX_SPLIT_BATCH + 1];
   long long warp_sum[THREADS / 32];
+  long long per_, more_;         // places of a block: per_, the first more_ one more
 
   // by all threads of the block; ends with a barrier
   __device__ void make(const TreeView& t) {
     const int tid = threadIdx.x, lane = tid & 31, per = (t.c.batch + THREADS - 1) / THREADS, b0 = min(tid * per, t.c.batch), b1 = min(b0 + per, t.c.batch);
     auto tiles_of = [&](int b) {
       const KeyRange k = key_range(t.c, b);
-      return (long long)t.c.num_kv_heads * tree_row_tiles(t, k.rq.tokens) * tree_key_tiles(t, k.keys);
+      return (long long)t.c.num_kv_heads * tree_row_tiles(t, k.rq.tokens) * (tree_key_tiles(t, k.keys) + TREE_SETUP);
     };
     long long mine = 0;
     for (int b = b0; b < b1; ++b) mine += tiles_of(b);
@@ -100,24 +112,46 @@ template <int THREADS> struct TreePlan {
     long long at = sum - mine;
     for (int w = 0; w < (tid >> 5); ++w) at += warp_sum[w];
     for (int b = b0; b < b1; ++b) { before[b] = at; at += per == 1 ? mine : tiles_of(b); }
-    if (tid == THREADS - 1) before[t.c.batch] = at;      // the last thread ends behind all
+    if (tid == THREADS - 1) { before[t.c.batch] = at; per_ = at / t.split; more_ = at % t.split; }   // the last thread ends behind all
     __syncthreads();
   }
   __device__ __forceinline__ long long all(const TreeView& t) const { return before[t.c.batch]; }
-  __device__ __forceinline__ long long bound(const TreeView& t, int block) const { return all(t) * block / t.split; }
-  // the piece from position `pos` on, at most to `end`
-  __device__ __forceinline__ TreePiece piece(const TreeView& t, long long pos, long long end) const {
+  __device__ __forceinline__ long long bound(int block) const { return block * per_ + min((long long)block, more_); }
+  // the first block whose stretch begins at or behind place `pos`
+  __device__ __forceinline__ int block_behind(const TreeView& t, long long pos) const {
+    int lo = 0, hi = t.split;
+    while (lo < hi) { const int mid = (lo + hi) / 2; if (bound(mid) < pos) lo = mid + 1; else hi = mid; }
+    return lo;
+  }
+  // what block x's first piece, from bound(x) on, leaves to be joined
+  __device__ __forceinline__ void note_join(const TreeView& t, int x, const TreePiece& pc, long long unit_end) const {
+    TreeJoin j;
+    j.rows = 0;
+    const long long first_tile = unit_end - pc.tiles;
+    if (x > 0 && bound(x) > first_tile && bound(x - 1) <= first_tile) {
+      const CacheRequest rq = cache_request(t.c, pc.b);
+      j.row0 = pc.row_tile * t.rows;
+      j.rows = (int)min((long long)t.rows, (long long)rq.tokens * t.group - j.row0);
+      j.to = block_behind(t, unit_end);
+      j.token0 = rq.row0; j.h = pc.h;
+    }
+    t.join[x] = j;
+  }
+  // the piece from place `pos` on, at most to `end`; `next` is behind it, `unit_end` behind its unit
+  __device__ __forceinline__ TreePiece piece(const TreeView& t, long long pos, long long end, long long* next, long long* unit_end) const {
     int lo = 0, hi = t.c.batch;                          // before[lo] <= pos < before[hi]
     while (hi - lo > 1) { const int mid = (lo + hi) / 2; if (before[mid] <= pos) lo = mid; else hi = mid; }
     const KeyRange k = key_range(t.c, lo);
     TreePiece p;
     p.b = lo;
     p.tiles = tree_key_tiles(t, k.keys);
-    const long long in = pos - before[lo], unit = in / p.tiles;
+    const long long in = pos - before[lo], unit = in / (p.tiles + TREE_SETUP), unit0 = before[lo] + unit * (p.tiles + TREE_SETUP);
     const int row_tiles = tree_row_tiles(t, k.rq.tokens);
     p.h = (int)(unit / row_tiles); p.row_tile = (int)(unit - (long long)p.h * row_tiles);
-    p.begin = (int)(in - unit * p.tiles);
-    p.end = (int)min((long long)p.tiles, p.begin + (end - pos));
+    *unit_end = unit0 + p.tiles + TREE_SETUP;
+    *next = min(end, *unit_end);
+    p.begin = (int)max(0ll, pos - unit0 - TREE_SETUP);
+    p.end = (int)max(0ll, *next - unit0 - TREE_SETUP);
     return p;
   }
 };
