@@ -56,7 +56,8 @@ enum DispatchKind {
   DK_HISTORY_APPEND = 21,
   DK_TREE_MMA = 22,         // attention over a paged cache, mma.sync
   DK_TOKEN_LOGPROBS = 23,
-  DK_COUNT = 24
+  DK_TREE_TC = 24,          // ... tcgen05 / TMEM
+  DK_COUNT = 25
 };
 void dispatch_note(int kind);
 

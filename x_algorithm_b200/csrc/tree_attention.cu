@@ -465,7 +465,7 @@ extern "C" phx_status phx_tree_workspace_bytes(int32_t device, int64_t* bytes_ou
   if (!bytes_out) { set_global_error("phx_tree_workspace_bytes: null argument"); return PHX_E_ARG; }
   DeviceScope scope(device);
   if (!scope.ok()) { set_global_error("phx_tree_workspace_bytes: cudaSetDevice failed"); return PHX_E_CUDA; }
-  *bytes_out = part_bytes(3 * device_sms(), 128, 128);   // the largest that a call may take
+  *bytes_out = part_bytes(tree_tc_blocks_per_sm() * device_sms(), 128, 128);   // the largest that a call may take
   return PHX_OK;
 }
 
@@ -496,8 +496,11 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   cudaStream_t st = (cudaStream_t)stream;
   std::string err;
 
+  // More than 16 rows a key head are the tensor cores' (tree_attention_sm100.cu); the mma.sync kernel would read the cache again for every 16.
+  const bool tc = tree_tc_supported(t) && (long long)t.a.max_tokens * t.group > ROWS;
   t.rows = ROWS; t.keys = KEYS * TREE_WARPS;
-  const int per_sm = t.c.key_size == 128 ? mma_blocks<128>() : mma_blocks<64>();
+  if (tc) tree_tc_shape(t);
+  const int per_sm = tc ? tree_tc_blocks_per_sm() : t.c.key_size == 128 ? mma_blocks<128>() : mma_blocks<64>();
   // Blocks share the tiles of all units where there are few units for them and long ones among them.
   const long long units = (long long)t.c.batch * t.c.num_kv_heads * (((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows);
   const long long tiles = (t.a.max_keys + t.keys - 1) / t.keys;
@@ -508,7 +511,7 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   t.part_ml = reinterpret_cast<float2*>(t.part_o + 2ll * t.split * t.rows * t.c.key_size);
   t.join = reinterpret_cast<TreeJoin*>(t.part_ml + 2ll * t.split * t.rows);
   if (t.c.num_pages == 0) return bad("an empty pool has no keys to attend to");
-  phx_status s = t.c.key_size == 32 ? tree_mma_launch<32>(t, st, err) : t.c.key_size == 64 ? tree_mma_launch<64>(t, st, err) : tree_mma_launch<128>(t, st, err);
+  phx_status s = tc ? tree_tc_launch(t, st, err) : t.c.key_size == 32 ? tree_mma_launch<32>(t, st, err) : t.c.key_size == 64 ? tree_mma_launch<64>(t, st, err) : tree_mma_launch<128>(t, st, err);
   if (s == PHX_OK && t.split) {
     const long long rows = (long long)t.a.max_tokens * t.group;
     const dim3 grid(t.split - 1, (unsigned)(rows < t.rows ? rows : t.rows)), block(32 * JOIN_WARPS);

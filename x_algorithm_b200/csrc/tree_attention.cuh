@@ -46,12 +46,13 @@ struct TreeCap {
   float scale, a, b;
   __device__ __forceinline__ TreeCap(const TreeView& t) {
     const float cap = t.a.cap;
-    scale = t.a.cap_method == 1 ? t.a.sm_scale : t.a.sm_scale * 2.0f * TREE_LOG2E / cap;
+    scale = t.a.cap_method == 0 ? t.csc : t.a.cap_method == 1 ? t.a.sm_scale : t.a.sm_scale * 2.0f * TREE_LOG2E / cap;
     a = t.a.cap_method == 1 ? 1.0f / cap : -2.0f * cap * TREE_LOG2E;
     b = cap * TREE_LOG2E;
   }
   template <int METHOD> __device__ __forceinline__ float of(float s) const {
     const float v = s * scale;
+    if (METHOD == 3) return v;                           // no cap, scaled in front of the mask: 0 * -inf is no mask
     if (METHOD == 1) return __fdividef(v, 1.0f + fabsf(v) * a) * TREE_LOG2E;
     return b + __fdividef(a, tree_ex2(v) + 1.0f);
   }
