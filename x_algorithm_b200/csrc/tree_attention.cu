@@ -371,7 +371,8 @@ __global__ void __launch_bounds__(32 * TREE_WARPS, mma_blocks<DH>()) tree_mma_ke
   if (*gave_up()) __nanosleep(1000000);                  // copies may still be on their way into this block's memory
 }
 
-// The parts of a unit that blocks x - 1, x, ... left, joined in the order of the keys: a block takes a row at a time, its warps every fourth part
+// The parts of a unit that blocks x - 1, x, ... left, joined in the order of the keys: a block takes four rows at a time, one a warp or, of
+// many parts, one after the other with every fourth part a warp
 constexpr int JOIN_WARPS = 4;
 template <int DH>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) tree_join_kernel(const TreeView t) {
@@ -381,41 +382,53 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) tree_join_kernel(const TreeVi
   const int x = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const TreeJoin j = t.join[x];
   constexpr int PER = DH / 32;
-  for (int row = blockIdx.y; row < j.rows; row += gridDim.y) {
-    const int parts = j.to - x + 1;
-    auto slot = [&](int k) { return ((long long)2 * (x - 1 + k) + (k == 0 ? 1 : 0)) * t.rows + row; };   // of part k
-    float top = -INFINITY;
-    for (int k = lane; k < parts; k += 32) top = fmaxf(top, t.part_ml[slot(k)].x);
+  const int parts = j.to - x + 1;
+  const bool alone = parts <= 2 * JOIN_WARPS;              // few parts: a warp takes a row for itself
+  for (int row = alone ? blockIdx.y * JOIN_WARPS + warp : blockIdx.y; row < j.rows; row += gridDim.y * (alone ? JOIN_WARPS : 1)) {
+      auto slot = [&](int k) { return ((long long)2 * (x - 1 + k) + (k == 0 ? 1 : 0)) * t.rows + row; };   // of part k
+      float top = -INFINITY;
+      for (int k = lane; k < parts; k += 32) top = fmaxf(top, t.part_ml[slot(k)].x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[PER];
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, acc[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+      for (int d = 0; d < PER; ++d) acc[d] = 0.f;
 #pragma unroll 4
-    for (int k = warp; k < parts; k += JOIN_WARPS) {
-      const float2 ml = t.part_ml[slot(k)];
-      const float* o = t.part_o + slot(k) * DH + lane * PER;
-      const float f = tree_ex2(ml.x - base);
-      sum += ml.y == 0.f ? 0.f : ml.y * f;
+      for (int k = alone ? 0 : warp; k < parts; k += alone ? 1 : JOIN_WARPS) {
+        const float2 ml = t.part_ml[slot(k)];
+        const float* o = t.part_o + slot(k) * DH + lane * PER;
+        const float f = tree_ex2(ml.x - base);
+        sum += ml.y == 0.f ? 0.f : ml.y * f;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) { const float v = o[i]; acc[i] += ml.y == 0.f ? 0.f : v * f; }   // a part that saw no key may hold anything
-    }
-    if (row >= (int)gridDim.y) __syncthreads();
-    if (lane == 0) sum_of[warp] = sum;
+        for (int d = 0; d < PER; ++d) { const float v = o[d]; acc[d] += ml.y == 0.f ? 0.f : v * f; }   // a part that saw no key may hold anything
+      }
+      if (!alone) {
+        __syncthreads();
+        if (lane == 0) sum_of[warp] = sum;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc_of[warp][lane * PER + i] = acc[i];
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d < DH) {
-      float s = 0.f, v = 0.f;
+        for (int d = 0; d < PER; ++d) acc_of[warp][lane * PER + d] = acc[d];
+        __syncthreads();
+        sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < JOIN_WARPS; ++w) { s += sum_of[w]; v += acc_of[w][d]; }
+        for (int d = 0; d < PER; ++d) acc[d] = 0.f;
+#pragma unroll
+        for (int w = 0; w < JOIN_WARPS; ++w) {
+          sum += sum_of[w];
+#pragma unroll
+          for (int d = 0; d < PER; ++d) acc[d] += acc_of[w][lane * PER + d];
+        }
+        if (warp != 0) continue;
+      }
       const int r = j.row0 + row, tk = r / t.group, head = j.h * t.group + r % t.group;
-      const bf16 y = f2bf(s == 0.f ? 0.f : v / s);
-      t.a.out[((long long)(j.token0 + tk) * t.a.num_q_heads + head) * DH + d] = *reinterpret_cast<const uint16_t*>(&y);
+      uint16_t* const out = t.a.out + ((long long)(j.token0 + tk) * t.a.num_q_heads + head) * DH + lane * PER;
+      uint16_t y[PER];
+#pragma unroll
+      for (int d = 0; d < PER; ++d) { const bf16 v = f2bf(sum == 0.f ? 0.f : acc[d] / sum); y[d] = *reinterpret_cast<const uint16_t*>(&v); }
+      if (PER == 4) *reinterpret_cast<uint2*>(out) = make_uint2(y[0] | (uint32_t)y[1 % PER] << 16, y[2 % PER] | (uint32_t)y[3 % PER] << 16);
+      else if (PER == 2) *reinterpret_cast<uint32_t*>(out) = y[0] | (uint32_t)y[1 % PER] << 16;
+      else out[0] = y[0];
     }
-  }
 }
 
 template <int DH, int CAP>
@@ -498,14 +511,14 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
 
   // More than 16 rows a key head are the tensor cores' (tree_attention_sm100.cu); the mma.sync kernel would read the cache again for every 16.
   const bool tc = tree_tc_supported(t) && (long long)t.a.max_tokens * t.group > ROWS;
-  t.rows = ROWS; t.keys = KEYS * TREE_WARPS;
+  t.rows = ROWS; t.keys = KEYS * TREE_WARPS; t.setup = 2;
   if (tc) tree_tc_shape(t);
   const int per_sm = tc ? tree_tc_blocks_per_sm() : t.c.key_size == 128 ? mma_blocks<128>() : mma_blocks<64>();
   // Blocks share the tiles of all units where there are few units for them and long ones among them.
   const long long units = (long long)t.c.batch * t.c.num_kv_heads * (((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows);
   const long long tiles = (t.a.max_keys + t.keys - 1) / t.keys;
-  const long long blocks = per_sm * device_sms(), fed = units * (tiles + TREE_SETUP) / 4;   // no block for less than four places
-  t.split = tiles >= 4 && units < 8 * blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)(fed < blocks ? fed : blocks) : 0;
+  const long long blocks = per_sm * device_sms(), fed = units * (tiles + t.setup) / 4;   // no block for less than four places
+  t.split = tiles >= 4 && units < (tc ? 2 : 8) * blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)(fed < blocks ? fed : blocks) : 0;
   if (part_bytes(t.split, t.rows, t.c.key_size) > t.a.workspace_bytes) return bad("workspace is smaller than phx_tree_workspace_bytes");
   t.part_o = static_cast<float*>(t.a.workspace);
   t.part_ml = reinterpret_cast<float2*>(t.part_o + 2ll * t.split * t.rows * t.c.key_size);
@@ -514,7 +527,9 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   phx_status s = tc ? tree_tc_launch(t, st, err) : t.c.key_size == 32 ? tree_mma_launch<32>(t, st, err) : t.c.key_size == 64 ? tree_mma_launch<64>(t, st, err) : tree_mma_launch<128>(t, st, err);
   if (s == PHX_OK && t.split) {
     const long long rows = (long long)t.a.max_tokens * t.group;
-    const dim3 grid(t.split - 1, (unsigned)(rows < t.rows ? rows : t.rows)), block(32 * JOIN_WARPS);
+    const unsigned most = (unsigned)(rows < t.rows ? rows : t.rows);
+    const bool many = t.split > JOIN_WARPS * units;                // parts of a unit: a block for each row, else for four
+    const dim3 grid(t.split - 1, many ? most : (most + JOIN_WARPS - 1) / JOIN_WARPS), block(32 * JOIN_WARPS);
     const cudaError_t e = t.c.key_size == 32 ? launch_programmatic(tree_join_kernel<32>, grid, block, 0, st, t)
                           : t.c.key_size == 64 ? launch_programmatic(tree_join_kernel<64>, grid, block, 0, st, t)
                                                : launch_programmatic(tree_join_kernel<128>, grid, block, 0, st, t);

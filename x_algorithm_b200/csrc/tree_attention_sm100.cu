@@ -23,7 +23,9 @@ constexpr int QT = 128;                 // query rows of a block
 constexpr int TC_THREADS = 192;
 constexpr int SLAB = QT * 128;          // bytes of one [128 rows x 64 bf16] swizzled tile
 constexpr int NEW_TILES = 2048;         // tiles of new keys that are classified; those behind count as seen in part
-__host__ __device__ constexpr int tc_keys(int dh) { return dh == 64 ? 128 : 64; }
+constexpr int KT = 64;                  // keys of a tile: S of two tiles and O share the block's 256 columns of tensor memory
+// K and V buffers each: 64 KB a block
+__host__ __device__ constexpr int tc_buffers(int dh) { return dh == 64 ? 4 : 2; }
 
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -49,14 +51,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 
 template <int DH>
 struct TcSmem {
-  static constexpr int KT = tc_keys(DH), DCH = DH / 64;
+  static constexpr int DCH = DH / 64, NB = tc_buffers(DH);
   uint8_t q[DCH * SLAB];
-  uint8_t k[2][DCH * KT * 128];
-  uint8_t v[2][DCH * KT * 128];
+  uint8_t k[NB][DCH * KT * 128];
+  uint8_t v[NB][DCH * KT * 128];
   int2 span[2][KT];                     // of a masked tile's keys
   uint32_t need[NEW_TILES / 32], mask[NEW_TILES / 32];
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half, p_ready, o_done;
-  uint32_t there[4];                    // which boxes of a tile lie in pages of the pool
+  uint64_t q_full, k_full[NB], k_empty[NB], v_full[NB], v_empty[NB], s_full[2], p_ready, o_done;
+  uint32_t there[8];                    // which boxes of a tile lie in pages of the pool
   uint32_t tmem;
   int odd;                              // a masked tile of the piece held infinities or NaN
   TreePlan<TC_THREADS> plan;
@@ -64,8 +66,7 @@ struct TcSmem {
 
 template <int DH, int CAP>
 struct TcBlock {
-  static constexpr int KT = tc_keys(DH), DCH = DH / 64;
-  static constexpr int NSB = KT == 64 ? 2 : 1;             // S buffers: S of the next tile is computed under the softmax of this one
+  static constexpr int DCH = DH / 64, NB = tc_buffers(DH);
   static constexpr uint32_t BLK = DCH * KT * 128, TM_S = 0, TM_O = 128;
   const TreeView& t;
   const CUtensorMap& map_q;
@@ -86,6 +87,15 @@ struct TcBlock {
       if (kr.keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
     }
     const uint32_t tmem = sm.tmem;
+    int first_page = -1;
+    if (warp == 0) {                                        // on their way under what follows
+      first_page = page_of(kr, pc.begin);
+      if (elect_one()) {
+        mbar_expect_tx(smem_u32(&sm.q_full), DCH * t.rows * 128);
+        for (int c = 0; c < DCH; ++c) tma_load_3d(smem_u32(sm.q) + c * SLAB, &map_q, smem_u32(&sm.q_full), c * 64, pc.h * group, rq.row0 + token0);
+      }
+      __syncwarp();
+    }
 
     // ---- which tiles of new keys the block's rows see ----------------------------------------------------------------
     const int new0 = rq.cached / KT, key_tiles = (kr.keys + KT - 1) / KT, last = min(pc.end, key_tiles);   // the first tile with new keys
@@ -129,7 +139,7 @@ struct TcBlock {
     const int first = next_tile(pc.begin);
 
     if (warp == 0) {
-      produce(kr, pc, token0, first, last, next_tile);
+      produce(kr, pc, first, last, next_tile, first == pc.begin ? first_page : page_of(kr, first));
     } else if (warp == 1) {
       if (elect_one()) issue(first, last, next_tile, tmem);
     } else {
@@ -142,54 +152,50 @@ struct TcBlock {
     tc_fence_after();
   }
 
+  // page of box `lane` of a tile, the last of which may lie behind the keys
+  __device__ __forceinline__ int page_of(const KeyRange& kr, int tile) const {
+    const int lane = threadIdx.x & 31;
+    const long long key = (long long)tile * KT + lane * box;
+    return lane < KT / box && key < kr.keys ? kr.table[(int)key / t.c.page_size] : -1;
+  }
   template <typename Next>
-  __device__ __forceinline__ void produce(const KeyRange& kr, const TreePiece& pc, int token0, int first, int last, const Next& next_tile) {
+  __device__ __forceinline__ void produce(const KeyRange& kr, const TreePiece& pc, int first, int last, const Next& next_tile, int page) {
     const int lane = threadIdx.x & 31, boxes = KT / box, v_off = t.c.num_kv_heads * t.c.page_size, no_row = (int)(2 * t.c.num_pages * v_off);
     volatile int* const verr = t.c.status_dev;
-    // row of the pool of box `lane` of a tile, the last of which may lie behind the keys
-    auto page_of = [&](int tile) {
-      const int key = tile * KT + lane * box;
-      return lane < boxes && tile < last && key < kr.keys ? kr.table[key / t.c.page_size] : -1;
-    };
+    // row of the pool of box `lane` of a tile
     auto row_of = [&](int tile, int page) {
       const int key = tile * KT + lane * box;
       return page >= 0 && page < t.c.num_pages ? (page * 2 * t.c.num_kv_heads + pc.h) * t.c.page_size + key % t.c.page_size : no_row;
     };
-    int page = page_of(first);
-    if (elect_one()) {
-      mbar_expect_tx(smem_u32(&sm.q_full), DCH * t.rows * 128);
-      for (int c = 0; c < DCH; ++c) tma_load_3d(smem_u32(sm.q) + c * SLAB, &map_q, smem_u32(&sm.q_full), c * 64, pc.h * t.group, kr.rq.row0 + token0);
-    }
-    __syncwarp();
-    int rows[8], before[8];                                // of this tile's boxes, of the tile's before
+    int rows[4], before[4];                                // of this tile's boxes, of the tile's before
     int j = seq;
-    // K runs a tile ahead of V: its buffer is free once S of two tiles before has been computed
+    // K runs a tile ahead of V: a buffer is free once S of the tile before in it has been computed
     for (int tile = first;; ++j) {
       const bool have = tile < last;
-      const int after = have ? next_tile(tile + 1) : last, page_after = page_of(after);
+      const int after = have ? next_tile(tile + 1) : last, page_after = page_of(kr, after);
       if (have) {
         const int row = row_of(tile, page);
         const uint32_t there = __ballot_sync(0xffffffffu, row != no_row);
         if (lane < boxes && row == no_row && tile * KT + lane * box < kr.keys) cache_report(t.c, CACHE_BAD_PAGE);
 #pragma unroll
-        for (int p = 0; p < 8; ++p) rows[p] = __shfl_sync(0xffffffffu, row, p);
+        for (int p = 0; p < 4; ++p) rows[p] = __shfl_sync(0xffffffffu, row, p);
         if (elect_one()) {
-          const int b = j & 1;
-          mbar_wait(smem_u32(&sm.k_empty[b]), (uint32_t)((j >> 1) & 1) ^ 1u, verr);
-          sm.there[j & 3] = there;
+          const int b = j % NB;
+          mbar_wait(smem_u32(&sm.k_empty[b]), (uint32_t)((j / NB) & 1) ^ 1u, verr);
+          sm.there[j & 7] = there;
           mbar_expect_tx(smem_u32(&sm.k_full[b]), BLK);
 #pragma unroll
-          for (int p = 0; p < 8; ++p)
+          for (int p = 0; p < 4; ++p)
             if (p < boxes)
               for (int c = 0; c < DCH; ++c) tma_load_2d(smem_u32(sm.k[b]) + c * KT * 128 + p * box * 128, &map_kv, smem_u32(&sm.k_full[b]), c * 64, rows[p]);
         }
       }
       if (j > seq && elect_one()) {
-        const int i = j - 1, b = i & 1;
-        mbar_wait(smem_u32(&sm.v_empty[b]), (uint32_t)((i >> 1) & 1) ^ 1u, verr);
+        const int i = j - 1, b = i % NB;
+        mbar_wait(smem_u32(&sm.v_empty[b]), (uint32_t)((i / NB) & 1) ^ 1u, verr);
         mbar_expect_tx(smem_u32(&sm.v_full[b]), BLK);
 #pragma unroll
-        for (int p = 0; p < 8; ++p)
+        for (int p = 0; p < 4; ++p)
           if (p < boxes)
             for (int c = 0; c < DCH; ++c)
               tma_load_2d(smem_u32(sm.v[b]) + c * KT * 128 + p * box * 128, &map_kv, smem_u32(&sm.v_full[b]), c * 64, before[p] == no_row ? no_row : before[p] + v_off);
@@ -197,7 +203,7 @@ struct TcBlock {
       __syncwarp();
       if (!have) break;
 #pragma unroll
-      for (int p = 0; p < 8; ++p) before[p] = rows[p];
+      for (int p = 0; p < 4; ++p) before[p] = rows[p];
       tile = after; page = page_after;
     }
   }
@@ -206,37 +212,33 @@ struct TcBlock {
   __device__ __forceinline__ void issue(int first, int last, const Next& next_tile, uint32_t tmem) {
     constexpr uint32_t idesc_s = make_idesc(QT, KT), idesc_o = make_idesc_b_mn(QT, DH);
     volatile int* const verr = t.c.status_dev;
-    auto issue_s = [&](int j) {                             // S(j) = Q K(j)^T into S buffer j % NSB
-      const int b = j & 1;
-      mbar_wait(smem_u32(&sm.k_full[b]), (uint32_t)((j >> 1) & 1), verr);
+    auto issue_s = [&](int j) {                             // S(j) = Q K(j)^T into S buffer j & 1
+      const int b = j % NB;
+      mbar_wait(smem_u32(&sm.k_full[b]), (uint32_t)((j / NB) & 1), verr);
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < DCH; ++c) {
         const uint64_t qd = make_smem_desc(smem_u32(sm.q) + c * SLAB), kd = make_smem_desc(smem_u32(sm.k[b]) + c * KT * 128);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_bf16(tmem + TM_S + (j % NSB) * KT, qd + (uint64_t)(k * 2), kd + (uint64_t)(k * 2), idesc_s, (c | k) != 0);
+        for (int k = 0; k < 4; ++k) umma_bf16(tmem + TM_S + (j & 1) * KT, qd + (uint64_t)(k * 2), kd + (uint64_t)(k * 2), idesc_s, (c | k) != 0);
       }
       umma_commit(smem_u32(&sm.k_empty[b]));
-      umma_commit(smem_u32(&sm.s_full[j % NSB]));
+      umma_commit(smem_u32(&sm.s_full[j & 1]));
     };
     mbar_wait(smem_u32(&sm.q_full), q_phase, verr);
     int ahead = first, j = seq, js = seq;                   // the next tile whose S is to be issued, its number
     auto issue_next = [&]() { if (ahead < last) { issue_s(js++); ahead = next_tile(ahead + 1); } };
-    for (int i = 0; i < NSB - 1; ++i) issue_next();
+    issue_next();
     for (int tile = first; tile < last; tile = next_tile(tile + 1), ++j) {
       issue_next();                                         // its S buffer was last read by the softmax whose P has been awaited below
-      const int b = j & 1;
-      mbar_wait(smem_u32(&sm.v_full[b]), (uint32_t)((j >> 1) & 1), verr);
-      mbar_wait(smem_u32(NSB == 1 ? &sm.p_half : &sm.p_ready), (uint32_t)(j & 1), verr);
+      const int b = j % NB;
+      mbar_wait(smem_u32(&sm.v_full[b]), (uint32_t)((j / NB) & 1), verr);
+      mbar_wait(smem_u32(&sm.p_ready), (uint32_t)(j & 1), verr);
       tc_fence_after();
 #pragma unroll
       for (int kk = 0; kk < KT / 16; ++kk) {
-        if (NSB == 1 && kk == KT / 32) {                    // S is single: the product's first half runs under the exponentials of the second
-          mbar_wait(smem_u32(&sm.p_ready), (uint32_t)(j & 1), verr);
-          tc_fence_after();
-        }
         const uint64_t vd = make_smem_desc_mn(smem_u32(sm.v[b]) + kk * 16 * 128, KT * 128, 1024);
-        umma_ts(tmem + TM_O, tmem + TM_S + (j % NSB) * KT + kk * 8, vd, idesc_o, (j - seq) | kk);
+        umma_ts(tmem + TM_O, tmem + TM_S + (j & 1) * KT + kk * 8, vd, idesc_o, (j - seq) | kk);
       }
       umma_commit(smem_u32(&sm.v_empty[b]));
       umma_commit(smem_u32(&sm.o_done));
@@ -259,10 +261,10 @@ struct TcBlock {
     int j = seq;
 
     for (int tile = first; tile < last; tile = next_tile(tile + 1), ++j) {
-      const uint32_t ph = (uint32_t)(j & 1), s_col = tmem + TM_S + (j % NSB) * KT + lane_base;
-      mbar_wait(smem_u32(&sm.s_full[j % NSB]), (uint32_t)((j / NSB) & 1), verr);
+      const uint32_t ph = (uint32_t)(j & 1), s_col = tmem + TM_S + (j & 1) * KT + lane_base;
+      mbar_wait(smem_u32(&sm.s_full[j & 1]), (uint32_t)((j >> 1) & 1), verr);
       tc_fence_after();
-      const uint32_t there = sm.there[j & 3];
+      const uint32_t there = sm.there[j & 7];
       const int i_new = tile - new0;
       const bool masked = there != (1u << (KT / box)) - 1 || (tile + 1) * KT > kr.keys ||
                           (i_new >= 0 && (i_new >= NEW_TILES || ((sm.mask[i_new >> 5] >> (i_new & 31)) & 1)));
@@ -275,8 +277,8 @@ struct TcBlock {
           sm.span[j & 1][r] = s;
         }
         // infinities and NaN among the values: out of the product
-        mbar_wait(smem_u32(&sm.v_full[j & 1]), (uint32_t)((j >> 1) & 1), verr);
-        uint4* const v = reinterpret_cast<uint4*>(sm.v[j & 1]);
+        mbar_wait(smem_u32(&sm.v_full[j % NB]), (uint32_t)((j / NB) & 1), verr);
+        uint4* const v = reinterpret_cast<uint4*>(sm.v[j % NB]);
         bool odd = false;
         for (int i = r; i < (int)BLK / 16; i += 128) {
           uint4 x = v[i];
@@ -298,7 +300,17 @@ struct TcBlock {
 #pragma unroll
         for (int c = 0; c < KT / 32; ++c) tmem_ld32_nowait(s_col + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
         tmem_ld_wait();
-        if (CAP) {
+        bool small = false;
+        if (CAP == 2) {                                      // tanh by its polynomial where all of the warp's logits are small against the cap
+          float big = 0.f;
+#pragma unroll
+          for (int k = 0; k < KT; ++k) big = fmaxf(big, fabsf(s[k]));
+          small = __all_sync(0xffffffffu, !valid || big * cap.small_scale <= TreeCap::SMALL);
+        }
+        if (CAP == 2 && small) {
+#pragma unroll
+          for (int k = 0; k < KT; k += 2) cap.of_small(s[k], s[k + 1]);
+        } else if (CAP) {
 #pragma unroll
           for (int k = 0; k < KT; ++k) s[k] = cap.template of<CAP>(s[k]);
         }
@@ -348,20 +360,13 @@ struct TcBlock {
             pw[k] = pack_bf2(x.x, x.y);                      // rounded for the product
           }
           tmem_st16(s_col + c * 16, pw);
-          if (NSB == 1 && c == KT / 64 - 1) {
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            tc_fence_before();
-            mbar_arrive(smem_u32(&sm.p_half));
-          }
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
-      } else if (NSB == 1) {
-        mbar_arrive(smem_u32(&sm.p_half));
       }
-      // where S of this tile did not wait for P V of the one before: its barrier must not run two phases ahead of the issuer
-      if (NSB > 1 && j > seq) mbar_wait(smem_u32(&sm.o_done), ph ^ 1u, verr);
+      // S of this tile did not wait for P V of the one before: its barrier must not run two phases ahead of the issuer
+      if (j > seq) mbar_wait(smem_u32(&sm.o_done), ph ^ 1u, verr);
       mbar_arrive(smem_u32(&sm.p_ready));
     }
 
@@ -438,11 +443,12 @@ __global__ void __launch_bounds__(TC_THREADS, 2) tree_tc_kernel(const __grid_con
   if (threadIdx.x == 0) {
     *gave_up() = 0;
     prefetch_map(&map_q); prefetch_map(&map_kv);
-    mbar_init(smem_u32(&sm.q_full), 1); mbar_init(smem_u32(&sm.p_half), 128); mbar_init(smem_u32(&sm.p_ready), 128); mbar_init(smem_u32(&sm.o_done), 1);
-    for (int i = 0; i < 2; ++i) {
+    mbar_init(smem_u32(&sm.q_full), 1); mbar_init(smem_u32(&sm.p_ready), 128); mbar_init(smem_u32(&sm.o_done), 1);
+    for (int i = 0; i < tc_buffers(DH); ++i) {
       mbar_init(smem_u32(&sm.k_full[i]), 1); mbar_init(smem_u32(&sm.k_empty[i]), 1);
-      mbar_init(smem_u32(&sm.v_full[i]), 1); mbar_init(smem_u32(&sm.v_empty[i]), 1); mbar_init(smem_u32(&sm.s_full[i]), 1);
+      mbar_init(smem_u32(&sm.v_full[i]), 1); mbar_init(smem_u32(&sm.v_empty[i]), 1);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.s_full[i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(smem_u32(&sm.tmem), 256);
@@ -501,7 +507,7 @@ phx_status launch(const TreeView& t, cudaStream_t stream, std::string& err) {
   static_assert(2 * (smem + 1024 + 64) <= 228 * 1024, "two blocks share an SM");
   static SmemLimit limit;
   PHX_CUDA_TRY(limit.raise(tree_tc_kernel<DH, CAP>, smem), err);
-  int box = tc_keys(DH);                                    // the largest power of two that a page is a multiple of, at most a tile
+  int box = KT;                                    // the largest power of two that a page is a multiple of, at most a tile
   while (t.c.page_size % box != 0) box /= 2;
   CUtensorMap map_q, map_kv;
   phx_status s = query_map(&map_q, t, err);
@@ -523,7 +529,7 @@ phx_status launch(const TreeView& t, cudaStream_t stream, std::string& err) {
 }  // namespace
 
 bool tree_tc_supported(const TreeView& t) { return (t.c.key_size == 64 || t.c.key_size == 128) && t.group <= QT; }
-void tree_tc_shape(TreeView& t) { t.rows = QT / t.group * t.group; t.keys = tc_keys(t.c.key_size); }
+void tree_tc_shape(TreeView& t) { t.rows = QT / t.group * t.group; t.keys = KT; t.setup = 6; }
 int tree_tc_blocks_per_sm() { return 2; }
 phx_status tree_tc_launch(const TreeView& t, cudaStream_t stream, std::string& err) {
   return t.c.key_size == 64 ? launch<64>(t, stream, err) : launch<128>(t, stream, err);
