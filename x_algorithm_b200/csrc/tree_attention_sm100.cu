@@ -49,6 +49,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
+// Wait for the tensor-memory loads in flight.  The 32 registers are operands, so that no use of them is scheduled in front of it.
+__device__ __forceinline__ void tmem_ld_wait_on(float* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]),
+                 "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]),
+                 "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+               :: "memory");
+}
+
 template <int DH>
 struct TcSmem {
   static constexpr int DCH = DH / 64, NB = tc_buffers(DH);
@@ -62,6 +71,38 @@ struct TcSmem {
   uint32_t tmem;
   int odd;                              // a masked tile of the piece held infinities or NaN
   TreePlan<TC_THREADS> plan;
+};
+
+// The tiles of a piece that are needed, one after the other; a role's own copy keeps the word of bits it is in
+template <int DH>
+struct TileWalk {
+  const TcSmem<DH>* sm;
+  int new0, last;                       // the first tile with new keys; behind the piece's last
+  int at = -1;
+  uint32_t need = 0, mask = 0;
+  __device__ __forceinline__ void fetch(int i) {
+    if ((i >> 5) != at) { at = i >> 5; need = sm->need[at]; mask = sm->mask[at]; }
+  }
+  // the first from `tile` on; `last`: none
+  __device__ __forceinline__ int next(int tile) {
+    while (tile < last) {
+      const int i = tile - new0;
+      if (i < 0 || i >= NEW_TILES) return tile;
+      fetch(i);
+      const uint32_t rest = need >> (i & 31);
+      if (rest & 1) return tile;
+      tile += rest ? __ffs(rest) - 1 : 32 - (i & 31);
+    }
+    return last;
+  }
+  // whether some of the block's rows do not see some of its keys (those of pages outside the pool and behind the last key aside)
+  __device__ __forceinline__ bool masked(int tile) {
+    const int i = tile - new0;
+    if (i < 0) return false;
+    if (i >= NEW_TILES) return true;
+    fetch(i);
+    return (mask >> (i & 31)) & 1;
+  }
 };
 
 template <int DH, int CAP>
@@ -129,23 +170,17 @@ struct TcBlock {
       }
     }
     __syncthreads();
-    auto next_tile = [&](int tile) {                        // the first from `tile` on that is needed; `last`: none
-      for (; tile < last; ++tile) {
-        const int i = tile - new0;
-        if (i < 0 || i >= NEW_TILES || ((sm.need[i >> 5] >> (i & 31)) & 1)) break;
-      }
-      return tile;
-    };
-    const int first = next_tile(pc.begin);
+    TileWalk<DH> walk{&sm, new0, last};
+    const int first = walk.next(pc.begin);
 
     if (warp == 0) {
-      produce(kr, pc, first, last, next_tile, first == pc.begin ? first_page : page_of(kr, first));
+      produce(kr, pc, first, walk, first == pc.begin ? first_page : page_of(kr, first));
     } else if (warp == 1) {
-      if (elect_one()) issue(first, last, next_tile, tmem);
+      if (elect_one()) issue(first, walk, tmem);
     } else {
-      softmax(kr, pc, token0, first, last, new0, next_tile, tmem);
+      softmax(kr, pc, token0, first, walk, tmem);
     }
-    for (int tile = first; tile < last; tile = next_tile(tile + 1)) ++seq;
+    for (int tile = first; tile < last; tile = walk.next(tile + 1)) ++seq;
     q_phase ^= 1;
     tc_fence_before();
     __syncthreads();                                        // Q, the buffers and O are free for the next piece
@@ -158,8 +193,8 @@ struct TcBlock {
     const long long key = (long long)tile * KT + lane * box;
     return lane < KT / box && key < kr.keys ? kr.table[(int)key / t.c.page_size] : -1;
   }
-  template <typename Next>
-  __device__ __forceinline__ void produce(const KeyRange& kr, const TreePiece& pc, int first, int last, const Next& next_tile, int page) {
+  __device__ __forceinline__ void produce(const KeyRange& kr, const TreePiece& pc, int first, TileWalk<DH> walk, int page) {
+    const int last = walk.last;
     const int lane = threadIdx.x & 31, boxes = KT / box, v_off = t.c.num_kv_heads * t.c.page_size, no_row = (int)(2 * t.c.num_pages * v_off);
     volatile int* const verr = t.c.status_dev;
     // row of the pool of box `lane` of a tile
@@ -172,7 +207,7 @@ struct TcBlock {
     // K runs a tile ahead of V: a buffer is free once S of the tile before in it has been computed
     for (int tile = first;; ++j) {
       const bool have = tile < last;
-      const int after = have ? next_tile(tile + 1) : last, page_after = page_of(kr, after);
+      const int after = have ? walk.next(tile + 1) : last, page_after = page_of(kr, after);
       if (have) {
         const int row = row_of(tile, page);
         const uint32_t there = __ballot_sync(0xffffffffu, row != no_row);
@@ -208,8 +243,8 @@ struct TcBlock {
     }
   }
 
-  template <typename Next>
-  __device__ __forceinline__ void issue(int first, int last, const Next& next_tile, uint32_t tmem) {
+  __device__ __forceinline__ void issue(int first, TileWalk<DH> walk, uint32_t tmem) {
+    const int last = walk.last;
     constexpr uint32_t idesc_s = make_idesc(QT, KT), idesc_o = make_idesc_b_mn(QT, DH);
     volatile int* const verr = t.c.status_dev;
     auto issue_s = [&](int j) {                             // S(j) = Q K(j)^T into S buffer j & 1
@@ -227,9 +262,9 @@ struct TcBlock {
     };
     mbar_wait(smem_u32(&sm.q_full), q_phase, verr);
     int ahead = first, j = seq, js = seq;                   // the next tile whose S is to be issued, its number
-    auto issue_next = [&]() { if (ahead < last) { issue_s(js++); ahead = next_tile(ahead + 1); } };
+    auto issue_next = [&]() { if (ahead < last) { issue_s(js++); ahead = walk.next(ahead + 1); } };
     issue_next();
-    for (int tile = first; tile < last; tile = next_tile(tile + 1), ++j) {
+    for (; j < js; ++j) {
       issue_next();                                         // its S buffer was last read by the softmax whose P has been awaited below
       const int b = j % NB;
       mbar_wait(smem_u32(&sm.v_full[b]), (uint32_t)((j / NB) & 1), verr);
@@ -245,8 +280,8 @@ struct TcBlock {
     }
   }
 
-  template <typename Next>
-  __device__ __forceinline__ void softmax(const KeyRange& kr, const TreePiece& pc, int token0, int first, int last, int new0, const Next& next_tile, uint32_t tmem) {
+  __device__ __forceinline__ void softmax(const KeyRange& kr, const TreePiece& pc, int token0, int first, TileWalk<DH> walk, uint32_t tmem) {
+    const int last = walk.last;
     const int lane = threadIdx.x & 31, quad = warp_index() & 3, r = quad * 32 + lane, group = t.group;
     const CacheRequest& rq = kr.rq;
     volatile int* const verr = t.c.status_dev;
@@ -260,14 +295,20 @@ struct TcBlock {
     float m = valid ? -INFINITY : 0.f, l = 0.f;
     int j = seq;
 
-    for (int tile = first; tile < last; tile = next_tile(tile + 1), ++j) {
+    const uint32_t all_there = (1u << (KT / box)) - 1;
+    for (int tile = first; tile < last; ++j) {
       const uint32_t ph = (uint32_t)(j & 1), s_col = tmem + TM_S + (j & 1) * KT + lane_base;
+      bool masked = walk.masked(tile) || (tile + 1) * KT > kr.keys;
       mbar_wait(smem_u32(&sm.s_full[j & 1]), (uint32_t)((j >> 1) & 1), verr);
       tc_fence_after();
+      float s[KT];
+      if (busy) {                                           // on its way under what follows
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) tmem_ld32_nowait(s_col + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
+      }
       const uint32_t there = sm.there[j & 7];
-      const int i_new = tile - new0;
-      const bool masked = there != (1u << (KT / box)) - 1 || (tile + 1) * KT > kr.keys ||
-                          (i_new >= 0 && (i_new >= NEW_TILES || ((sm.mask[i_new >> 5] >> (i_new & 31)) & 1)));
+      masked |= there != all_there;
+      const int after = walk.next(tile + 1);
       if (masked) {                                         // the same for all 128 threads
         if (r < KT) {
           const int key = tile * KT + r;
@@ -296,10 +337,8 @@ struct TcBlock {
       }
       float alpha = 1.0f;
       if (busy) {
-        float s[KT];
-#pragma unroll
-        for (int c = 0; c < KT / 32; ++c) tmem_ld32_nowait(s_col + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
-        tmem_ld_wait();
+        tmem_ld_wait_on(s);
+        tmem_ld_wait_on(s + 32);
         bool small = false;
         if (CAP == 2) {                                      // tanh by its polynomial where all of the warp's logits are small against the cap
           float big = 0.f;
@@ -368,6 +407,7 @@ struct TcBlock {
       // S of this tile did not wait for P V of the one before: its barrier must not run two phases ahead of the issuer
       if (j > seq) mbar_wait(smem_u32(&sm.o_done), ph ^ 1u, verr);
       mbar_arrive(smem_u32(&sm.p_ready));
+      tile = after;
     }
 
     // ---- the row: normalised and stored, or left as a part ---------------------------------------------------------------
@@ -411,9 +451,8 @@ struct TcBlock {
     // what the row sees of the infinities and NaN that were taken out of the masked tiles, onto what has been stored
     if (sm.odd != 0 && valid && !none) {
 #pragma unroll 1
-      for (int tile = first; tile < last; tile = next_tile(tile + 1)) {
-        const int i = tile - new0;
-        bool masked = (tile + 1) * KT > kr.keys || (i >= 0 && (i >= NEW_TILES || ((sm.mask[i >> 5] >> (i & 31)) & 1)));
+      for (int tile = first; tile < last; tile = walk.next(tile + 1)) {
+        bool masked = (tile + 1) * KT > kr.keys || walk.masked(tile);
         for (int key = tile * KT; key < min((tile + 1) * KT, kr.keys); key += box) masked |= (unsigned)kr.table[key / t.c.page_size] >= (unsigned)t.c.num_pages;
         if (!masked) continue;
 #pragma unroll 1
