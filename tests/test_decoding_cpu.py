@@ -61,6 +61,19 @@ def test_struct_layouts():
     assert C.sizeof(_lib.LogprobsArgs) == 7 * 8 + 8 * 4
 
 
+def test_argument_blocks_are_filled_field_by_field():
+    from x_algorithm_b200 import decoding
+    mine = decoding._Structs()
+    decoding._BATCH(mine.batch, 0, *range(1, 14))
+    assert [getattr(mine.batch, n) for n, _ in _lib.CacheBatch._fields_] == list(range(1, 14))
+    decoding._APPEND(mine.append, 0, *range(1, 13))
+    assert [getattr(mine.append, n) for n, _ in _lib.AppendArgs._fields_] == list(range(1, 13))
+    decoding._TREE(mine.tree, 0, *range(1, 14))
+    assert [getattr(mine.tree, n) for n, _ in _lib.TreeArgs._fields_] == list(range(1, 14))
+    decoding._LOGPROBS(mine.logprobs, 0, *range(1, 16))
+    assert [getattr(mine.logprobs, n) for n, _ in _lib.LogprobsArgs._fields_] == list(range(1, 16))
+
+
 @pytest.mark.parametrize("wrong", [dict(key_size=48), dict(page_size=8), dict(page_size=40), dict(num_kv_heads=0), dict(batch=-1), dict(status_dev=None),
                                    dict(q_start=None), dict(lengths=None), dict(block_table=None), dict(table_stride=3), dict(pages=8), dict(pages=None),
                                    dict(table_cols=2 ** 30), dict(num_pages=2 ** 40), dict(num_tokens=-1)])

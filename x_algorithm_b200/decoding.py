@@ -10,6 +10,8 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
+import threading
 from typing import Optional
 
 import numpy as np
@@ -31,9 +33,23 @@ class _Kept:
         self.workspace = torch.empty(need.value, dtype=torch.uint8, device=f"cuda:{device}")
         # made on torch's current stream, used on others: both must be there before any of them reads
         torch.cuda.current_stream(device).synchronize()
+        self.status_ptr, self.workspace_ptr, self.workspace_bytes = self.status.data_ptr(), self.workspace.data_ptr(), need.value
 
 
 _kept = {}
+
+
+class _Structs(threading.local):
+    """One set of argument blocks a thread, filled anew for every call: a call costs the host less than its launch."""
+
+    def __init__(self):
+        self.batch, self.append, self.tree, self.logprobs = _lib.CacheBatch(), _lib.AppendArgs(), _lib.TreeArgs(), _lib.LogprobsArgs()
+        self.batch_ref, self.append_ref, self.tree_ref, self.logprobs_ref = (C.byref(x) for x in (self.batch, self.append, self.tree, self.logprobs))
+
+
+_structs = _Structs()
+_BATCH, _APPEND, _TREE, _LOGPROBS = (struct.Struct(f).pack_into for f in ("=7q6i", "=8q2ifi", "=7q2i2f2i", "=7q5i2fi"))   # the blocks' fields, in order
+_BF16, _F32, _I32, _I64, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.int64, torch.uint8
 
 
 def _ok(status: int) -> None:
@@ -42,7 +58,7 @@ def _ok(status: int) -> None:
 
 
 def _stream(device: int, stream: Optional[int]) -> int:
-    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream
 
 
 def _keep(device: int, stream: int) -> _Kept:
@@ -52,35 +68,35 @@ def _keep(device: int, stream: int) -> _Kept:
     return kept
 
 
-def _is(t, name: str, dtype, ndim: int, device: Optional[torch.device] = None):
-    """`t` is a CUDA tensor of this type and rank whose last dimension is dense."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != ndim or not t.is_cuda:
+def _need(t, name: str, dtype, shape, device):
+    """`t` is a contiguous tensor of this type and shape on this device."""
+    if type(t) is torch.Tensor or isinstance(t, torch.Tensor):
+        if t.dtype is dtype and t.get_device() == device and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+    raise ValueError(f"{name} must be a contiguous {list(shape)} {dtype} tensor on cuda:{device}")
+
+
+def _rows(t, name: str, dtype, ndim: int):
+    """The device of `t`, a CUDA tensor of this type and rank whose last dimension is dense."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != ndim or not t.is_cuda:
         raise ValueError(f"{name} must be a {ndim}-dimensional {dtype} tensor on a CUDA device")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must be dense in its last dimension")
-    return t
+    return t.get_device()
 
 
-def _dense(t, name: str, dtype, shape, device):
-    _is(t, name, dtype, len(shape), device)
-    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {list(shape)} tensor, got {list(t.shape)}")
-    return t
-
-
-def _batch(pages, q_start, lengths, block_table, tokens: int, kept: _Kept) -> _lib.CacheBatch:
-    _is(pages, "pages", torch.bfloat16, 5)
-    if pages.shape[1] != 2 or not pages.is_contiguous():
+def _batch(block, pages, q_start, lengths, block_table, tokens: int, device: int, kept: _Kept):
+    """Fills the cache's block; (kv heads, page size, head dim, table columns)."""
+    if _rows(pages, "pages", _BF16, 5) != device or _rows(block_table, "block_table", _I32, 2) != device:
+        raise ValueError(f"pages and block_table must be on cuda:{device}")
+    num_pages, two, kv_heads, page_size, dh = pages.shape
+    if two != 2 or not pages.is_contiguous():
         raise ValueError("pages must be a contiguous [pages, 2, kv heads, page size, head dim] tensor")
-    _is(block_table, "block_table", torch.int32, 2, pages.device)
-    batch = block_table.shape[0]
-    _dense(q_start, "q_start", torch.int32, (batch + 1,), pages.device)
-    _dense(lengths, "lengths", torch.int32, (batch,), pages.device)
-    return _lib.CacheBatch(pages.data_ptr(), pages.shape[0], q_start.data_ptr(), lengths.data_ptr(), block_table.data_ptr(),
-                           max(block_table.stride(0), block_table.shape[1]), kept.status.data_ptr(), block_table.shape[1], pages.shape[3],
-                           pages.shape[2], pages.shape[4], batch, tokens)
+    batch, cols = block_table.shape
+    stride = block_table.stride(0)
+    _BATCH(block, 0, pages.data_ptr(), num_pages, _need(q_start, "q_start", _I32, (batch + 1,), device), _need(lengths, "lengths", _I32, (batch,), device),
+           block_table.data_ptr(), stride if stride > cols else cols, kept.status_ptr, cols, page_size, kv_heads, dh, batch, tokens)
+    return kv_heads, page_size, dh, cols
 
 
 def rope_tables(num_positions: int, head_dim: int, base: float = 10000.0, device="cuda"):
@@ -106,31 +122,29 @@ def history_append(qkv, pages, q_start, lengths, block_table, positions, cos=Non
     """qkv bf16 [N, (num_q_heads + 2 kv heads) * head dim] in the merged order [kv head][queries, key, value] (rows may be apart).  Query and key heads are
     normed (q_gain, k_gain fp32 [head dim]; None: not) and rotated by positions int32 [N] (cos, sin fp32 [positions, head dim / 2];
     None: not); keys and values go to the cache behind `lengths`, the queries come back as bf16 [N, num_q_heads, head dim]."""
-    _is(qkv, "qkv", torch.bfloat16, 2)
-    device, n = qkv.device, qkv.shape[0]
-    stream = _stream(device.index, stream)
-    kept = _keep(device.index, stream)
-    batch = _batch(pages, q_start, lengths, block_table, n, kept)
-    _is(pages, "pages", torch.bfloat16, 5, device)
-    dh = batch.key_size
-    if qkv.shape[1] != (num_q_heads + 2 * batch.num_kv_heads) * dh:
-        raise ValueError(f"qkv rows have {qkv.shape[1]} columns, {(num_q_heads + 2 * batch.num_kv_heads) * dh} are needed")
+    device = _rows(qkv, "qkv", _BF16, 2)
+    n, width = qkv.shape
+    stream = _stream(device, stream)
+    mine = _structs
+    kv_heads, _, dh, _ = _batch(mine.batch, pages, q_start, lengths, block_table, n, device, _keep(device, stream))
+    if width != (num_q_heads + 2 * kv_heads) * dh:
+        raise ValueError(f"qkv rows have {width} columns, {(num_q_heads + 2 * kv_heads) * dh} are needed")
+    places = at = cos_ptr = sin_ptr = q_gain_ptr = k_gain_ptr = 0
     if cos is not None or sin is not None:
-        _is(cos, "cos", torch.float32, 2, device)
-        _dense(cos, "cos", torch.float32, (cos.shape[0], dh // 2), device)
-        _dense(sin, "sin", torch.float32, (cos.shape[0], dh // 2), device)
-        _dense(positions, "positions", torch.int32, (n,), device)
-    for g, name in ((q_gain, "q_gain"), (k_gain, "k_gain")):
-        if g is not None:
-            _dense(g, name, torch.float32, (dh,), device)
+        _rows(cos, "cos", _F32, 2)
+        places = cos.shape[0]
+        cos_ptr, sin_ptr = _need(cos, "cos", _F32, (places, dh // 2), device), _need(sin, "sin", _F32, (places, dh // 2), device)
+        at = _need(positions, "positions", _I32, (n,), device)
+    if q_gain is not None:
+        q_gain_ptr = _need(q_gain, "q_gain", _F32, (dh,), device)
+    if k_gain is not None:
+        k_gain_ptr = _need(k_gain, "k_gain", _F32, (dh,), device)
+    shape = (n, num_q_heads, dh)
     if out is None:
-        out = torch.empty((n, num_q_heads, dh), dtype=torch.bfloat16, device=device)
-    else:
-        _dense(out, "out", torch.bfloat16, (n, num_q_heads, dh), device)
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    args = _lib.AppendArgs(qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], p(positions), p(cos), p(sin), p(q_gain), p(k_gain), out.data_ptr(), num_q_heads,
-                           0 if cos is None else cos.shape[0], eps, 0)
-    _ok(lib.phx_history_append_device(device.index, C.byref(batch), C.byref(args), stream))
+        out = torch.empty_strided(shape, (num_q_heads * dh, dh, 1), dtype=_BF16, device=qkv.device)
+    _APPEND(mine.append, 0, qkv.data_ptr(), qkv.stride(0) if n > 1 else width, at, cos_ptr, sin_ptr, q_gain_ptr, k_gain_ptr, _need(out, "out", _BF16, shape, device),
+            num_q_heads, places, eps, 0)
+    _ok(lib.phx_history_append_device(device, mine.batch_ref, mine.append_ref, stream))
     return out
 
 
@@ -142,31 +156,26 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
     chain).  sm_scale defaults to sqrt(128) / head dim (scaling.py:46-47).  max_tokens and max_keys: the most new tokens and keys
     (cached + new) of a request, if the caller knows them; they only choose kernels.  workspace: uint8, phx_tree_workspace_bytes; the stream's own if None.
     Returns bf16 [N, heads, head dim]."""
-    _is(q, "q", torch.bfloat16, 3)
-    n, heads, dh = q.shape
-    device = q.device
-    stream = _stream(device.index, stream)
-    kept = _keep(device.index, stream)
-    batch = _batch(pages, q_start, lengths, block_table, n, kept)
-    _is(pages, "pages", torch.bfloat16, 5, device)
-    if batch.key_size != dh or (heads > 1 and q.stride(1) != dh):
+    device = _rows(q, "q", _BF16, 3)
+    n, heads, dh = shape = q.shape
+    stream = _stream(device, stream)
+    kept, mine = _keep(device, stream), _structs
+    _, page_size, cache_dh, cols = _batch(mine.batch, pages, q_start, lengths, block_table, n, device, kept)
+    if cache_dh != dh or (heads > 1 and q.stride(1) != dh):
         raise ValueError("q must have the cache's head dim, its heads side by side")
     if cap_method not in CAP_METHODS:
         raise ValueError(f"cap_method must be one of {list(CAP_METHODS)}")
-    if spans is not None:
-        _dense(spans, "spans", torch.int32, (n, 2), device)
     if out is None:
-        out = torch.empty((n, heads, dh), dtype=torch.bfloat16, device=device)
-    else:
-        _dense(out, "out", torch.bfloat16, (n, heads, dh), device)
+        out = torch.empty_strided(shape, (heads * dh, dh, 1), dtype=_BF16, device=q.device)
     if workspace is None:
-        workspace = kept.workspace
+        space, size = kept.workspace_ptr, kept.workspace_bytes
     else:
-        _is(workspace, "workspace", torch.uint8, 1, device)
-    args = _lib.TreeArgs(q.data_ptr(), q.stride(0) if n > 1 else heads * dh, None if spans is None else spans.data_ptr(), out.data_ptr(), workspace.data_ptr(), workspace.numel(),
-                         batch.table_cols * batch.page_size if max_keys is None else max_keys, n if max_tokens is None else max_tokens, heads,
-                         math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], 0)
-    _ok(lib.phx_tree_attention_device(device.index, C.byref(batch), C.byref(args), stream))
+        size = workspace.numel()
+        space = _need(workspace, "workspace", _U8, (size,), device)
+    _TREE(mine.tree, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, 0 if spans is None else _need(spans, "spans", _I32, (n, 2), device),
+          _need(out, "out", _BF16, shape, device), space, size, cols * page_size if max_keys is None else max_keys, n if max_tokens is None else max_tokens, heads,
+          math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], 0)
+    _ok(lib.phx_tree_attention_device(device, mine.batch_ref, mine.tree_ref, stream))
     return out
 
 
@@ -174,24 +183,26 @@ def token_logprobs(logits, given=None, *, top_k: int = 0, cap: float = 0.0, temp
     """logits fp32 or bf16 [N, vocab] (rows may be apart; -inf: not allowed), given int64 [N, n] or [N] ids (outside the
     vocabulary: none).  Returns (log probabilities of given fp32, of its shape, None without given; entropy fp32 [N]; the top_k best ids' log probabilities fp32
     [N, top_k]; the ids int64 [N, top_k]) of softmax(cap tanh(logits / cap) / temperature), best first, ties by the lower id."""
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError("logits must be a float32 or bfloat16 tensor")
-    _is(logits, "logits", logits.dtype, 2)
+    bf16 = isinstance(logits, torch.Tensor) and logits.dtype is _BF16
+    device = _rows(logits, "logits", _BF16 if bf16 else _F32, 2)
     rows, vocab = logits.shape
-    device = logits.device
     if not 0 <= top_k <= vocab:
         raise ValueError(f"top_k must be 0 to vocab ({vocab})")
-    given_out = None
+    where = logits.device
+    given_out, given_ptr, given_out_ptr, num_given = None, 0, 0, 0
     if given is not None:
-        _dense(given, "given", torch.int64, (rows,) if given.dim() == 1 else (rows, given.shape[-1]), device)
-        given_out = torch.empty(given.shape, dtype=torch.float32, device=device)
-    entropy = torch.empty((rows,), dtype=torch.float32, device=device)
-    top = torch.empty((rows, top_k), dtype=torch.float32, device=device)
-    ids = torch.empty((rows, top_k), dtype=torch.int64, device=device)
-    args = _lib.LogprobsArgs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, None if given is None else given.data_ptr(), None if given is None else given_out.data_ptr(), entropy.data_ptr(), top.data_ptr(),
-                             ids.data_ptr(), rows, vocab, 0 if given is None else given.numel() // max(rows, 1), top_k,
-                             int(logits.dtype == torch.bfloat16), cap, temperature, 0)
-    _ok(lib.phx_token_logprobs_device(device.index, C.byref(args), _stream(device.index, stream)))
+        shape = tuple(given.shape)
+        num_given = shape[-1] if len(shape) == 2 else 1
+        given_ptr = _need(given, "given", _I64, (rows,) if len(shape) == 1 else (rows, num_given), device)
+        given_out = torch.empty_strided(shape, given.stride(), dtype=_F32, device=where)
+        given_out_ptr = given_out.data_ptr()
+    entropy = torch.empty_strided((rows,), (1,), dtype=_F32, device=where)
+    top = torch.empty_strided((rows, top_k), (top_k, 1), dtype=_F32, device=where)
+    ids = torch.empty_strided((rows, top_k), (top_k, 1), dtype=_I64, device=where)
+    mine = _structs
+    _LOGPROBS(mine.logprobs, 0, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, given_ptr, given_out_ptr, entropy.data_ptr(), top.data_ptr(), ids.data_ptr(),
+              rows, vocab, num_given, top_k, bf16, cap, temperature, 0)
+    _ok(lib.phx_token_logprobs_device(device, mine.logprobs_ref, _stream(device, stream)))
     return given_out, entropy, top, ids
 
 
