@@ -5,10 +5,11 @@
 //   h' = h / sqrt(mean(h^2) + eps) * gain,   (a, b) -> (a cos - b sin, b cos + a sin) over the halves a, b of h'
 //
 // in fp32, rounded once.  Bound by memory: each element is read once and written once, 16 bytes at a time.  key_size / 16
-// threads hold one head: thread i the 8 elements from 8 i on and the 8 that the rotation pairs them with, so that norm
-// (a shuffle over the head's threads) and rotation stay in registers.  A warp takes 4 x 32 / (key_size / 16) heads of one token with all its loads
-// issued before the first is used, and reads the token's cosines once for all of them; what a head's place in the cache needs - the
-// request by a 32-way search in q_start, its length, the page - is looked up under those loads.
+// threads hold one head: thread i the 8 elements from 8 i on and the 8 that the rotation pairs them with, so that norm (a
+// shuffle over the head's threads) and rotation stay in registers.  A round is 32 / (key_size / 16) heads of one token, queries or keys or values; a
+// warp takes four rounds that follow one another, of the queries or of keys and values, with all loads in flight before the first is used.  So gains, cosines and
+// sines are the same for all heads until the token changes, and are multiplied into four factors once, x' = (x A - y B) / rms, y' = (y C + x D) / rms, and
+// only the warps of keys and values look up their token's place in the cache - the request by a 32-way search in q_start, its length, the page.
 #include <string>
 
 #include "cache_batch.cuh"
@@ -17,7 +18,21 @@ namespace phx {
 namespace {
 
 constexpr int APPEND_WARPS = 4;
-constexpr int APPEND_ROUNDS = 4;   // heads of a warp that follow one another, all loads in flight
+constexpr int APPEND_ROUNDS = 4;
+
+// n / d for n below 2^16 or d a power of two: by a product with m = 2^32 / d rounded up
+struct SmallDivisor {
+  uint32_t d, m;
+  SmallDivisor() = default;
+  explicit SmallDivisor(uint32_t divisor) : d(divisor), m((uint32_t)((0x100000000ull + divisor - 1) / divisor)) {}
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return d == 1 ? n : __umulhi(n, m); }
+};
+struct AppendShape {
+  SmallDivisor group;               // query heads of a key head
+  unsigned q_blocks, kv_blocks;     // rounds of a token's queries, keys (or values)
+  unsigned q_rounds, kv_rounds;     // of all tokens
+  unsigned q_warps;
+};
 
 __device__ __forceinline__ uint4 load_stream(const uint16_t* p) {
   uint4 v;
@@ -52,97 +67,130 @@ __device__ __forceinline__ int find_request(const phx_cache_batch& c, int n, int
 }
 
 template <int DH>
-__global__ void __launch_bounds__(32 * APPEND_WARPS) history_append_kernel(const phx_cache_batch c, const phx_append_args a, int chunks) {
+__global__ void __launch_bounds__(32 * APPEND_WARPS, 5) history_append_kernel(const phx_cache_batch c, const phx_append_args a, const AppendShape shape) {
   constexpr int TPH = DH / 16;                 // threads of a head
   constexpr int HPR = 32 / TPH;                // heads of a round
   const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * APPEND_WARPS + (threadIdx.x >> 5);
-  const int n = (int)(item / chunks), chunk = (int)(item % chunks);
-  if (n >= c.num_tokens) return;
-  const int group = a.num_q_heads / c.num_kv_heads, per = group + 2, heads = c.num_kv_heads * per;
-  const int head0 = chunk * (APPEND_ROUNDS * HPR) + lane / TPH, e0 = (lane % TPH) * 8;
+  const unsigned warp = blockIdx.x * APPEND_WARPS + (threadIdx.x >> 5);
+  const bool kv = warp >= shape.q_warps;       // keys and values, or queries
+  const unsigned round0 = (kv ? warp - shape.q_warps : warp) * APPEND_ROUNDS, rounds = kv ? shape.kv_rounds : shape.q_rounds;
+  if (round0 >= rounds) return;
+  const int group = (int)shape.group.d, e0 = (lane % TPH) * 8, heads = kv ? c.num_kv_heads : a.num_q_heads;
 
-  const uint16_t* row = a.qkv + (long long)n * a.qkv_stride + e0;
+  // round i: token, head of this lane, whether of the values
+  int token[APPEND_ROUNDS], head[APPEND_ROUNDS];
+  bool value[APPEND_ROUNDS];
   uint4 lo[APPEND_ROUNDS], hi[APPEND_ROUNDS];
+  {
+    const unsigned per = kv ? 2 * shape.kv_blocks : shape.q_blocks;
+    unsigned n = round0 / per, block = round0 - n * per;
 #pragma unroll
-  for (int i = 0; i < APPEND_ROUNDS; ++i) {
-    const int head = head0 + i * HPR;
-    if (head < heads) { lo[i] = load_stream(row + head * DH); hi[i] = load_stream(row + head * DH + DH / 2); }
-    else lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
-  }
-  float cs[8], sn[8];
-  const bool rotary = a.cos_tab != nullptr, norm = a.q_gain != nullptr;
-  if (rotary) {
-    int pos = a.positions[n];
-    if (pos < 0 || pos >= a.num_positions) {
-      if (lane == 0) cache_report(c, CACHE_BAD_POSITION);
-      pos = max(0, min(pos, a.num_positions - 1));
+    for (int i = 0; i < APPEND_ROUNDS; ++i) {
+      value[i] = kv && block >= shape.kv_blocks;
+      token[i] = (int)n;
+      head[i] = (int)(value[i] ? block - shape.kv_blocks : block) * HPR + lane / TPH;
+      if (round0 + i >= rounds) head[i] = heads;            // none
+      const int of = kv ? head[i] : (int)shape.group.of((unsigned)head[i]), part = kv ? group + (value[i] ? 1 : 0) : head[i] - of * group;
+      if (head[i] < heads) {
+        const uint16_t* const src = a.qkv + (long long)n * a.qkv_stride + (of * (group + 2) + part) * DH + e0;
+        lo[i] = load_stream(src); hi[i] = load_stream(src + DH / 2);
+      } else {
+        lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
+      }
+      if (++block == per) { block = 0; ++n; }
     }
-    load8(a.cos_tab + (long long)pos * (DH / 2) + e0, cs);
-    load8(a.sin_tab + (long long)pos * (DH / 2) + e0, sn);
   }
-  // the token's place in the cache
-  const int b = find_request(c, n, lane);
-  const CacheRequest rq = cache_request(c, b);
-  const bool mine = n >= rq.row0 && n < rq.row0 + rq.tokens;
-  const long long at = (long long)rq.cached + (n - rq.row0);
-  const int col = (int)(at / c.page_size), slot = (int)(at - (long long)col * c.page_size);
-  const int page = mine && at < cache_columns(c) ? c.block_table[(long long)b * c.table_stride + col] : -1;
-  const bool stored = page >= 0 && page < c.num_pages;
-  if (!stored && lane == 0) cache_report(c, mine ? CACHE_BAD_PAGE : CACHE_BAD_OFFSETS);
-  uint16_t* const place = c.pages + (long long)slot * DH + e0;
 
+  const bool rotary = a.cos_tab != nullptr, norm = a.q_gain != nullptr;
+  float A[8], B[8], C[8], D[8];                // x' = x A - y B, y' = y C + x D
+  uint16_t* out = nullptr;
+  bool stored = true;
 #pragma unroll
   for (int i = 0; i < APPEND_ROUNDS; ++i) {
-    const int head = head0 + i * HPR;
-    const int kv = head / per, part = head - kv * per;         // part < group: a query head, group: the key, group + 1: the value
-    if (__all_sync(0xffffffffu, head >= heads)) break;
-    if (part <= group && (norm || rotary)) {
-      float x[8], y[8];
-      unpack8(lo[i], x); unpack8(hi[i], y);
+    if (round0 + i >= rounds) break;
+    const int n = token[i];
+    if (i == 0 || n != token[i - 1]) {         // the same for the whole warp
+      if (rotary) {
+        int pos = a.positions[n];
+        if (pos < 0 || pos >= a.num_positions) {
+          if (lane == 0) cache_report(c, CACHE_BAD_POSITION);
+          pos = max(0, min(pos, a.num_positions - 1));
+        }
+        load8(a.cos_tab + (long long)pos * (DH / 2) + e0, A);
+        load8(a.sin_tab + (long long)pos * (DH / 2) + e0, B);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { A[k] = 1.f; B[k] = 0.f; }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) { C[k] = A[k]; D[k] = B[k]; }
       if (norm) {
-        float ss = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) ss += x[k] * x[k] + y[k] * y[k];
-        const unsigned who = ((TPH == 32 ? 0u : (1u << TPH)) - 1u) << (lane & ~(TPH - 1));   // the head's threads: neighbours may hold a value
-#pragma unroll
-        for (int o = TPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(who, ss, o);
-        const float inv = 1.0f / sqrtf(ss * (1.0f / DH) + a.eps);
         float gx[8], gy[8];
-        const float* gain = (part == group ? a.k_gain : a.q_gain) + e0;
+        const float* const gain = (kv ? a.k_gain : a.q_gain) + e0;
         load8(gain, gx); load8(gain + DH / 2, gy);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) { x[k] *= inv * gx[k]; y[k] *= inv * gy[k]; }
+        for (int k = 0; k < 8; ++k) { A[k] *= gx[k]; D[k] *= gx[k]; B[k] *= gy[k]; C[k] *= gy[k]; }
       }
-      if (rotary) {
+      if (kv) {
+        const int b = find_request(c, n, lane);
+        const CacheRequest rq = cache_request(c, b);
+        const bool owned = n >= rq.row0 && n < rq.row0 + rq.tokens;
+        const long long at = (long long)rq.cached + (n - rq.row0);
+        const int col = owned && at < cache_columns(c) ? (int)at / c.page_size : -1, slot = (int)at - col * c.page_size;
+        const int page = col >= 0 ? c.block_table[(long long)b * c.table_stride + col] : -1;
+        stored = page >= 0 && page < c.num_pages;
+        if (!stored && lane == 0) cache_report(c, owned ? CACHE_BAD_PAGE : CACHE_BAD_OFFSETS);
+        out = c.pages + (stored ? cache_row0(c, page, 0, 0) + (long long)slot * DH : 0) + e0;
+      } else {
+        out = a.q_out + (long long)n * a.num_q_heads * DH + e0;
+      }
+    }
+    if ((norm || rotary) && !value[i]) {
+      float x[8], y[8];
+      unpack8(lo[i], x); unpack8(hi[i], y);
+      float inv = 1.0f;
+      if (norm) {
+        float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float u = x[k] * cs[k] - y[k] * sn[k];
-          y[k] = y[k] * cs[k] + x[k] * sn[k];
-          x[k] = u;
+        for (int k = 0; k < 8; k += 2) {
+          ss = __ffma2_rn(make_float2(x[k], x[k + 1]), make_float2(x[k], x[k + 1]), ss);
+          ss = __ffma2_rn(make_float2(y[k], y[k + 1]), make_float2(y[k], y[k + 1]), ss);
         }
+        float sum = ss.x + ss.y;
+#pragma unroll
+        for (int o = TPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        inv = rsqrtf(sum * (1.0f / DH) + a.eps);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) {
+        const float2 x2 = __fmul2_rn(make_float2(x[k], x[k + 1]), make_float2(inv, inv)), y2 = __fmul2_rn(make_float2(y[k], y[k + 1]), make_float2(inv, inv));
+        const float2 u = __ffma2_rn(x2, make_float2(A[k], A[k + 1]), __fmul2_rn(y2, make_float2(-B[k], -B[k + 1])));
+        const float2 v = __ffma2_rn(y2, make_float2(C[k], C[k + 1]), __fmul2_rn(x2, make_float2(D[k], D[k + 1])));
+        x[k] = u.x; x[k + 1] = u.y; y[k] = v.x; y[k + 1] = v.y;
       }
       lo[i] = pack8(x); hi[i] = pack8(y);
     }
-    if (head < heads) {
-      uint16_t* out = nullptr;
-      if (part < group) out = a.q_out + ((long long)n * a.num_q_heads + kv * group + part) * DH + e0;
-      else if (stored) out = place + cache_row0(c, page, part - group, kv);
-      if (out) {
-        *reinterpret_cast<uint4*>(out) = lo[i];
-        *reinterpret_cast<uint4*>(out + DH / 2) = hi[i];
-      }
+    if (head[i] < heads && stored) {
+      uint16_t* const to = out + (kv ? (long long)(head[i] + (value[i] ? c.num_kv_heads : 0)) * c.page_size * DH : (long long)head[i] * DH);
+      *reinterpret_cast<uint4*>(to) = lo[i];
+      *reinterpret_cast<uint4*>(to + DH / 2) = hi[i];
     }
   }
 }
 
 template <int DH>
 cudaError_t append_launch(const phx_cache_batch& c, const phx_append_args& a, cudaStream_t stream) {
-  constexpr int heads_per_warp = APPEND_ROUNDS * 32 / (DH / 16);
-  const int heads = a.num_q_heads + 2 * c.num_kv_heads;
-  const int chunks = (heads + heads_per_warp - 1) / heads_per_warp;
-  const long long warps = (long long)c.num_tokens * chunks;
-  history_append_kernel<DH><<<(unsigned)((warps + APPEND_WARPS - 1) / APPEND_WARPS), 32 * APPEND_WARPS, 0, stream>>>(c, a, chunks);
+  constexpr int per_round = 32 / (DH / 16);
+  AppendShape shape;
+  shape.group = SmallDivisor((uint32_t)(a.num_q_heads / c.num_kv_heads));
+  shape.q_blocks = (unsigned)(a.num_q_heads + per_round - 1) / per_round;
+  shape.kv_blocks = (unsigned)(c.num_kv_heads + per_round - 1) / per_round;
+  const long long q = (long long)c.num_tokens * shape.q_blocks, kv = 2ll * c.num_tokens * shape.kv_blocks;
+  if (q + kv > 0xF0000000ll) return cudaErrorInvalidValue;
+  shape.q_rounds = (unsigned)q; shape.kv_rounds = (unsigned)kv;
+  shape.q_warps = (unsigned)((q + APPEND_ROUNDS - 1) / APPEND_ROUNDS);
+  const unsigned warps = shape.q_warps + (unsigned)((kv + APPEND_ROUNDS - 1) / APPEND_ROUNDS);
+  history_append_kernel<DH><<<(warps + APPEND_WARPS - 1) / APPEND_WARPS, 32 * APPEND_WARPS, 0, stream>>>(c, a, shape);
   return cudaGetLastError();
 }
 
