@@ -13,10 +13,12 @@
 // The best ids are found by words first: a word's key is its largest logit's order-preserving image, then its place, first come first.
 // The top_k-th largest key of any set of words bounds what the row's best ids can be in - a word below it holds nothing that is not
 // beaten by a logit in each of top_k other words - so after the first batch the threads' best words give a bound, and from then on the words at
-// or above it, few, are noted in shared memory.  After 2, 4, 8, ... batches the bound is taken anew from the notes, if they have grown, and the rest is dropped.  At the end the notes' words are
+// or above it, few, are noted in shared memory.  After 2, 4, 8, ... batches the bound is taken anew from the notes, if they
+// fill a quarter of their room, and the rest is dropped.  At the end the notes' words are
 // read again, their (logit, id) keys bounded in the same way, and the survivors ranked by counting.  Rows whose order defeats the
 // bounds (sorted ones: more words than the notes hold) take the exact bound from a radix select over the keys, a byte a pass.  Keys are
-// distinct, so ties need no care and the result does not depend on the order of the atomics.
+// distinct, so ties need no care and the result does not depend on the order of the atomics.  More ids than lanes give a bound for (over 24) of
+// a row that a warp has for itself are found exactly: the row's images in registers, their top_k-th largest by halving.
 #include <math.h>
 #include <string.h>
 
@@ -28,6 +30,7 @@ namespace phx {
 namespace {
 
 constexpr int WARP_ROWS = 4;        // rows of a block whose warps take one each
+constexpr int WARP_ROW = 1024;      // the longest of them
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float FLOOR = -1e38f, DEEP = -1e37f;
 constexpr float ROOM = 16.0f;       // powers of two that the exponentials may grow to before the reference moves
@@ -215,7 +218,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
   };
 
   Stat st = {-INFINITY, 0.f, 0.f};
-  const bool want_top = a.top_k > 0 && (a.top_out || a.top_ids_out);
+  const bool want_top = a.top_k > 0 && (a.top_out || a.top_ids_out), exactly = NT == 32 && a.top_k > 24;
   u64 bound = ~0ull;              // of words
   float bound_x = INFINITY;       // its logit
   bool lost = false;              // more words than the notes hold
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
       top = max_nan(top, tops[i]);
     }
 
-    if (want_top) {
+    if (want_top && !exactly) {
       if (it == 0) {              // the first bound
         u64 best = 0;
 #pragma unroll
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
         const int n = mem.count;
         G::sync();
         if (n > KEEP) { lost = true; bound = ~0ull; bound_x = INFINITY; }   // not worth noting any more
-        else if (n > 3 * a.top_k) {
+        else if (n > KEEP / 4) {
           const u64 closer = tighten(mem.keep, n);
           if (closer > bound) { bound = closer; bound_x = value_of(bound); }
         }
@@ -375,7 +378,36 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
   // the team's best keys, of single logits, over the rings
   u64* const single = reinterpret_cast<u64*>(&mem.word[0][0]);
   int n = 0;
-  if (want_top) {
+  if (NT == 32 && exactly && want_top) {
+    uint32_t img[WARP_ROW / 32];                             // of logits lane, lane + 32, ...; 0: behind the row
+#pragma unroll
+    for (int i = 0; i < WARP_ROW / 32; ++i) img[i] = i * 32 + lane < a.vocab ? image(Words<T>::at(row, i * 32 + lane)) : 0;
+    uint32_t low = 1, high = 0xFFFFFFFFu;                    // at least top_k are at or above low
+    for (int have = a.vocab; have > a.top_k && low < high;) {
+      const uint32_t mid = low + (high - low) / 2 + 1;
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < WARP_ROW / 32; ++i) c += img[i] >= mid;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (c >= a.top_k) { low = mid; have = c; }
+      else high = mid - 1;
+    }
+    int more = 0;                                            // above low: all of them, so of low itself the rest, lowest ids first
+#pragma unroll
+    for (int i = 0; i < WARP_ROW / 32; ++i) more += img[i] > low;
+    int equal = a.top_k - __reduce_add_sync(0xffffffffu, more);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < WARP_ROW / 32; ++i) {
+      const unsigned same = __ballot_sync(0xffffffffu, img[i] == low);
+      const bool take = img[i] > low || (img[i] == low && __popc(same & ((1u << lane) - 1)) < equal);
+      const unsigned who = __ballot_sync(0xffffffffu, take);
+      if (take) single[n + __popc(who & ((1u << lane) - 1))] = (u64)img[i] << 32 | (uint32_t)~(i * 32 + lane);
+      n += __popc(who);
+      equal = max(0, equal - __popc(same));
+    }
+    __syncwarp();
+  } else if (want_top) {
     G::sync();
     int notes = mem.count;
     G::sync();
@@ -501,13 +533,13 @@ cudaError_t logprobs_launch(const phx_logprobs_args& a, int blocks, cudaStream_t
   return cudaLaunchKernelEx(&lc, logprobs_kernel<T, NT, CAP>, a, blocks);
 }
 // Threads of a row: enough for its words in one batch, as far as the device has room for all rows at once (148 SMs of 1024 threads at
-// this kernel's registers); a warp for rows it can hold (and ids it can bound by its lanes), else a block, else a cluster of up to eight.
+// this kernel's registers); a warp for rows it can hold, else a block, else a cluster of up to eight.
 template <typename T, bool CAP>
 cudaError_t logprobs_dispatch(const phx_logprobs_args& a, cudaStream_t stream) {
   const long long need = (a.vocab + 2ll * Words<T>::N) / (Words<T>::N * 4) + 1;
   const long long room = (long long)device_sms() * 1024 / a.rows;
   const long long threads = need < room ? need : room;
-  if (a.vocab <= 1024 && a.top_k <= 24) return logprobs_launch<T, 32, CAP>(a, 1, stream);
+  if (a.vocab <= WARP_ROW) return logprobs_launch<T, 32, CAP>(a, 1, stream);
   if (threads <= 512 || a.rows > 1 << 27) return logprobs_launch<T, 256, CAP>(a, 1, stream);
   const int blocks = threads <= 1024 ? 1 : threads <= 2048 ? 2 : threads <= 4096 ? 4 : 8;
   return logprobs_launch<T, 1024, CAP>(a, blocks, stream);
