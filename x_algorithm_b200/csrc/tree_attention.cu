@@ -519,6 +519,7 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   const long long tiles = (t.a.max_keys + t.keys - 1) / t.keys;
   const long long blocks = per_sm * device_sms(), fed = units * (tiles + t.setup) / 4;   // no block for less than four places
   t.split = tiles >= 4 && units < (tc ? 2 : 8) * blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)(fed < blocks ? fed : blocks) : 0;
+  t.turns = tc && !t.split && units > blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)blocks : 0;
   if (part_bytes(t.split, t.rows, t.c.key_size) > t.a.workspace_bytes) return bad("workspace is smaller than phx_tree_workspace_bytes");
   t.part_o = static_cast<float*>(t.a.workspace);
   t.part_ml = reinterpret_cast<float2*>(t.part_o + 2ll * t.split * t.rows * t.c.key_size);

@@ -24,6 +24,7 @@ struct TreeView {
   int rows, keys;        // of a tile
   int setup;             // places in front of a unit's tiles
   int split;             // blocks that share the tiles; 0: a block takes whole units
+  int turns;             // blocks that take whole units in turns (tcgen05 kernel); 0: a block for each
   float* part_o;         // [2 split][rows][key_size]
   float2* part_ml;       // [2 split][rows]: reference (log2 domain), sum
   struct TreeJoin* join; // [split]: what block x's bound in front leaves to be joined
@@ -104,7 +105,7 @@ struct TreePiece {
 __device__ __forceinline__ int tree_row_tiles(const TreeView& t, int tokens) { return (int)(((long long)tokens * t.group + t.rows - 1) / t.rows); }
 __device__ __forceinline__ int tree_key_tiles(const TreeView& t, int keys) { return keys > 0 ? (keys - 1) / t.keys + 1 : 1; }
 
-// Tiles in front of each request, in shared memory
+// Places in front of each request, in shared memory; without a split, units
 template <int THREADS> struct TreePlan {
   long long before[TREE_MAX_SPLIT_BATCH + 1];
   long long warp_sum[THREADS / 32];
@@ -115,7 +116,7 @@ template <int THREADS> struct TreePlan {
     const int tid = threadIdx.x, lane = tid & 31, per = (t.c.batch + THREADS - 1) / THREADS, b0 = min(tid * per, t.c.batch), b1 = min(b0 + per, t.c.batch);
     auto tiles_of = [&](int b) {
       const KeyRange k = key_range(t.c, b);
-      return (long long)t.c.num_kv_heads * tree_row_tiles(t, k.rq.tokens) * (tree_key_tiles(t, k.keys) + t.setup);
+      return (long long)t.c.num_kv_heads * tree_row_tiles(t, k.rq.tokens) * (t.split ? tree_key_tiles(t, k.keys) + t.setup : 1);
     };
     long long mine = 0;
     for (int b = b0; b < b1; ++b) mine += tiles_of(b);
@@ -127,11 +128,23 @@ template <int THREADS> struct TreePlan {
     long long at = sum - mine;
     for (int w = 0; w < (tid >> 5); ++w) at += warp_sum[w];
     for (int b = b0; b < b1; ++b) { before[b] = at; at += per == 1 ? mine : tiles_of(b); }
-    if (tid == THREADS - 1) { before[t.c.batch] = at; per_ = at / t.split; more_ = at % t.split; }   // the last thread ends behind all
+    if (tid == THREADS - 1) { before[t.c.batch] = at; if (t.split) { per_ = at / t.split; more_ = at % t.split; } }   // the last thread ends behind all
     __syncthreads();
   }
   __device__ __forceinline__ long long all(const TreeView& t) const { return before[t.c.batch]; }
   __device__ __forceinline__ long long bound(int block) const { return block * per_ + min((long long)block, more_); }
+  __device__ __forceinline__ int request_at(const TreeView& t, long long pos) const {
+    int lo = 0, hi = t.c.batch;                          // before[lo] <= pos < before[hi]
+    while (hi - lo > 1) { const int mid = (lo + hi) / 2; if (before[mid] <= pos) lo = mid; else hi = mid; }
+    return lo;
+  }
+  // unit `pos`
+  __device__ __forceinline__ TreePiece unit(const TreeView& t, long long pos) const {
+    const int b = request_at(t, pos);
+    const KeyRange k = key_range(t.c, b);
+    const int row_tiles = tree_row_tiles(t, k.rq.tokens), in = (int)(pos - before[b]), tiles = tree_key_tiles(t, k.keys);
+    return TreePiece{b, in / row_tiles, in % row_tiles, 0, tiles, tiles};
+  }
   // the first block whose stretch begins at or behind place `pos`
   __device__ __forceinline__ int block_behind(const TreeView& t, long long pos) const {
     int lo = 0, hi = t.split;
@@ -154,8 +167,7 @@ template <int THREADS> struct TreePlan {
   }
   // the piece from place `pos` on, at most to `end`; `next` is behind it, `unit_end` behind its unit
   __device__ __forceinline__ TreePiece piece(const TreeView& t, long long pos, long long end, long long* next, long long* unit_end) const {
-    int lo = 0, hi = t.c.batch;                          // before[lo] <= pos < before[hi]
-    while (hi - lo > 1) { const int mid = (lo + hi) / 2; if (before[mid] <= pos) lo = mid; else hi = mid; }
+    const int lo = request_at(t, pos);
     const KeyRange k = key_range(t.c, lo);
     TreePiece p;
     p.b = lo;
