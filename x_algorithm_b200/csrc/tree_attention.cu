@@ -514,11 +514,15 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   t.rows = ROWS; t.keys = KEYS * TREE_WARPS; t.setup = 2;
   if (tc) tree_tc_shape(t);
   const int per_sm = tc ? tree_tc_blocks_per_sm() : t.c.key_size == 128 ? mma_blocks<128>() : mma_blocks<64>();
-  // Blocks share the tiles of all units where there are few units for them and long ones among them.
+  // Blocks share the tiles of all units where there are few units for them and long ones among them.  Measured on the tensor cores (us, shared / whole): 2 to 4
+  // units a block, 16 tiles each 141 / 110, 64 tiles 350 / 370, 128 tiles 646 / 716: whole ones cost the last round's empty blocks, shared ones about 24 tiles for parts and
+  // their join.  Up to two a block they are shared all the same: lengths are seldom equal.
   const long long units = (long long)t.c.batch * t.c.num_kv_heads * (((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows);
   const long long tiles = (t.a.max_keys + t.keys - 1) / t.keys;
-  const long long blocks = per_sm * device_sms(), fed = units * (tiles + t.setup) / 4;   // no block for less than four places
-  t.split = tiles >= 4 && units < (tc ? 2 : 8) * blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)(fed < blocks ? fed : blocks) : 0;
+  const long long blocks = per_sm * device_sms(), fed = units * (tiles + t.setup) / (tc ? 8 : 4);   // no block for fewer places: parts and joins take longer than that many
+  const long long idle = (units + blocks - 1) / blocks * blocks - units;                  // blocks without a unit in the last round of whole ones
+  const bool few = tc ? tiles >= 8 && (units < 2 * blocks || idle * tiles > 24 * blocks) : tiles >= 4 && units < 8 * blocks;
+  t.split = few && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)(fed < blocks ? fed : blocks) : 0;
   t.turns = tc && !t.split && units > blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)blocks : 0;
   if (part_bytes(t.split, t.rows, t.c.key_size) > t.a.workspace_bytes) return bad("workspace is smaller than phx_tree_workspace_bytes");
   t.part_o = static_cast<float*>(t.a.workspace);
