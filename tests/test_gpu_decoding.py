@@ -575,3 +575,99 @@ def test_refusals():
     assert decoding.history_append(qkv[:0], c.pages, zero, c.lengths, c.table, pos[:0], num_q_heads=4).shape == (0, 4, 64)
     assert decoding.token_logprobs(x[:0], top_k=3)[3].shape == (0, 3)
     decoding.check_status()
+
+
+# ---- which kernels run, and the ends of the ranges -------------------------------------------------------------------------
+
+def _ran(f):
+    from x_algorithm_b200.engine import dispatch_counts
+    before = dispatch_counts()
+    f()
+    return {k for k, v in dispatch_counts().items() if v != before[k]}
+
+
+def test_kernels_by_rows_of_a_key_head():
+    """Up to 16 query rows of a key head, heads of 32 and groups of more than 128 are the mma.sync kernel's, the rest the tensor cores'."""
+    assert _ran(lambda: _tree_case([1, 3], [100, 5], 16, 4, 128, 16)) == {"tree.mma"}
+    assert _ran(lambda: _tree_case([2, 5], [100, 5], 16, 4, 128, 16, max_tokens=5)) == {"tree.tcgen05"}
+    assert _ran(lambda: _tree_case([40], [100], 4, 4, 32, 16)) == {"tree.mma"}
+    assert _ran(lambda: _tree_case([2], [90], 144, 1, 64, 16)) == {"tree.mma"}
+
+
+@pytest.mark.parametrize("batch,tokens,heads,kv_heads,dh", [(50, 140, 8, 8, 64), (90, 40, 16, 4, 128), (1100, 1, 16, 4, 128), (1100, 20, 4, 2, 64), (700, 2, 8, 8, 64)])
+def test_many_requests(batch, tokens, heads, kv_heads, dh):
+    """More units than blocks (a block takes several), more requests than the shared plan holds; empty requests among them."""
+    rng = np.random.default_rng(batch)
+    t = [int(x) for x in rng.integers(0, tokens + 1, batch)]
+    t[3] = tokens
+    _tree_case(t, [int(x) for x in rng.integers(0, 200, batch)], heads, kv_heads, dh, 16, "tree", seed=batch)
+
+
+@pytest.mark.parametrize("tokens,cached,heads,kv_heads,dh,page", [([1], [40001], 8, 8, 64, 128), ([9], [30003], 16, 1, 128, 48), ([2, 30], [20000, 17], 10, 2, 64, 16),
+                                                                   ([33], [12345], 24, 8, 128, 32), ([1100], [3], 4, 1, 64, 64), ([300, 2], [2500, 4001], 16, 4, 128, 112)])
+@pytest.mark.parametrize("shape", ["chain", "whole", "tree"])
+def test_long_caches_are_cut_and_joined(tokens, cached, heads, kv_heads, dh, page, shape):
+    _tree_case(tokens, cached, heads, kv_heads, dh, page, shape, padding=1, seed=len(tokens))
+
+
+def test_odd_values_in_parts():
+    """Infinities and NaN of new tokens where the keys are cut into parts."""
+    from x_algorithm_b200 import decoding
+    torch = _torch()
+    for tokens, heads, kv_heads, dh in ((3, 16, 4, 128), (60, 16, 4, 128), (40, 8, 8, 64)):
+        c = Cache([tokens], [9000], kv_heads, dh, 16, seed=2)
+        q = torch.randn((c.n, heads, dh), device=DEV, generator=c.g).to(torch.bfloat16)
+        spans = torch.tensor(_spans("tree", tokens, 1, 4), dtype=torch.int32, device=DEV)
+        for j, value in ((0, math.inf), (tokens - 1, math.nan), (1, -math.inf)):
+            at = 9000 + j
+            c.pages[c.table_host[0][at // 16], 1, 0, at % 16, j + 2] = value
+        out = decoding.tree_attention(q, *c.args(), spans)
+        _check(out, *_attend(c, q, spans, math.sqrt(128.0) / dh))
+
+
+def test_offsets_past_32_bits():
+    """A pool of more than 2^32 elements, its last pages in use; logits and rows further apart than 2^31 elements."""
+    from x_algorithm_b200 import decoding
+    torch = _torch()
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    total, kv, page, dh, heads = 18000, 8, 128, 128, 16
+    pages = torch.empty((total, 2, kv, page, dh), dtype=torch.bfloat16, device=DEV)
+    assert pages.numel() > 2 ** 32
+    for tokens in (1, 70):
+        small = Cache([tokens], [300], kv, dh, page, seed=tokens)
+        numbers = [total - 1 - i for i in range(len(small.table_host[0]) - 1)]
+        for i, p in enumerate(numbers):
+            pages[p] = small.pages[small.table_host[0][i]]
+        table = torch.tensor([numbers + [-1]], dtype=torch.int32, device=DEV)
+        q = torch.randn((tokens, heads, dh), device=DEV, generator=small.g).to(torch.bfloat16)
+        want = decoding.tree_attention(q, *small.args())
+        assert torch.equal(decoding.tree_attention(q, pages, small.q_start, small.lengths, table), want)
+        qkv = torch.randn((tokens, (heads + 2 * kv) * dh), device=DEV, generator=small.g).to(torch.bfloat16)
+        a = decoding.history_append(qkv, *small.args(), None, num_q_heads=heads)
+        b = decoding.history_append(qkv, pages, small.q_start, small.lengths, table, None, num_q_heads=heads)
+        assert torch.equal(a, b)
+        for i, p in enumerate(numbers):
+            assert torch.equal(pages[p], small.pages[small.table_host[0][i]])
+        decoding.check_status()
+    del pages
+    wide = torch.empty(2 ** 31 + 5000, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn((2, 4001), device=DEV, generator=g).to(torch.bfloat16)
+    far = wide.as_strided((2, 4001), (2 ** 31 + 8, 1), 3)
+    far.copy_(x)
+    _logprobs_check(far, torch.tensor([[0, 4000]] * 2, device=DEV), 9)    # (its words begin elsewhere than x's: the sums' last bits may differ)
+
+
+def test_a_wait_that_ran_out_is_reported_once():
+    """The flag that a bounded wait raises, raised by the host."""
+    from x_algorithm_b200 import PhoenixError, decoding
+    torch = _torch()
+    _tree_case([40], [100], 8, 8, 64, 16)
+    kept = decoding._kept[(0, torch._C._cuda_getCurrentRawStream(0))]
+    kept.status[0] = 1
+    with pytest.raises(PhoenixError) as e:
+        decoding.check_status()
+    assert e.value.status == 4
+    decoding.check_status()
+    _tree_case([40], [100], 8, 8, 64, 16)

@@ -142,8 +142,9 @@ def history_append(qkv, pages, q_start, lengths, block_table, positions, cos=Non
     shape = (n, num_q_heads, dh)
     if out is None:
         out = torch.empty_strided(shape, (num_q_heads * dh, dh, 1), dtype=_BF16, device=qkv.device)
-    _APPEND(mine.append, 0, qkv.data_ptr(), qkv.stride(0) if n > 1 else width, at, cos_ptr, sin_ptr, q_gain_ptr, k_gain_ptr, _need(out, "out", _BF16, shape, device),
-            num_q_heads, places, eps, 0)
+    else:
+        _need(out, "out", _BF16, shape, device)
+    _APPEND(mine.append, 0, qkv.data_ptr(), qkv.stride(0) if n > 1 else width, at, cos_ptr, sin_ptr, q_gain_ptr, k_gain_ptr, out.data_ptr(), num_q_heads, places, eps, 0)
     _ok(lib.phx_history_append_device(device, mine.batch_ref, mine.append_ref, stream))
     return out
 
@@ -167,13 +168,15 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
         raise ValueError(f"cap_method must be one of {list(CAP_METHODS)}")
     if out is None:
         out = torch.empty_strided(shape, (heads * dh, dh, 1), dtype=_BF16, device=q.device)
+    else:
+        _need(out, "out", _BF16, shape, device)
     if workspace is None:
         space, size = kept.workspace_ptr, kept.workspace_bytes
     else:
         size = workspace.numel()
         space = _need(workspace, "workspace", _U8, (size,), device)
     _TREE(mine.tree, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, 0 if spans is None else _need(spans, "spans", _I32, (n, 2), device),
-          _need(out, "out", _BF16, shape, device), space, size, cols * page_size if max_keys is None else max_keys, n if max_tokens is None else max_tokens, heads,
+          out.data_ptr(), space, size, cols * page_size if max_keys is None else max_keys, n if max_tokens is None else max_tokens, heads,
           math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], 0)
     _ok(lib.phx_tree_attention_device(device, mine.batch_ref, mine.tree_ref, stream))
     return out
