@@ -169,7 +169,7 @@ __device__ __forceinline__ V* in_block(V* p, uint32_t rank) {   // the same plac
 
 // shape of a team: words it notes (all of a warp's row), words that a thread takes at a time, such batches in its ring, blocks that share an SM
 template <int NT> struct Shape {
-  static constexpr int KEEP = NT == 32 ? 320 : 1024, BATCH = NT == 256 ? 4 : 2, RING = NT == 32 ? 3 : 2, RESIDENT = NT == 1024 ? 1 : 4;
+  static constexpr int KEEP = NT == 32 ? 320 : 1024, BATCH = NT == 256 ? 4 : 2, RING = NT == 32 ? 3 : 2, RESIDENT = NT == 1024 ? 1 : 5;
   typedef TeamMemory<NT, KEEP, RING * BATCH> Memory;
 };
 

@@ -43,26 +43,27 @@ __device__ __forceinline__ float tree_ex2(float x) {
   return y;
 }
 // cap(s * scale) in the log2 domain: method 1 s / (1 + |s| / cap), 2 cap tanh(s / cap) as cap (1 - 2 / (e^(2 s / cap) + 1)), good to 1e-7 of the cap
-// tanh also as an odd polynomial for |z| <= SMALL (least maximum error over it, 1.9e-7, found by reweighted least squares on Chebyshev nodes): on the fma pipe,
-// two at a time, where two special-function operations a logit bound the kernel (24 trees of 32 over 8192 keys, 32 heads of 128: 178 -> 136 us without a cap)
+// tanh also as an odd polynomial for |z| <= SMALL (least maximum error over it, 1.3e-7, found by reweighted least squares on Chebyshev nodes), in the
+// raw logit with all factors in the coefficients: on the fma pipe, two at a time, where two more special-function operations a logit bound the kernel (24 trees of 32
+// over 8192 keys, 32 heads of 128: 178 us against 136 without a cap, when it was first measured)
 struct TreeCap {
-  static constexpr float SMALL = 0.75f;
-  float scale, a, b, small_scale, c[5];
+  static constexpr float SMALL = 0.5f;
+  float scale, a, b, small_scale, c[4];
   __device__ __forceinline__ TreeCap(const TreeView& t) {
     const float cap = t.a.cap;
     scale = t.a.cap_method == 0 ? t.csc : t.a.cap_method == 1 ? t.a.sm_scale : t.a.sm_scale * 2.0f * TREE_LOG2E / cap;
     a = t.a.cap_method == 1 ? 1.0f / cap : -2.0f * cap * TREE_LOG2E;
     b = cap * TREE_LOG2E;
-    small_scale = fabsf(t.a.sm_scale) / cap;
-    const float sign = t.a.sm_scale < 0.f ? -b : b;
-    c[0] = sign * 0.999997228f; c[1] = sign * -0.333230764f; c[2] = sign * 0.132260913f; c[3] = sign * -0.049280439f; c[4] = sign * 0.0123188247f;
+    const float z = t.a.sm_scale / cap, z2 = z * z;
+    small_scale = fabsf(z);
+    c[0] = b * z * 0.999997676f; c[1] = b * z * z2 * -0.333206551f; c[2] = b * z * z2 * z2 * 0.13145145f; c[3] = b * z * z2 * z2 * z2 * -0.0433724655f;
   }
   __device__ __forceinline__ void of_small(float& s0, float& s1) const {
     auto two = [](float x) { return make_float2(x, x); };
-    const float2 z = __fmul2_rn(make_float2(s0, s1), two(small_scale)), z2 = __fmul2_rn(z, z);
-    float2 p = __ffma2_rn(two(c[4]), z2, two(c[3]));
-    p = __ffma2_rn(p, z2, two(c[2])); p = __ffma2_rn(p, z2, two(c[1])); p = __ffma2_rn(p, z2, two(c[0]));
-    p = __fmul2_rn(p, z);
+    const float2 s = make_float2(s0, s1), s2 = __fmul2_rn(s, s);
+    float2 p = __ffma2_rn(two(c[3]), s2, two(c[2]));
+    p = __ffma2_rn(p, s2, two(c[1])); p = __ffma2_rn(p, s2, two(c[0]));
+    p = __fmul2_rn(p, s);
     s0 = p.x; s1 = p.y;
   }
   template <int METHOD> __device__ __forceinline__ float of(float s) const {

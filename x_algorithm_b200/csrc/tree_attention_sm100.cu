@@ -34,6 +34,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // D[tmem] (+)= A[tmem] * B[smem desc]
 __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
   asm volatile(
@@ -371,16 +376,38 @@ struct TcBlock {
         if (busy) {
           tmem_ld_wait_on(s);
           tmem_ld_wait_on(s + 32);
-          bool small = false;
-          if (CAP == 2) {                                   // tanh by its polynomial where all of the warp's logits are small against the cap
-            float big = 0.f;
+          // Four chains of three-input max.  tanh is monotone: without a mask one of the raw maximum serves for the row, and with the raw minimum it says
+          // whether all of the warp's logits are small enough against the cap for its polynomial.
+          float bm;
+          auto top_of = [&]() {
+            float b4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int k = 0; k < KT; ++k) big = fmaxf(big, fabsf(s[k]));
-            small = __all_sync(0xffffffffu, !valid || big * cap.small_scale <= TreeCap::SMALL);
-          }
-          if (CAP == 2 && small) {
+            for (int k = 4; k + 7 < KT; k += 8) {
+              b4[0] = max3(b4[0], s[k], s[k + 1]); b4[1] = max3(b4[1], s[k + 2], s[k + 3]);
+              b4[2] = max3(b4[2], s[k + 4], s[k + 5]); b4[3] = max3(b4[3], s[k + 6], s[k + 7]);
+            }
+            return max3(fmaxf(b4[0], b4[1]), max3(b4[2], b4[3], s[KT - 4]), max3(s[KT - 3], s[KT - 2], s[KT - 1]));   // and the tail that the loop leaves
+          };
+          if (CAP == 2) {
+            float low[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int k = 0; k < KT; k += 2) cap.of_small(s[k], s[k + 1]);
+            for (int k = 4; k + 7 < KT; k += 8) {
+              low[0] = min3(low[0], s[k], s[k + 1]); low[1] = min3(low[1], s[k + 2], s[k + 3]);
+              low[2] = min3(low[2], s[k + 4], s[k + 5]); low[3] = min3(low[3], s[k + 6], s[k + 7]);
+            }
+            float least = min3(fminf(low[0], low[1]), min3(low[2], low[3], s[KT - 4]), min3(s[KT - 3], s[KT - 2], s[KT - 1]));
+            bm = top_of();
+            const bool small = __all_sync(0xffffffffu, !valid || fmaxf(fabsf(bm), fabsf(least)) * cap.small_scale <= TreeCap::SMALL);
+            if (cap.scale < 0.f) bm = least;                 // a negative scale turns the order round
+            if (small) {
+              cap.of_small(bm, least);
+#pragma unroll
+              for (int k = 0; k < KT; k += 2) cap.of_small(s[k], s[k + 1]);
+            } else {
+              bm = cap.template of<2>(bm);
+#pragma unroll
+              for (int k = 0; k < KT; ++k) s[k] = cap.template of<2>(s[k]);
+            }
           } else if (CAP) {
 #pragma unroll
             for (int k = 0; k < KT; ++k) s[k] = cap.template of<CAP>(s[k]);
@@ -389,15 +416,7 @@ struct TcBlock {
 #pragma unroll
             for (int k = 0; k < KT; ++k) { const int2 sp = sm.span[j & 1][k]; if (!(sp.x <= pre && pre < sp.y)) s[k] = -INFINITY; }
           }
-          float b4[4] = {s[0], s[1], s[2], s[3]};            // four chains of three-input max
-#pragma unroll
-          for (int k = 4; k + 7 < KT; k += 8) {
-            b4[0] = max3(b4[0], s[k], s[k + 1]); b4[1] = max3(b4[1], s[k + 2], s[k + 3]);
-            b4[2] = max3(b4[2], s[k + 4], s[k + 5]); b4[3] = max3(b4[3], s[k + 6], s[k + 7]);
-          }
-          float bm = fmaxf(max3(b4[0], b4[1], b4[2]), b4[3]);
-#pragma unroll
-          for (int k = KT - 4; k < KT; ++k) bm = fmaxf(bm, s[k]);   // the tail that the 8-wide loop leaves
+          if (CAP != 2 || masked) bm = top_of();
           // The reference only has to bound the exponentials: it moves when the maximum has outgrown it by 2^8 (P stays below 256, as exact in bf16 as below
           // 1), which spares rescaling O for almost every tile.  Each row moves its own.
           const float m_true = fmaxf(m, bm * csc);
