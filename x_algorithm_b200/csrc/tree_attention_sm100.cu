@@ -132,11 +132,11 @@ struct TcBlock {
   uint32_t tmem;
 
   __device__ __forceinline__ bool wait(const uint64_t& bar, int phase) const { return mbar_wait(smem_u32(&bar), (uint32_t)(phase & 1), t.c.status_dev); }
-  // page of box `lane` of a tile, the last of which may lie behind the keys
+  // Page of box `lane` of a tile; behind the keys, some page.  (This and the spans below are asked for a tile ahead, by loads without a condition: a value
+  // that is chosen between a load and a constant has to wait for the load, and the producer was 2000 cycles a tile behind.)
   __device__ __forceinline__ int page_of(const KeyRange& kr, int tile) const {
-    const int lane = threadIdx.x & 31;
-    const long long key = (long long)tile * KT + lane * box;
-    return lane < KT / box && key < kr.keys ? kr.table[(int)key / t.c.page_size] : -1;
+    const long long key = (long long)tile * KT + (threadIdx.x & 31) * box;
+    return kr.keys > 0 ? kr.table[(int)min(key, (long long)kr.keys - 1) / t.c.page_size] : -1;
   }
 
   // ---- TMA producer (a whole warp; one lane issues) ----------------------------------------------------------------------
@@ -176,10 +176,7 @@ struct TcBlock {
       auto ask = [&](int tile) {
         spans_of = tile;
 #pragma unroll
-        for (int i = 0; i < KT / 32; ++i) {
-          const long long key = (long long)tile * KT + i * 32 + lane;
-          spans[i] = key >= kr.keys ? make_int2(0x7fffffff, -1) : key < rq.cached ? make_int2(-1, 0x7fffffff) : span_of(t, rq, (int)key - rq.cached);
-        }
+        for (int i = 0; i < KT / 32; ++i) spans[i] = span_of(t, rq, (int)max(0ll, min((long long)tile * KT + i * 32 + lane - rq.cached, (long long)rq.tokens - 1)));
       };
       // the first tile from `tile` on of which some row sees some key (`last`: none); *masked: not every row every key
       auto next_tile = [&](int tile, bool* masked) {
@@ -191,8 +188,10 @@ struct TcBlock {
           bool any = false, all = true;
 #pragma unroll
           for (int i = 0; i < KT / 32; ++i) {
-            any |= spans[i].x <= hi && spans[i].y > lo;
-            all &= spans[i].x <= lo && spans[i].y > hi;
+            const long long key = (long long)tile * KT + i * 32 + lane;
+            const bool there = key < kr.keys, cached = key < rq.cached;
+            any |= there && (cached || (spans[i].x <= hi && spans[i].y > lo));
+            all &= there && (cached || (spans[i].x <= lo && spans[i].y > hi));
           }
           if (tile + 1 < last) ask(tile + 1);
           any = __any_sync(0xffffffffu, any) && hi >= 0;
@@ -224,7 +223,7 @@ struct TcBlock {
       };
       for (int first = j;; ++j) {                            // K runs a tile ahead of V
         const int key = tile * KT + lane * box;
-        const int row = page >= 0 && page < t.c.num_pages ? (page * 2 * t.c.num_kv_heads + pc.h) * t.c.page_size + key % t.c.page_size : no_row;
+        const int row = lane < boxes && key < kr.keys && page >= 0 && page < t.c.num_pages ? (page * 2 * t.c.num_kv_heads + pc.h) * t.c.page_size + key % t.c.page_size : no_row;
         const uint32_t there = __ballot_sync(0xffffffffu, row != no_row);
         if (lane < boxes && row == no_row && key < kr.keys) cache_report(t.c, CACHE_BAD_PAGE);
         int rows[4];
