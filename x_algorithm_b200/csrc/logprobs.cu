@@ -217,6 +217,14 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
+  // the first given id of this thread and its logit, on their way under the row
+  long long given_id = -1;
+  float given_x = 0.f;
+  if (a.given_out && rank == 0 && tid < a.num_given) {
+    given_id = a.given[(long long)r * a.num_given + tid];
+    if (given_id >= 0 && given_id < a.vocab) given_x = Words<T>::at(row, given_id);
+  }
+
   Stat st = {-INFINITY, 0.f, 0.f};
   const bool want_top = a.top_k > 0 && (a.top_out || a.top_ids_out), exactly = NT == 32 && a.top_k > 24;
   u64 bound = ~0ull;              // of words
@@ -412,7 +420,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
     int notes = mem.count;
     G::sync();
     lost |= notes > KEEP;
-    if (!lost && notes > 2 * a.top_k) {
+    if (!lost && notes > max(2 * a.top_k, NT / 4)) {         // (a bound takes as long as reading so many words at once)
       const u64 closer = tighten(mem.keep, notes);
       bound = closer > bound ? closer : bound;
       notes = mem.count;
@@ -461,7 +469,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
     G::sync();
     n = mem.count;
     G::sync();
-    if (n > a.top_k + a.top_k / 2) {
+    if (n > 64 + 2 * a.top_k) {                              // (or as counting over so many keys)
       tighten(single, n);
       n = mem.count;
     }
@@ -503,8 +511,8 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
   if (a.entropy_out && tid == 0) a.entropy_out[r] = st.z == 0.f ? 0.f : logz - st.s / st.z / a.temperature;
   if (a.given_out)
     for (int i = tid; i < a.num_given; i += NT) {
-      const long long id = a.given[(long long)r * a.num_given + i];
-      a.given_out[(long long)r * a.num_given + i] = id < 0 || id >= a.vocab ? 0.f : logp(Words<T>::at(row, id));
+      const long long id = i == tid ? given_id : a.given[(long long)r * a.num_given + i];
+      a.given_out[(long long)r * a.num_given + i] = id < 0 || id >= a.vocab ? 0.f : logp(i == tid ? given_x : Words<T>::at(row, id));
     }
   for (int i = tid; i < n; i += NT) {
     const u64 key = single[i];

@@ -70,32 +70,48 @@ def _keep(device: int, stream: int) -> _Kept:
 
 def _need(t, name: str, dtype, shape, device):
     """`t` is a contiguous tensor of this type and shape on this device."""
-    if type(t) is torch.Tensor or isinstance(t, torch.Tensor):
+    try:
         if t.dtype is dtype and t.get_device() == device and t.shape == shape and t.is_contiguous():
             return t.data_ptr()
+    except AttributeError:
+        pass
     raise ValueError(f"{name} must be a contiguous {list(shape)} {dtype} tensor on cuda:{device}")
 
 
 def _rows(t, name: str, dtype, ndim: int):
     """The device of `t`, a CUDA tensor of this type and rank whose last dimension is dense."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != ndim or not t.is_cuda:
-        raise ValueError(f"{name} must be a {ndim}-dimensional {dtype} tensor on a CUDA device")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name} must be dense in its last dimension")
-    return t.get_device()
+    try:
+        if t.dtype is dtype and t.is_cuda:
+            shape, stride = t.shape, t.stride()
+            if len(shape) == ndim:
+                if stride[-1] == 1 or shape[-1] < 2:
+                    return t.get_device()
+                raise ValueError(f"{name} must be dense in its last dimension")
+    except AttributeError:
+        pass
+    raise ValueError(f"{name} must be a {ndim}-dimensional {dtype} tensor on a CUDA device")
 
 
 def _batch(block, pages, q_start, lengths, block_table, tokens: int, device: int, kept: _Kept):
     """Fills the cache's block; (kv heads, page size, head dim, table columns)."""
-    if _rows(pages, "pages", _BF16, 5) != device or _rows(block_table, "block_table", _I32, 2) != device:
-        raise ValueError(f"pages and block_table must be on cuda:{device}")
-    num_pages, two, kv_heads, page_size, dh = pages.shape
-    if two != 2 or not pages.is_contiguous():
+    try:
+        num_pages, two, kv_heads, page_size, dh = pages.shape
+        batch, cols = block_table.shape
+        good = (pages.dtype is _BF16 and pages.get_device() == device and pages.is_contiguous() and two == 2 and
+                block_table.dtype is _I32 and block_table.get_device() == device and (cols < 2 or block_table.stride(1) == 1) and
+                q_start.dtype is _I32 and q_start.get_device() == device and q_start.shape == (batch + 1,) and q_start.is_contiguous() and
+                lengths.dtype is _I32 and lengths.get_device() == device and lengths.shape == (batch,) and lengths.is_contiguous())
+    except (AttributeError, ValueError, TypeError):
+        good = False
+    if not good:                                             # say which
+        if _rows(pages, "pages", _BF16, 5) != device or _rows(block_table, "block_table", _I32, 2) != device:
+            raise ValueError(f"pages and block_table must be on cuda:{device}")
+        _need(q_start, "q_start", _I32, (block_table.shape[0] + 1,), device)
+        _need(lengths, "lengths", _I32, (block_table.shape[0],), device)
         raise ValueError("pages must be a contiguous [pages, 2, kv heads, page size, head dim] tensor")
-    batch, cols = block_table.shape
     stride = block_table.stride(0)
-    _BATCH(block, 0, pages.data_ptr(), num_pages, _need(q_start, "q_start", _I32, (batch + 1,), device), _need(lengths, "lengths", _I32, (batch,), device),
-           block_table.data_ptr(), stride if stride > cols else cols, kept.status_ptr, cols, page_size, kv_heads, dh, batch, tokens)
+    _BATCH(block, 0, pages.data_ptr(), num_pages, q_start.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), stride if stride > cols else cols,
+           kept.status_ptr, cols, page_size, kv_heads, dh, batch, tokens)
     return kv_heads, page_size, dh, cols
 
 
