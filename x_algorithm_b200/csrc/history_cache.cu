@@ -10,6 +10,7 @@
 // warp takes four rounds that follow one another, of the queries or of keys and values, with all loads in flight before the first is used.  So gains, cosines and
 // sines are the same for all heads until the token changes, and are multiplied into four factors once, x' = (x A - y B) / rms, y' = (y C + x D) / rms, and
 // only the warps of keys and values look up their token's place in the cache - the request by a 32-way search in q_start, its length, the page.
+// Measured: 31 k tokens' rows of 32 + 8 + 8 heads of 128 with norms 147 us = 5.4 TB/s, 16384 tokens of 8 + 8 + 8 heads of 64 25 us = 4.0 TB/s, one token 3.0 us.
 #include <string>
 
 #include "cache_batch.cuh"

@@ -20,8 +20,8 @@
 // distinct, so ties need no care and the result does not depend on the order of the atomics.  More ids than lanes give a bound for (over 24) of
 // a row that a warp has for itself are found exactly: the row's images in registers, their top_k-th largest by halving.
 //
-// Measured: 2048 rows of 100003 bf16 logits 85 us = 4.8 TB/s without best ids, 118 with eight, 152 and 183 capped; 1024 rows of 100004 fp32 71 us = 5.8 TB/s and 85;
-// one row of 131072 fp32, best 20, 12.3 us on eight blocks.  A block's selection, a dozen barriers behind its last word, is what the eight cost.
+// Measured: 2048 rows of 100003 bf16 logits 85 us = 4.8 TB/s without best ids, 118 with eight, 151 and 183 capped; 1024 rows of 100004 fp32 72 us = 5.6 TB/s and 88;
+// one row of 131072 fp32, best 20, 12.2 us on eight blocks.  The selection behind a row's last word is what the eight cost.
 #include <math.h>
 #include <string.h>
 

@@ -11,9 +11,9 @@
 // output; they are joined once at the end.  Masked logits
 // become -inf before the maximum; a value row that some of the tile's rows do not see must not reach them as 0 * NaN either, so tiles that are
 // not seen whole are searched for infinities and NaN, which are then added to the rows that do see them, one by one.
-// Bound by memory: 16 padded rows cost the tensor pipe 4 of the 22 cycles that a key of 128 columns takes from HBM.  Two stages a warp and three blocks an
-// SM: 96 single tokens over up to 4096 keys, 4 key heads of 128 (382 MB), take 75 us = 5.1 TB/s, 139 us = 5.8 TB/s where all have 4096; three stages and two blocks took 90
-// for the first, 32 keys a warp copied by cp.async 139.
+// Bound by memory: 16 operations a byte of the cache, padded rows counted.  96 single tokens over up to 4096 keys, 4 key heads of 128 (382 MB), take 75 us = 5.1 TB/s, 138 us =
+// 5.8 TB/s where all have 4096.  Two stages a warp and three blocks an SM against three and two: 75 / 78 us for the first, 138 / 137 for the second, 89 / 104 for
+// 400 tokens over up to 1000 keys.
 #include <math.h>
 
 #include <string>
@@ -517,14 +517,15 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   t.rows = ROWS; t.keys = KEYS * TREE_WARPS; t.setup = 2;
   if (tc) tree_tc_shape(t);
   const int per_sm = tc ? tree_tc_blocks_per_sm() : t.c.key_size == 128 ? mma_blocks<128>() : mma_blocks<64>();
-  // Blocks share the tiles of all units where there are few units for them and long ones among them.  Measured on the tensor cores (us, shared / whole): 2 to 4
-  // units a block, 16 tiles each 141 / 110, 64 tiles 350 / 370, 128 tiles 646 / 716: whole ones cost the last round's empty blocks, shared ones about 24 tiles for parts and
-  // their join.  Up to two a block they are shared all the same: lengths are seldom equal.
+  // Blocks share the tiles of all units where there are few units for them and long ones among them.  Measured on the tensor cores (us, shared / whole): 2 to 3
+  // units a block, heads of 128, with 0.4 of the last round's blocks empty and 16, 64, 128 tiles a unit 108 / 87, 285 / 273, 523 / 523; with 0.84 empty 97 / 82, 245 / 253,
+  // 443 / 482; with none 104 / 94, 307 / 299, 575 / 564.  Whole ones cost the empty blocks, shared ones about 48 tiles for parts and their join.  Up to
+  // two a block they are shared all the same: lengths are seldom equal.
   const long long units = (long long)t.c.batch * t.c.num_kv_heads * (((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows);
   const long long tiles = (t.a.max_keys + t.keys - 1) / t.keys;
   const long long blocks = per_sm * device_sms(), fed = units * (tiles + t.setup) / (tc ? 8 : 4);   // no block for fewer places: parts and joins take longer than that many
   const long long idle = (units + blocks - 1) / blocks * blocks - units;                  // blocks without a unit in the last round of whole ones
-  const bool few = tc ? tiles >= 8 && (units < 2 * blocks || idle * tiles > 24 * blocks) : tiles >= 4 && units < 8 * blocks;
+  const bool few = tc ? tiles >= 8 && (units < 2 * blocks || idle * tiles > 48 * blocks) : tiles >= 4 && units < 8 * blocks;
   t.split = few && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)(fed < blocks ? fed : blocks) : 0;
   t.turns = tc && !t.split && units > blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)blocks : 0;
   if (part_bytes(t.split, t.rows, t.c.key_size) > t.a.workspace_bytes) return bad("workspace is smaller than phx_tree_workspace_bytes");

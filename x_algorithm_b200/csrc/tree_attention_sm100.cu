@@ -12,9 +12,9 @@
 // seen, some, or all of them by all rows), and only tiles of the second kind are masked.  Those are searched for infinities and NaN among the values as well, which
 // 0 * V would spread to rows that do not see them: they are taken out of shared memory and added to the rows that do at the end.
 // Waits are bounded; when one runs out the flag is raised, every later wait of any role fails at once, and a role whose wait failed is done.
-// Measured: 8192 tokens that see themselves, 16 heads of 128, 502 us = 1095 TFLOP/s (bound by a tile's chain of load, maximum, exponentials and store, 1800
-// cycles of two blocks in turns, and by the special-function unit, 1024 of them); 24 trees of 32 over up to 8192 keys, 32 heads of 128 (465 MB), 101 us = 4.6 TB/s,
-// with capped logits 112; 74 such trees over 8192 keys each 400 us = 6.3 TB/s.
+// Measured: 8192 tokens that see themselves, 16 heads of 128, 506 us = 1086 TFLOP/s (bound by a tile's chain of load, maximum, exponentials and store, 1800
+// cycles of two blocks in turns, and by the special-function unit, 1024 of them); 24 trees of 32 over up to 8192 keys, 32 heads of 128 (465 MB), 100 us = 4.6 TB/s,
+// with capped logits 112; 74 such trees over 8192 keys each 405 us = 6.2 TB/s.
 #include <string.h>
 
 #include "sm100_ptx.cuh"
@@ -138,7 +138,7 @@ struct TcBlock {
   // ---- TMA producer (a whole warp; one lane issues) ----------------------------------------------------------------------
   // Its chain of instructions for a tile has to be shorter than the tile's softmax, beside whose warps it issues: pages and spans are asked for a tile
   // ahead, by loads without a condition (a value chosen between a load and a constant waits for the load), and places in pages are counted on, not divided.
-  // (8192 tokens that see themselves, 16 heads of 128: 716 us before the first, 577 before the second.)
+  // (8192 tokens that see themselves, 16 heads of 128: 716 us before the first, 577 before the second, 502 then.)
   __device__ __forceinline__ void produce(PieceWalk<DH> walk) {
     const int lane = threadIdx.x & 31, boxes = KT / box, page_size = t.c.page_size, v_off = t.c.num_kv_heads * page_size, page_rows = 2 * v_off;
     const int no_row = (int)(t.c.num_pages * page_rows), tokens_per_tile = t.rows / t.group, cols_on = KT / page_size, slots_on = KT % page_size;
