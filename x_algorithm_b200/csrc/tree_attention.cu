@@ -519,13 +519,14 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   const int per_sm = tc ? tree_tc_blocks_per_sm() : t.c.key_size == 128 ? mma_blocks<128>() : mma_blocks<64>();
   // Blocks share the tiles of all units where there are few units for them and long ones among them.  Measured on the tensor cores (us, shared / whole): 2 to 3
   // units a block, heads of 128, with 0.4 of the last round's blocks empty and 16, 64, 128 tiles a unit 108 / 87, 285 / 273, 523 / 523; with 0.84 empty 97 / 82, 245 / 253,
-  // 443 / 482; with none 104 / 94, 307 / 299, 575 / 564.  Whole ones cost the empty blocks, shared ones about 48 tiles for parts and their join.  Up to
-  // two a block they are shared all the same: lengths are seldom equal.
+  // 443 / 482; with none 104 / 94, 307 / 299, 575 / 564.  Heads of 64, 0.4 empty: 81 / 64, 193 / 196, 356 / 377;
+  // 0.84 empty and 32, 64, 128 tiles: 102 / 98, 166 / 177, 299 / 340.  Whole ones cost the empty blocks; shared ones the parts and their join, as wide as a head:
+  // about 48 tiles for 128, 24 for 64.  Up to two a block they are shared all the same: lengths are seldom equal.
   const long long units = (long long)t.c.batch * t.c.num_kv_heads * (((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows);
   const long long tiles = (t.a.max_keys + t.keys - 1) / t.keys;
   const long long blocks = per_sm * device_sms(), fed = units * (tiles + t.setup) / (tc ? 8 : 4);   // no block for fewer places: parts and joins take longer than that many
   const long long idle = (units + blocks - 1) / blocks * blocks - units;                  // blocks without a unit in the last round of whole ones
-  const bool few = tc ? tiles >= 8 && (units < 2 * blocks || idle * tiles > 48 * blocks) : tiles >= 4 && units < 8 * blocks;
+  const bool few = tc ? tiles >= 8 && (units < 2 * blocks || idle * tiles > 3 * t.c.key_size / 8 * blocks) : tiles >= 4 && units < 8 * blocks;
   t.split = few && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)(fed < blocks ? fed : blocks) : 0;
   t.turns = tc && !t.split && units > blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)blocks : 0;
   if (part_bytes(t.split, t.rows, t.c.key_size) > t.a.workspace_bytes) return bad("workspace is smaller than phx_tree_workspace_bytes");
