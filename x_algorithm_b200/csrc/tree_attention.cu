@@ -528,6 +528,7 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   const long long idle = (units + blocks - 1) / blocks * blocks - units;                  // blocks without a unit in the last round of whole ones
   const bool few = tc ? tiles >= 8 && (units < 2 * blocks || idle * tiles > 3 * t.c.key_size / 8 * blocks) : tiles >= 4 && units < 8 * blocks;
   t.split = few && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)(fed < blocks ? fed : blocks) : 0;
+  if (t.split < 2) t.split = 0;                                                            // one block takes whole units: there is no bound between blocks, nothing to join
   t.turns = tc && !t.split && units > blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)blocks : 0;
   if (part_bytes(t.split, t.rows, t.c.key_size) > t.a.workspace_bytes) return bad("workspace is smaller than phx_tree_workspace_bytes");
   t.part_o = static_cast<float*>(t.a.workspace);
