@@ -19,3 +19,26 @@ def test_one_request_with_one_key_head(heads, dh, page, tokens, keys, hints):
     again = decoding.history_append(qkv, *c.args(), None, num_q_heads=heads)
     assert torch.equal(again, qkv.view(tokens, heads + 2, dh)[:, :heads])
     decoding.check_status()
+
+
+def test_an_error_of_the_runtime_is_not_left_for_the_next_call():
+    """A device that is not there is refused by the runtime; the next call, on one that is, succeeds."""
+    import ctypes as C
+    from x_algorithm_b200 import _lib, decoding
+    torch = _torch()
+    c = Cache([2], [30], 2, 64, 16, seed=1)
+    qkv = torch.randn((2, 8 * 64), device=DEV, generator=c.g).to(torch.bfloat16)
+    x = torch.randn((2, 100), device=DEV, generator=c.g)
+    q = decoding.history_append(qkv, *c.args(), None, num_q_heads=4)
+    out, probs = decoding.tree_attention(q, *c.args()), decoding.token_logprobs(x, top_k=3)
+    mine, stream, bits = decoding._structs, torch.cuda.current_stream().cuda_stream, C.c_int32()
+    status = decoding._kept[(0, stream)].status.data_ptr()
+    none = 10 ** 6
+    for f, a in ((_lib.lib.phx_history_append_device, (mine.batch_ref, mine.append_ref)), (_lib.lib.phx_tree_attention_device, (mine.batch_ref, mine.tree_ref)),
+                 (_lib.lib.phx_token_logprobs_device, (mine.logprobs_ref,)), (_lib.lib.phx_decode_status, (status, stream, C.byref(bits)))):
+        assert f(none, *a, *(() if f is _lib.lib.phx_decode_status else (stream,))) == 2   # PHX_E_CUDA
+        assert torch.equal(decoding.history_append(qkv, *c.args(), None, num_q_heads=4), q)
+    assert _lib.lib.phx_tree_workspace_bytes(none, C.byref(C.c_int64())) == 2
+    assert torch.equal(decoding.tree_attention(q, *c.args()), out)
+    assert all(torch.equal(a, b) for a, b in zip(decoding.token_logprobs(x, top_k=3)[1:], probs[1:]))
+    decoding.check_status()

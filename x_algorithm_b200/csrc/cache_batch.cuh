@@ -44,11 +44,17 @@ inline const char* cache_check(const phx_cache_batch* c) {
 }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// `e`; a failure is the entry point's answer, so it is taken back as the runtime's last error, which the next launch would report as its own
+inline cudaError_t taken_back(cudaError_t e) {
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e;
+}
+
 // makes `device` current for the calls of one entry point and puts the caller's back
 class DeviceScope {
  public:
   explicit DeviceScope(int device) {
-    ok_ = cudaGetDevice(&before_) == cudaSuccess && (before_ == device || cudaSetDevice(device) == cudaSuccess);
+    ok_ = taken_back(cudaGetDevice(&before_)) == cudaSuccess && (before_ == device || taken_back(cudaSetDevice(device)) == cudaSuccess);
     changed_ = ok_ && before_ != device;
   }
   ~DeviceScope() { if (changed_) cudaSetDevice(before_); }

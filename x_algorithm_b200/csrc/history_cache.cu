@@ -221,7 +221,7 @@ extern "C" phx_status phx_history_append_device(int32_t device, const phx_cache_
   DeviceScope scope(device);
   if (!scope.ok()) { set_global_error("phx_history_append_device: cudaSetDevice failed"); return PHX_E_CUDA; }
   cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = c.key_size == 32 ? append_launch<32>(c, a, st) : c.key_size == 64 ? append_launch<64>(c, a, st) : append_launch<128>(c, a, st);
+  const cudaError_t e = taken_back(c.key_size == 32 ? append_launch<32>(c, a, st) : c.key_size == 64 ? append_launch<64>(c, a, st) : append_launch<128>(c, a, st));
   if (e != cudaSuccess) { set_global_error(std::string("phx_history_append_device: ") + cudaGetErrorString(e)); return PHX_E_CUDA; }
   dispatch_note(DK_HISTORY_APPEND);
   return PHX_OK;
@@ -241,7 +241,7 @@ extern "C" phx_status phx_decode_status(int32_t device, int32_t* status_dev, voi
     e = cudaMemsetAsync(status_dev, 0, 4, st);
     if (e == cudaSuccess) e = cudaMemsetAsync(status_dev + 2, 0, 4, st);
   }
-  if (e != cudaSuccess) return fail(cudaGetErrorString(e), PHX_E_CUDA);
+  if (taken_back(e) != cudaSuccess) return fail(cudaGetErrorString(e), PHX_E_CUDA);
   *bits_out = now[2];
   if (now[0] != 0) return fail("a bounded wait ran out", PHX_E_TIMEOUT);
   if (now[2] != 0) {

@@ -608,8 +608,8 @@ extern "C" phx_status phx_token_logprobs_device(int32_t device, const phx_logpro
   DeviceScope scope(device);
   if (!scope.ok()) { set_global_error("phx_token_logprobs_device: cudaSetDevice failed"); return PHX_E_CUDA; }
   cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = a.is_bf16 ? (a.cap > 0.f ? logprobs_dispatch<bf16, true>(a, st) : logprobs_dispatch<bf16, false>(a, st))
-                                  : (a.cap > 0.f ? logprobs_dispatch<float, true>(a, st) : logprobs_dispatch<float, false>(a, st));
+  const cudaError_t e = taken_back(a.is_bf16 ? (a.cap > 0.f ? logprobs_dispatch<bf16, true>(a, st) : logprobs_dispatch<bf16, false>(a, st))
+                                             : (a.cap > 0.f ? logprobs_dispatch<float, true>(a, st) : logprobs_dispatch<float, false>(a, st)));
   if (e != cudaSuccess) { set_global_error(std::string("phx_token_logprobs_device: ") + cudaGetErrorString(e)); return PHX_E_CUDA; }
   dispatch_note(DK_TOKEN_LOGPROBS);
   return PHX_OK;

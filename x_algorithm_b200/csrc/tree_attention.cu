@@ -546,7 +546,10 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
                                                : launch_programmatic(tree_join_kernel<128>, grid, block, 0, st, t);
     if (e != cudaSuccess) { err = cudaGetErrorString(e); s = PHX_E_CUDA; }
   }
-  if (s != PHX_OK) set_global_error("phx_tree_attention_device: " + err);
+  if (s != PHX_OK) {
+    (void)cudaGetLastError();
+    set_global_error("phx_tree_attention_device: " + err);
+  }
   return s;
 }
 
