@@ -111,3 +111,23 @@ def test_entry_points_refuse_wrong_arguments():
         assert f(0, None, None, None) == 1 and f(0, C.byref(c), None, None) == 1
     assert _lib.lib.phx_token_logprobs_device(0, None, None) == 1
     assert _lib.lib.phx_decode_status(0, None, None, None) == 1 and _lib.lib.phx_tree_workspace_bytes(0, None) == 1
+
+
+def test_the_rows_of_a_block_table_keep_their_distance():
+    """A table that is broadcast over requests reaches the entry point with its stride of 0, which refuses it; one row has no distance to a next."""
+    import torch
+    from types import SimpleNamespace as Fake
+    from x_algorithm_b200 import decoding
+
+    def on_gpu(t):
+        return Fake(shape=t.shape, dtype=t.dtype, stride=t.stride, is_contiguous=t.is_contiguous, get_device=lambda: 0, data_ptr=lambda: 16)
+
+    pages = on_gpu(torch.zeros((4, 2, 2, 16, 64), dtype=torch.bfloat16))
+    kept, flat = Fake(status_ptr=16), torch.zeros(40, dtype=torch.int32)
+    for table, stride in ((flat.view(4, 10), 10), (flat[:10].expand(4, 10), 0), (flat.as_strided((4, 10), (3, 1)), 3), (flat.as_strided((4, 5), (10, 1)), 10), (flat.as_strided((1, 10), (1, 1)), 10)):
+        n, mine = table.shape[0], decoding._Structs()
+        decoding._batch(mine.batch, pages, on_gpu(torch.zeros(n + 1, dtype=torch.int32)), on_gpu(torch.zeros(n, dtype=torch.int32)), on_gpu(table), n, 0, kept)
+        assert mine.batch.table_stride == stride and mine.batch.table_cols == table.shape[1]
+        if stride < table.shape[1]:
+            a = _lib.AppendArgs(16, 512, 16, None, None, None, None, 16, 4, 0, 1e-6, 0)
+            assert _lib.lib.phx_history_append_device(0, mine.batch_ref, C.byref(a), None) == 1 and b"table_cols apart" in _lib.lib.phx_global_error()

@@ -42,3 +42,20 @@ def test_an_error_of_the_runtime_is_not_left_for_the_next_call():
     assert torch.equal(decoding.tree_attention(q, *c.args()), out)
     assert all(torch.equal(a, b) for a, b in zip(decoding.token_logprobs(x, top_k=3)[1:], probs[1:]))
     decoding.check_status()
+
+
+def test_a_table_that_is_broadcast_over_requests_is_refused():
+    from x_algorithm_b200 import PhoenixError, decoding
+    torch = _torch()
+    c = Cache([1, 1, 1], [20, 20, 20], 2, 64, 16)
+    q = torch.zeros((3, 4, 64), dtype=torch.bfloat16, device=DEV)
+    qkv = torch.zeros((3, 8 * 64), dtype=torch.bfloat16, device=DEV)
+    flat = torch.arange(16, dtype=torch.int32, device=DEV)
+    for table in (c.table[:1].expand(3, -1), flat.as_strided((3, 3), (1, 1))):
+        for f in (lambda: decoding.tree_attention(q, c.pages, c.q_start, c.lengths, table), lambda: decoding.history_append(qkv, c.pages, c.q_start, c.lengths, table, None, num_q_heads=4)):
+            with pytest.raises((ValueError, PhoenixError)):
+                f()
+    one = Cache([1], [20], 2, 64, 16)                            # one row has no distance to a next
+    want = decoding.tree_attention(q[:1], *one.args())
+    assert torch.equal(decoding.tree_attention(q[:1], one.pages, one.q_start, one.lengths, one.table.as_strided(one.table.shape, (1, 1))), want)
+    decoding.check_status()

@@ -109,8 +109,8 @@ def _batch(block, pages, q_start, lengths, block_table, tokens: int, device: int
         _need(q_start, "q_start", _I32, (block_table.shape[0] + 1,), device)
         _need(lengths, "lengths", _I32, (block_table.shape[0],), device)
         raise ValueError("pages must be a contiguous [pages, 2, kv heads, page size, head dim] tensor")
-    stride = block_table.stride(0)
-    _BATCH(block, 0, pages.data_ptr(), num_pages, q_start.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), stride if stride > cols else cols,
+    # one row has no distance to a next, whatever its stride says; rows that overlap (a table broadcast over requests) are refused below
+    _BATCH(block, 0, pages.data_ptr(), num_pages, q_start.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), block_table.stride(0) if batch > 1 else cols,
            kept.status_ptr, cols, page_size, kv_heads, dh, batch, tokens)
     return kv_heads, page_size, dh, cols
 
