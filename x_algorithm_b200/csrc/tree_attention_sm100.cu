@@ -238,11 +238,11 @@ struct TcBlock {
         __syncwarp();
         if (elect_one()) {
           const int b = j % NB;
-          mbar_expect_tx(smem_u32(&sm.k_full[b]), BLK);
           TileNote n;
           n.tile = tile;
           n.flags = there | (masked || there != (1u << boxes) - 1 ? MASKED : 0u) | (follows >= last ? LAST | (more ? 0u : FINAL) : 0u);
-          sm.note[j & 7] = n;
+          sm.note[j & 7] = n;                              // in front of the arrival, which publishes it
+          mbar_expect_tx(smem_u32(&sm.k_full[b]), BLK);
 #pragma unroll
           for (int p = 0; p < 4; ++p)
             if (p < boxes)
