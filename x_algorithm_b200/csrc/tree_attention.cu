@@ -264,6 +264,7 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
             }
             asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
           }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // a later tile is copied over these stores
           __syncwarp();
         }
       }
