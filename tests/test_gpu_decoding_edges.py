@@ -1,7 +1,9 @@
 """Calls at the edges of the operators on a cached history.  Oracles and tolerances are test_gpu_decoding's unless a test says its own."""
+import math
+
 import pytest
 
-from test_gpu_decoding import DEV, Cache, _torch, _tree_case
+from test_gpu_decoding import DEV, Cache, _logprobs_check, _torch, _tree_case
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +61,26 @@ def test_a_table_that_is_broadcast_over_requests_is_refused():
     want = decoding.tree_attention(q[:1], *one.args())
     assert torch.equal(decoding.tree_attention(q[:1], one.pages, one.q_start, one.lengths, one.table.as_strided(one.table.shape, (1, 1))), want)
     decoding.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,vocab", [(6, 300), (6, 1001), (6, 5000), (600, 9001), (1, 66000), (6, 131072)])
+def test_token_logprobs_of_a_types_highest_value(dtype, rows, vocab):
+    """An id that is forced by the largest number of the type, among ordinary, banned and lowest ones: all finite but what fp32 does not hold."""
+    torch = _torch()
+    t = getattr(torch, dtype)
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    x = torch.randn((rows, vocab), device=DEV, generator=g).to(t)
+    high = torch.finfo(t).max
+    x[0, vocab // 2] = high
+    if rows > 1:
+        x[1, torch.rand(vocab, device=DEV, generator=g) < 0.5] = -math.inf
+        x[1, vocab - 1] = high
+        x[2, :] = high                                          # all of them
+        x[3, :] = -math.inf
+        x[3, 1] = high
+        x[4, 0] = 2.5e38
+        x[5, 0], x[5, vocab - 1], x[5, 3] = 1.2e38, -1.2e38, -math.inf
+    given = torch.tensor([[0, vocab // 2, vocab - 1]] * rows, device=DEV)
+    for temperature in (1.0, 0.5, 2.0):
+        _logprobs_check(x, given, min(vocab, 9), temperature=temperature)

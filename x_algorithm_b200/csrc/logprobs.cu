@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
         }
       }
       if (!one_by_one) {
-        // what lies below FLOOR weighs nothing; raised to it, it has a finite distance from the reference
+        // a distance below FLOOR weighs nothing; raised to it, it is finite (-inf has one too, and so has the lowest logit under the highest reference)
         float2 z2 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);
         const float2 m2 = make_float2(-st.m, -st.m), c2 = make_float2(scale, scale);
 #pragma unroll
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
 #pragma unroll
           for (int k = 0; k < N; k += 2) {
             const float y0 = CAP ? (x[k] == -INFINITY ? x[k] : cap.small(x[k])) : x[k], y1 = CAP ? (x[k + 1] == -INFINITY ? x[k + 1] : cap.small(x[k + 1])) : x[k + 1];
-            const float2 d = __fadd2_rn(make_float2(max_nan(y0, FLOOR), max_nan(y1, FLOOR)), m2);
+            const float2 far = __fadd2_rn(make_float2(y0, y1), m2), d = make_float2(max_nan(far.x, FLOOR), max_nan(far.y, FLOOR));
             const float2 t = __fmul2_rn(d, c2);
             const float2 e = make_float2(ex2(t.x), ex2(t.y));
             z2 = __fadd2_rn(z2, e);
