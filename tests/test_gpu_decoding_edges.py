@@ -84,3 +84,13 @@ def test_token_logprobs_of_a_types_highest_value(dtype, rows, vocab):
     given = torch.tensor([[0, vocab // 2, vocab - 1]] * rows, device=DEV)
     for temperature in (1.0, 0.5, 2.0):
         _logprobs_check(x, given, min(vocab, 9), temperature=temperature)
+
+
+@pytest.mark.parametrize("vocab", [300, 5000, 66000])
+def test_banned_ids_weigh_nothing_at_any_temperature(vocab):
+    torch = _torch()
+    x = torch.zeros((2, vocab), device=DEV)
+    x[:, ::2] = -math.inf
+    x[1, 1] = 3.0
+    for temperature in (1e-6, 1e30, 1e37, 3e38):
+        _logprobs_check(x, torch.tensor([[0, 1, 3]] * 2, device=DEV), 5, temperature=float(torch.tensor(temperature, dtype=torch.float32)))

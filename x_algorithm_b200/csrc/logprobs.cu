@@ -202,6 +202,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
   const int tid = G::tid(), lane = threadIdx.x & 31, warp = tid >> 5;
   const T* const row = static_cast<const T*>(a.logits) + (long long)r * a.stride;
   const float scale = LOG2E / a.temperature;
+  const bool flat = FLOOR * scale > -150.0f;                // a temperature (above 1e36) at which a distance of FLOOR would weigh something
   const Cap cap(CAP ? a.cap : 1.0f);
 
   // 16-byte words of the row, the first and last of them perhaps in part
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
         const Stat none = {ctop, 0.f, 0.f};
         st = join(st, none, scale);
       }
-      bool one_by_one = !(st.m > DEEP);         // all logits so far are at a type's lowest values, or NaN
+      bool one_by_one = !(st.m > DEEP) || flat; // all logits so far are at a type's lowest values, or NaN
       if (CAP && !one_by_one) {                 // or some, that are allowed, are not small against the cap
         one_by_one = !(top <= cap.most);
         float low = INFINITY;
