@@ -3,7 +3,7 @@ import math
 
 import pytest
 
-from test_gpu_decoding import DEV, Cache, _logprobs_check, _torch, _tree_case
+from test_gpu_decoding import DEV, Cache, _logprobs_check, _logprobs_want, _torch, _tree_case
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +94,27 @@ def test_banned_ids_weigh_nothing_at_any_temperature(vocab):
     x[1, 1] = 3.0
     for temperature in (1e-6, 1e30, 1e37, 3e38):
         _logprobs_check(x, torch.tensor([[0, 1, 3]] * 2, device=DEV), 5, temperature=float(torch.tensor(temperature, dtype=torch.float32)))
+
+
+@pytest.mark.parametrize("dtype,vocab", [("float32", 100003), ("bfloat16", 100003), ("float32", 1024), ("bfloat16", 1000), ("float32", 300000)])
+@pytest.mark.parametrize("late", [False, True])
+def test_token_logprobs_of_peaked_rows(dtype, vocab, late):
+    """The best id 8.5 above all others, early and late in the row.  With the row's maximum as the reference its own exponential is 1, and log p = -ln Z, Z = 1 + r
+    with r at most about 0.5.  Roundings after the 1 has been added, taken as independent, of a half ulp (2^-24) at most and so 2^-24 / sqrt(3) in the mean square: 16 within a
+    batch, 74 batches at most (300000 in a cluster of blocks: fewer), 10 in the joins, 2 behind the logarithm: sqrt(102) 2^-24 / sqrt(3) = 3.5e-7, but a 1 that has equal chances to stand
+    anywhere sees half of them, 2.5e-7; the exponentials' own 2^-22 on r adds 1e-7 if all were off the same way.  Root mean square at most 3.2e-7."""
+    from x_algorithm_b200 import decoding
+    torch = _torch()
+    rows = 64 if vocab > 2000 else 512
+    t = getattr(torch, dtype)
+    g = torch.Generator(device=DEV).manual_seed(vocab + late)
+    x = torch.randn((rows, vocab), device=DEV, generator=g).to(t)
+    at = torch.randint(0, vocab // 4, (rows,), device=DEV, generator=g)
+    at = vocab - 1 - at if late else at % 32
+    best = (x.float().amax(1) + 8.5).to(t)
+    x[torch.arange(rows, device=DEV), at] = best
+    lp, _, top, ids = decoding.token_logprobs(x, at, top_k=1)
+    assert torch.equal(ids[:, 0], at) and torch.equal(lp, top[:, 0])
+    want = _logprobs_want(x, 0.0, 1.0)[0].gather(1, at[:, None])[:, 0]
+    off = (lp.double() - want).square().mean().sqrt().item()
+    assert off <= 3.2e-7, off

@@ -7,8 +7,9 @@
 //
 // One pass over the logits, bound by memory.  A row belongs to a warp, to a block, or to a cluster of blocks that each take a
 // stretch of it.  A thread fetches its own 16-byte words, cp.async into a ring of its own in shared memory (no barriers), takes a few
-// of them at a time, and keeps a reference, the sum of e^t and the sum of e^t t against it.  The reference is the maximum of the warp's first batch and moves only
-// when the exponentials could outgrow fp32: a running maximum moved in some lane of a warp at almost every batch, a third of the instructions.
+// of them at a time, and keeps a reference, the sum of e^t and the sum of e^t t against it.  The reference is the running maximum of the warp: the best id's
+// own exponential is 1 at the end, and log p near 0 and the entropy keep their bits (a reference that may be 11 below it cost log p 1e-6).  It moves a few times a row; a lane's
+// own maximum moved in some lane of a warp at almost every batch, a third of the instructions.
 //
 // The best ids are found by words first: a word's key is its largest logit's order-preserving image, then its place, first come first.
 // The top_k-th largest key of any set of words bounds what the row's best ids can be in - a word below it holds nothing that is not
@@ -36,7 +37,6 @@ constexpr int WARP_ROWS = 4;        // rows of a block whose warps take one each
 constexpr int WARP_ROW = 1024;      // the longest of them
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float FLOOR = -1e38f, DEEP = -1e37f;
-constexpr float ROOM = 16.0f;       // powers of two that the exponentials may grow to before the reference moves
 typedef unsigned long long u64;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -334,18 +334,14 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
       }
     }
 
-    if (it == 0) {
-      float first = CAP ? cap.of(top) : top;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) first = max_nan(first, __shfl_xor_sync(0xffffffffu, first, o));
-      st.m = first;
-    }
     const float ctop = CAP ? cap.of(top) : top;
+    if (__any_sync(0xffffffffu, !(ctop <= st.m))) {   // the warp's maximum has grown, or there is a NaN
+      Stat grown = {max_nan(ctop, st.m), 0.f, 0.f};
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) grown.m = max_nan(grown.m, __shfl_xor_sync(0xffffffffu, grown.m, o));
+      st = join(st, grown, scale);
+    }
     if (top != -INFINITY) {
-      if (!((ctop - st.m) * scale <= ROOM)) {   // grown too far, the first that is allowed, or NaN
-        const Stat none = {ctop, 0.f, 0.f};
-        st = join(st, none, scale);
-      }
       bool one_by_one = !(st.m > DEEP) || flat; // all logits so far are at a type's lowest values, or NaN
       if (CAP && !one_by_one) {                 // or some, that are allowed, are not small against the cap
         one_by_one = !(top <= cap.most);
