@@ -118,3 +118,19 @@ def test_token_logprobs_of_peaked_rows(dtype, vocab, late):
     want = _logprobs_want(x, 0.0, 1.0)[0].gather(1, at[:, None])[:, 0]
     off = (lp.double() - want).square().mean().sqrt().item()
     assert off <= 3.2e-7, off
+
+
+@pytest.mark.parametrize("cap", [1e-3, 1e-5, 1e-20, 1e-38, 1e-41])
+@pytest.mark.parametrize("vocab", [300, 5000, 66000])
+def test_token_logprobs_of_very_small_caps(cap, vocab):
+    torch = _torch()
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    x = torch.randn((5, vocab), device=DEV, generator=g)
+    x[1] = 0.0
+    x[2] *= cap
+    x[3, ::3] = 0.0
+    x[4, ::2] = -math.inf
+    given = torch.tensor([[0, 1, vocab - 1]] * 5, device=DEV)
+    cap32 = float(torch.tensor(cap, dtype=torch.float32))
+    for k in (0, 5):
+        _logprobs_check(x, given, k, cap=cap32)

@@ -95,7 +95,8 @@ __device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float scale) 
 // by 1e-7 of the cap, log probabilities near 0 were off by 1e-5 of themselves.
 struct Cap {
   float cap, most, c[6];
-  __device__ __forceinline__ explicit Cap(float limit) : cap(limit), most(0.75f * limit) {
+  // (below 1e-3 the powers of 1 / cap leave fp32: no logit counts as small there)
+  __device__ __forceinline__ explicit Cap(float limit) : cap(limit), most(limit >= 1e-3f ? 0.75f * limit : -1.0f) {
     const float z = 1.0f / limit, z2 = z * z;
     c[0] = 0.999999832f; c[1] = -0.333324709f * z2; c[2] = 0.133205796f * z2 * z2; c[3] = -0.0531492588f * z2 * z2 * z2;
     c[4] = 0.0192372317f * z2 * z2 * z2 * z2; c[5] = -0.0044934523f * z2 * z2 * z2 * z2 * z2;
