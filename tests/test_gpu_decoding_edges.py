@@ -3,7 +3,7 @@ import math
 
 import pytest
 
-from test_gpu_decoding import DEV, Cache, _logprobs_check, _logprobs_want, _torch, _tree_case
+from test_gpu_decoding import DEV, Cache, _attend, _check, _logprobs_check, _logprobs_want, _spans, _torch, _tree_case
 
 pytestmark = pytest.mark.gpu
 
@@ -134,3 +134,20 @@ def test_token_logprobs_of_very_small_caps(cap, vocab):
     cap32 = float(torch.tensor(cap, dtype=torch.float32))
     for k in (0, 5):
         _logprobs_check(x, given, k, cap=cap32)
+
+
+@pytest.mark.parametrize("method", ["tanh", "soft_sign"])
+@pytest.mark.parametrize("cap", [1e-3, 1e-7, 1e-20, 1e-38, 1e-41])
+@pytest.mark.parametrize("heads,kv_heads,dh,tokens", [(4, 4, 32, 3), (16, 4, 128, 3), (16, 4, 128, 50), (8, 8, 64, 40)])
+def test_tree_attention_with_very_small_caps(method, cap, heads, kv_heads, dh, tokens):
+    """Logits that are zero, and others, under a cap that makes them all nearly equal."""
+    from x_algorithm_b200 import decoding
+    torch = _torch()
+    c = Cache([tokens], [200], kv_heads, dh, 16, seed=5)
+    q = torch.randn((c.n, heads, dh), device=DEV, generator=c.g).to(torch.bfloat16)
+    q[0] = 0
+    spans = torch.tensor(_spans("tree", tokens, 1, 1), dtype=torch.int32, device=DEV)
+    cap = float(torch.tensor(cap, dtype=torch.float32))
+    out = decoding.tree_attention(q, *c.args(), spans, cap=cap, cap_method=method)
+    decoding.check_status()
+    _check(out, *_attend(c, q, spans, math.sqrt(128.0) / dh, cap, method))

@@ -47,16 +47,17 @@ __device__ __forceinline__ float tree_ex2(float x) {
 // raw logit with all factors in the coefficients: on the fma pipe, two at a time, where two more special-function operations a logit bound the kernel (24 trees of 32
 // over 8192 keys, 32 heads of 128: 178 us against 136 without a cap, when it was first measured)
 struct TreeCap {
-  static constexpr float SMALL = 0.5f;
+  static constexpr float SMALL = 0.5f, MOST = 3e38f;
   float scale, a, b, small_scale, c[4];
   __device__ __forceinline__ TreeCap(const TreeView& t) {
     const float cap = t.a.cap;
-    scale = t.a.cap_method == 0 ? t.csc : t.a.cap_method == 1 ? t.a.sm_scale : t.a.sm_scale * 2.0f * TREE_LOG2E / cap;
-    a = t.a.cap_method == 1 ? 1.0f / cap : -2.0f * cap * TREE_LOG2E;
+    auto finite = [](float x) { return fmaxf(-MOST, fminf(x, MOST)); };   // 0 times it is 0 under the smallest caps, too
+    scale = t.a.cap_method == 0 ? t.csc : t.a.cap_method == 1 ? t.a.sm_scale : finite(t.a.sm_scale * 2.0f * TREE_LOG2E / cap);
+    a = t.a.cap_method == 1 ? finite(1.0f / cap) : -2.0f * cap * TREE_LOG2E;
     b = cap * TREE_LOG2E;
     const float z = t.a.sm_scale / cap, z2 = z * z;
-    small_scale = fabsf(z);
     c[0] = b * z * 0.999997676f; c[1] = b * z * z2 * -0.333206551f; c[2] = b * z * z2 * z2 * 0.13145145f; c[3] = b * z * z2 * z2 * z2 * -0.0433724655f;
+    small_scale = fabsf(c[3]) <= MOST ? fabsf(z) : INFINITY;              // no logit is small where the coefficients leave fp32
   }
   __device__ __forceinline__ void of_small(float& s0, float& s1) const {
     auto two = [](float x) { return make_float2(x, x); };
