@@ -151,3 +151,37 @@ def test_tree_attention_with_very_small_caps(method, cap, heads, kv_heads, dh, t
     out = decoding.tree_attention(q, *c.args(), spans, cap=cap, cap_method=method)
     decoding.check_status()
     _check(out, *_attend(c, q, spans, math.sqrt(128.0) / dh, cap, method))
+
+
+@pytest.mark.parametrize("method,cap", [("tanh", 5.0), ("tanh", 30.0), ("soft_sign", 5.0)])
+@pytest.mark.parametrize("heads,kv_heads,dh,tokens,cached", [(4, 4, 32, 9, 70), (8, 8, 64, 9, 70), (16, 4, 128, 4, 70), (16, 4, 128, 60, 70), (8, 8, 64, 150, 70), (32, 8, 128, 17, 3000)])
+def test_keys_that_are_not_seen_leave_no_trace_under_a_cap(method, cap, heads, kv_heads, dh, tokens, cached):
+    """Large keys, NaN and infinities of padding tokens, of another branch and behind the last key: the same bits as without them."""
+    from x_algorithm_b200 import decoding
+    torch = _torch()
+    c = Cache([tokens, tokens], [cached, 3], kv_heads, dh, 32, seed=5)
+    q = torch.randn((c.n, heads, dh), device=DEV, generator=c.g).to(torch.bfloat16)
+    spans = torch.tensor(_spans("tree", tokens, 2, 1) + _spans("isolated", tokens, 0), dtype=torch.int32, device=DEV)
+    run = lambda: decoding.tree_attention(q, *c.args(), spans, cap=cap, cap_method=method)  # noqa: E731
+    clean = run()
+    _check(clean, *_attend(c, q, spans, math.sqrt(128.0) / dh, cap, method))
+    for value in (50.0, 1000.0, math.inf, math.nan):
+        for b, (t, k) in enumerate(zip(c.tokens, c.cached)):       # behind the last key
+            c.pages[c.table_host[b][(t + k - 1) // 32], :, :, (t + k - 1) % 32 + 1:] = value
+        for j in (tokens - 2, tokens - 1):                         # the padding tokens of request 0
+            c.pages[c.table_host[0][(cached + j) // 32], :, :, (cached + j) % 32] = value
+        assert torch.equal(run(), clean), value
+    # candidates that see themselves only: what the key of one holds is its own row's
+    at = 3 + tokens // 2
+    c.pages[c.table_host[1][at // 32], 0, :, at % 32] *= 40.0
+    out = run()
+    rest = [i for i in range(c.n) if i != tokens + tokens // 2]
+    assert torch.equal(out[rest], clean[rest]) and not torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("method", ["tanh", "soft_sign"])
+@pytest.mark.parametrize("heads,kv_heads,dh,tokens", [(4, 4, 32, 5), (8, 8, 64, 1), (16, 4, 128, 4), (16, 4, 128, 60), (8, 8, 64, 150)])
+@pytest.mark.parametrize("scale", [0.3, -0.3, 3.0])
+def test_logits_that_reach_their_cap(method, heads, kv_heads, dh, tokens, scale):
+    """Logits of up to several times the cap beside small ones, both signs of the scale."""
+    _tree_case([tokens, 2], [900, 40], heads, kv_heads, dh, 32, "tree", cap=4.0, method=method, seed=7, scale=scale)

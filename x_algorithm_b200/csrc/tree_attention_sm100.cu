@@ -314,6 +314,41 @@ struct TcBlock {
     }
   }
 
+  // The polynomial and the exponential form of tanh differ in their last bits, so a key that a row does not see must not choose between them.  In a masked tile a row
+  // goes by the logits that it sees, 16 keys at a time, in tensor memory and in a loop of its own: beside the code for whole tiles, where a warp takes one form
+  // for all, such choices made that code 3 to 20 % slower (registers).  24 trees of 32 over up to 8192 keys, 32 heads of 128: 106 us, 152 with logits around the cap; 110 and 151 when
+  // masked tiles were capped there by the warp's choice; 32 x 512 candidates under a cap 97 and 132, were 111 and 128.
+  __device__ __forceinline__ void cap_masked(const TreeCap& cap, uint32_t s_col, const int2* span, int pre) const {
+    tmem_ld_wait();
+#pragma unroll 1
+    for (int c = 0; c < KT / 16; ++c) {
+      float x[16];
+      tmem_ld16_nowait(s_col + c * 16, reinterpret_cast<uint32_t*>(x));
+      tmem_ld_wait();
+      uint32_t seen = 0;
+      float most = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int2 sp = span[c * 16 + k];
+        if (sp.x <= pre && pre < sp.y) { seen |= 1u << k; most = fmaxf(most, fabsf(x[k])); }
+      }
+      if (most * cap.small_scale <= TreeCap::SMALL) {
+        if (seen != 0) {
+#pragma unroll
+          for (int k = 0; k < 16; k += 2) cap.of_small(x[k], x[k + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[k] = cap.template of<2>(x[k]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 16; ++k) if (!((seen >> k) & 1)) x[k] = -INFINITY;
+      tmem_st16(s_col + c * 16, reinterpret_cast<uint32_t*>(x));
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+  }
+
   // ---- softmax (128 threads, one a row) ------------------------------------------------------------------------------------
   __device__ __forceinline__ void softmax(PieceWalk<DH> walk) {
     const int lane = threadIdx.x & 31, quad = warp_index() & 3, r = quad * 32 + lane, group = t.group;
@@ -383,10 +418,15 @@ struct TcBlock {
         }
         float alpha = 1.0f;
         if (busy) {
+          if (CAP == 2 && masked) {
+            cap_masked(cap, s_col, sm.span[j & 1], pre);
+#pragma unroll
+            for (int c = 0; c < KT / 32; ++c) tmem_ld32_nowait(s_col + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
+          }
           tmem_ld_wait_on(s);
           tmem_ld_wait_on(s + 32);
           // Four chains of three-input max.  tanh is monotone: without a mask one of the raw maximum serves for the row, and with the raw minimum it says
-          // whether all of the warp's logits are small enough against the cap for its polynomial.
+          // whether all of the warp's logits are small enough against the cap for its polynomial (but a padding token's, whose query has no part in others' rows).
           float bm;
           auto top_of = [&]() {
             float b4[4] = {s[0], s[1], s[2], s[3]};
@@ -397,7 +437,7 @@ struct TcBlock {
             }
             return max3(fmaxf(b4[0], b4[1]), max3(b4[2], b4[3], s[KT - 4]), max3(s[KT - 3], s[KT - 2], s[KT - 1]));   // and the tail that the loop leaves
           };
-          if (CAP == 2) {
+          if (CAP == 2 && !masked) {
             float low[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
             for (int k = 4; k + 7 < KT; k += 8) {
@@ -406,7 +446,7 @@ struct TcBlock {
             }
             float least = min3(fminf(low[0], low[1]), min3(low[2], low[3], s[KT - 4]), min3(s[KT - 3], s[KT - 2], s[KT - 1]));
             bm = top_of();
-            const bool small = __all_sync(0xffffffffu, !valid || fmaxf(fabsf(bm), fabsf(least)) * cap.small_scale <= TreeCap::SMALL);
+            const bool small = __all_sync(0xffffffffu, pre < 0 || fmaxf(fabsf(bm), fabsf(least)) * cap.small_scale <= TreeCap::SMALL);
             if (cap.scale < 0.f) bm = least;                 // a negative scale turns the order round
             if (small) {
               cap.of_small(bm, least);
@@ -417,11 +457,11 @@ struct TcBlock {
 #pragma unroll
               for (int k = 0; k < KT; ++k) s[k] = cap.template of<2>(s[k]);
             }
-          } else if (CAP) {
+          } else if (CAP && CAP != 2) {
 #pragma unroll
             for (int k = 0; k < KT; ++k) s[k] = cap.template of<CAP>(s[k]);
           }
-          if (masked) {
+          if (masked && CAP != 2) {
 #pragma unroll
             for (int k = 0; k < KT; ++k) { const int2 sp = sm.span[j & 1][k]; if (!(sp.x <= pre && pre < sp.y)) s[k] = -INFINITY; }
           }
