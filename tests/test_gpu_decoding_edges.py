@@ -185,3 +185,11 @@ def test_keys_that_are_not_seen_leave_no_trace_under_a_cap(method, cap, heads, k
 def test_logits_that_reach_their_cap(method, heads, kv_heads, dh, tokens, scale):
     """Logits of up to several times the cap beside small ones, both signs of the scale."""
     _tree_case([tokens, 2], [900, 40], heads, kv_heads, dh, 32, "tree", cap=4.0, method=method, seed=7, scale=scale)
+
+
+@pytest.mark.parametrize("method", ["tanh", "soft_sign"])
+@pytest.mark.parametrize("cap", [1e3, 1e5, 1e7, 1e30, 3e38])
+@pytest.mark.parametrize("heads,kv_heads,dh,tokens", [(4, 4, 32, 5), (8, 8, 64, 3), (16, 4, 128, 4), (16, 4, 128, 60), (8, 8, 64, 150)])
+def test_caps_far_above_the_logits(method, cap, heads, kv_heads, dh, tokens):
+    """As good as no cap: the error does not grow with the cap."""
+    _tree_case([tokens, 2], [900, 40], heads, kv_heads, dh, 32, "tree", cap=cap, method=method, seed=11)

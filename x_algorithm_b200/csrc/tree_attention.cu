@@ -29,6 +29,7 @@ constexpr int TREE_WARPS = 4;
 constexpr int ROWS = 16;         // query rows of a tile
 constexpr int KEYS = 16;         // keys of a warp's tile; a page holds whole tiles
 constexpr int STAGES = 2;
+constexpr int WIDE_CAP = 4;      // tanh under a cap so large that 1e-7 of it counts: small logits by the polynomial
 using namespace sm100;
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -170,13 +171,27 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
       const int key0 = tile * KEYS;
       const bool whole = key0 + KEYS <= min(rq.cached, kr.keys) && there;
       uint32_t seen[2] = {0xffu, 0xffu};               // bit 2 n + c: key 8 n + (lane & 3) * 2 + c, for either row
+      if (CAP == WIDE_CAP) {
+        float most = 0.f;
 #pragma unroll
-      for (int n = 0; n < KEYS / 8; ++n)
+        for (int n = 0; n < KEYS / 8; ++n) most = fmaxf(fmaxf(fmaxf(most, fabsf(s[n][0])), fmaxf(fabsf(s[n][1]), fabsf(s[n][2]))), fabsf(s[n][3]));
+        const bool small = __all_sync(0xffffffffu, most * cap.small_scale <= TreeCap::SMALL);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float v = s[n][c];
-          s[n][c] = CAP == 0 ? v * t.csc : cap.of<CAP>(v);
-        }
+        for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            if (small) cap.of_small(s[n][c], s[n][c + 1]);
+            else cap.of_any(s[n][c], s[n][c + 1]);           // the same bits for those that are small
+          }
+      } else {
+#pragma unroll
+        for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float v = s[n][c];
+            s[n][c] = CAP == 0 ? v * t.csc : cap.of<CAP>(v);
+          }
+      }
       if (!whole) {
         seen[0] = seen[1] = 0;
 #pragma unroll
@@ -453,6 +468,9 @@ phx_status tree_mma_launch(const TreeView& t, cudaStream_t stream, std::string& 
 }
 template <int DH>
 phx_status tree_mma_launch(const TreeView& t, cudaStream_t stream, std::string& err) {
+  // Up to 1000 the exponential form's error, 1e-7 of the cap, is far below the bf16 rounding of the probabilities, and it is the faster one here: 76.6 us against 82.1 for 96
+  // single tokens over up to 4096 keys, 103 against 105 (113 with logits around the cap) for prompts of 512 with heads of 32.
+  if (t.a.cap_method == 2 && t.a.cap > 1000.0f) return tree_mma_launch<DH, WIDE_CAP>(t, stream, err);
   return t.a.cap_method == 0 ? tree_mma_launch<DH, 0>(t, stream, err) : t.a.cap_method == 1 ? tree_mma_launch<DH, 1>(t, stream, err) : tree_mma_launch<DH, 2>(t, stream, err);
 }
 

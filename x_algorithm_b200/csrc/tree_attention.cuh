@@ -42,8 +42,8 @@ __device__ __forceinline__ float tree_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// cap(s * scale) in the log2 domain: method 1 s / (1 + |s| / cap), 2 cap tanh(s / cap) as cap (1 - 2 / (e^(2 s / cap) + 1)), good to 1e-7 of the cap
-// tanh also as an odd polynomial for |z| <= SMALL (least maximum error over it, 1.3e-7, found by reweighted least squares on Chebyshev nodes), in the
+// cap(s * scale) in the log2 domain: method 1 s / (1 + |s| / cap), 2 cap tanh(s / cap) as cap (1 - 2 / (e^(2 s / cap) + 1)), good to 1e-7 of the cap: for logits that
+// are not small against it, or under a cap of ordinary size.  Small ones take tanh as an odd polynomial for |z| <= SMALL (least maximum error over it, 1.3e-7, found by reweighted least squares on Chebyshev nodes), in the
 // raw logit with all factors in the coefficients: on the fma pipe, two at a time, where two more special-function operations a logit bound the kernel (24 trees of 32
 // over 8192 keys, 32 heads of 128: 178 us against 136 without a cap, when it was first measured)
 struct TreeCap {
@@ -55,8 +55,8 @@ struct TreeCap {
     scale = t.a.cap_method == 0 ? t.csc : t.a.cap_method == 1 ? t.a.sm_scale : finite(t.a.sm_scale * 2.0f * TREE_LOG2E / cap);
     a = t.a.cap_method == 1 ? finite(1.0f / cap) : -2.0f * cap * TREE_LOG2E;
     b = cap * TREE_LOG2E;
-    const float z = t.a.sm_scale / cap, z2 = z * z;
-    c[0] = b * z * 0.999997676f; c[1] = b * z * z2 * -0.333206551f; c[2] = b * z * z2 * z2 * 0.13145145f; c[3] = b * z * z2 * z2 * z2 * -0.0433724655f;
+    const float z = t.a.sm_scale / cap, z2 = z * z, bz = t.a.sm_scale * TREE_LOG2E;   // b z
+    c[0] = bz * 0.999997676f; c[1] = bz * z2 * -0.333206551f; c[2] = bz * z2 * z2 * 0.13145145f; c[3] = bz * z2 * z2 * z2 * -0.0433724655f;
     small_scale = fabsf(c[3]) <= MOST ? fabsf(z) : INFINITY;              // no logit is small where the coefficients leave fp32
   }
   __device__ __forceinline__ void of_small(float& s0, float& s1) const {
@@ -66,6 +66,17 @@ struct TreeCap {
     p = __ffma2_rn(p, s2, two(c[1])); p = __ffma2_rn(p, s2, two(c[0]));
     p = __fmul2_rn(p, s);
     s0 = p.x; s1 = p.y;
+  }
+  // either form of tanh, each logit by its own size alone
+  __device__ __forceinline__ void of_any(float& s0, float& s1) const {
+    auto pick = [](float size, float small, float large) {   // both are there: no branch around the one that is not taken
+      float y;
+      asm("{\n .reg .pred p;\n setp.le.f32 p, %1, %2;\n selp.f32 %0, %3, %4, p;\n}" : "=f"(y) : "f"(size), "f"(SMALL), "f"(small), "f"(large));
+      return y;
+    };
+    const float size0 = fabsf(s0) * small_scale, size1 = fabsf(s1) * small_scale, e0 = of<2>(s0), e1 = of<2>(s1);
+    of_small(s0, s1);
+    s0 = pick(size0, s0, e0); s1 = pick(size1, s1, e1);
   }
   template <int METHOD> __device__ __forceinline__ float of(float s) const {
     const float v = s * scale;
