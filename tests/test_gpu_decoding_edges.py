@@ -193,3 +193,13 @@ def test_logits_that_reach_their_cap(method, heads, kv_heads, dh, tokens, scale)
 def test_caps_far_above_the_logits(method, cap, heads, kv_heads, dh, tokens):
     """As good as no cap: the error does not grow with the cap."""
     _tree_case([tokens, 2], [900, 40], heads, kv_heads, dh, 32, "tree", cap=cap, method=method, seed=11)
+
+
+def test_a_cap_without_its_method_is_refused():
+    from x_algorithm_b200 import decoding
+    torch = _torch()
+    c = Cache([2], [20], 2, 64, 16)
+    q = torch.randn((2, 4, 64), device=DEV, generator=c.g).to(torch.bfloat16)
+    with pytest.raises(ValueError, match="cap_method"):
+        decoding.tree_attention(q, *c.args(), cap=30.0)
+    assert torch.equal(decoding.tree_attention(q, *c.args(), cap=0.0, cap_method="tanh"), decoding.tree_attention(q, *c.args()))

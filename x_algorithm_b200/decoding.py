@@ -170,7 +170,7 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
                    stream: Optional[int] = None):
     """q bf16 [N, heads, head dim] (tokens may be apart) attends to the cached keys of its request and to the new ones - appended
     already - that spans int32 [N, 2] lets it see: (pre, end) per token, i sees j where pre[j] <= pre[i] < end[j] (`tree_spans`; None: a
-    chain).  sm_scale defaults to sqrt(128) / head dim (scaling.py:46-47).  max_tokens and max_keys: the most new tokens and keys
+    chain).  sm_scale defaults to sqrt(128) / head dim (scaling.py:46-47).  cap > 0 caps the logits by cap_method.  max_tokens and max_keys: the most new tokens and keys
     (cached + new) of a request, if the caller knows them; they only choose kernels.  workspace: uint8, phx_tree_workspace_bytes; the stream's own if None.
     Returns bf16 [N, heads, head dim]."""
     device = _rows(q, "q", _BF16, 3)
@@ -182,6 +182,8 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
         raise ValueError("q must have the cache's head dim, its heads side by side")
     if cap_method not in CAP_METHODS:
         raise ValueError(f"cap_method must be one of {list(CAP_METHODS)}")
+    if cap > 0 and cap_method is None:
+        raise ValueError("a cap needs its cap_method")
     if out is None:
         out = torch.empty_strided(shape, (heads * dh, dh, 1), dtype=_BF16, device=q.device)
     else:
