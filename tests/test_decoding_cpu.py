@@ -131,3 +131,23 @@ def test_the_rows_of_a_block_table_keep_their_distance():
         if stride < table.shape[1]:
             a = _lib.AppendArgs(16, 512, 16, None, None, None, None, 16, 4, 0, 1e-6, 0)
             assert _lib.lib.phx_history_append_device(0, mine.batch_ref, C.byref(a), None) == 1 and b"table_cols apart" in _lib.lib.phx_global_error()
+
+
+def test_check_status_asks_the_current_device(monkeypatch):
+    import torch
+    from types import SimpleNamespace as Fake
+    from x_algorithm_b200 import decoding
+    asked = []
+
+    def decode_status(device, status, stream, bits):
+        asked.append((device, status, stream))
+        return 0
+
+    monkeypatch.setattr(decoding, "lib", Fake(phx_decode_status=decode_status))
+    monkeypatch.setattr(decoding, "_kept", {(d, 70 + d): Fake(status=Fake(data_ptr=lambda d=d: 100 + d)) for d in (0, 1)})
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 70 + d, raising=False)
+    decoding.check_status()
+    decoding.check_status(0)
+    decoding.check_status(device=0, stream=70)
+    assert asked == [(1, 101, 71), (0, 100, 70), (0, 100, 70)]

@@ -227,9 +227,10 @@ def token_logprobs(logits, given=None, *, top_k: int = 0, cap: float = 0.0, temp
     return given_out, entropy, top, ids
 
 
-def check_status(device: int = 0, stream: Optional[int] = None) -> None:
-    """Waits for the stream and raises PhoenixError if a call on it since the last check met a page, position or offset out of range
+def check_status(device: Optional[int] = None, stream: Optional[int] = None) -> None:
+    """Waits for the stream (torch's current one of `device`, of the current device if None) and raises PhoenixError if a call on it since the last check met a page, position or offset out of range
     (PHX_E_ARG: what it named was left out) or a bounded wait that ran out (PHX_E_TIMEOUT)."""
+    device = torch.cuda.current_device() if device is None else device
     stream = _stream(device, stream)
     kept = _kept.get((device, stream))
     if kept is not None:
