@@ -203,3 +203,41 @@ def test_a_cap_without_its_method_is_refused():
     with pytest.raises(ValueError, match="cap_method"):
         decoding.tree_attention(q, *c.args(), cap=30.0)
     assert torch.equal(decoding.tree_attention(q, *c.args(), cap=0.0, cap_method="tanh"), decoding.tree_attention(q, *c.args()))
+
+
+def _dropped(torch, shape, dtype):
+    """The address of a block that the current stream's pool will hand out next for this size."""
+    t = torch.empty(shape, dtype=dtype, device=DEV)
+    return t.data_ptr()
+
+
+def test_results_of_a_named_stream_are_that_streams():
+    """stream=: what a call allocates comes from that stream's pool, so neither a block that queued work of the current stream still uses is written, nor a
+    result that is dropped early is handed to the current stream."""
+    from x_algorithm_b200 import decoding
+    torch = _torch()
+    c = Cache([300], [500], 2, 64, 16, seed=3)
+    qkv = torch.randn((300, 12 * 64), device=DEV, generator=c.g).to(torch.bfloat16)
+    x = torch.randn((700, 5000), device=DEV, generator=c.g)
+    given = torch.randint(0, 5000, (700, 900), device=DEV, generator=c.g)
+    want_q = decoding.history_append(qkv, *c.args(), None, num_q_heads=8)
+    want = decoding.tree_attention(want_q, *c.args())
+    want_p = decoding.token_logprobs(x, given, top_k=100)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    calls = [(lambda: [decoding.history_append(qkv, *c.args(), None, num_q_heads=8, stream=side.cuda_stream)], [want_q]),
+             (lambda: [decoding.tree_attention(want_q, *c.args(), stream=side.cuda_stream)], [want]),
+             (lambda: list(decoding.token_logprobs(x, given, top_k=100, stream=side.cuda_stream)), list(want_p))]
+    for f, wants in calls:
+        free = [_dropped(torch, w.shape, w.dtype) for w in wants]
+        got = f()
+        assert not set(free) & {g.data_ptr() for g in got}
+        side.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, wants))
+        addresses = {g.data_ptr() for g in got}
+        del got
+        assert not addresses & {torch.empty(w.shape, dtype=w.dtype, device=DEV).data_ptr() for w in wants}
+    assert torch.cuda.current_stream() == torch.cuda.default_stream()
+    decoding.check_status(stream=side.cuda_stream)
+    same = decoding.tree_attention(want_q, *c.args(), stream=0)      # the default stream by its number
+    assert torch.equal(same, want)

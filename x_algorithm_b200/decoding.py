@@ -1,7 +1,8 @@
 """Serving over a cached history: rows enter a paged cache (`history_append`), a tree of new tokens attends to it
 (`tree_attention`), logits become log probabilities, entropy and best alternatives (`token_logprobs`).  torch CUDA tensors in
-and out, asynchronous on torch's current stream unless `stream` says otherwise; nothing here waits for the GPU but
-`check_status`.
+and out, asynchronous on torch's current stream; nothing here waits for the GPU but `check_status`.  `stream`, a raw handle, names another
+as `with torch.cuda.stream(...)` around the call would: what the call allocates is that stream's, and what it reads has to be there and stay until it
+has run.
 
 The cache is a tensor `pages` bf16 [num_pages, 2 (key, value), kv heads, page size, head dim] that the caller owns and hands out page by
 page; `block_table` int32 [B, columns] names a request's pages in order, `lengths` int32 [B] counts its cached keys, and the new tokens of
@@ -59,6 +60,16 @@ def _ok(status: int) -> None:
 
 def _stream(device: int, stream: Optional[int]) -> int:
     return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream
+
+
+def _elsewhere(device: int, stream: Optional[int]) -> bool:
+    """Whether `stream` is another than torch's current one.  A call for it runs under it: outputs from the current stream's pool could still be in
+    use by work that is queued there, or be handed out again there while the call writes them."""
+    return stream is not None and stream != torch._C._cuda_getCurrentRawStream(device)
+
+
+def _under(device: int, stream: int):
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
 def _keep(device: int, stream: int) -> _Kept:
@@ -139,6 +150,9 @@ def history_append(qkv, pages, q_start, lengths, block_table, positions, cos=Non
     normed (q_gain, k_gain fp32 [head dim]; None: not) and rotated by positions int32 [N] (cos, sin fp32 [positions, head dim / 2];
     None: not); keys and values go to the cache behind `lengths`, the queries come back as bf16 [N, num_q_heads, head dim]."""
     device = _rows(qkv, "qkv", _BF16, 2)
+    if _elsewhere(device, stream):
+        with _under(device, stream):
+            return history_append(qkv, pages, q_start, lengths, block_table, positions, cos, sin, num_q_heads=num_q_heads, q_gain=q_gain, k_gain=k_gain, eps=eps, out=out)
     n, width = qkv.shape
     stream = _stream(device, stream)
     mine = _structs
@@ -174,6 +188,10 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
     (cached + new) of a request, if the caller knows them; they only choose kernels.  workspace: uint8, phx_tree_workspace_bytes; the stream's own if None.
     Returns bf16 [N, heads, head dim]."""
     device = _rows(q, "q", _BF16, 3)
+    if _elsewhere(device, stream):
+        with _under(device, stream):
+            return tree_attention(q, pages, q_start, lengths, block_table, spans, sm_scale=sm_scale, cap=cap, cap_method=cap_method, max_tokens=max_tokens,
+                                  max_keys=max_keys, out=out, workspace=workspace)
     n, heads, dh = shape = q.shape
     stream = _stream(device, stream)
     kept, mine = _keep(device, stream), _structs
@@ -206,6 +224,9 @@ def token_logprobs(logits, given=None, *, top_k: int = 0, cap: float = 0.0, temp
     [N, top_k]; the ids int64 [N, top_k]) of softmax(cap tanh(logits / cap) / temperature), best first, ties by the lower id."""
     bf16 = isinstance(logits, torch.Tensor) and logits.dtype is _BF16
     device = _rows(logits, "logits", _BF16 if bf16 else _F32, 2)
+    if _elsewhere(device, stream):
+        with _under(device, stream):
+            return token_logprobs(logits, given, top_k=top_k, cap=cap, temperature=temperature)
     rows, vocab = logits.shape
     if not 0 <= top_k <= vocab:
         raise ValueError(f"top_k must be 0 to vocab ({vocab})")
