@@ -151,3 +151,32 @@ def test_check_status_asks_the_current_device(monkeypatch):
     decoding.check_status(0)
     decoding.check_status(device=0, stream=70)
     assert asked == [(1, 101, 71), (0, 100, 70), (0, 100, 70)]
+
+
+def test_threads_that_meet_on_a_stream_keep_one_block(monkeypatch):
+    """Both make the first call on a stream at once: one status block and one workspace, not one each."""
+    import threading
+    import time
+    from x_algorithm_b200 import decoding
+
+    class Slow:
+        made = 0
+
+        def __init__(self, *_):
+            Slow.made += 1
+            time.sleep(0.05)
+
+    monkeypatch.setattr(decoding, "_Kept", Slow)
+    monkeypatch.setattr(decoding, "_kept", {})
+    got, start = [], threading.Barrier(4)
+
+    def first():
+        start.wait()
+        got.append(decoding._keep(0, 5))
+
+    threads = [threading.Thread(target=first) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert Slow.made == 1 and len({id(k) for k in got}) == 1 and len(got) == 4

@@ -37,7 +37,7 @@ class _Kept:
         self.status_ptr, self.workspace_ptr, self.workspace_bytes = self.status.data_ptr(), self.workspace.data_ptr(), need.value
 
 
-_kept = {}
+_kept, _kept_lock = {}, threading.Lock()
 
 
 class _Structs(threading.local):
@@ -75,7 +75,10 @@ def _under(device: int, stream: int):
 def _keep(device: int, stream: int) -> _Kept:
     kept = _kept.get((device, stream))
     if kept is None:
-        kept = _kept[(device, stream)] = _Kept(device)
+        with _kept_lock:                                     # made once: what a second one held would be lost, or freed under a kernel
+            kept = _kept.get((device, stream))
+            if kept is None:
+                kept = _kept[(device, stream)] = _Kept(device)
     return kept
 
 
