@@ -241,3 +241,62 @@ def test_results_of_a_named_stream_are_that_streams():
     decoding.check_status(stream=side.cuda_stream)
     same = decoding.tree_attention(want_q, *c.args(), stream=0)      # the default stream by its number
     assert torch.equal(same, want)
+
+
+def _all_three(c, qkv, x):
+    from x_algorithm_b200 import decoding
+    q = decoding.history_append(qkv, *c.args(), None, num_q_heads=16)
+    return decoding.tree_attention(q, *c.args()), decoding.token_logprobs(x, top_k=4)[2]
+
+
+def test_a_capture_on_a_stream_of_its_own():
+    """Warmed up on one stream, captured on the graph's own, on which nothing has run before; what a replay reports is found under the stream of the capture."""
+    from x_algorithm_b200 import PhoenixError, decoding
+    torch = _torch()
+    c = Cache([3, 40], [9000, 700], 4, 128, 16, seed=1)
+    qkv = torch.randn((c.n, 24 * 128), device=DEV, generator=c.g).to(torch.bfloat16)
+    x = torch.randn((3, 9000), device=DEV, generator=c.g)
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        _all_three(c, qkv, x)
+    warm.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = torch.cuda.current_stream().cuda_stream
+        out = _all_three(c, qkv, x)
+    qkv.copy_(torch.randn(qkv.shape, device=DEV, generator=c.g))
+    graph.replay()
+    got = [t.clone() for t in out]
+    for a, b in zip(got, _all_three(c, qkv, x)):
+        assert torch.equal(a, b)
+    decoding.check_status()
+    decoding.check_status(stream=captured)
+    c.table[0, 2] = -1
+    graph.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(PhoenixError, match="page"):
+        decoding.check_status(stream=captured)
+
+
+def test_the_first_call_on_a_stream_does_not_wait_for_it():
+    """Work that is queued on a new stream is still running when the first call returns."""
+    from x_algorithm_b200 import decoding
+    torch = _torch()
+    c = Cache([3], [50], 2, 64, 16, seed=1)
+    q = torch.randn((3, 4, 64), device=DEV, generator=c.g).to(torch.bfloat16)
+    decoding.tree_attention(q, *c.args())
+    torch.cuda.synchronize()
+    for _ in range(40):                                            # one that has no call behind it
+        side = torch.cuda.Stream()
+        if (0, side.cuda_stream) not in decoding._kept:
+            break
+    else:
+        pytest.skip("every stream of the pool has been used")
+    done = torch.cuda.Event()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)                             # about 0.1 s
+        done.record()
+        decoding.tree_attention(q, *c.args())
+        assert not done.query()
+    side.synchronize()

@@ -1,6 +1,6 @@
 """Serving over a cached history: rows enter a paged cache (`history_append`), a tree of new tokens attends to it
 (`tree_attention`), logits become log probabilities, entropy and best alternatives (`token_logprobs`).  torch CUDA tensors in
-and out, asynchronous on torch's current stream; nothing here waits for the GPU but `check_status`.  `stream`, a raw handle, names another
+and out, asynchronous on torch's current stream; nothing here waits for what is queued but `check_status`.  `stream`, a raw handle, names another
 as `with torch.cuda.stream(...)` around the call would: what the call allocates is that stream's, and what it reads has to be there and stay until it
 has run.
 
@@ -21,6 +21,7 @@ import torch
 from . import _lib
 from ._lib import PhoenixError, lib
 
+STATUS_BLOCKS = 1024                # cleared at a time, one a stream
 CAP_METHODS = {None: 0, "soft_sign": 1, "tanh": 2}
 
 
@@ -28,16 +29,29 @@ class _Kept:
     """What one stream of one device keeps between calls: the status block and the attention's workspace."""
 
     def __init__(self, device: int):
-        self.status = torch.zeros(4, dtype=torch.int32, device=f"cuda:{device}")
+        self.status = _status_block(device)
         need = C.c_int64()
         _ok(lib.phx_tree_workspace_bytes(device, C.byref(need)))
         self.workspace = torch.empty(need.value, dtype=torch.uint8, device=f"cuda:{device}")
-        # made on torch's current stream, used on others: both must be there before any of them reads
-        torch.cuda.current_stream(device).synchronize()
         self.status_ptr, self.workspace_ptr, self.workspace_bytes = self.status.data_ptr(), self.workspace.data_ptr(), need.value
 
 
 _kept, _kept_lock = {}, threading.Lock()
+_cleared = {}                       # device -> status blocks that no stream has yet
+
+
+def _status_block(device: int):
+    """A status block of zeros.  They are cleared many at a time, on a stream of its own whose work is waited for: neither the caller's queue is, nor is
+    the clearing recorded where the caller is capturing a graph."""
+    blocks = _cleared.setdefault(device, [])
+    if not blocks:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call on a device must not be captured: make one before")
+        side = torch.cuda.Stream(device, priority=-1)
+        with torch.cuda.stream(side):
+            blocks.extend(torch.zeros((STATUS_BLOCKS, 4), dtype=torch.int32, device=f"cuda:{device}").unbind(0))
+        side.synchronize()
+    return blocks.pop()
 
 
 class _Structs(threading.local):
