@@ -300,3 +300,37 @@ def test_the_first_call_on_a_stream_does_not_wait_for_it():
         decoding.tree_attention(q, *c.args())
         assert not done.query()
     side.synchronize()
+
+
+def test_graphs_that_are_replayed_beside_each_other_share_no_workspace():
+    from x_algorithm_b200 import decoding
+    torch = _torch()
+    caches = [Cache([3, 40], [9000, 7000], 4, 128, 16, seed=s) for s in (1, 2, 3)]
+    q = [torch.randn((c.n, 16, 128), device=DEV, generator=c.g).to(torch.bfloat16) for c in caches]
+    want = [decoding.tree_attention(r, *c.args()) for c, r in zip(caches, q)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs, used = [], [], []
+    with torch.cuda.stream(side):
+        decoding.tree_attention(q[0], *caches[0].args())     # the stream has a workspace of its own
+        for c, r in zip(caches, q):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                outs.append([decoding.tree_attention(r, *c.args()) for _ in range(4)])
+                used.append(decoding._structs.tree.workspace)
+            graphs.append(graph)
+        used.append(decoding._kept[(0, side.cuda_stream)].workspace.data_ptr())
+    assert len(set(used)) == 4
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(10):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        with torch.cuda.stream(side):
+            last = decoding.tree_attention(q[0], *caches[0].args())
+    torch.cuda.synchronize()
+    assert torch.equal(last, want[0])
+    for o, w in zip(outs, want):
+        assert all(torch.equal(t, w) for t in o)
+    decoding.check_status()

@@ -202,7 +202,7 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
     """q bf16 [N, heads, head dim] (tokens may be apart) attends to the cached keys of its request and to the new ones - appended
     already - that spans int32 [N, 2] lets it see: (pre, end) per token, i sees j where pre[j] <= pre[i] < end[j] (`tree_spans`; None: a
     chain).  sm_scale defaults to sqrt(128) / head dim (scaling.py:46-47).  cap > 0 caps the logits by cap_method.  max_tokens and max_keys: the most new tokens and keys
-    (cached + new) of a request, if the caller knows them; they only choose kernels.  workspace: uint8, phx_tree_workspace_bytes; the stream's own if None.
+    (cached + new) of a request, if the caller knows them; they only choose kernels.  workspace: uint8, phx_tree_workspace_bytes; the stream's own if None, in a capture the graph's own.
     Returns bf16 [N, heads, head dim]."""
     device = _rows(q, "q", _BF16, 3)
     if _elsewhere(device, stream):
@@ -225,6 +225,9 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
         _need(out, "out", _BF16, shape, device)
     if workspace is None:
         space, size = kept.workspace_ptr, kept.workspace_bytes
+        if torch._C._cuda_isCurrentStreamCapturing():        # a graph may be replayed on any stream: it has a workspace of its own, from its own pool
+            workspace = torch.empty(size, dtype=_U8, device=q.device)
+            space = workspace.data_ptr()
     else:
         size = workspace.numel()
         space = _need(workspace, "workspace", _U8, (size,), device)
