@@ -334,3 +334,23 @@ def test_graphs_that_are_replayed_beside_each_other_share_no_workspace():
     for o, w in zip(outs, want):
         assert all(torch.equal(t, w) for t in o)
     decoding.check_status()
+
+
+def test_appending_keeps_no_workspace_and_it_can_be_given_back():
+    from x_algorithm_b200 import decoding
+    torch = _torch()
+    c = Cache([3], [50], 2, 64, 16, seed=1)
+    qkv = torch.randn((3, 8 * 64), device=DEV, generator=c.g).to(torch.bfloat16)
+    side = torch.cuda.Stream()
+    decoding.release(stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        before = torch.cuda.memory_allocated()
+        q = decoding.history_append(qkv, *c.args(), None, num_q_heads=4)
+        assert torch.cuda.memory_allocated() - before < 1 << 20
+        out = decoding.tree_attention(q, *c.args())
+        assert torch.cuda.memory_allocated() - before > 1 << 20
+        decoding.release()
+        assert torch.cuda.memory_allocated() - before < 1 << 20
+        assert torch.equal(decoding.tree_attention(q, *c.args()), out)
+        decoding.check_status()

@@ -26,14 +26,25 @@ CAP_METHODS = {None: 0, "soft_sign": 1, "tanh": 2}
 
 
 class _Kept:
-    """What one stream of one device keeps between calls: the status block and the attention's workspace."""
+    """What one stream of one device keeps between calls: the status block and, from its first attention on, that one's workspace."""
 
     def __init__(self, device: int):
         self.status = _status_block(device)
-        need = C.c_int64()
-        _ok(lib.phx_tree_workspace_bytes(device, C.byref(need)))
-        self.workspace = torch.empty(need.value, dtype=torch.uint8, device=f"cuda:{device}")
-        self.status_ptr, self.workspace_ptr, self.workspace_bytes = self.status.data_ptr(), self.workspace.data_ptr(), need.value
+        self.status_ptr, self.workspace, self.space = self.status.data_ptr(), None, None
+
+
+def _take_space(kept, device: int):
+    with _kept_lock:
+        if kept.space is None:
+            kept.workspace = _workspace(device)
+            kept.space = kept.workspace.data_ptr(), kept.workspace.numel()
+        return kept.space
+
+
+def _workspace(device: int):
+    need = C.c_int64()
+    _ok(lib.phx_tree_workspace_bytes(device, C.byref(need)))
+    return torch.empty(need.value, dtype=torch.uint8, device=f"cuda:{device}")
 
 
 _kept, _kept_lock = {}, threading.Lock()
@@ -224,10 +235,11 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
     else:
         _need(out, "out", _BF16, shape, device)
     if workspace is None:
-        space, size = kept.workspace_ptr, kept.workspace_bytes
-        if torch._C._cuda_isCurrentStreamCapturing():        # a graph may be replayed on any stream: it has a workspace of its own, from its own pool
-            workspace = torch.empty(size, dtype=_U8, device=q.device)
-            space = workspace.data_ptr()
+        if stream != 0 and torch._C._cuda_isCurrentStreamCapturing():   # (the default stream cannot be captured)
+            workspace = _workspace(device)                   # a graph may be replayed on any stream: it has a workspace of its own, from its own pool
+            space, size = workspace.data_ptr(), workspace.numel()
+        else:
+            space, size = kept.space or _take_space(kept, device)
     else:
         size = workspace.numel()
         space = _need(workspace, "workspace", _U8, (size,), device)
@@ -266,6 +278,14 @@ def token_logprobs(logits, given=None, *, top_k: int = 0, cap: float = 0.0, temp
               rows, vocab, num_given, top_k, bf16, cap, temperature, 0)
     _ok(lib.phx_token_logprobs_device(device, mine.logprobs_ref, _stream(device, stream)))
     return given_out, entropy, top, ids
+
+
+def release(device: Optional[int] = None, stream: Optional[int] = None) -> None:
+    """Gives the workspace of a stream (torch's current one if None) back to torch's allocator, 39 MB on a B200; its next attention takes one again."""
+    device = torch.cuda.current_device() if device is None else device
+    kept = _kept.get((device, _stream(device, stream)))
+    if kept is not None:
+        kept.workspace = kept.space = None
 
 
 def check_status(device: Optional[int] = None, stream: Optional[int] = None) -> None:
