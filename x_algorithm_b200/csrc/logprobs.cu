@@ -49,6 +49,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
+__device__ __forceinline__ float warp_max_nan(float x) {       // of a warp's lanes
+  float y;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
 // order-preserving: larger logit, larger image; the two zeros are equal, NaN is largest
 __device__ __forceinline__ uint32_t image(float x) {
   if (x != x) return 0xFFFFFFFFu;
@@ -337,9 +342,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
 
     const float ctop = CAP ? cap.of(top) : top;
     if (__any_sync(0xffffffffu, !(ctop <= st.m))) {   // the warp's maximum has grown, or there is a NaN
-      Stat grown = {max_nan(ctop, st.m), 0.f, 0.f};
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) grown.m = max_nan(grown.m, __shfl_xor_sync(0xffffffffu, grown.m, o));
+      const Stat grown = {warp_max_nan(max_nan(ctop, st.m)), 0.f, 0.f};
       st = join(st, grown, scale);
     }
     if (top != -INFINITY) {
@@ -398,9 +401,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * WARP_ROWS : NT, Shape<NT>::RES
 
   // the team's sums, in a fixed order
   auto fold = [&]() {
-    Stat all = {st.m, 0.f, 0.f};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all.m = max_nan(all.m, __shfl_xor_sync(0xffffffffu, all.m, o));
+    const Stat all = {warp_max_nan(st.m), 0.f, 0.f};
     st = join(st, all, scale);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) { st.z += __shfl_xor_sync(0xffffffffu, st.z, o); st.s += __shfl_xor_sync(0xffffffffu, st.s, o); }
