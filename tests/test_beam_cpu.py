@@ -1,0 +1,57 @@
+"""What the beam search decides on the host, with stand-ins for the operators."""
+import contextlib
+
+import pytest
+import torch
+
+from x_algorithm_b200 import beam, decoding
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The operators in plain torch on the CPU (attention as an average of the queries); what they were called with."""
+    seen = dict(gemm=[], status=[], device=[], tables=[])
+
+    def gemm(a, wt, residual=None, epilogue=0, impl=0, device=0):
+        seen["gemm"].append(device)
+        c = a.float() @ wt.float().T
+        c = torch.nn.functional.gelu(c) if epilogue == 2 else c + residual.float() if epilogue == 1 else c
+        return c.to(torch.bfloat16), 0.0
+
+    def history_append(qkv, pages, q_start, lengths, table, positions, cos, sin, *, num_q_heads, q_gain, k_gain, eps):
+        seen["tables"].append(table.clone())
+        return qkv[:, :num_q_heads * pages.shape[-1]].reshape(qkv.shape[0], num_q_heads, -1)
+
+    def token_logprobs(logits, given=None, *, top_k=0, cap=0.0, temperature=1.0):
+        lp = torch.log_softmax(logits.float(), -1)
+        best, ids = lp.topk(top_k, dim=1)
+        return None, None, best, ids
+
+    @contextlib.contextmanager
+    def device(index):
+        seen["device"].append(index)
+        yield
+
+    monkeypatch.setattr(beam, "gemm", gemm)
+    monkeypatch.setattr(decoding, "history_append", history_append)
+    monkeypatch.setattr(decoding, "tree_attention", lambda q, *a, **k: q)
+    monkeypatch.setattr(decoding, "token_logprobs", token_logprobs)
+    monkeypatch.setattr(decoding, "check_status", lambda device=None, stream=None: seen["status"].append(device))
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 2)
+    return seen
+
+
+def _decoder(**kw):
+    cfg = beam.BeamConfig(emb_size=64, num_layers=1, ffn_size=64, vocab=32, **kw)
+    return beam.SemanticIdBeam(cfg, beam.make_weights(cfg, device="cpu"), max_users=4, device="cpu")
+
+
+def test_every_call_goes_to_the_decoders_device(host):
+    d = _decoder()
+    assert d.index == 2                                      # "cuda" is the current device
+    d.index = 3
+    d.remember([0, 1], [torch.randn(5, 64).to(torch.bfloat16), torch.randn(2, 64).to(torch.bfloat16)])
+    ids, scores = d.search([1, 0], [3, 4], steps=2, beam=3)
+    assert ids.shape == (2, 3, 2) and scores.shape == (2, 3)
+    assert set(host["gemm"]) == {3} and host["status"] == [3] and host["device"] == [3, 3]

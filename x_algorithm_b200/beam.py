@@ -53,6 +53,7 @@ class SemanticIdBeam:
 
     def __init__(self, cfg: BeamConfig, weights, max_users: int, device="cuda"):
         self.cfg, self.w, self.device = cfg, weights, torch.device(device)
+        self.index = self.device.index if self.device.index is not None else torch.cuda.current_device()
         shape = (cfg.num_pages, 2, cfg.num_kv_heads, cfg.page_size, cfg.key_size)
         self.pages = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(cfg.num_layers)]
         self.cos, self.sin = decoding.rope_tables(cfg.max_positions, cfg.key_size, device=device)
@@ -64,6 +65,9 @@ class SemanticIdBeam:
         """Pages for so many keys of the user."""
         while len(self.owned[user]) * self.cfg.page_size < keys:
             self.owned[user].append(self.free.pop())
+
+    def _gemm(self, a, wt, residual=None, epilogue=0):
+        return gemm(a, wt, residual, epilogue=epilogue, device=self.index)[0]
 
     def _norm(self, x, gain):
         x = x.float()
@@ -81,13 +85,13 @@ class SemanticIdBeam:
         q_start = torch.tensor([0] + counts, **dev).cumsum(0).to(torch.int32)
         most = dict(max_tokens=max(counts), max_keys=max(self.length[u] + n for u, n in zip(users, counts)))
         for w, pages in zip(self.w["layers"], self.pages):
-            qkv, _ = gemm(self._norm(x, w["pre_attn"]), w["qkv"])
+            qkv = self._gemm(self._norm(x, w["pre_attn"]), w["qkv"])
             q = decoding.history_append(qkv, pages, q_start, lengths, table, positions, self.cos, self.sin, num_q_heads=cfg.num_q_heads,
                                         q_gain=w["q_gain"], k_gain=w["k_gain"], eps=cfg.rms_eps)
             a = decoding.tree_attention(q, pages, q_start, lengths, table, spans, **most)
-            x, _ = gemm(a.view(a.shape[0], -1), w["out"], x, epilogue=1)
-            h, _ = gemm(self._norm(x, w["pre_ffn"]), w["up"], epilogue=2)
-            x, _ = gemm(h, w["down"], x, epilogue=1)
+            x = self._gemm(a.view(a.shape[0], -1), w["out"], x, epilogue=1)
+            h = self._gemm(self._norm(x, w["pre_ffn"]), w["up"], epilogue=2)
+            x = self._gemm(h, w["down"], x, epilogue=1)
         return x
 
     def remember(self, users: List[int], rows: List[torch.Tensor]):
@@ -98,7 +102,8 @@ class SemanticIdBeam:
                 raise ValueError(f"user {u} has a history already: forget it first")
         positions = torch.cat([torch.arange(n, dtype=torch.int32, device=self.device) for n in counts])
         spans = torch.tensor([[0, 1]], dtype=torch.int32, device=self.device).repeat(sum(counts), 1)
-        self._layers(torch.cat(rows), users, counts, positions, spans)
+        with torch.cuda.device(self.index):
+            self._layers(torch.cat(rows), users, counts, positions, spans)
         for u, n in zip(users, counts):
             self.length[u] = n
 
@@ -109,6 +114,10 @@ class SemanticIdBeam:
     def search(self, users: List[int], first_ids: List[int], steps: int, beam: int):
         """The `beam` best continuations of `steps` ids behind each user's history and first id: (ids int64 [users, beam, steps],
         log probabilities fp32 [users, beam])."""
+        with torch.cuda.device(self.index):
+            return self._search(users, first_ids, steps, beam)
+
+    def _search(self, users, first_ids, steps, beam):
         cfg, count = self.cfg, len(users)
         # a user's tree: ids, parents (-1: behind the history), depth of each token; leaves of the last level and their scores
         ids, parents, depth = [[f] for f in first_ids], [[-1] for _ in users], [[0] for _ in users]
@@ -121,7 +130,7 @@ class SemanticIdBeam:
             x = self._layers(x, users, counts, positions, spans)
             starts = [sum(counts[:i]) for i in range(count)]
             last = torch.tensor([s + leaf for s, ls in zip(starts, leaves) for leaf in ls], device=self.device)
-            logits, _ = gemm(self._norm(x[last], self.w["final"]), self.w["unembed"])
+            logits = self._gemm(self._norm(x[last], self.w["final"]), self.w["unembed"])
             width = len(leaves[0])
             _, _, best, best_ids = decoding.token_logprobs(logits, top_k=min(beam, cfg.vocab), cap=cfg.logit_cap)
             total = scores[:, :, None] + best.view(count, width, -1)
@@ -133,7 +142,7 @@ class SemanticIdBeam:
                     parent = leaves[u][leaf]
                     ids[u].append(i); parents[u].append(parent); depth[u].append(step + 1)
                 leaves[u] = list(range(first_new, first_new + beam))
-        decoding.check_status(self.device.index or 0)
+        decoding.check_status(self.index)
         paths = []
         for u in range(count):
             rows = []
