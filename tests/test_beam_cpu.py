@@ -55,3 +55,15 @@ def test_every_call_goes_to_the_decoders_device(host):
     ids, scores = d.search([1, 0], [3, 4], steps=2, beam=3)
     assert ids.shape == (2, 3, 2) and scores.shape == (2, 3)
     assert set(host["gemm"]) == {3} and host["status"] == [3] and host["device"] == [3, 3]
+
+
+def test_a_user_may_be_named_once_a_call(host):
+    d = _decoder()
+    row = torch.randn(5, 64).to(torch.bfloat16)
+    with pytest.raises(ValueError, match="once"):
+        d.remember([1, 1], [row, row])
+    assert d.length == [0] * 4 and len(d.free) == d.cfg.num_pages
+    d.remember([1], [row])
+    with pytest.raises(ValueError, match="once"):
+        d.search([1, 1], [3, 4], steps=1, beam=2)
+    d.search([1], [3], steps=1, beam=2)

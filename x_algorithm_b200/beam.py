@@ -61,6 +61,12 @@ class SemanticIdBeam:
         self.owned: List[List[int]] = [[] for _ in range(max_users)]
         self.length = [0] * max_users
 
+    @staticmethod
+    def _distinct(users: List[int]):
+        """Two rows of one call for the same user would write the same places of its pages."""
+        if len(set(users)) != len(users):
+            raise ValueError("a user may be named once a call")
+
     def _reserve(self, user: int, keys: int):
         """Pages for so many keys of the user."""
         while len(self.owned[user]) * self.cfg.page_size < keys:
@@ -97,6 +103,7 @@ class SemanticIdBeam:
     def remember(self, users: List[int], rows: List[torch.Tensor]):
         """History rows bf16 [n, D] of each user join the cache (a user's first: its rows see each other, none comes later than its history)."""
         counts = [r.shape[0] for r in rows]
+        self._distinct(users)
         for u in users:
             if self.length[u]:
                 raise ValueError(f"user {u} has a history already: forget it first")
@@ -114,6 +121,7 @@ class SemanticIdBeam:
     def search(self, users: List[int], first_ids: List[int], steps: int, beam: int):
         """The `beam` best continuations of `steps` ids behind each user's history and first id: (ids int64 [users, beam, steps],
         log probabilities fp32 [users, beam])."""
+        self._distinct(users)
         with torch.cuda.device(self.index):
             return self._search(users, first_ids, steps, beam)
 
