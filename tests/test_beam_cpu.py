@@ -67,3 +67,20 @@ def test_a_user_may_be_named_once_a_call(host):
     with pytest.raises(ValueError, match="once"):
         d.search([1, 1], [3, 4], steps=1, beam=2)
     d.search([1], [3], steps=1, beam=2)
+
+
+def test_a_pool_that_is_too_small_hands_out_nothing(host):
+    d = _decoder(num_pages=4, page_size=16)
+    row = torch.randn(40, 64).to(torch.bfloat16)                 # three pages
+    with pytest.raises(MemoryError, match="6 pages"):
+        d.remember([0, 1], [row, row])
+    assert len(d.free) == 4 and d.owned == [[]] * 4 and d.length == [0] * 4
+    d.remember([0], [row])
+    d.search([0], [3], steps=2, beam=3)
+    with pytest.raises(MemoryError):
+        d.remember([1], [row])
+    assert d.length[1] == 0 and len(d.free) + len(d.owned[0]) == 4
+    d.forget(0)
+    d.remember([1], [row])
+    tables = host["tables"]
+    assert all(len(set(t[t >= 0].tolist())) == int((t >= 0).sum()) for t in tables)

@@ -67,10 +67,13 @@ class SemanticIdBeam:
         if len(set(users)) != len(users):
             raise ValueError("a user may be named once a call")
 
-    def _reserve(self, user: int, keys: int):
-        """Pages for so many keys of the user."""
-        while len(self.owned[user]) * self.cfg.page_size < keys:
-            self.owned[user].append(self.free.pop())
+    def _reserve(self, users: List[int], keys: List[int]):
+        """Pages for so many keys of each user: all that are missing, or none and an error."""
+        more = [max(0, -(-k // self.cfg.page_size) - len(self.owned[u])) for u, k in zip(users, keys)]
+        if sum(more) > len(self.free):
+            raise MemoryError(f"{sum(more)} pages are needed, {len(self.free)} are free: forget a user, or make the pool larger")
+        for u, n in zip(users, more):
+            self.owned[u] += [self.free.pop() for _ in range(n)]
 
     def _gemm(self, a, wt, residual=None, epilogue=0):
         return gemm(a, wt, residual, epilogue=epilogue, device=self.index)[0]
@@ -82,8 +85,7 @@ class SemanticIdBeam:
     def _layers(self, x, users: List[int], counts: List[int], positions, spans):
         """Token rows x bf16 [N, D] of the users, counts[i] each, behind what their caches hold; appends their keys, returns the rows."""
         cfg = self.cfg
-        for u, n in zip(users, counts):
-            self._reserve(u, self.length[u] + n)
+        self._reserve(users, [self.length[u] + n for u, n in zip(users, counts)])
         cols = max(len(self.owned[u]) for u in users)
         dev = dict(dtype=torch.int32, device=self.device)
         table = torch.tensor([self.owned[u] + [-1] * (cols - len(self.owned[u])) for u in users], **dev)
