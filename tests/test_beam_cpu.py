@@ -84,3 +84,18 @@ def test_a_pool_that_is_too_small_hands_out_nothing(host):
     d.remember([1], [row])
     tables = host["tables"]
     assert all(len(set(t[t >= 0].tolist())) == int((t >= 0).sum()) for t in tables)
+
+
+def test_what_has_no_position_or_no_candidates_is_refused(host):
+    d = _decoder(max_positions=40)
+    row = torch.randn(41, 64).to(torch.bfloat16)
+    with pytest.raises(ValueError, match="41 positions"):
+        d.remember([0], [row])
+    assert d.length[0] == 0 and not d.owned[0]
+    d.remember([0], [row[:38]])
+    with pytest.raises(ValueError, match="41 positions"):
+        d.search([0], [3], steps=3, beam=2)
+    for beam_size in (0, 33, 129):
+        with pytest.raises(ValueError, match="beam"):
+            d.search([0], [3], steps=2, beam=beam_size)
+    assert d.search([0], [3], steps=2, beam=32)[0].shape == (1, 32, 2)

@@ -67,6 +67,10 @@ class SemanticIdBeam:
         if len(set(users)) != len(users):
             raise ValueError("a user may be named once a call")
 
+    def _placed(self, positions: int):
+        if positions > self.cfg.max_positions:
+            raise ValueError(f"{positions} positions are needed, the rotation has {self.cfg.max_positions}")
+
     def _reserve(self, users: List[int], keys: List[int]):
         """Pages for so many keys of each user: all that are missing, or none and an error."""
         more = [max(0, -(-k // self.cfg.page_size) - len(self.owned[u])) for u, k in zip(users, keys)]
@@ -109,6 +113,7 @@ class SemanticIdBeam:
         for u in users:
             if self.length[u]:
                 raise ValueError(f"user {u} has a history already: forget it first")
+        self._placed(max(counts, default=0))
         positions = torch.cat([torch.arange(n, dtype=torch.int32, device=self.device) for n in counts])
         spans = torch.tensor([[0, 1]], dtype=torch.int32, device=self.device).repeat(sum(counts), 1)
         with torch.cuda.device(self.index):
@@ -124,6 +129,9 @@ class SemanticIdBeam:
         """The `beam` best continuations of `steps` ids behind each user's history and first id: (ids int64 [users, beam, steps],
         log probabilities fp32 [users, beam])."""
         self._distinct(users)
+        if not 1 <= beam <= min(self.cfg.vocab, 128):
+            raise ValueError("beam must be 1 to the vocabulary, at most 128")
+        self._placed(max((self.length[u] for u in users), default=0) + steps)
         with torch.cuda.device(self.index):
             return self._search(users, first_ids, steps, beam)
 
