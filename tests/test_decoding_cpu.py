@@ -180,3 +180,16 @@ def test_threads_that_meet_on_a_stream_keep_one_block(monkeypatch):
     for t in threads:
         t.join()
     assert Slow.made == 1 and len({id(k) for k in got}) == 1 and len(got) == 4
+
+
+def test_parents_are_integers_and_keep_all_their_bits():
+    from x_algorithm_b200.decoding import tree_spans
+    for parents in (np.array([-1, 2 ** 32]), np.array([-1, 2 ** 32 - 2]), np.array([2 ** 64 - 1, 0], np.uint64), [-1, 2 ** 40]):
+        with pytest.raises(PhoenixError) as e:
+            tree_spans(parents)
+        assert e.value.status == 1
+    for parents in ([-1, 0.5], np.array([-1.0, 0.0])):
+        with pytest.raises(ValueError):
+            tree_spans(parents)
+    np.testing.assert_array_equal(tree_spans(np.array([-1, 0], np.int8)), [[0, 2], [1, 2]])
+    assert tree_spans([]).shape == (0, 2)

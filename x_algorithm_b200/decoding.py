@@ -164,9 +164,12 @@ def rope_tables(num_positions: int, head_dim: int, base: float = 10000.0, device
 def tree_spans(parents) -> np.ndarray:
     """int32 [n, 2] (pre, end) of one request's tokens from their parents (host ints: the parent's place among them, -1: hangs on
     the cached history, -2: padding), any order."""
-    p = np.ascontiguousarray(parents, dtype=np.int32)
-    if p.ndim != 1:
-        raise ValueError("parents must be one-dimensional")
+    p = np.asarray(parents)
+    if p.ndim != 1 or (p.size and p.dtype.kind not in "iu"):
+        raise ValueError("parents must be one-dimensional integers")
+    if p.size and (p.min() < -2 or p.max() >= p.size):         # before they are narrowed to 32 bits
+        raise PhoenixError(1, "a parent must be -1, -2 (padding) or another token that is no padding")
+    p = np.ascontiguousarray(p, dtype=np.int32)
     out = np.empty((p.shape[0], 2), np.int32)
     _ok(lib.phx_tree_spans(p.ctypes.data, p.shape[0], out.ctypes.data))
     return out
