@@ -770,7 +770,7 @@ phx_status phx_dpp_rescore_device(int32_t device, const phx_dpp_config* cfg, con
  *
  * What the host cannot check is checked on the device, and reads or writes nothing out of range: a token whose page is
  * outside the pool or behind the table's columns is not stored, a key in such a page is left out (as if it did not exist), a
- * position outside the rotation tables takes the nearest one inside.  Each raises a bit of status_dev[2]: 1 a page, 2 a
+ * position outside the rotation tables takes the nearest one inside; rows of no request are neither read nor written by the attention.  Each raises a bit of status_dev[2]: 1 a page, 2 a
  * position, 4 offsets that do not ascend or leave the token rows (such a request is left out).  status_dev (int32 [4],
  * required) starts as zeros; [0] is raised when a bounded wait ran out (as phx_sync reports by PHX_E_TIMEOUT), [1] is the limit of those waits in
  * microseconds (0 = 2 s).  phx_decode_status waits for `stream`, returns PHX_OK, PHX_E_TIMEOUT, or PHX_E_ARG with the
@@ -820,7 +820,7 @@ phx_status phx_history_append_device(int32_t device, const phx_cache_batch* cach
  * j an ancestor of i (phx_tree_spans makes them from parents, in any order of the tokens); (0, 1) everywhere lets all see
  * all, as a history does, (i, i + 1) only themselves, as candidates do.  spans NULL: a chain, j <= i.  pre = -1 (end <= 0):
  * a padding token, seen by none, output zeros; so is the output of a token that sees no key.  A key that a token does not see leaves no trace in its
- * output, whatever the key's value rows hold (infinities, NaN).  cap > 0: logits go through cap_method (1 soft sign, 2 tanh).
+ * output, whatever its key and value rows hold (infinities, NaN).  cap > 0: logits go through cap_method (1 soft sign, 2 tanh).
  * max_tokens and max_keys (cached + new) say how large a request may be; they choose kernels and splits only: larger
  * requests are computed all the same.  workspace: phx_tree_workspace_bytes of device memory, not shared by calls that may
  * overlap; nothing in it has to be kept or cleared between calls.  The order of every sum follows from the sizes alone: equal calls

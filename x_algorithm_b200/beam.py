@@ -1,11 +1,11 @@
-"""Beam search over semantic ids behind a user's cached history: the operators of `decoding` run together as a serving path
-would use them.
+"""Beam search over semantic ids behind a user's cached history: an example of the operators of `decoding` run together.
 
 A small decoder in the trunk's arithmetic (pre-norm layers, merged QKV, rotation, GELU feed-forward; transformer.py:461-618) keeps the keys and
 values of every user's history in one paged cache a layer.  `remember` sends history rows through the layers once, each
 seeing the whole history; `search` grows a tree of ids behind it: every step sends the tree's tokens through the layers, appended behind the history
 and seeing it and their own branch, and extends the best branches by the best alternatives of the next id.  The projections are the
-engine's GEMM; norms, GELU and the choice of branches are plain torch."""
+engine's GEMM call, which waits for the device each time; norms and the choice of branches are plain torch.  (A new token sees all that is cached, so a tree is not
+cached level by level: each step sends it whole.)"""
 from __future__ import annotations
 
 import math

@@ -21,8 +21,9 @@
 // distinct, so ties need no care and the result does not depend on the order of the atomics.  More ids than lanes give a bound for (over 24) of
 // a row that a warp has for itself are found exactly: the row's images in registers, their top_k-th largest by halving.
 //
-// Measured: 2048 rows of 100003 bf16 logits 85 us = 4.8 TB/s without best ids, 118 with eight, 151 and 183 capped; 1024 rows of 100004 fp32 72 us = 5.6 TB/s and 88;
-// one row of 131072 fp32, best 20, 12.2 us on eight blocks.  The selection behind a row's last word is what the eight cost.
+// Measured: 2048 rows of 100003 bf16 logits 83 us = 4.9 TB/s without best ids, 117 with eight, 150 and 180 capped; 1024 rows of 100004 fp32 72 us = 5.6 TB/s and 85;
+// one row of 131072 fp32, best 20, 11.9 us on eight blocks.  The selection behind a row's last word is what the eight cost.  A cap that logits reach costs more: beyond 3/4 of it a
+// thread takes its batch one by one, 630 us for the 2048 rows with logits of 4 times a standard normal under a cap of 10.
 #include <math.h>
 #include <string.h>
 
@@ -572,8 +573,9 @@ cudaError_t logprobs_launch(const phx_logprobs_args& a, int blocks, cudaStream_t
   lc.attrs = at; lc.numAttrs = 1;
   return cudaLaunchKernelEx(&lc, logprobs_kernel<T, NT, CAP>, a, blocks);
 }
-// Threads of a row: enough for its words in one batch, as far as the device has room for all rows at once (148 SMs of 1024 threads at
-// this kernel's registers); a warp for rows it can hold, else a block, else a cluster of up to eight.
+// Threads of a row: enough for its words in one batch, up to the row's part of the device's (148 SMs of 1024 threads at this kernel's registers), rounded up to
+// what there is: a warp for rows it can hold, else a block of 256, of 1024, else a cluster of up to eight of those.  Rounding up makes 149 to 295 long rows two rounds of blocks (148
+// fp32 rows of 131072 with best 8 take 23 us, 149 take 41, 296 take 40), 75 to 147 pairs that do not all fit (74 rows 18 us, 75 rows 30).
 template <typename T, bool CAP>
 cudaError_t logprobs_dispatch(const phx_logprobs_args& a, cudaStream_t stream) {
   const long long need = (a.vocab + 2ll * Words<T>::N) / (Words<T>::N * 4) + 1;

@@ -227,7 +227,7 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
         for (int n = 0; n < KEYS / 8; ++n) {
           const float e0 = tree_ex2(s[n][2 * i] - base), e1 = tree_ex2(s[n][2 * i + 1] - base);
           sum += e0 + e1;
-          p[n >> 1][(n & 1) * 2 + i] = pack_bf2(e0, e1);   // rounded to bf16 for the product; the sum keeps fp32
+          p[n >> 1][(n & 1) * 2 + i] = pack_bf2(e0, e1);   // rounded to bf16 for the product with bf16 values; the sum keeps fp32
         }
         l[i] = l[i] * alpha + sum;
         if (__any_sync(0xffffffffu, alpha != 1.0f)) {

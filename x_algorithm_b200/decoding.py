@@ -255,7 +255,7 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
 
 def token_logprobs(logits, given=None, *, top_k: int = 0, cap: float = 0.0, temperature: float = 1.0, stream: Optional[int] = None):
     """logits fp32 or bf16 [N, vocab] (rows may be apart; -inf: not allowed), given int64 [N, n] or [N] ids (outside the
-    vocabulary: none).  Returns (log probabilities of given fp32, of its shape, None without given; entropy fp32 [N]; the top_k best ids' log probabilities fp32
+    vocabulary: none), top_k at most 128.  Returns (log probabilities of given fp32, of its shape, None without given; entropy fp32 [N]; the top_k best ids' log probabilities fp32
     [N, top_k]; the ids int64 [N, top_k]) of softmax(cap tanh(logits / cap) / temperature), best first, ties by the lower id."""
     bf16 = isinstance(logits, torch.Tensor) and logits.dtype is _BF16
     device = _rows(logits, "logits", _BF16 if bf16 else _F32, 2)
