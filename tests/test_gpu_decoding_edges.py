@@ -153,7 +153,7 @@ def test_tree_attention_with_very_small_caps(method, cap, heads, kv_heads, dh, t
     _check(out, *_attend(c, q, spans, math.sqrt(128.0) / dh, cap, method))
 
 
-@pytest.mark.parametrize("method,cap", [("tanh", 5.0), ("tanh", 30.0), ("soft_sign", 5.0)])
+@pytest.mark.parametrize("method,cap", [("tanh", 5.0), ("tanh", 30.0), ("tanh", 2000.0), ("soft_sign", 5.0)])
 @pytest.mark.parametrize("heads,kv_heads,dh,tokens,cached", [(4, 4, 32, 9, 70), (8, 8, 64, 9, 70), (16, 4, 128, 4, 70), (16, 4, 128, 60, 70), (8, 8, 64, 150, 70), (32, 8, 128, 17, 3000)])
 def test_keys_that_are_not_seen_leave_no_trace_under_a_cap(method, cap, heads, kv_heads, dh, tokens, cached):
     """Large keys, NaN and infinities of padding tokens, of another branch and behind the last key: the same bits as without them."""
