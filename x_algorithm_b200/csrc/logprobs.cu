@@ -8,7 +8,7 @@
 // One pass over the logits, bound by memory.  A row belongs to a warp, to a block, or to a cluster of blocks that each take a
 // stretch of it.  A thread fetches its own 16-byte words, cp.async into a ring of its own in shared memory (no barriers), takes a few
 // of them at a time, and keeps a reference, the sum of e^t and the sum of e^t t against it.  The reference is the running maximum of the warp: the best id's
-// own exponential is 1 at the end, and log p near 0 and the entropy keep their bits (a reference that may be 11 below it cost log p 1e-6).  It moves a few times a row; a lane's
+// own exponential is 1 at the end, and its log p near 0 is good to 1e-7 (a reference that may be 11 below it cost 1e-6).  It moves a few times a row; a lane's
 // own maximum moved in some lane of a warp at almost every batch, a third of the instructions.
 //
 // The best ids are found by words first: a word's key is its largest logit's order-preserving image, then its place, first come first.
