@@ -842,6 +842,70 @@ typedef struct phx_tree_args {
 } phx_tree_args;
 phx_status phx_tree_workspace_bytes(int32_t device, int64_t* bytes_out);
 phx_status phx_tree_attention_device(int32_t device, const phx_cache_batch* cache, const phx_tree_args* args, void* stream);
+
+/* The same with a window: of the keys that token i may see, it sees those whose place is behind its own place - window, and those whose place is in front of
+ * `sinks` (the first keys of a history keep taking the weight that a softmax has to put somewhere).  A cached key's place is its number in the cache, a new
+ * token's positions[token] (a draft's depth behind the cache: lengths[b] + depth), at least lengths[b]; positions NULL: lengths[b] + i for token i of a chain
+ * (spans NULL), lengths[b] for tokens with spans.  A window counts the token's own key: 1 leaves a chain's token itself and the first keys.  window 0: none.
+ * Tiles of keys that no token of a block's rows sees are not read, nor are the pages in such a gap looked up for a chain or behind the cache: a caller may hand out pages that lie
+ * wholly in front of all windows and behind the first keys anew, with -1 in the table.  lse_out [num_tokens][num_q_heads] fp32: ln sum e^x over the keys
+ * seen, of the logits x that the softmax takes (scaled, capped); -inf for a token that sees none.  Everything else as above. */
+typedef struct phx_window_args {
+  phx_tree_args attention;
+  const int32_t* positions;    /* [num_tokens] or NULL */
+  float* lse_out;
+  int32_t window;
+  int32_t sinks;
+} phx_window_args;
+phx_status phx_window_attention_device(int32_t device, const phx_cache_batch* cache, const phx_window_args* args, void* stream);
+
+/* The attention weight that the keys of the cache receive: for every key j of a request and key head, the sum over the new tokens that see it and the
+ * head's queries of e^(x_ij - lse[i]), with the logits x of the attention above (same sm_scale, cap, spans, positions, window and sinks) and lse
+ * [num_tokens][num_q_heads] as phx_window_attention_device gave it.  A cached key's weights[page][kv head][slot] becomes decay * weight + sum, a new one's
+ * (behind lengths[b]) the sum: nothing has to be cleared when a page is handed out.  Places of no key are left as they are.  A row whose lse is infinite adds
+ * nothing: -inf is a row that saw nothing, +inf leaves a row out.  With decay 1 the keys that no window reaches keep their weights and are not touched.  The order of
+ * every sum follows from the sizes alone.  max_tokens and max_keys choose kernels and launch sizes only, as above.  workspace: phx_tree_workspace_bytes, not shared by
+ * calls that may overlap.  Asynchronous on `stream`. */
+typedef struct phx_key_weights_args {
+  const uint16_t* q;           /* [num_tokens][num_q_heads][key_size], rows q_stride apart */
+  int64_t q_stride;
+  const int32_t* spans;        /* [num_tokens][2] or NULL */
+  const int32_t* positions;    /* [num_tokens] or NULL */
+  const float* lse;
+  float* weights;              /* [num_pages][num_kv_heads][page_size] */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t max_keys;
+  int32_t max_tokens;
+  int32_t num_q_heads;
+  int32_t window;              /* 0: none */
+  int32_t sinks;
+  float sm_scale;
+  float cap;
+  int32_t cap_method;
+  float decay;
+} phx_key_weights_args;
+phx_status phx_key_weights_device(int32_t device, const phx_cache_batch* cache, const phx_key_weights_args* args, void* stream);
+
+/* Keys leave the cache until no request has more than `budget`: of each key head the first `sinks` and the last `recent` keys stay, and of those between the
+ * ones with the largest weights (ties: the lower place; NaN counts as largest; a key whose page is outside the pool as lowest).  What stays moves to places 0, 1, ... budget - 1
+ * in its order, key, value and weight, in the request's own pages; places behind are left as they are, and the pages behind the budget are the caller's to
+ * hand out.  A request with at most `budget` keys stays as it is.  kept_out [batch][num_kv_heads][budget]: the places that the kept keys had, ascending,
+ * -1 behind a shorter request's last; lengths_out [batch]: keys per request now (may be `lengths` itself).  A page may belong to one request of the call only.
+ * max_keys (the most that a request has) chooses launch sizes only.  Of the cache block q_start and num_tokens are not used.  Bad pages and lengths raise
+ * status bits as above.  Asynchronous on `stream`. */
+typedef struct phx_evict_args {
+  float* weights;              /* [num_pages][num_kv_heads][page_size] */
+  int32_t* lengths_out;
+  int32_t* kept_out;
+  int64_t max_keys;
+  int32_t budget;
+  int32_t sinks;
+  int32_t recent;
+  int32_t _pad;
+} phx_evict_args;
+phx_status phx_evict_device(int32_t device, const phx_cache_batch* cache, const phx_evict_args* args, void* stream);
+
 /* Spans of one request's tokens from their parents (host arrays; parent -1: hangs on the cached history, -2: padding;
  * any order, cycles and parents out of range are refused with PHX_E_ARG).  Host code only. */
 phx_status phx_tree_spans(const int32_t* parents, int32_t n, int32_t* spans_out);

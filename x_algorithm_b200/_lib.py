@@ -115,6 +115,21 @@ class TreeArgs(C.Structure):   # phx_tree_args
                 ("sm_scale", C.c_float), ("cap", C.c_float), ("cap_method", C.c_int32), ("_pad", C.c_int32)]
 
 
+class WindowArgs(C.Structure):   # phx_window_args
+    _fields_ = [("attention", TreeArgs), ("positions", C.c_void_p), ("lse_out", C.c_void_p), ("window", C.c_int32), ("sinks", C.c_int32)]
+
+
+class KeyWeightsArgs(C.Structure):   # phx_key_weights_args
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64)] + [(n, C.c_void_p) for n in ("spans", "positions", "lse", "weights", "workspace")] + [
+        ("workspace_bytes", C.c_int64), ("max_keys", C.c_int64)] + [(n, C.c_int32) for n in ("max_tokens", "num_q_heads", "window", "sinks")] + [
+        ("sm_scale", C.c_float), ("cap", C.c_float), ("cap_method", C.c_int32), ("decay", C.c_float)]
+
+
+class EvictArgs(C.Structure):   # phx_evict_args
+    _fields_ = [(n, C.c_void_p) for n in ("weights", "lengths_out", "kept_out")] + [("max_keys", C.c_int64)] + [
+        (n, C.c_int32) for n in ("budget", "sinks", "recent", "_pad")]
+
+
 class LogprobsArgs(C.Structure):   # phx_logprobs_args
     _fields_ = [("logits", C.c_void_p), ("stride", C.c_int64)] + [(n, C.c_void_p) for n in (
         "given", "given_out", "entropy_out", "top_out", "top_ids_out")] + [(n, C.c_int32) for n in (
@@ -232,6 +247,9 @@ SIGNATURES = {
     "phx_history_append_device": (C.c_int32, [C.c_int32, C.POINTER(CacheBatch), C.POINTER(AppendArgs), _P]),
     "phx_tree_workspace_bytes": (C.c_int32, [C.c_int32, C.POINTER(C.c_int64)]),
     "phx_tree_attention_device": (C.c_int32, [C.c_int32, C.POINTER(CacheBatch), C.POINTER(TreeArgs), _P]),
+    "phx_window_attention_device": (C.c_int32, [C.c_int32, C.POINTER(CacheBatch), C.POINTER(WindowArgs), _P]),
+    "phx_key_weights_device": (C.c_int32, [C.c_int32, C.POINTER(CacheBatch), C.POINTER(KeyWeightsArgs), _P]),
+    "phx_evict_device": (C.c_int32, [C.c_int32, C.POINTER(CacheBatch), C.POINTER(EvictArgs), _P]),
     "phx_tree_spans": (C.c_int32, [_P, C.c_int32, _P]),
     "phx_token_logprobs_device": (C.c_int32, [C.c_int32, C.POINTER(LogprobsArgs), _P]),
     "phx_corpus_sync": (C.c_int32, [_P]),

@@ -57,7 +57,10 @@ enum DispatchKind {
   DK_TREE_MMA = 22,         // attention over a paged cache, mma.sync
   DK_TOKEN_LOGPROBS = 23,
   DK_TREE_TC = 24,          // ... tcgen05 / TMEM
-  DK_COUNT = 25
+  DK_KEY_WEIGHTS_MMA = 25,  // attention weight of cached keys, mma.sync
+  DK_KEY_WEIGHTS_TC = 26,   // ... tcgen05 / TMEM
+  DK_CACHE_EVICT = 27,
+  DK_COUNT = 28
 };
 void dispatch_note(int kind);
 

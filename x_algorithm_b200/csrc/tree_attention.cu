@@ -61,15 +61,20 @@ struct TreeSmem {
   TreePlan<32 * TREE_WARPS> plan;
 };
 
-template <int DH, int CAP>
-__device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensorMap& map, TreeSmem<DH>& sm, const TreePiece& pc, int& seq) {
+template <int DH, int CAP, class View>
+__device__ __forceinline__ void tree_mma_piece(const View& t, const CUtensorMap& map, TreeSmem<DH>& sm, const TreePiece& pc, int& seq) {
   constexpr int PIECES = DH / 8, KSTEPS = DH / 16, NT = DH / 8;
+  constexpr bool WINDOW = has_window<View>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = pc.h, b = pc.b, group = t.group;
   const KeyRange kr = key_range(t.c, b);
   const CacheRequest& rq = kr.rq;
   const long long rows = (long long)rq.tokens * group, r0 = (long long)pc.row_tile * ROWS;
-  const int n_tiles = min((kr.keys + KEYS - 1) / KEYS, pc.end * TREE_WARPS);
+  // with a window tiles are counted without the gap between the first keys and the window; `at` is where one lies
+  TileRange range{0, 0, 0};
+  if constexpr (WINDOW) range = tile_range(t, kr, (int)(r0 / group), (int)(min(r0 + ROWS, rows) - 1) / group);
+  auto at_tile = [&](int i) { return WINDOW ? range.at(i / TREE_WARPS) * TREE_WARPS + i % TREE_WARPS : i; };
+  const int n_tiles = WINDOW ? pc.end * TREE_WARPS : min((kr.keys + KEYS - 1) / KEYS, pc.end * TREE_WARPS);
   if (threadIdx.x == 0 && kr.keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
   const int v_off = t.c.num_kv_heads * t.c.page_size;                         // rows of the pool from a key to its value
   const int no_row = (int)(2 * t.c.num_pages * v_off);                        // behind the pool: zeros
@@ -78,33 +83,48 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
 
   {
     // rows lane / 4 and lane / 4 + 8 of the tile: token, its place in the walk, A fragments of the query
-    int pre[2];
+    int pre[2], behind[2] = {0, 0};                    // a row's window: keys whose place is behind
     const uint16_t* qrow[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const long long r = min(r0 + lane / 4 + 8 * i, rows - 1);
       const int tok = (int)(r / group), head = h * group + (int)(r - (long long)tok * group);
       pre[i] = span_of(t, rq, tok).x;
+      if constexpr (WINDOW) behind[i] = place_of(t, rq, tok) - t.window;
       qrow[i] = t.a.q + (long long)(rq.row0 + tok) * t.a.q_stride + head * DH;
+    }
+    int behind_least = min(behind[0], behind[1]), behind_last = max(behind[0], behind[1]);
+    if constexpr (WINDOW) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        behind_least = min(behind_least, __shfl_xor_sync(0xffffffffu, behind_least, o));
+        behind_last = max(behind_last, __shfl_xor_sync(0xffffffffu, behind_last, o));
+      }
     }
     int lo = 0, hi = -2;                               // the places that the tile's rows take in the walk, once they are asked for
     int next = pc.begin * TREE_WARPS + warp;           // the next tile of this warp that may be needed
     int ahead = -1, ahead_page = 0;                    // a tile whose page has been looked up
     auto page_of = [&](int tile) { return kr.table[tile * KEYS / t.c.page_size]; };
-    auto load = [&](int at) {                          // the copy of the next tile that is needed into stage `at`, or a note that there is none
+    auto load = [&](int stage) {                       // the copy of the next tile that is needed into stage `stage`, or a note that there is none
       int tile = -1;
       for (; next < n_tiles; next += TREE_WARPS) {
-        if ((next + 1) * KEYS <= rq.cached) { tile = next; break; }
+        const int at = at_tile(next);
+        if constexpr (WINDOW) {
+          if (at >= (kr.keys + KEYS - 1) / KEYS) break;
+          if ((at + 1) * KEYS <= rq.cached && (at + 1) * KEYS - 1 <= behind_least && at * KEYS >= t.sinks) continue;
+        }
+        if ((at + 1) * KEYS <= rq.cached) { tile = at; break; }
         if (hi == -2) {
           lo = min(pre[0] < 0 ? 0x7fffffff : pre[0], pre[1] < 0 ? 0x7fffffff : pre[1]);
           hi = max(pre[0], pre[1]);
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) { lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o)); }
         }
-        const int key = next * KEYS + (lane & (KEYS - 1)), j = key - rq.cached;   // this lane's key, among the new ones if j >= 0
+        const int key = at * KEYS + (lane & (KEYS - 1)), j = key - rq.cached;   // this lane's key, among the new ones if j >= 0
         bool seen = key < kr.keys && hi >= 0;
         if (seen && j >= 0) { const int2 s = span_of(t, rq, j); seen = s.x <= hi && s.y > lo; }
-        if (__any_sync(0xffffffffu, seen)) { tile = next; break; }
+        if constexpr (WINDOW) { if (seen) seen = key_place(t, rq, key) > behind_least; }
+        if (__any_sync(0xffffffffu, seen)) { tile = at; break; }
       }
       if (tile >= 0) {
         const int key = tile * KEYS, page = tile == ahead ? ahead_page : page_of(tile);
@@ -112,7 +132,7 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
         const int row = ok ? (page * 2 * t.c.num_kv_heads + h) * t.c.page_size + key % t.c.page_size : no_row;
         __syncwarp();                                  // the stage's last reads are done
         if (elect_one()) {
-          const uint32_t bar = smem_u32(&sm.full[warp][at]), dst = kv_smem + at * (2 * KEYS * DH * 2);
+          const uint32_t bar = smem_u32(&sm.full[warp][stage]), dst = kv_smem + stage * (2 * KEYS * DH * 2);
           mbar_expect_tx(bar, 2 * KEYS * DH * 2);
 #pragma unroll
           for (int c = 0; c < (DH + 63) / 64; ++c) {
@@ -121,14 +141,15 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
           }
         }
         if (lane == 0) {
-          sm.there[warp][at] = ok;
+          sm.there[warp][stage] = ok;
           if (!ok) cache_report(t.c, CACHE_BAD_PAGE);
         }
         next += TREE_WARPS;
-        ahead = next;
-        if (ahead < n_tiles) ahead_page = page_of(ahead);
+        ahead = at_tile(next);
+        if (next < n_tiles && (!WINDOW || ahead < (kr.keys + KEYS - 1) / KEYS)) ahead_page = page_of(ahead);
+        else ahead = -1;
       }
-      if (lane == 0) sm.tile[warp][at] = tile;
+      if (lane == 0) sm.tile[warp][stage] = tile;
     };
     const int seq0 = seq;                              // tiles that this warp has taken so far, over all pieces: stage and parity of the next
 #pragma unroll
@@ -169,7 +190,8 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
 
       // seen by every row: cached keys in pages of the pool
       const int key0 = tile * KEYS;
-      const bool whole = key0 + KEYS <= min(rq.cached, kr.keys) && there;
+      bool whole = key0 + KEYS <= min(rq.cached, kr.keys) && there;
+      if constexpr (WINDOW) whole &= key0 > behind_last || key0 + KEYS <= t.sinks;
       uint32_t seen[2] = {0xffu, 0xffu};               // bit 2 n + c: key 8 n + (lane & 3) * 2 + c, for either row
       if (CAP == WIDE_CAP) {
         float most = 0.f;
@@ -202,9 +224,12 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
             const bool ok = key < kr.keys && there;
             int2 span = make_int2(0, 0x7fffffff);      // cached: seen by all
             if (ok && key >= rq.cached) span = span_of(t, rq, key - rq.cached);
+            int place = 0;
+            if constexpr (WINDOW) place = ok ? key_place(t, rq, key) : 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const bool see = ok && span.x <= pre[i] && pre[i] < span.y;
+              bool see = ok && span.x <= pre[i] && pre[i] < span.y;
+              if constexpr (WINDOW) see &= place > behind[i];
               seen[i] |= see ? 1u << (2 * n + c) : 0u;
               if (!see) s[n][2 * i + c] = -INFINITY;
             }
@@ -343,6 +368,7 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
       for (int k = 0; k < 8; ++k) o[k] = none ? 0.f : o[k] * inv;
       const uint4 v = make_uint4(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]), pack_bf2(o[4], o[5]), pack_bf2(o[6], o[7]));
       *reinterpret_cast<uint4*>(t.a.out + ((long long)(rq.row0 + tk) * t.a.num_q_heads + head) * DH + piece * 8) = v;
+      if constexpr (WINDOW) { if (piece == 0) t.lse[(long long)(rq.row0 + tk) * t.a.num_q_heads + head] = none ? -INFINITY : (top + log2f(sum)) * TREE_LN2; }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next piece's tiles are copied over this
     __syncthreads();
@@ -352,8 +378,8 @@ __device__ __forceinline__ void tree_mma_piece(const TreeView& t, const CUtensor
 // blocks that share an SM: by shared memory (72 KB of tiles at key_size 128), and as many registers
 template <int DH> constexpr int mma_blocks() { return DH == 128 ? 3 : 4; }
 
-template <int DH, int CAP>
-__global__ void __launch_bounds__(32 * TREE_WARPS, mma_blocks<DH>()) tree_mma_kernel(const TreeView t, const __grid_constant__ CUtensorMap map) {
+template <int DH, int CAP, class View>
+__global__ void __launch_bounds__(32 * TREE_WARPS, mma_blocks<DH>()) tree_mma_kernel(const View t, const __grid_constant__ CUtensorMap map) {
   extern __shared__ uint8_t smem_bytes[];
   TreeSmem<DH>& sm = *reinterpret_cast<TreeSmem<DH>*>(smem_bytes + ((1024u - (smem_u32(smem_bytes) & 1023u)) & 1023u));
   if (threadIdx.x == 0) {
@@ -368,8 +394,8 @@ __global__ void __launch_bounds__(32 * TREE_WARPS, mma_blocks<DH>()) tree_mma_ke
     const int b = blockIdx.z;
     const KeyRange kr = key_range(t.c, b);
     if (!kr.rq.ok && threadIdx.x == 0) cache_report(t.c, CACHE_BAD_OFFSETS);
-    const int row_tiles = tree_row_tiles(t, kr.rq.tokens), tiles = tree_key_tiles(t, kr.keys);
-    for (int rt = blockIdx.x; rt < row_tiles; rt += gridDim.x) tree_mma_piece<DH, CAP>(t, map, sm, TreePiece{b, (int)blockIdx.y, rt, 0, tiles, tiles}, seq);
+    const int row_tiles = tree_row_tiles(t, kr.rq.tokens), tiles = unit_tiles(t, kr);
+    for (int rt = blockIdx.x; rt < row_tiles; rt += gridDim.x) tree_mma_piece<DH, CAP, View>(t, map, sm, TreePiece{b, (int)blockIdx.y, rt, 0, tiles, tiles}, seq);
   } else {
     sm.plan.make(t);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join's blocks may make their plan beside this
@@ -384,7 +410,7 @@ __global__ void __launch_bounds__(32 * TREE_WARPS, mma_blocks<DH>()) tree_mma_ke
       long long unit_end;
       const TreePiece pc = sm.plan.piece(t, pos, end, &pos, &unit_end);
       if (first && threadIdx.x == 0) sm.plan.note_join(t, blockIdx.x, pc, unit_end);
-      if (pc.begin < pc.end) tree_mma_piece<DH, CAP>(t, map, sm, pc, seq);
+      if (pc.begin < pc.end) tree_mma_piece<DH, CAP, View>(t, map, sm, pc, seq);
     }
   }
   if (*gave_up()) __nanosleep(1000000);                  // copies may still be on their way into this block's memory
@@ -393,8 +419,8 @@ __global__ void __launch_bounds__(32 * TREE_WARPS, mma_blocks<DH>()) tree_mma_ke
 // The parts of a unit that blocks x - 1, x, ... left, joined in the order of the keys: a block takes four rows at a time, one a warp or, of
 // many parts, one after the other with every fourth part a warp
 constexpr int JOIN_WARPS = 4;
-template <int DH>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) tree_join_kernel(const TreeView t) {
+template <int DH, class View>
+__global__ void __launch_bounds__(32 * JOIN_WARPS) tree_join_kernel(const View t) {
   __shared__ float acc_of[JOIN_WARPS][DH];
   __shared__ float sum_of[JOIN_WARPS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -447,31 +473,36 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) tree_join_kernel(const TreeVi
       if (PER == 4) *reinterpret_cast<uint2*>(out) = make_uint2(y[0] | (uint32_t)y[1 % PER] << 16, y[2 % PER] | (uint32_t)y[3 % PER] << 16);
       else if (PER == 2) *reinterpret_cast<uint32_t*>(out) = y[0] | (uint32_t)y[1 % PER] << 16;
       else out[0] = y[0];
+      if constexpr (has_window<View>) { if (lane == 0) t.lse[(long long)(j.token0 + tk) * t.a.num_q_heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * TREE_LN2; }
     }
 }
 
-template <int DH, int CAP>
-phx_status tree_mma_launch(const TreeView& t, cudaStream_t stream, std::string& err) {
+template <int DH, int CAP, class View>
+phx_status tree_mma_launch(const View& t, cudaStream_t stream, std::string& err) {
   constexpr int smem = (int)sizeof(TreeSmem<DH>) + 1024;
   static SmemLimit limit;
-  PHX_CUDA_TRY(limit.raise(tree_mma_kernel<DH, CAP>, smem), err);
+  PHX_CUDA_TRY(limit.raise(tree_mma_kernel<DH, CAP, View>, smem), err);
   CUtensorMap map;
   const phx_status st = tree_pool_map(&map, t, KEYS, err);
   if (st != PHX_OK) return st;
   const long long rows = (long long)t.a.max_tokens * t.group;
   const unsigned tiles = (unsigned)((rows + ROWS - 1) / ROWS < 65535 ? (rows + ROWS - 1) / ROWS : 65535);
   const dim3 grid = t.split ? dim3(t.split) : dim3(tiles, t.c.num_kv_heads, t.c.batch);
-  tree_mma_kernel<DH, CAP><<<grid, 32 * TREE_WARPS, smem, stream>>>(t, map);
+  tree_mma_kernel<DH, CAP, View><<<grid, 32 * TREE_WARPS, smem, stream>>>(t, map);
   PHX_CUDA_TRY(cudaGetLastError(), err);
   dispatch_note(DK_TREE_MMA);
   return PHX_OK;
 }
-template <int DH>
-phx_status tree_mma_launch(const TreeView& t, cudaStream_t stream, std::string& err) {
+template <int DH, class View>
+phx_status tree_mma_launch(const View& t, cudaStream_t stream, std::string& err) {
   // Up to 1000 the exponential form's error, 1e-7 of the cap, is far below the bf16 rounding of the probabilities, and it is the faster one here: 76.6 us against 82.1 for 96
   // single tokens over up to 4096 keys, 103 against 105 (113 with logits around the cap) for prompts of 512 with heads of 32.
   if (t.a.cap_method == 2 && t.a.cap > 1000.0f) return tree_mma_launch<DH, WIDE_CAP>(t, stream, err);
   return t.a.cap_method == 0 ? tree_mma_launch<DH, 0>(t, stream, err) : t.a.cap_method == 1 ? tree_mma_launch<DH, 1>(t, stream, err) : tree_mma_launch<DH, 2>(t, stream, err);
+}
+template <int DH, class View>
+cudaError_t tree_join_launch(const View& t, dim3 grid, cudaStream_t stream) {
+  return launch_programmatic(tree_join_kernel<DH, View>, grid, dim3(32 * JOIN_WARPS), 0, stream, t);
 }
 
 long long part_bytes(int split, int rows, int dh) { return 2ll * split * rows * (dh * 4 + 8) + split * (long long)sizeof(TreeJoin); }
@@ -504,13 +535,17 @@ extern "C" phx_status phx_tree_workspace_bytes(int32_t device, int64_t* bytes_ou
   return PHX_OK;
 }
 
-extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_batch* cache, const phx_tree_args* args, void* stream) {
-  auto bad = [](const char* m) { set_global_error(std::string("phx_tree_attention_device: ") + m); return PHX_E_ARG; };
+namespace {
+
+inline bool is_chain_call(const WindowView& t) { return !t.positions && !t.a.spans; }
+
+// A call of either entry point, its arguments in t.a (and the window's)
+template <class View>
+phx_status attend(int32_t device, const phx_cache_batch* cache, View& t, cudaStream_t st, const char* name) {
+  auto bad = [&](const char* m) { set_global_error(std::string(name) + ": " + m); return PHX_E_ARG; };
   const char* what = cache_check(cache);
   if (*what) return bad(what);
-  if (!args) return bad("null argument");
-  TreeView t;
-  t.c = *cache; t.a = *args;
+  t.c = *cache;
   if (t.a.num_q_heads < 1 || t.a.num_q_heads > 4096 || t.a.num_q_heads % t.c.num_kv_heads != 0) return bad("num_q_heads must be a multiple of num_kv_heads, at most 4096");
   if (t.a.cap_method < 0 || t.a.cap_method > 2) return bad("cap_method must be 0, 1 or 2");
   if (!isfinite(t.a.sm_scale) || !isfinite(t.a.cap)) return bad("sm_scale and cap must be finite");
@@ -527,8 +562,7 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   t.csc = t.a.sm_scale * TREE_LOG2E;
   t.group = t.a.num_q_heads / t.c.num_kv_heads;
   DeviceScope scope(device);
-  if (!scope.ok()) { set_global_error("phx_tree_attention_device: cudaSetDevice failed"); return PHX_E_CUDA; }
-  cudaStream_t st = (cudaStream_t)stream;
+  if (!scope.ok()) { set_global_error(std::string(name) + ": cudaSetDevice failed"); return PHX_E_CUDA; }
   std::string err;
 
   // More than 16 rows a key head are the tensor cores' (tree_attention_sm100.cu); the mma.sync kernel would read the cache again for every 16.
@@ -542,7 +576,12 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
   // 0.84 empty and 32, 64, 128 tiles: 102 / 98, 166 / 177, 299 / 340.  Whole ones cost the empty blocks; shared ones the parts and their join, as wide as a head:
   // about 48 tiles for 128, 24 for 64.  Up to two a block they are shared all the same: lengths are seldom equal.
   const long long units = (long long)t.c.batch * t.c.num_kv_heads * (((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows);
-  const long long tiles = (t.a.max_keys + t.keys - 1) / t.keys;
+  long long tiles = (t.a.max_keys + t.keys - 1) / t.keys;
+  if constexpr (has_window<View>) {                                                       // no more than the first keys', the window's, and the new tokens' that it does not bound
+    const long long in_rows = (t.rows + t.group - 2) / t.group + 1, behind = is_chain_call(t) && in_rows < t.a.max_tokens ? in_rows : t.a.max_tokens;
+    const long long seen = ((long long)t.sinks + t.keys - 1) / t.keys + ((long long)t.window + behind + t.keys - 3) / t.keys + 1;
+    if (seen < tiles) tiles = seen;
+  }
   const long long blocks = per_sm * device_sms(), fed = units * (tiles + t.setup) / (tc ? 8 : 4);   // no block for fewer places: parts and joins take longer than that many
   const long long idle = (units + blocks - 1) / blocks * blocks - units;                  // blocks without a unit in the last round of whole ones
   const bool few = tc ? tiles >= 8 && (units < 2 * blocks || idle * tiles > 3 * t.c.key_size / 8 * blocks) : tiles >= 4 && units < 8 * blocks;
@@ -559,17 +598,37 @@ extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_
     const long long rows = (long long)t.a.max_tokens * t.group;
     const unsigned most = (unsigned)(rows < t.rows ? rows : t.rows);
     const bool many = t.split > JOIN_WARPS * units;                // parts of a unit: a block for each row, else for four
-    const dim3 grid(t.split - 1, many ? most : (most + JOIN_WARPS - 1) / JOIN_WARPS), block(32 * JOIN_WARPS);
-    const cudaError_t e = t.c.key_size == 32 ? launch_programmatic(tree_join_kernel<32>, grid, block, 0, st, t)
-                          : t.c.key_size == 64 ? launch_programmatic(tree_join_kernel<64>, grid, block, 0, st, t)
-                                               : launch_programmatic(tree_join_kernel<128>, grid, block, 0, st, t);
+    const dim3 grid(t.split - 1, many ? most : (most + JOIN_WARPS - 1) / JOIN_WARPS);
+    const cudaError_t e = t.c.key_size == 32 ? tree_join_launch<32>(t, grid, st) : t.c.key_size == 64 ? tree_join_launch<64>(t, grid, st) : tree_join_launch<128>(t, grid, st);
     if (e != cudaSuccess) { err = cudaGetErrorString(e); s = PHX_E_CUDA; }
   }
   if (s != PHX_OK) {
     (void)cudaGetLastError();
-    set_global_error("phx_tree_attention_device: " + err);
+    set_global_error(std::string(name) + ": " + err);
   }
   return s;
+}
+
+}  // namespace
+
+extern "C" phx_status phx_tree_attention_device(int32_t device, const phx_cache_batch* cache, const phx_tree_args* args, void* stream) {
+  if (!args) { set_global_error("phx_tree_attention_device: null argument"); return PHX_E_ARG; }
+  TreeView t;
+  t.a = *args;
+  return attend(device, cache, t, (cudaStream_t)stream, "phx_tree_attention_device");
+}
+
+extern "C" phx_status phx_window_attention_device(int32_t device, const phx_cache_batch* cache, const phx_window_args* args, void* stream) {
+  auto bad = [](const char* m) { set_global_error(std::string("phx_window_attention_device: ") + m); return PHX_E_ARG; };
+  if (!args) return bad("null argument");
+  if (args->window < 0 || args->sinks < 0) return bad("window and sinks must not be negative");
+  WindowView t;
+  t.a = args->attention;
+  t.positions = args->positions; t.lse = args->lse_out;
+  t.window = args->window > 0 ? args->window : 0x7fffffff;
+  t.sinks = args->sinks;
+  if (cache && cache->num_tokens > 0 && cache->batch > 0 && !t.lse) return bad("lse_out is required");
+  return attend(device, cache, t, (cudaStream_t)stream, "phx_window_attention_device");
 }
 
 // Depth-first places of a forest given by parents, without recursion: tokens below each token are counted from the leaves up

@@ -9,11 +9,13 @@
 // 30-60 us.)
 #pragma once
 
+#include <type_traits>
+
 #include "cache_batch.cuh"
 
 namespace phx {
 
-constexpr float TREE_LOG2E = 1.4426950408889634f;
+constexpr float TREE_LOG2E = 1.4426950408889634f, TREE_LN2 = 0.69314718055994531f;
 constexpr int TREE_MAX_SPLIT_BATCH = 1024;      // requests whose tiles the blocks may share
 
 struct TreeView {
@@ -29,6 +31,14 @@ struct TreeView {
   float2* part_ml;       // [2 split][rows]: reference (log2 domain), sum
   struct TreeJoin* join; // [split]: what block x's bound in front leaves to be joined
 };
+// The view of a call with a window: of the keys that a row may see, those whose place is behind the row's place - window, or in front of `sinks`, and the rows' ln sum e^x.
+// (A type of its own, so that calls without one pass the kernels no more than they need.)
+struct WindowView : TreeView {
+  const int* positions;
+  float* lse;
+  int window, sinks;
+};
+template <class View> constexpr bool has_window = std::is_same<View, WindowView>::value;
 // A unit cut by the bound between blocks x - 1 and x, the first that cuts it: block x - 1 has its first tiles, blocks x .. to - 1 the others
 struct TreeJoin {
   int rows;              // 0: nothing to join here
@@ -118,6 +128,39 @@ struct TreePiece {
 __device__ __forceinline__ int tree_row_tiles(const TreeView& t, int tokens) { return (int)(((long long)tokens * t.group + t.rows - 1) / t.rows); }
 __device__ __forceinline__ int tree_key_tiles(const TreeView& t, int keys) { return keys > 0 ? (keys - 1) / t.keys + 1 : 1; }
 
+// The place of new token j, at which its window ends and which a window has to reach for its key to be seen
+__device__ __forceinline__ int place_of(const WindowView& t, const CacheRequest& rq, int j) {
+  return t.positions ? max(rq.cached, t.positions[rq.row0 + j]) : t.a.spans ? rq.cached : rq.cached + j;
+}
+// The same for key `key`, one that every window reaches where it is one of the first
+__device__ __forceinline__ int key_place(const WindowView& t, const CacheRequest& rq, int key) {
+  const int place = key < rq.cached ? key : place_of(t, rq, key - rq.cached);
+  return place < t.sinks ? 0x7fffffff : place;
+}
+// The tiles of keys that rows of some tokens may see: [0, sinks) and [first, end).  A unit's tiles are counted without the gap.
+struct TileRange {
+  int sinks, first, end;
+  __device__ __forceinline__ int at(int i) const { return i < sinks ? i : i - sinks + first; }
+};
+__device__ __forceinline__ bool is_chain(const WindowView& t) { return !t.positions && !t.a.spans; }
+__device__ __forceinline__ TileRange tile_range(const WindowView& t, const KeyRange& k, int token0, int token1) {   // tokens token0 .. token1
+  TileRange r;
+  r.end = tree_key_tiles(t, k.keys);
+  r.sinks = min(r.end, t.sinks > 0 ? (t.sinks - 1) / t.keys + 1 : 0);
+  r.first = max(r.sinks, max(0, k.rq.cached + (is_chain(t) ? token0 : 0) - t.window + 1) / t.keys);
+  if (is_chain(t)) r.end = max(r.sinks, min(r.end, (k.rq.cached + token1) / t.keys + 1));
+  return r;
+}
+// Tiles of a unit of this request: the most that a tile of its rows may see
+__device__ __forceinline__ int unit_tiles(const TreeView& t, const KeyRange& k) { return tree_key_tiles(t, k.keys); }
+__device__ __forceinline__ int unit_tiles(const WindowView& t, const KeyRange& k) {
+  const TileRange r = tile_range(t, k, 0, k.rq.tokens - 1);
+  const int all = r.sinks + max(0, tree_key_tiles(t, k.keys) - r.first);
+  if (!is_chain(t)) return max(1, all);
+  const int tokens = (t.rows + t.group - 2) / t.group + 1;   // that a tile of rows may touch: its windows reach over window + tokens - 1 keys
+  return (int)max(1ll, min((long long)all, r.sinks + ((long long)t.window + tokens + t.keys - 3) / t.keys + 1));
+}
+
 // Places in front of each request, in shared memory; without a split, units
 template <int THREADS> struct TreePlan {
   long long before[TREE_MAX_SPLIT_BATCH + 1];
@@ -125,11 +168,11 @@ template <int THREADS> struct TreePlan {
   long long per_, more_;         // places of a block: per_, the first more_ one more
 
   // by all threads of the block; ends with a barrier
-  __device__ void make(const TreeView& t) {
+  template <class View> __device__ void make(const View& t) {
     const int tid = threadIdx.x, lane = tid & 31, per = (t.c.batch + THREADS - 1) / THREADS, b0 = min(tid * per, t.c.batch), b1 = min(b0 + per, t.c.batch);
     auto tiles_of = [&](int b) {
       const KeyRange k = key_range(t.c, b);
-      return (long long)t.c.num_kv_heads * tree_row_tiles(t, k.rq.tokens) * (t.split ? tree_key_tiles(t, k.keys) + t.setup : 1);
+      return (long long)t.c.num_kv_heads * tree_row_tiles(t, k.rq.tokens) * (t.split ? unit_tiles(t, k) + t.setup : 1);
     };
     long long mine = 0;
     for (int b = b0; b < b1; ++b) mine += tiles_of(b);
@@ -152,10 +195,10 @@ template <int THREADS> struct TreePlan {
     return lo;
   }
   // unit `pos`
-  __device__ __forceinline__ TreePiece unit(const TreeView& t, long long pos) const {
+  template <class View> __device__ __forceinline__ TreePiece unit(const View& t, long long pos) const {
     const int b = request_at(t, pos);
     const KeyRange k = key_range(t.c, b);
-    const int row_tiles = tree_row_tiles(t, k.rq.tokens), in = (int)(pos - before[b]), tiles = tree_key_tiles(t, k.keys);
+    const int row_tiles = tree_row_tiles(t, k.rq.tokens), in = (int)(pos - before[b]), tiles = unit_tiles(t, k);
     return TreePiece{b, in / row_tiles, in % row_tiles, 0, tiles, tiles};
   }
   // the first block whose stretch begins at or behind place `pos`
@@ -179,12 +222,12 @@ template <int THREADS> struct TreePlan {
     t.join[x] = j;
   }
   // the piece from place `pos` on, at most to `end`; `next` is behind it, `unit_end` behind its unit
-  __device__ __forceinline__ TreePiece piece(const TreeView& t, long long pos, long long end, long long* next, long long* unit_end) const {
+  template <class View> __device__ __forceinline__ TreePiece piece(const View& t, long long pos, long long end, long long* next, long long* unit_end) const {
     const int lo = request_at(t, pos);
     const KeyRange k = key_range(t.c, lo);
     TreePiece p;
     p.b = lo;
-    p.tiles = tree_key_tiles(t, k.keys);
+    p.tiles = unit_tiles(t, k);
     const long long in = pos - before[lo], unit = in / (p.tiles + t.setup), unit0 = before[lo] + unit * (p.tiles + t.setup);
     const int row_tiles = tree_row_tiles(t, k.rq.tokens);
     p.h = (int)(unit / row_tiles); p.row_tile = (int)(unit - (long long)p.h * row_tiles);
@@ -202,5 +245,6 @@ bool tree_tc_supported(const TreeView& t);
 void tree_tc_shape(TreeView& t);                 // rows and keys of a tile
 int tree_tc_blocks_per_sm();
 phx_status tree_tc_launch(const TreeView& t, cudaStream_t stream, std::string& err);
+phx_status tree_tc_launch(const WindowView& t, cudaStream_t stream, std::string& err);
 
 }  // namespace phx

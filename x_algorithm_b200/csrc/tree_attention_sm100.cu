@@ -74,13 +74,14 @@ struct TileNote {
 };
 constexpr uint32_t MASKED = 16, LAST = 32, FINAL = 64, BOXES = 15;
 
-template <int DH>
+template <int DH, class View>
 struct TcSmem {
   static constexpr int DCH = DH / 64, NB = tc_buffers(DH);
   uint8_t q[DCH * SLAB];
   uint8_t k[NB][DCH * KT * 128];
   uint8_t v[NB][DCH * KT * 128];
   int2 span[2][KT];                     // of a masked tile's keys
+  int place[2][has_window<View> ? KT : 1];
   TileNote note[8];
   uint64_t q_full, q_empty, k_full[NB], k_empty[NB], v_full[NB], v_empty[NB], s_full[2], p_ready, o_done, o_empty, together;
   uint32_t tmem;
@@ -89,13 +90,13 @@ struct TcSmem {
 };
 
 // The pieces of a block, the same for every role: its stretch of the places, every gridDim.x-th unit, or the units of its place in the grid
-template <int DH>
+template <int DH, class View>
 struct PieceWalk {
-  const TreeView& t;
-  const TcSmem<DH>& sm;
+  const View& t;
+  const TcSmem<DH, View>& sm;
   long long pos, end;
   int row_tile;
-  __device__ __forceinline__ PieceWalk(const TreeView& view, const TcSmem<DH>& mem) : t(view), sm(mem), pos(0), end(0), row_tile(blockIdx.x) {
+  __device__ __forceinline__ PieceWalk(const View& view, const TcSmem<DH, View>& mem) : t(view), sm(mem), pos(0), end(0), row_tile(blockIdx.x) {
     if (t.split) { pos = sm.plan.bound(blockIdx.x); end = sm.plan.bound(blockIdx.x + 1); }
     else if (t.turns) { pos = blockIdx.x; end = sm.plan.all(t); }
   }
@@ -116,21 +117,22 @@ struct PieceWalk {
     }
     const KeyRange k = key_range(t.c, blockIdx.z);
     if (row_tile >= tree_row_tiles(t, k.rq.tokens)) return false;
-    const int tiles = tree_key_tiles(t, k.keys);
+    const int tiles = unit_tiles(t, k);
     *p = TreePiece{(int)blockIdx.z, (int)blockIdx.y, row_tile, 0, tiles, tiles};
     row_tile += gridDim.x;
     return true;
   }
 };
 
-template <int DH, int CAP>
+template <int DH, int CAP, class View>
 struct TcBlock {
+  static constexpr bool WINDOW = has_window<View>;
   static constexpr int DCH = DH / 64, NB = tc_buffers(DH);
   static constexpr uint32_t BLK = DCH * KT * 128, TM_S = 0, TM_O = 128;
-  const TreeView& t;
+  const View& t;
   const CUtensorMap& map_q;
   const CUtensorMap& map_kv;
-  TcSmem<DH>& sm;
+  TcSmem<DH, View>& sm;
   int box;                                                 // rows of a K / V copy
   uint32_t tmem;
 
@@ -139,7 +141,7 @@ struct TcBlock {
   // Its chain of instructions for a tile has to be shorter than the tile's softmax, beside whose warps it issues: pages and spans are asked for a tile
   // ahead, by loads without a condition (a value chosen between a load and a constant waits for the load), and places in pages are counted on, not divided.
   // (8192 tokens that see themselves, 16 heads of 128: 716 us before the first, 577 before the second, 502 then.)
-  __device__ __forceinline__ void produce(PieceWalk<DH> walk) {
+  __device__ __forceinline__ void produce(PieceWalk<DH, View> walk) {
     const int lane = threadIdx.x & 31, boxes = KT / box, page_size = t.c.page_size, v_off = t.c.num_kv_heads * page_size, page_rows = 2 * v_off;
     const int no_row = (int)(t.c.num_pages * page_rows), tokens_per_tile = t.rows / t.group, cols_on = KT / page_size, slots_on = KT % page_size;
     TreePiece pc, after;
@@ -149,14 +151,31 @@ struct TcBlock {
       pc = after;
       const KeyRange kr = key_range(t.c, pc.b);
       const CacheRequest& rq = kr.rq;
-      const int keys = kr.keys, token0 = pc.row_tile * tokens_per_tile, last = min(pc.end, (keys + KT - 1) / KT), last_col = keys > 0 ? (keys - 1) / page_size : 0;
+      const int keys = kr.keys, token0 = pc.row_tile * tokens_per_tile, last_col = keys > 0 ? (keys - 1) / page_size : 0;
+      int begin = pc.begin, last = min(pc.end, (keys + KT - 1) / KT);
+      // with a window: the tiles of the rows, and the places behind which the least and the last of the rows' windows begin
+      TileRange range{0, 0, 0};
+      int behind_least = 0, behind_last = 0;
+      if constexpr (WINDOW) {
+        const int token1 = min(token0 + tokens_per_tile, rq.tokens) - 1;
+        range = tile_range(t, kr, token0, token1);
+        begin = range.at(pc.begin);
+        last = min(min(range.at(pc.end - 1) + 1, (keys + KT - 1) / KT), range.end);
+        if (t.positions) {
+          int least = 0x7fffffff, most = 0;
+          for (int i = token0 + lane; i <= token1; i += 32) { const int p = place_of(t, rq, i); least = min(least, p); most = max(most, p); }
+          behind_least = (int)__reduce_min_sync(0xffffffffu, least) - t.window; behind_last = (int)__reduce_max_sync(0xffffffffu, most) - t.window;
+        } else {
+          behind_least = place_of(t, rq, token0) - t.window; behind_last = place_of(t, rq, token1) - t.window;
+        }
+      }
       const int old_tiles = min(rq.cached, keys) / KT, head_row = pc.h * page_size;   // tiles in front of the first with new keys
       if (lane == 0 && keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
       // box `lane` of the tile that is looked up: column of the table, place in the page, page
       int col, slot, page;
       auto look_up = [&](int tile) { const int key = tile * KT + lane * box; col = key / page_size; slot = key - col * page_size; };
       auto ask_page = [&]() { page = keys > 0 ? kr.table[min(col, last_col)] : -1; };
-      look_up(pc.begin);
+      look_up(begin);
       ask_page();
       if (piece > 0 && !wait(sm.q_empty, piece - 1)) return;
       __syncwarp();
@@ -185,8 +204,15 @@ struct TcBlock {
       // the first tile from `tile` on of which some row sees some key (`last`: none); *masked: not every row every key
       auto next_tile = [&](int tile, bool* masked) {
         for (; tile < last; ++tile) {
+          if constexpr (WINDOW) {
+            if (tile >= range.sinks && tile < range.first) tile = range.first;
+            if (tile >= last) break;
+          }
           *masked = false;
-          if (tile < old_tiles) return tile;
+          if (tile < old_tiles) {
+            if constexpr (WINDOW) *masked = tile * KT <= behind_last && (tile + 1) * KT > t.sinks;
+            return tile;
+          }
           if (hi == -2) places();
           if (spans_of != tile) ask_spans(tile);
           bool any = false, all = true;
@@ -194,8 +220,13 @@ struct TcBlock {
           for (int i = 0; i < KT / 32; ++i) {
             const int key = tile * KT + i * 32 + lane;
             const bool there = key < keys, cached = key < rq.cached;
-            any |= there && (cached || (spans[i].x <= hi && spans[i].y > lo));
-            all &= there && (cached || (spans[i].x <= lo && spans[i].y > hi));
+            bool some = there, every = there;
+            if constexpr (WINDOW) {
+              const int place = there ? key_place(t, rq, key) : 0;
+              some &= place > behind_least; every &= place > behind_last;
+            }
+            any |= some && (cached || (spans[i].x <= hi && spans[i].y > lo));
+            all &= every && (cached || (spans[i].x <= lo && spans[i].y > hi));
           }
           ask_spans(tile + 1);
           any = __any_sync(0xffffffffu, any) && hi >= 0;
@@ -205,9 +236,9 @@ struct TcBlock {
         return last;
       };
       bool masked = false, masked_next = false;
-      int tile = next_tile(pc.begin, &masked);
-      if (tile >= last) { tile = pc.begin; masked = true; }  // a piece that no row sees anything of is one masked tile all the same
-      if (tile != pc.begin) { look_up(tile); ask_page(); }
+      int tile = next_tile(begin, &masked);
+      if (tile >= last) { tile = begin; masked = true; }     // a piece that no row sees anything of is one masked tile all the same
+      if (tile != begin) { look_up(tile); ask_page(); }
       more = walk.next(&after);
       int before[4] = {no_row, no_row, no_row, no_row};      // rows of the pool of the boxes of the tile whose V is still to be asked for
       auto values = [&](int i) {
@@ -314,11 +345,19 @@ struct TcBlock {
     }
   }
 
+  // whether the row at `pre`, whose window begins behind place `behind`, sees key k of the masked tile in buffer `at`
+  __device__ __forceinline__ bool sees(int at, int k, int pre, int behind) const {
+    const int2 sp = sm.span[at][k];
+    bool see = sp.x <= pre && pre < sp.y;
+    if constexpr (WINDOW) see &= sm.place[at][k] > behind;
+    return see;
+  }
+
   // The polynomial and the exponential form of tanh differ in their last bits, so a key that a row does not see must not choose between them.  In a masked tile a row
   // goes by the logits that it sees, 16 keys at a time, in tensor memory and in a loop of its own: beside the code for whole tiles, where a warp takes one form
   // for all, such choices made that code 3 to 20 % slower (registers).  24 trees of 32 over up to 8192 keys, 32 heads of 128: 106 us, 152 with logits around the cap; 110 and 151 when
   // masked tiles were capped there by the warp's choice; 32 x 512 candidates under a cap 97 and 132, were 111 and 128.
-  __device__ __forceinline__ void cap_masked(const TreeCap& cap, uint32_t s_col, const int2* span, int pre) const {
+  __device__ __forceinline__ void cap_masked(const TreeCap& cap, uint32_t s_col, int at, int pre, int behind) const {
     tmem_ld_wait();
 #pragma unroll 1
     for (int c = 0; c < KT / 16; ++c) {
@@ -329,8 +368,7 @@ struct TcBlock {
       float most = 0.f;
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
-        const int2 sp = span[c * 16 + k];
-        if (sp.x <= pre && pre < sp.y) { seen |= 1u << k; most = fmaxf(most, fabsf(x[k])); }
+        if (sees(at, c * 16 + k, pre, behind)) { seen |= 1u << k; most = fmaxf(most, fabsf(x[k])); }
       }
       if (most * cap.small_scale <= TreeCap::SMALL) {
         if (seen != 0) {
@@ -350,7 +388,7 @@ struct TcBlock {
   }
 
   // ---- softmax (128 threads, one a row) ------------------------------------------------------------------------------------
-  __device__ __forceinline__ void softmax(PieceWalk<DH> walk) {
+  __device__ __forceinline__ void softmax(PieceWalk<DH, View> walk) {
     const int lane = threadIdx.x & 31, quad = warp_index() & 3, r = quad * 32 + lane, group = t.group;
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16, all_there = (1u << (KT / box)) - 1;
     const TreeCap cap(t);
@@ -360,13 +398,14 @@ struct TcBlock {
     bool more = walk.next(&after);
     // this row of the piece to come: its request, token, place in the walk
     KeyRange kr_after;
-    int pre_after = -1;
+    int pre_after = -1, behind_after = 0;
     bool valid_after = false;
     auto look = [&]() {
       kr_after = key_range(t.c, after.b);
       const int token = after.row_tile * (t.rows / group) + token_of;
       valid_after = r < t.rows && token < kr_after.rq.tokens;
       pre_after = valid_after ? span_of(t, kr_after.rq, token).x : -1;
+      if constexpr (WINDOW) behind_after = valid_after ? place_of(t, kr_after.rq, token) - t.window : 0;
     };
     if (more) look();
     int j = 0, together = 0;
@@ -374,7 +413,7 @@ struct TcBlock {
       pc = after;
       const KeyRange kr = kr_after;
       const CacheRequest& rq = kr.rq;
-      const int pre = pre_after, token = pc.row_tile * (t.rows / group) + token_of;
+      const int pre = pre_after, behind = behind_after, token = pc.row_tile * (t.rows / group) + token_of;
       const bool valid = valid_after, busy = __any_sync(0xffffffffu, valid);   // a warp without rows only keeps the others company
       float m = valid ? -INFINITY : 0.f, l = 0.f;
       const int first = j;
@@ -396,6 +435,7 @@ struct TcBlock {
             if (key >= kr.keys || !((note.flags >> (r / box)) & 1)) sp = make_int2(0x7fffffff, -1);
             else if (key >= rq.cached) sp = span_of(t, rq, key - rq.cached);
             sm.span[j & 1][r] = sp;
+            if constexpr (WINDOW) sm.place[j & 1][r] = key < kr.keys ? key_place(t, rq, key) : 0;
           }
           // infinities and NaN among the values: out of the product
           if (!wait(sm.v_full[j % NB], j / NB)) return;
@@ -419,7 +459,7 @@ struct TcBlock {
         float alpha = 1.0f;
         if (busy) {
           if (CAP == 2 && masked) {
-            cap_masked(cap, s_col, sm.span[j & 1], pre);
+            cap_masked(cap, s_col, j & 1, pre, behind);
 #pragma unroll
             for (int c = 0; c < KT / 32; ++c) tmem_ld32_nowait(s_col + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
           }
@@ -463,7 +503,7 @@ struct TcBlock {
           }
           if (masked && CAP != 2) {
 #pragma unroll
-            for (int k = 0; k < KT; ++k) { const int2 sp = sm.span[j & 1][k]; if (!(sp.x <= pre && pre < sp.y)) s[k] = -INFINITY; }
+            for (int k = 0; k < KT; ++k) if (!sees(j & 1, k, pre, behind)) s[k] = -INFINITY;
           }
           if (CAP != 2 || masked) bm = top_of();
           // The reference only has to bound the exponentials: it moves when the maximum has outgrown it by 2^8 (P stays below 256, as exact in bf16 as below
@@ -541,15 +581,25 @@ struct TcBlock {
           }
         }
         if (valid && !pc.whole()) t.part_ml[part_row] = none ? make_float2(-INFINITY, 0.f) : make_float2(m, l);
+        if constexpr (WINDOW) { if (valid && pc.whole()) t.lse[(long long)(rq.row0 + token) * t.a.num_q_heads + head] = none ? -INFINITY : (m + log2f(l)) * TREE_LN2; }
       } else {
         mbar_arrive(smem_u32(&sm.o_empty));
       }
       // What the row sees of the infinities and NaN that were taken out of masked tiles, onto what has been stored.  (One of an unmasked tile is in there
       // already: adding it again changes nothing.)
       if (sm.odd[piece & 1] == piece + 1 && valid && !none) {
-        const long long behind = min((long long)pc.end * KT, (long long)kr.keys);
+        TileRange range{0, 0, 0};
+        if constexpr (WINDOW) range = tile_range(t, kr, pc.row_tile * (t.rows / group), min((pc.row_tile + 1) * (t.rows / group), rq.tokens) - 1);
+        const long long end = WINDOW ? pc.end * (long long)KT : min((long long)pc.end * KT, (long long)kr.keys);
 #pragma unroll 1
-        for (int key = pc.begin * KT; key < behind; ++key) {
+        for (long long i = pc.begin * (long long)KT; i < end; ++i) {
+          int key = (int)i;
+          if constexpr (WINDOW) {
+            const long long at = (long long)range.at((int)(i / KT)) * KT + i % KT;
+            if (at >= kr.keys) break;
+            key = (int)at;
+            if (key_place(t, rq, key) <= behind) continue;
+          }
           const int page = kr.table[key / t.c.page_size];
           const int2 sp = key >= rq.cached ? span_of(t, rq, key - rq.cached) : make_int2(0, 0x7fffffff);
           if ((unsigned)page >= (unsigned)t.c.num_pages || !(sp.x <= pre && pre < sp.y)) continue;
@@ -567,10 +617,10 @@ struct TcBlock {
   }
 };
 
-template <int DH, int CAP>
-__global__ void __launch_bounds__(TC_THREADS, 2) tree_tc_kernel(const __grid_constant__ TreeView t, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, int box) {
+template <int DH, int CAP, class View>
+__global__ void __launch_bounds__(TC_THREADS, 2) tree_tc_kernel(const __grid_constant__ View t, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, int box) {
   extern __shared__ uint8_t smem_bytes[];
-  TcSmem<DH>& sm = *reinterpret_cast<TcSmem<DH>*>(smem_bytes + ((1024u - (smem_u32(smem_bytes) & 1023u)) & 1023u));
+  TcSmem<DH, View>& sm = *reinterpret_cast<TcSmem<DH, View>*>(smem_bytes + ((1024u - (smem_u32(smem_bytes) & 1023u)) & 1023u));
   const int warp = warp_index();
   if (threadIdx.x == 0) {
     *gave_up() = 0;
@@ -607,12 +657,12 @@ __global__ void __launch_bounds__(TC_THREADS, 2) tree_tc_kernel(const __grid_con
     for (int b = threadIdx.x; b < t.c.batch; b += TC_THREADS)
       if (!cache_request(t.c, b).ok) cache_report(t.c, CACHE_BAD_OFFSETS);
 
-  TcBlock<DH, CAP> block{t, map_q, map_kv, sm, box, sm.tmem};
-  const PieceWalk<DH> walk(t, sm);
+  TcBlock<DH, CAP, View> block{t, map_q, map_kv, sm, box, sm.tmem};
+  const PieceWalk<DH, View> walk(t, sm);
   if (warp == 0) {
     block.produce(walk);
   } else if (warp == 1) {
-    PieceWalk<DH> mine = walk;
+    PieceWalk<DH, View> mine = walk;
     TreePiece pc;
     if (mine.next(&pc) && elect_one()) block.issue();
   } else {
@@ -640,12 +690,12 @@ phx_status query_map(CUtensorMap* map, const TreeView& t, std::string& err) {
   return PHX_OK;
 }
 
-template <int DH, int CAP>
-phx_status launch(const TreeView& t, cudaStream_t stream, std::string& err) {
-  constexpr int smem = (int)sizeof(TcSmem<DH>) + 1024;
+template <int DH, int CAP, class View>
+phx_status launch(const View& t, cudaStream_t stream, std::string& err) {
+  constexpr int smem = (int)sizeof(TcSmem<DH, View>) + 1024;
   static_assert(2 * (smem + 1024 + 64) <= 228 * 1024, "two blocks share an SM");
   static SmemLimit limit;
-  PHX_CUDA_TRY(limit.raise(tree_tc_kernel<DH, CAP>, smem), err);
+  PHX_CUDA_TRY(limit.raise(tree_tc_kernel<DH, CAP, View>, smem), err);
   int box = KT;                                    // the largest power of two that a page is a multiple of, at most a tile
   while (t.c.page_size % box != 0) box /= 2;
   CUtensorMap map_q, map_kv;
@@ -654,15 +704,19 @@ phx_status launch(const TreeView& t, cudaStream_t stream, std::string& err) {
   if (s != PHX_OK) return s;
   const long long row_tiles = ((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows;
   const dim3 grid = t.split || t.turns ? dim3(t.split ? t.split : t.turns) : dim3((unsigned)(row_tiles < 65535 ? row_tiles : 65535), t.c.num_kv_heads, t.c.batch);
-  tree_tc_kernel<DH, CAP><<<grid, TC_THREADS, smem, stream>>>(t, map_q, map_kv, box);
+  tree_tc_kernel<DH, CAP, View><<<grid, TC_THREADS, smem, stream>>>(t, map_q, map_kv, box);
   PHX_CUDA_TRY(cudaGetLastError(), err);
   dispatch_note(DK_TREE_TC);
   return PHX_OK;
 }
-template <int DH>
-phx_status launch(const TreeView& t, cudaStream_t stream, std::string& err) {
-  if (t.a.cap_method == 0 && !(t.a.sm_scale > 0.f)) return launch<DH, 3>(t, stream, err);
-  return t.a.cap_method == 0 ? launch<DH, 0>(t, stream, err) : t.a.cap_method == 1 ? launch<DH, 1>(t, stream, err) : launch<DH, 2>(t, stream, err);
+template <class View>
+phx_status launch_any(const View& t, cudaStream_t stream, std::string& err) {
+  auto of = [&](auto dh) {
+    constexpr int DH = decltype(dh)::value;
+    if (t.a.cap_method == 0 && !(t.a.sm_scale > 0.f)) return launch<DH, 3>(t, stream, err);
+    return t.a.cap_method == 0 ? launch<DH, 0>(t, stream, err) : t.a.cap_method == 1 ? launch<DH, 1>(t, stream, err) : launch<DH, 2>(t, stream, err);
+  };
+  return t.c.key_size == 64 ? of(std::integral_constant<int, 64>()) : of(std::integral_constant<int, 128>());
 }
 
 }  // namespace
@@ -670,8 +724,7 @@ phx_status launch(const TreeView& t, cudaStream_t stream, std::string& err) {
 bool tree_tc_supported(const TreeView& t) { return (t.c.key_size == 64 || t.c.key_size == 128) && t.group <= QT; }
 void tree_tc_shape(TreeView& t) { t.rows = QT / t.group * t.group; t.keys = KT; t.setup = 6; }
 int tree_tc_blocks_per_sm() { return 2; }
-phx_status tree_tc_launch(const TreeView& t, cudaStream_t stream, std::string& err) {
-  return t.c.key_size == 64 ? launch<64>(t, stream, err) : launch<128>(t, stream, err);
-}
+phx_status tree_tc_launch(const TreeView& t, cudaStream_t stream, std::string& err) { return launch_any(t, stream, err); }
+phx_status tree_tc_launch(const WindowView& t, cudaStream_t stream, std::string& err) { return launch_any(t, stream, err); }
 
 }  // namespace phx

@@ -1,5 +1,6 @@
 """Serving over a cached history: rows enter a paged cache (`history_append`), a tree of new tokens attends to it
-(`tree_attention`), logits become log probabilities, entropy and best alternatives (`token_logprobs`).  torch CUDA tensors in
+(`tree_attention`, or to its first keys and a window: `window_attention`), logits become log probabilities, entropy and best alternatives
+(`token_logprobs`).  What the keys of a cache receive of the attention is added up (`key_weights`), and the keys that received the least leave it (`evict`).  torch CUDA tensors in
 and out, asynchronous on torch's current stream; nothing here waits for what is queued but `check_status`.  `stream`, a raw handle, names another
 as `with torch.cuda.stream(...)` around the call would: what the call allocates is that stream's, and what it reads has to be there and stay until it
 has run.
@@ -23,6 +24,7 @@ from ._lib import PhoenixError, lib
 
 STATUS_BLOCKS = 1024                # cleared at a time, one a stream
 CAP_METHODS = {None: 0, "soft_sign": 1, "tanh": 2}
+_NO_ROWS = object()
 
 
 class _Kept:
@@ -71,10 +73,13 @@ class _Structs(threading.local):
     def __init__(self):
         self.batch, self.append, self.tree, self.logprobs = _lib.CacheBatch(), _lib.AppendArgs(), _lib.TreeArgs(), _lib.LogprobsArgs()
         self.batch_ref, self.append_ref, self.tree_ref, self.logprobs_ref = (C.byref(x) for x in (self.batch, self.append, self.tree, self.logprobs))
+        self.window, self.weights, self.evict = _lib.WindowArgs(), _lib.KeyWeightsArgs(), _lib.EvictArgs()
+        self.window_ref, self.weights_ref, self.evict_ref = (C.byref(x) for x in (self.window, self.weights, self.evict))
 
 
 _structs = _Structs()
 _BATCH, _APPEND, _TREE, _LOGPROBS = (struct.Struct(f).pack_into for f in ("=7q6i", "=8q2ifi", "=7q2i2f2i", "=7q5i2fi"))   # the blocks' fields, in order
+_WINDOW, _WEIGHTS, _EVICT = (struct.Struct(f).pack_into for f in ("=7q2i2f2i2q2i", "=9q4i2fif", "=4q4i"))
 _BF16, _F32, _I32, _I64, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.int64, torch.uint8
 
 
@@ -132,24 +137,25 @@ def _rows(t, name: str, dtype, ndim: int):
 
 
 def _batch(block, pages, q_start, lengths, block_table, tokens: int, device: int, kept: _Kept):
-    """Fills the cache's block; (kv heads, page size, head dim, table columns)."""
+    """Fills the cache's block (q_start _NO_ROWS: a call without new tokens); (kv heads, page size, head dim, table columns)."""
     try:
         num_pages, two, kv_heads, page_size, dh = pages.shape
         batch, cols = block_table.shape
         good = (pages.dtype is _BF16 and pages.get_device() == device and pages.is_contiguous() and two == 2 and
                 block_table.dtype is _I32 and block_table.get_device() == device and (cols < 2 or block_table.stride(1) == 1) and
-                q_start.dtype is _I32 and q_start.get_device() == device and q_start.shape == (batch + 1,) and q_start.is_contiguous() and
+                (q_start is _NO_ROWS or (q_start.dtype is _I32 and q_start.get_device() == device and q_start.shape == (batch + 1,) and q_start.is_contiguous())) and
                 lengths.dtype is _I32 and lengths.get_device() == device and lengths.shape == (batch,) and lengths.is_contiguous())
     except (AttributeError, ValueError, TypeError):
         good = False
     if not good:                                             # say which
         if _rows(pages, "pages", _BF16, 5) != device or _rows(block_table, "block_table", _I32, 2) != device:
             raise ValueError(f"pages and block_table must be on cuda:{device}")
-        _need(q_start, "q_start", _I32, (block_table.shape[0] + 1,), device)
+        if q_start is not _NO_ROWS:
+            _need(q_start, "q_start", _I32, (block_table.shape[0] + 1,), device)
         _need(lengths, "lengths", _I32, (block_table.shape[0],), device)
         raise ValueError("pages must be a contiguous [pages, 2, kv heads, page size, head dim] tensor")
     # one row has no distance to a next, whatever its stride says; rows that overlap (a table broadcast over requests) are refused below
-    _BATCH(block, 0, pages.data_ptr(), num_pages, q_start.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), block_table.stride(0) if batch > 1 else cols,
+    _BATCH(block, 0, pages.data_ptr(), num_pages, 0 if q_start is _NO_ROWS else q_start.data_ptr(), lengths.data_ptr(), block_table.data_ptr(), block_table.stride(0) if batch > 1 else cols,
            kept.status_ptr, cols, page_size, kv_heads, dh, batch, tokens)
     return kv_heads, page_size, dh, cols
 
@@ -237,20 +243,133 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
         out = torch.empty_strided(shape, (heads * dh, dh, 1), dtype=_BF16, device=q.device)
     else:
         _need(out, "out", _BF16, shape, device)
-    if workspace is None:
-        if stream != 0 and torch._C._cuda_isCurrentStreamCapturing():   # (the default stream cannot be captured)
-            workspace = _workspace(device)                   # a graph may be replayed on any stream: it has a workspace of its own, from its own pool
-            space, size = workspace.data_ptr(), workspace.numel()
-        else:
-            space, size = kept.space or _take_space(kept, device)
-    else:
-        size = workspace.numel()
-        space = _need(workspace, "workspace", _U8, (size,), device)
+    space, size = _space(workspace, kept, device, stream)
     _TREE(mine.tree, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, 0 if spans is None else _need(spans, "spans", _I32, (n, 2), device),
           out.data_ptr(), space, size, cols * page_size if max_keys is None else max_keys, n if max_tokens is None else max_tokens, heads,
           math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], 0)
     _ok(lib.phx_tree_attention_device(device, mine.batch_ref, mine.tree_ref, stream))
     return out
+
+
+def _seen(spans, positions, window, sinks, n: int, device: int):
+    """(spans, positions, window, sinks) of a call as its block has them."""
+    if window is not None and not 1 <= window <= 2**31 - 1:
+        raise ValueError("window must be at least 1 key (None: no window)")
+    if not 0 <= sinks <= 2**31 - 1:
+        raise ValueError("sinks must not be negative")
+    return (0 if spans is None else _need(spans, "spans", _I32, (n, 2), device), 0 if positions is None else _need(positions, "positions", _I32, (n,), device),
+            0 if window is None else window, sinks)
+
+
+def _space(workspace, kept, device: int, stream: int):
+    """(address, bytes) of the workspace of a call."""
+    if workspace is not None:
+        size = workspace.numel()
+        return _need(workspace, "workspace", _U8, (size,), device), size
+    if stream != 0 and torch._C._cuda_isCurrentStreamCapturing():   # (the default stream cannot be captured)
+        workspace = _workspace(device)                       # a graph may be replayed on any stream: it has a workspace of its own, from its own pool
+        return workspace.data_ptr(), workspace.numel()
+    return kept.space or _take_space(kept, device)
+
+
+def _queries(q, cache_dh: int, cap: float, cap_method: Optional[str]):
+    if cache_dh != q.shape[2] or (q.shape[1] > 1 and q.stride(1) != cache_dh):
+        raise ValueError("q must have the cache's head dim, its heads side by side")
+    if cap_method not in CAP_METHODS:
+        raise ValueError(f"cap_method must be one of {list(CAP_METHODS)}")
+    if cap > 0 and cap_method is None:
+        raise ValueError("a cap needs its cap_method")
+
+
+def window_attention(q, pages, q_start, lengths, block_table, spans=None, positions=None, *, window: Optional[int], sinks: int = 0, sm_scale: Optional[float] = None,
+                     cap: float = 0.0, cap_method: Optional[str] = None, max_tokens: Optional[int] = None, max_keys: Optional[int] = None, out=None, lse=None,
+                     workspace=None, stream: Optional[int] = None):
+    """`tree_attention` over a window and the first keys of the cache, with the rows' statistics: of the keys that it may see, a token at place p sees those at places behind
+    p - window (None: all) and the first `sinks`.  A cached key's place is its number; a new token's is positions int32 [N], at least lengths (in a tree: lengths +
+    depth), by default lengths + i in a chain and lengths for tokens with spans.  Pages between the first keys and a window are not read.  Returns (bf16 [N, heads,
+    head dim], the logits' ln sum exp fp32 [N, heads], -inf where a token sees nothing)."""
+    device = _rows(q, "q", _BF16, 3)
+    if _elsewhere(device, stream):
+        with _under(device, stream):
+            return window_attention(q, pages, q_start, lengths, block_table, spans, positions, window=window, sinks=sinks, sm_scale=sm_scale, cap=cap, cap_method=cap_method,
+                                    max_tokens=max_tokens, max_keys=max_keys, out=out, lse=lse, workspace=workspace)
+    n, heads, dh = shape = q.shape
+    stream = _stream(device, stream)
+    kept, mine = _keep(device, stream), _structs
+    _, page_size, cache_dh, cols = _batch(mine.batch, pages, q_start, lengths, block_table, n, device, kept)
+    _queries(q, cache_dh, cap, cap_method)
+    spans, positions, window, sinks = _seen(spans, positions, window, sinks, n, device)
+    if out is None:
+        out = torch.empty_strided(shape, (heads * dh, dh, 1), dtype=_BF16, device=q.device)
+    else:
+        _need(out, "out", _BF16, shape, device)
+    if lse is None:
+        lse = torch.empty_strided((n, heads), (heads, 1), dtype=_F32, device=q.device)
+    else:
+        _need(lse, "lse", _F32, (n, heads), device)
+    space, size = _space(workspace, kept, device, stream)
+    _WINDOW(mine.window, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, spans, out.data_ptr(), space, size, cols * page_size if max_keys is None else max_keys,
+            n if max_tokens is None else max_tokens, heads, math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], 0, positions, lse.data_ptr(), window, sinks)
+    _ok(lib.phx_window_attention_device(device, mine.batch_ref, mine.window_ref, stream))
+    return out, lse
+
+
+def key_weights(q, pages, q_start, lengths, block_table, lse, weights, spans=None, positions=None, *, window: Optional[int] = None, sinks: int = 0,
+                sm_scale: Optional[float] = None, cap: float = 0.0, cap_method: Optional[str] = None, decay: float = 1.0, max_tokens: Optional[int] = None,
+                max_keys: Optional[int] = None, workspace=None, stream: Optional[int] = None):
+    """The attention weight that every key of the requests receives from the new tokens, summed over them and the queries of the key's head, joins weights fp32 [num_pages,
+    kv heads, page size], in place: decay * weight + sum for cached keys, the sum alone for new ones.  lse fp32 [N, heads] is what `window_attention` gave for the same
+    queries, spans, positions, window, sinks, scale and cap (a row with an infinite one adds nothing).  Returns weights."""
+    device = _rows(q, "q", _BF16, 3)
+    if _elsewhere(device, stream):
+        with _under(device, stream):
+            return key_weights(q, pages, q_start, lengths, block_table, lse, weights, spans, positions, window=window, sinks=sinks, sm_scale=sm_scale, cap=cap,
+                               cap_method=cap_method, decay=decay, max_tokens=max_tokens, max_keys=max_keys, workspace=workspace)
+    n, heads, dh = q.shape
+    stream = _stream(device, stream)
+    kept, mine = _keep(device, stream), _structs
+    kv_heads, page_size, cache_dh, cols = _batch(mine.batch, pages, q_start, lengths, block_table, n, device, kept)
+    _queries(q, cache_dh, cap, cap_method)
+    spans, positions, window, sinks = _seen(spans, positions, window, sinks, n, device)
+    lse_ptr = _need(lse, "lse", _F32, (n, heads), device)
+    weights_ptr = _need(weights, "weights", _F32, (pages.shape[0], kv_heads, page_size), device)
+    space, size = _space(workspace, kept, device, stream)
+    _WEIGHTS(mine.weights, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, spans, positions, lse_ptr, weights_ptr, space, size,
+             cols * page_size if max_keys is None else max_keys, n if max_tokens is None else max_tokens, heads, window, sinks,
+             math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], decay)
+    _ok(lib.phx_key_weights_device(device, mine.batch_ref, mine.weights_ref, stream))
+    return weights
+
+
+def evict(weights, pages, lengths, block_table, *, budget: int, sinks: int = 0, recent: int = 0, max_keys: Optional[int] = None, lengths_out=None, kept=None,
+          stream: Optional[int] = None):
+    """Requests with more than `budget` keys keep, in each key head, the first `sinks`, the last `recent`, and of the others the ones with the largest weights (ties: the
+    earlier); keys, values and weights move together in their order, in place, to the front of the request's own pages.  Returns (lengths int32 [B] now, the
+    places that the kept keys had, ascending, int32 [B, kv heads, budget], -1 behind the last of a shorter request).  lengths_out may be `lengths`.  A page may belong
+    to one request of the call only; the pages behind a request's new length are the caller's to hand out."""
+    device = _rows(weights, "weights", _F32, 3)
+    if _elsewhere(device, stream):
+        with _under(device, stream):
+            return evict(weights, pages, lengths, block_table, budget=budget, sinks=sinks, recent=recent, max_keys=max_keys, lengths_out=lengths_out, kept=kept)
+    stream = _stream(device, stream)
+    mine = _structs
+    kv_heads, page_size, _, cols = _batch(mine.batch, pages, _NO_ROWS, lengths, block_table, 0, device, _keep(device, stream))
+    _need(weights, "weights", _F32, (pages.shape[0], kv_heads, page_size), device)
+    if not (1 <= budget <= 2**31 - 1 and sinks >= 0 and recent >= 0 and sinks + recent <= budget):
+        raise ValueError("budget must be at least 1 and hold sinks + recent keys")
+    batch = block_table.shape[0]
+    if lengths_out is None:
+        lengths_out = torch.empty_strided((batch,), (1,), dtype=_I32, device=weights.device)
+    else:
+        _need(lengths_out, "lengths_out", _I32, (batch,), device)
+    shape = (batch, kv_heads, budget)
+    if kept is None:
+        kept = torch.empty_strided(shape, (kv_heads * budget, budget, 1), dtype=_I32, device=weights.device)
+    else:
+        _need(kept, "kept", _I32, shape, device)
+    _EVICT(mine.evict, 0, weights.data_ptr(), lengths_out.data_ptr(), kept.data_ptr(), cols * page_size if max_keys is None else max_keys, budget, sinks, recent, 0)
+    _ok(lib.phx_evict_device(device, mine.batch_ref, mine.evict_ref, stream))
+    return lengths_out, kept
 
 
 def token_logprobs(logits, given=None, *, top_k: int = 0, cap: float = 0.0, temperature: float = 1.0, stream: Optional[int] = None):
