@@ -287,3 +287,54 @@ def test_evict(case, values):
     assert torch.equal(lengths, want[2]) and torch.equal(kept, want[3])
     assert torch.equal(c["pages"].view(torch.int16), want[0].view(torch.int16))
     assert torch.equal(c["weights"].view(torch.int32), want[1].view(torch.int32))
+
+
+MANY_ROWS = [
+    (1, 17, 40, 4, 4, 64, 16, "chain", None),
+    (2, 700, 900, 24, 8, 128, 48, "chain", None),
+    (2, 333, 0, 10, 2, 64, 16, "whole", None),
+    (1, 2048, 60, 16, 2, 64, 64, "isolated", None),
+    (1, 1500, 100, 16, 4, 128, 128, "whole", None),
+    (1, 900, 3000, 32, 1, 64, 32, "chain", None),
+    (1, 4, 300, 128, 1, 128, 32, "chain", None),
+    (4, 64, 700, 8, 8, 64, 48, "tree", "spread"),
+]
+
+
+@pytest.mark.parametrize("shape", MANY_ROWS, ids=lambda s: "-".join(map(str, s)))
+@pytest.mark.parametrize("window,sinks", [(None, 0), (130, 4), (1, 200)])
+def test_key_weights_of_many_rows(shape, window, sinks):
+    """The tensor cores' kernel: groups that do not divide a tile, rows in chunks that are joined, hints that say too little."""
+    from x_algorithm_b200 import decoding
+    from x_algorithm_b200.engine import dispatch_counts
+    c = make_case(*shape[:-1], seed=11, positions=shape[-1], padding=3 if shape[-2] != "chain" else 0, stride=24)
+    args = (c["q"], c["pages"], c["q_start"], c["lengths"], c["table"])
+    lse = plain(c, window, sinks)[1].float()
+    lse[::7, 0] = math.inf                                    # rows that the caller leaves out
+    lse[3 % len(lse), -1] = -math.inf
+    before = dispatch_counts()["key_weights.tcgen05"]
+    for decay in (1.0, 0.5):
+        want, tol = plain_weights(c, lse, window, sinks, decay=decay)
+        first = None
+        for hints in ({}, dict(max_tokens=max(c["n_new"]), max_keys=max(a + b for a, b in zip(c["n_new"], c["n_old"]))), dict(max_tokens=17 * 4, max_keys=1)):
+            got = decoding.key_weights(*args, lse, c["weights"].clone(), c["spans"], c["positions"], window=window, sinks=sinks, decay=decay, **hints)
+            close(got, want, tol, f"weights, decay {decay}, {hints}")
+            if hints == {}:
+                first = got
+        again = decoding.key_weights(*args, lse, c["weights"].clone(), c["spans"], c["positions"], window=window, sinks=sinks, decay=decay)
+        assert torch.equal(again, first)                      # the order of every sum follows from the sizes
+    assert dispatch_counts()["key_weights.tcgen05"] > before
+    decoding.check_status()
+
+
+def test_key_weights_of_more_requests_than_a_block_plans():
+    from x_algorithm_b200 import decoding
+    c = make_case(1500, 20, 40, 4, 2, 64, 16, "chain", seed=2)
+    args = (c["q"], c["pages"], c["q_start"], c["lengths"], c["table"])
+    lse = plain(c, None, 0)[1].float()
+    got = decoding.key_weights(*args, lse, c["weights"].clone())
+    close(got, *plain_weights(c, lse, None, 0), "weights")
+    out, got_lse = decoding.window_attention(*args, window=13, sinks=2)
+    want, want_lse, tol, tol_lse = plain(c, 13, 2)
+    close(out, want, tol, "out")
+    close(got_lse, want_lse, tol_lse, "lse")

@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(32 * KW_WARPS, DH == 128 && NB == 2 ? 1 : 2) k
     if (!rq.ok) cache_report(t.c, CACHE_BAD_OFFSETS);
     if (kr.keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
   }
-  const TreeCap cap(t);
+  const WeightCap cap(t);
   const int rows = rq.tokens * group;
   // tiles of 16 keys, without those between the first keys and the first token's window - unless their weights fade
   const int tiles = (kr.keys + KW_KEYS - 1) / KW_KEYS;
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(32 * KW_WARPS, DH == 128 && NB == 2 ? 1 : 2) k
           for (int j = 0; j < 4; ++j) s[n][j] *= t.csc;
         } else if (CAP == 1) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[n][j] = cap.of<1>(s[n][j]);
+          for (int j = 0; j < 4; ++j) s[n][j] = cap.form.of<1>(s[n][j]);
         } else {
           cap.of_any(s[n][0], s[n][1]); cap.of_any(s[n][2], s[n][3]);
         }
@@ -243,6 +243,7 @@ extern "C" phx_status phx_key_weights_device(int32_t device, const phx_cache_bat
   if ((long long)t.c.num_tokens * t.a.num_q_heads > 2147483647ll) return bad("num_tokens x num_q_heads must fit 31 bits");
   if (!t.a.q || !aligned16(t.a.q)) return bad("q must be a 16-byte aligned buffer");
   if (!t.lse || !t.weights) return bad("lse and weights are required");
+  if (t.a.workspace_bytes < 0 || (t.a.workspace_bytes > 0 && (!t.a.workspace || !aligned16(t.a.workspace)))) return bad("workspace must be a 16-byte aligned buffer");
   if ((reinterpret_cast<uintptr_t>(t.a.spans) & 7) != 0) return bad("spans must be 8-byte aligned");
   if (t.c.num_pages == 0) return bad("an empty pool has no keys");
   const long long columns = (long long)t.c.table_cols * t.c.page_size;
@@ -255,7 +256,7 @@ extern "C" phx_status phx_key_weights_device(int32_t device, const phx_cache_bat
   if (!scope.ok()) { set_global_error("phx_key_weights_device: cudaSetDevice failed"); return PHX_E_CUDA; }
   std::string err;
   cudaStream_t st = (cudaStream_t)stream;
-  const phx_status s = t.c.key_size == 32 ? launch<32>(t, st, err) : t.c.key_size == 64 ? launch<64>(t, st, err) : launch<128>(t, st, err);
+  const phx_status s = weights_tc_supported(t) ? weights_tc_launch(t, st, err) : t.c.key_size == 32 ? launch<32>(t, st, err) : t.c.key_size == 64 ? launch<64>(t, st, err) : launch<128>(t, st, err);
   if (s != PHX_OK) {
     (void)cudaGetLastError();
     set_global_error("phx_key_weights_device: " + err);

@@ -1,0 +1,473 @@
+// The attention weight that cached keys receive, on Blackwell tensor cores (tcgen05 + TMEM + TMA), for requests of more than 16 query rows a key head; the semantics are
+// key_weights.cu's.  S^T = K Q^T: 128 keys are the rows of the product and 128 query rows its columns, so that a key's sum over the queries is the sum along one thread's row of
+// tensor memory, and no thread needs another's.  A block (one an SM) takes unit after unit - a request, key head and tile of 128 keys, with all tiles of rows or a
+// chunk of them - K once, then the tiles of rows that see one of its keys:
+//   warp 0      producer: K (page by page) and Q tiles by TMA, the rows' lse and what they see, and which of a tile's four groups of 32 rows have rows at all, and
+//               some key that some row does not see; what its 128 keys are, once a unit
+//   warp 1      MMA issuer: S^T into one of four buffers of tensor memory
+//   warps 4-11  thread = key and 64 of the rows: e^(x - lse) summed up in a register; at the unit's end one half hands its sums to the other, which writes the weight (or
+//               a part, where chunks of rows are joined by key_weights_join_kernel)
+// Waits are bounded; when one runs out the flag is raised, every later wait of any role fails at once, and a role whose wait failed is done.
+#include <string.h>
+
+#include <string>
+
+#include "key_weights.cuh"
+#include "sm100_ptx.cuh"
+
+namespace phx {
+namespace {
+
+using namespace sm100;
+
+constexpr int KT = 128, RT = 128;        // keys and rows of a tile
+constexpr int KW_THREADS = 384, KW_FIRST = 4, KW_SUM = 8;   // warps 4 .. 11 sum
+constexpr int NK = 2, NS = 4;            // K tiles in shared memory, S^T buffers in tensor memory
+__host__ __device__ constexpr int q_buffers(int dh) { return dh == 64 ? 4 : 3; }
+constexpr int NU = 8;                    // units whose keys are described: none begins before the tile NS in front of its first has been read
+
+struct RowNote { float lse[RT]; int2 sees[RT]; };   // lse in the log2 domain, infinite: no weight; (place in the walk or -1, place behind which the window begins)
+struct KeyNote { int x, y, place, at; };            // span, place in the window's terms, word of the weights or -1: no key
+constexpr uint32_t ROWS_OF = 0xf, MASKED_AT = 4, LAST = 256, FINAL = 512;   // bits 0-3: the group has rows, 4-7: and some do not see some key
+
+template <int DH>
+struct KwSmem {
+  static constexpr int DCH = DH / 64, NQ = q_buffers(DH);
+  uint8_t k[NK][DCH * KT * 128];
+  uint8_t q[NQ][DCH * RT * 128];
+  RowNote rows[NS];
+  KeyNote keys[NU][KT];
+  float half[NU][KT];
+  uint32_t flags[NS];
+  int part[NS];                          // of the tile's unit: the place of its sums among the parts
+  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], rows_full[NS], s_full[NS], s_empty[NS], half_full[NU];
+  uint32_t tmem;
+  TreePlan<KW_THREADS> plan;
+};
+
+struct KwUnit { int b, h, key_tile, chunk; };
+
+// The tiles of keys that rows may see; all of them where weights fade
+__device__ __forceinline__ TileRange key_tiles(const WeightsView& t, const KeyRange& k) {
+  const int all = (k.keys + KT - 1) / KT;
+  if (t.decay != 1.0f || all == 0) return TileRange{all, all, all};
+  return tile_range(t, k, 0, k.rq.tokens - 1);
+}
+__device__ __forceinline__ long long key_tiles_of(const WeightsView& t, const KeyRange& k) {
+  if (k.rq.tokens == 0 && t.decay == 1.0f) return 0;
+  const TileRange r = key_tiles(t, k);
+  return r.sinks + max(0, r.end - r.first);
+}
+
+// What the join finds in front of the parts
+struct PartsHead { long long units; int chunks, pad; };
+__host__ __device__ constexpr long long parts_bytes(long long units, int chunks) { return (long long)sizeof(PartsHead) + units * KT * 4 * (chunks + 1); }
+
+template <int DH, int CAP>
+struct KwBlock {
+  static constexpr int DCH = DH / 64, NQ = q_buffers(DH);
+  static constexpr uint32_t BLK = DCH * KT * 128;
+  const WeightsView& t;
+  const CUtensorMap& map_q;
+  const CUtensorMap& map_k;
+  KwSmem<DH>& sm;
+  int box, chunks;                       // chunks that a request's tiles of rows are taken in
+  uint32_t tmem;
+
+  __device__ __forceinline__ bool wait(const uint64_t& bar, int phase) const { return mbar_wait(smem_u32(&bar), (uint32_t)(phase & 1), t.c.status_dev); }
+
+  // unit `pos` of the call
+  __device__ __forceinline__ KwUnit unit_at(long long pos) const {
+    KwUnit u;
+    u.b = sm.plan.request_at(t, pos / chunks);
+    const KeyRange k = key_range(t.c, u.b);
+    long long in = pos - sm.plan.before[u.b] * chunks;
+    u.chunk = (int)(in % chunks); in /= chunks;
+    u.h = (int)(in % t.c.num_kv_heads);
+    u.key_tile = key_tiles(t, k).at((int)(in / t.c.num_kv_heads));
+    return u;
+  }
+
+  // ---- producer (a whole warp; one lane issues) ----
+  __device__ __forceinline__ void produce(long long units) {
+    const int lane = threadIdx.x & 31, boxes = KT / box, page_size = t.c.page_size, page_rows = 2 * t.c.num_kv_heads * page_size;
+    const int no_row = (int)(t.c.num_pages * page_rows), group = t.group, per_tile = t.rows / group;   // tokens of a tile
+    int j = 0, n = 0;                                       // tiles and units so far
+    for (long long pos = blockIdx.x; pos < units; pos += gridDim.x, ++n) {
+      const KwUnit u = unit_at(pos);
+      const KeyRange kr = key_range(t.c, u.b);
+      const CacheRequest& rq = kr.rq;
+      const int key0 = u.key_tile * KT, tiles = (rq.tokens + per_tile - 1) / per_tile, per = (tiles + chunks - 1) / chunks;
+      int begin = min(u.chunk * per, tiles), end = min(begin + per, tiles);
+      if (lane == 0 && u.key_tile == 0 && u.h == 0 && u.chunk == 0 && kr.keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
+      // ---- K, box by box
+      if (!wait(sm.k_empty[n % NK], n / NK - 1)) return;    // the first wait passes
+      int page = -1;
+      bool there = false;
+      if (lane < boxes && key0 + lane * box < kr.keys) {
+        const int key = key0 + lane * box, col = key / page_size;
+        page = kr.table[col];
+        there = (unsigned)page < (unsigned)t.c.num_pages;
+        if (!there) cache_report(t.c, CACHE_BAD_PAGE);
+      }
+      const int row = there ? page * page_rows + u.h * page_size + (key0 + lane * box) % page_size : no_row;
+      __syncwarp();
+      if (elect_one()) mbar_expect_tx(smem_u32(&sm.k_full[n % NK]), BLK);
+      __syncwarp();
+      for (int p = 0; p < boxes; ++p) {
+        const int at = __shfl_sync(0xffffffffu, row, p);
+        if (elect_one())
+          for (int c = 0; c < DCH; ++c) tma_load_2d(smem_u32(sm.k[n % NK]) + c * KT * 128 + p * box * 128, &map_k, smem_u32(&sm.k_full[n % NK]), c * 64, at);
+        __syncwarp();
+      }
+      // ---- this lane's four keys: what a row has to be to see all of them, or any
+      KeyNote mine[KT / 32];
+      int x_most = -1, y_least = 0x7fffffff, place_least = 0x7fffffff, x_least = 0x7fffffff, y_most = -1, place_most = -1;
+#pragma unroll
+      for (int i = 0; i < KT / 32; ++i) {
+        const int in = i * 32 + lane, key = key0 + in;
+        const int owner = in / box, of = __shfl_sync(0xffffffffu, page, owner);
+        const bool ok = __shfl_sync(0xffffffffu, (int)there, owner) && key < kr.keys;
+        KeyNote m{0x7fffffff, -1, 0, -1};
+        if (ok) {
+          m.x = 0; m.y = 0x7fffffff;
+          if (key >= rq.cached) { const int2 s = span_of(t, rq, key - rq.cached); m.x = s.x; m.y = s.y; }
+          m.place = key_place(t, rq, key);
+          m.at = (of * t.c.num_kv_heads + u.h) * page_size + key % page_size;
+          if (key >= rq.cached) m.at = -2 - m.at;           // a new key: no weight before
+          x_least = min(x_least, m.x); y_most = max(y_most, m.y); place_most = max(place_most, m.place);
+        }
+        x_most = max(x_most, m.x); y_least = min(y_least, m.y); place_least = min(place_least, ok ? m.place : -1);
+        mine[i] = m;
+      }
+      x_most = __reduce_max_sync(0xffffffffu, x_most); y_least = __reduce_min_sync(0xffffffffu, y_least); place_least = __reduce_min_sync(0xffffffffu, place_least);
+      x_least = __reduce_min_sync(0xffffffffu, x_least); y_most = __reduce_max_sync(0xffffffffu, y_most); place_most = __reduce_max_sync(0xffffffffu, place_most);
+
+      // ---- tiles of rows.  In a chain those in front of the keys, and those whose windows lie behind them, are not looked at.
+      if (is_chain(t)) {
+        if (key0 > rq.cached) begin = max(begin, min(end, (key0 - rq.cached) / per_tile));
+        if (key0 >= t.sinks) end = max(begin, (int)min((long long)end, ((long long)key0 + KT - 1 + t.window - rq.cached - 1 + per_tile) / per_tile));
+      }
+      // rows 4 groups of 32: row r is token r / group, head r % group
+      struct Ask { float lse[4]; int pre[4], behind[4]; } ask;
+      auto ask_rows = [&](int tile) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int r = g * 32 + lane, token = tile * per_tile + r / group;
+          const bool valid = r < t.rows && token < rq.tokens;
+          ask.lse[g] = INFINITY; ask.pre[g] = -1; ask.behind[g] = 0;
+          if (valid) {
+            ask.lse[g] = t.lse[(long long)(rq.row0 + token) * t.a.num_q_heads + u.h * group + r % group];
+            ask.pre[g] = span_of(t, rq, token).x;
+            ask.behind[g] = place_of(t, rq, token) - t.window;
+          }
+        }
+      };
+      auto look = [&](int tile, uint32_t* flags) {           // of the rows asked for
+        uint32_t f = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (isinf(ask.lse[g])) ask.pre[g] = -1;
+          const bool live = ask.pre[g] >= 0;
+          if (!live) { ask.lse[g] = INFINITY; ask.pre[g] = -0x7fffffff - 1; }
+          const bool any = live && ask.pre[g] >= x_least && ask.pre[g] < y_most && place_most > ask.behind[g];
+          const bool all = live && x_most <= ask.pre[g] && ask.pre[g] < y_least && place_least > ask.behind[g];
+          if (__any_sync(0xffffffffu, any)) f |= 1u << g;
+          if (!__all_sync(0xffffffffu, all)) f |= 1u << (MASKED_AT + g);
+        }
+        *flags = f;
+        return (f & ROWS_OF) != 0;
+      };
+      // the first tile from `tile` on with a token that may see new keys alone, by the tokens' places; 128 tokens a round trip
+      const bool sparse = t.a.spans && key0 >= rq.cached;
+      auto candidate = [&](int tile) {
+        if (!sparse) return tile;
+        for (int tok = tile * per_tile; tok < min(end * per_tile, rq.tokens); tok += 128) {
+          int pre[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pre[i] = span_of(t, rq, min(tok + i * 32 + lane, rq.tokens - 1)).x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t hit = __ballot_sync(0xffffffffu, tok + i * 32 + lane < rq.tokens && pre[i] >= x_least && pre[i] < y_most);
+            if (hit) return (tok + i * 32 + __ffs(hit) - 1) / per_tile;
+          }
+        }
+        return end;
+      };
+      uint32_t flags = 0, flags_next = 0;
+      int tile = begin;
+      bool found = false;
+      while (!found && (tile = candidate(tile)) < end) {
+        ask_rows(tile);
+        found = look(tile, &flags);
+        if (!found) ++tile;
+      }
+      if (!found) { tile = max(0, min(begin, tiles - 1)); flags = 0; }   // no row sees any: a tile without rows, which ends the unit all the same
+      for (bool first = true;; first = false) {
+        const Ask now = ask;
+        int next = tile + 1;
+        if (found && next < end) ask_rows(next);             // on its way under what follows
+        if (!wait(sm.q_empty[j % NQ], j / NQ - 1)) return;
+        if (!wait(sm.s_empty[j % NS], j / NS - 1)) return;
+        __syncwarp();
+        if (elect_one()) {
+          mbar_expect_tx(smem_u32(&sm.q_full[j % NQ]), DCH * t.rows * 128);
+          for (int c = 0; c < DCH; ++c)
+            tma_load_3d(smem_u32(sm.q[j % NQ]) + c * RT * 128, &map_q, smem_u32(&sm.q_full[j % NQ]), c * 64, u.h * group, rq.row0 + tile * per_tile);
+        }
+        __syncwarp();
+        if (first) {
+#pragma unroll
+          for (int i = 0; i < KT / 32; ++i) sm.keys[n % NU][i * 32 + lane] = mine[i];
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          sm.rows[j % NS].lse[g * 32 + lane] = found ? now.lse[g] * TREE_LOG2E : INFINITY;
+          sm.rows[j % NS].sees[g * 32 + lane] = make_int2(now.pre[g], now.behind[g]);
+        }
+        bool more = false;
+        if (found) {
+          for (bool asked = true; next < end; asked = false) {
+            if (!asked) { next = candidate(next); if (next >= end) break; ask_rows(next); }
+            if (look(next, &flags_next)) { more = true; break; }
+            ++next;
+          }
+        }
+        if (lane == 0) sm.flags[j % NS] = flags | (more ? 0u : LAST | (pos + gridDim.x < units ? 0u : FINAL));
+        if (lane == 0) sm.part[j % NS] = (int)(pos / chunks) * chunks + u.chunk;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.rows_full[j % NS]));
+        ++j;
+        if (!more) break;
+        tile = next; flags = flags_next;
+      }
+    }
+  }
+
+  // ---- MMA issuer (one thread) ----
+  __device__ __forceinline__ void issue() {
+    constexpr uint32_t idesc = make_idesc(KT, RT);
+    int n = 0;
+    bool first = true;
+    for (int j = 0;; ++j) {
+      if (!wait(sm.rows_full[j % NS], j / NS)) return;
+      const uint32_t flags = sm.flags[j % NS];
+      if (first && !wait(sm.k_full[n % NK], n / NK)) return;
+      if (!wait(sm.q_full[j % NQ], j / NQ)) return;         // (the producer has waited for the buffer of S^T)
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < DCH; ++c) {
+        const uint64_t kd = make_smem_desc(smem_u32(sm.k[n % NK]) + c * KT * 128), qd = make_smem_desc(smem_u32(sm.q[j % NQ]) + c * RT * 128);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_bf16(tmem + (j % NS) * RT, kd + (uint64_t)(k * 2), qd + (uint64_t)(k * 2), idesc, (c | k) != 0);
+      }
+      umma_commit(smem_u32(&sm.q_empty[j % NQ]));
+      umma_commit(smem_u32(&sm.s_full[j % NS]));
+      first = flags & LAST;
+      if (first) { umma_commit(smem_u32(&sm.k_empty[n % NK])); ++n; }
+      if (flags & FINAL) return;
+    }
+  }
+
+  // ---- sums ----
+  __device__ __forceinline__ void sum_up() {
+    const int warp = warp_index() - KW_FIRST, lane = threadIdx.x & 31, half = warp >> 2, in = (warp & 3) * 32 + lane;
+    const uint32_t column = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 64;
+    const WeightCap cap(t);
+    const float csc = CAP ? 1.0f : t.csc;
+    int n = 0;
+    KeyNote key{0, 0, 0, -1};
+    float sum = 0.f;
+    bool first = true;
+    for (int j = 0;; ++j) {
+      if (!wait(sm.rows_full[j % NS], j / NS) || !wait(sm.s_full[j % NS], j / NS)) return;
+      tc_fence_after();
+      const uint32_t flags = sm.flags[j % NS];
+      const int part = sm.part[j % NS];
+      if (first) { key = sm.keys[n % NU][in]; sum = 0.f; }
+      const RowNote& rows = sm.rows[j % NS];
+#pragma unroll
+      for (int g2 = 0; g2 < 2; ++g2) {
+        const int g = half * 2 + g2;
+        if (!((flags >> g) & 1)) continue;
+        float s[32];
+        tmem_ld32_nowait(column + (j % NS) * RT + g2 * 32, reinterpret_cast<uint32_t*>(s));
+        tmem_ld_wait_on(s);
+        if (CAP == 1) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) s[k] = cap.form.template of<1>(s[k]);
+        } else if (CAP == 2) {
+          float most = 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) most = fmaxf(most, fabsf(s[k]));
+          if (__all_sync(0xffffffffu, cap.small(most))) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) cap.of_small(s[k], s[k + 1]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) cap.of_any(s[k], s[k + 1]);
+          }
+        }
+        const float4* const lse = reinterpret_cast<const float4*>(rows.lse + g * 32);
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!((flags >> (MASKED_AT + g)) & 1)) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 l = lse[k];
+            acc[0] += tree_ex2(fmaf(s[4 * k], csc, -l.x)); acc[1] += tree_ex2(fmaf(s[4 * k + 1], csc, -l.y));
+            acc[2] += tree_ex2(fmaf(s[4 * k + 2], csc, -l.z)); acc[3] += tree_ex2(fmaf(s[4 * k + 3], csc, -l.w));
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const int2 see = rows.sees[g * 32 + k];
+            const float p = tree_ex2(fmaf(s[k], csc, -rows.lse[g * 32 + k]));
+            acc[k & 3] += key.x <= see.x && see.x < key.y && key.place > see.y ? p : 0.f;
+          }
+        }
+        sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+      }
+      tc_fence_before();
+      const bool last = flags & LAST;
+      if (last && half == 1) { sm.half[n % NU][in] = sum; mbar_arrive(smem_u32(&sm.half_full[n % NU])); }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sm.s_empty[j % NS]));
+      if (last && half == 0) {
+        if (!wait(sm.half_full[n % NU], n / NU)) return;
+        sum += sm.half[n % NU][in];
+        if (chunks > 1) {                                    // behind the places of the weights
+          t.part[((sm.plan.all(t) + part) * KT) + in] = sum;
+          if (part % chunks == 0) reinterpret_cast<int*>(t.part)[(long long)(part / chunks) * KT + in] = key.at;
+        } else if (key.at != -1) {
+          if (key.at >= 0) { float* const w = t.weights + key.at; *w = fmaf(*w, t.decay, sum); }
+          else t.weights[-2 - key.at] = sum;
+        }
+      }
+      first = last;
+      n += last;
+      if (flags & FINAL) return;
+    }
+  }
+};
+
+template <int DH, int CAP>
+__global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __grid_constant__ WeightsView t, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, int box) {
+  extern __shared__ uint8_t smem_bytes[];
+  KwSmem<DH>& sm = *reinterpret_cast<KwSmem<DH>*>(smem_bytes + ((1024u - (smem_u32(smem_bytes) & 1023u)) & 1023u));
+  const int warp = warp_index();
+  if (threadIdx.x == 0) {
+    *gave_up() = 0;
+    prefetch_map(&map_q); prefetch_map(&map_k);
+    for (int i = 0; i < NK; ++i) { mbar_init(smem_u32(&sm.k_full[i]), 1); mbar_init(smem_u32(&sm.k_empty[i]), 1); }
+    for (int i = 0; i < q_buffers(DH); ++i) { mbar_init(smem_u32(&sm.q_full[i]), 1); mbar_init(smem_u32(&sm.q_empty[i]), 1); }
+    for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&sm.rows_full[i]), 1); mbar_init(smem_u32(&sm.s_full[i]), 1); mbar_init(smem_u32(&sm.s_empty[i]), KW_SUM); }
+    for (int i = 0; i < NU; ++i) mbar_init(smem_u32(&sm.half_full[i]), KT);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&sm.tmem), NS * RT);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  sm.plan.make_of(t, [&](const KeyRange& k) { return key_tiles_of(t, k) * t.c.num_kv_heads; });
+  const int chunks = parts_bytes(sm.plan.all(t), t.chunks) <= t.a.workspace_bytes ? t.chunks : 1;   // more keys than the caller said: no room for parts
+  const long long units = sm.plan.all(t) * chunks;
+  if (t.chunks > 1) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (blockIdx.x == 0 && threadIdx.x == 0) *static_cast<PartsHead*>(t.a.workspace) = PartsHead{sm.plan.all(t), chunks, 0};
+  }
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < t.c.batch; b += KW_THREADS)
+      if (!cache_request(t.c, b).ok) cache_report(t.c, CACHE_BAD_OFFSETS);
+  KwBlock<DH, CAP> block{t, map_q, map_k, sm, box, chunks, sm.tmem};
+  if (blockIdx.x < units) {
+    if (warp == 0) block.produce(units);
+    else if (warp == 1) { if (elect_one()) block.issue(); }
+    else if (warp >= KW_FIRST) block.sum_up();
+  }
+  settle();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(sm.tmem, NS * RT);
+  }
+}
+
+// Sums of a key's chunks of rows, in their order
+__global__ void __launch_bounds__(256) key_weights_join_kernel(const WeightsView t) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const PartsHead head = *static_cast<const PartsHead*>(t.a.workspace);
+  if (head.chunks == 1) return;
+  const int* const at_of = reinterpret_cast<const int*>(t.part);
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < head.units * KT; i += (long long)gridDim.x * 256) {
+    const int at = at_of[i];
+    if (at == -1) continue;
+    const float* const part = t.part + (head.units + i / KT * head.chunks) * KT + i % KT;
+    float sum = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < head.chunks; ++c) sum += part[c * KT];
+    if (at >= 0) t.weights[at] = fmaf(t.weights[at], t.decay, sum);
+    else t.weights[-2 - at] = sum;
+  }
+}
+
+template <int DH, int CAP>
+phx_status launch(const WeightsView& t, const CUtensorMap& map_q, const CUtensorMap& map_k, int box, int blocks, cudaStream_t stream, std::string& err) {
+  constexpr int smem = (int)sizeof(KwSmem<DH>) + 1024;
+  static_assert(smem <= 227 * 1024, "a block's shared memory");
+  static SmemLimit limit;
+  PHX_CUDA_TRY(limit.raise(key_weights_tc_kernel<DH, CAP>, smem), err);
+  key_weights_tc_kernel<DH, CAP><<<blocks, KW_THREADS, smem, stream>>>(t, map_q, map_k, box);
+  PHX_CUDA_TRY(cudaGetLastError(), err);
+  dispatch_note(DK_KEY_WEIGHTS_TC);
+  return PHX_OK;
+}
+
+template <int DH>
+phx_status launch(const WeightsView& t, const CUtensorMap& map_q, const CUtensorMap& map_k, int box, int blocks, cudaStream_t stream, std::string& err) {
+  return t.a.cap_method == 0 ? launch<DH, 0>(t, map_q, map_k, box, blocks, stream, err) : t.a.cap_method == 1 ? launch<DH, 1>(t, map_q, map_k, box, blocks, stream, err)
+                                                                                                               : launch<DH, 2>(t, map_q, map_k, box, blocks, stream, err);
+}
+
+}  // namespace
+
+bool weights_tc_supported(const WeightsView& t) { return (t.c.key_size == 64 || t.c.key_size == 128) && t.group <= RT && (long long)t.a.max_tokens * t.group > 16; }
+
+phx_status weights_tc_launch(WeightsView& t, cudaStream_t stream, std::string& err) {
+  t.rows = RT / t.group * t.group; t.keys = KT;
+  int box = KT;                                    // the largest power of two that a page is a multiple of, at most a tile
+  while (t.c.page_size % box != 0) box /= 2;
+  CUtensorMap map_q, map_k;
+  phx_status s = tree_query_map(&map_q, t, err);
+  if (s == PHX_OK) s = tree_pool_map(&map_k, t, box, err);
+  // Tiles of rows in chunks where units alone leave blocks idle in a last round: about eight rounds then, of four tiles at least
+  const WeightsView whole = t;
+  const int per_tile = t.rows / t.group, sms = device_sms();
+  for (int b0 = 0; s == PHX_OK && b0 < whole.c.batch; b0 += TREE_MAX_SPLIT_BATCH) {   // as many requests as a block plans
+    t = whole;
+    t.c.batch = whole.c.batch - b0 < TREE_MAX_SPLIT_BATCH ? whole.c.batch - b0 : TREE_MAX_SPLIT_BATCH;
+    t.c.q_start += b0; t.c.lengths += b0; t.c.block_table += b0 * t.c.table_stride;
+    long long tiles = (t.a.max_keys + KT - 1) / KT;
+    if (t.decay == 1.0f) {
+      const long long seen = ((long long)t.sinks + KT - 1) / KT + ((long long)t.window + t.a.max_tokens + KT - 3) / KT + 1;
+      if (seen < tiles) tiles = seen;
+    }
+    const long long units = tiles * t.c.num_kv_heads * t.c.batch, row_tiles = (t.a.max_tokens + per_tile - 1) / per_tile;
+    t.chunks = 1;
+    if (units < 4 * sms) {
+      const long long want = (8ll * sms + units - 1) / units, most = row_tiles / 4;
+      t.chunks = (int)(want < most ? want : most);
+      if (t.chunks < 1) t.chunks = 1;
+      while (t.chunks > 1 && parts_bytes(units, t.chunks) > t.a.workspace_bytes) --t.chunks;
+    }
+    t.part = reinterpret_cast<float*>(static_cast<uint8_t*>(t.a.workspace) + sizeof(PartsHead));
+    const int blocks = (int)(units * t.chunks < sms ? units * t.chunks : sms);
+    s = t.c.key_size == 64 ? launch<64>(t, map_q, map_k, box, blocks, stream, err) : launch<128>(t, map_q, map_k, box, blocks, stream, err);
+    if (s == PHX_OK && t.chunks > 1) {
+      const long long joins = (units * KT + 255) / 256;
+      const cudaError_t e = launch_programmatic(key_weights_join_kernel, dim3((unsigned)(joins < 4 * sms ? joins : 4 * sms)), dim3(256), 0, stream, t);
+      if (e != cudaSuccess) { err = cudaGetErrorString(e); s = PHX_E_CUDA; }
+    }
+  }
+  return s;
+}
+
+}  // namespace phx

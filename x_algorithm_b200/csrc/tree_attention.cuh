@@ -169,11 +169,12 @@ template <int THREADS> struct TreePlan {
 
   // by all threads of the block; ends with a barrier
   template <class View> __device__ void make(const View& t) {
+    make_of(t, [&](const KeyRange& k) { return (long long)t.c.num_kv_heads * tree_row_tiles(t, k.rq.tokens) * (t.split ? unit_tiles(t, k) + t.setup : 1); });
+  }
+  // places(request's keys): its places
+  template <class View, class Places> __device__ __forceinline__ void make_of(const View& t, Places places) {
     const int tid = threadIdx.x, lane = tid & 31, per = (t.c.batch + THREADS - 1) / THREADS, b0 = min(tid * per, t.c.batch), b1 = min(b0 + per, t.c.batch);
-    auto tiles_of = [&](int b) {
-      const KeyRange k = key_range(t.c, b);
-      return (long long)t.c.num_kv_heads * tree_row_tiles(t, k.rq.tokens) * (t.split ? unit_tiles(t, k) + t.setup : 1);
-    };
+    auto tiles_of = [&](int b) { return places(key_range(t.c, b)); };
     long long mine = 0;
     for (int b = b0; b < b1; ++b) mine += tiles_of(b);
     long long sum = mine;
@@ -240,6 +241,7 @@ template <int THREADS> struct TreePlan {
 };
 
 phx_status tree_pool_map(CUtensorMap* map, const TreeView& t, int box_rows, std::string& err);
+phx_status tree_query_map(CUtensorMap* map, const TreeView& t, std::string& err);
 // tcgen05 kernel (tree_attention_sm100.cu): whether it takes the call, its tile shape, its launch
 bool tree_tc_supported(const TreeView& t);
 void tree_tc_shape(TreeView& t);                 // rows and keys of a tile

@@ -58,15 +58,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
-// Wait for the tensor-memory loads in flight.  The 32 registers are operands, so that no use of them is scheduled in front of it.
-__device__ __forceinline__ void tmem_ld_wait_on(float* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]),
-                 "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]),
-                 "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
-               :: "memory");
-}
-
 // what the producer notes about a tile
 struct TileNote {
   int tile;
@@ -676,20 +667,6 @@ __global__ void __launch_bounds__(TC_THREADS, 2) tree_tc_kernel(const __grid_con
   }
 }
 
-// Queries as [token][head][column]; a box is 64 columns of the group's heads of as many tokens as 128 rows hold
-phx_status query_map(CUtensorMap* map, const TreeView& t, std::string& err) {
-  EncodeTiledFn fn = get_encode_fn(err);
-  if (!fn) return PHX_E_CUDA;
-  const cuuint64_t dh = (cuuint64_t)t.c.key_size;
-  cuuint64_t dims[3] = {dh, (cuuint64_t)t.a.num_q_heads, (cuuint64_t)t.c.num_tokens};
-  cuuint64_t strides[2] = {dh * 2, (cuuint64_t)t.a.q_stride * 2};
-  cuuint32_t box[3] = {64, (cuuint32_t)t.group, (cuuint32_t)(t.rows / t.group)}, estr[3] = {1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t*>(t.a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) { err = "cuTensorMapEncodeTiled (queries) failed with code " + std::to_string((int)r); return PHX_E_CUDA; }
-  return PHX_OK;
-}
-
 template <int DH, int CAP, class View>
 phx_status launch(const View& t, cudaStream_t stream, std::string& err) {
   constexpr int smem = (int)sizeof(TcSmem<DH, View>) + 1024;
@@ -699,7 +676,7 @@ phx_status launch(const View& t, cudaStream_t stream, std::string& err) {
   int box = KT;                                    // the largest power of two that a page is a multiple of, at most a tile
   while (t.c.page_size % box != 0) box /= 2;
   CUtensorMap map_q, map_kv;
-  phx_status s = query_map(&map_q, t, err);
+  phx_status s = tree_query_map(&map_q, t, err);
   if (s == PHX_OK) s = tree_pool_map(&map_kv, t, box, err);
   if (s != PHX_OK) return s;
   const long long row_tiles = ((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows;
@@ -720,6 +697,20 @@ phx_status launch_any(const View& t, cudaStream_t stream, std::string& err) {
 }
 
 }  // namespace
+
+// Queries as [token][head][column]; a box is 64 columns of the group's heads of as many tokens as 128 rows hold
+phx_status tree_query_map(CUtensorMap* map, const TreeView& t, std::string& err) {
+  EncodeTiledFn fn = get_encode_fn(err);
+  if (!fn) return PHX_E_CUDA;
+  const cuuint64_t dh = (cuuint64_t)t.c.key_size;
+  cuuint64_t dims[3] = {dh, (cuuint64_t)t.a.num_q_heads, (cuuint64_t)t.c.num_tokens};
+  cuuint64_t strides[2] = {dh * 2, (cuuint64_t)t.a.q_stride * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)t.group, (cuuint32_t)(t.rows / t.group)}, estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t*>(t.a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { err = "cuTensorMapEncodeTiled (queries) failed with code " + std::to_string((int)r); return PHX_E_CUDA; }
+  return PHX_OK;
+}
 
 bool tree_tc_supported(const TreeView& t) { return (t.c.key_size == 64 || t.c.key_size == 128) && t.group <= QT; }
 void tree_tc_shape(TreeView& t) { t.rows = QT / t.group * t.group; t.keys = KT; t.setup = 6; }
