@@ -2,9 +2,9 @@
 // key_weights.cu's.  S^T = K Q^T: 128 keys are the rows of the product and 128 query rows its columns, so that a key's sum over the queries is the sum along one thread's row of
 // tensor memory, and no thread needs another's.  A block (one an SM) takes unit after unit - a request, key head and tile of 128 keys, with all tiles of rows or a
 // chunk of them - K once, then the tiles of rows that see one of its keys:
-//   warp 0      producer: K (page by page) and Q tiles by TMA, the rows' lse and what they see, and which of a tile's four groups of 32 rows have rows at all, and
-//               some key that some row does not see; what its 128 keys are, once a unit
+//   warp 0      producer: K (page by page) and Q tiles by TMA, and a note about each; what the unit's 128 keys are
 //   warp 1      MMA issuer: S^T into one of four buffers of tensor memory
+//   warps 2, 3  every other tile of rows each: the rows' lse and what they see, which of the four groups of 32 rows see keys at all, and which not all
 //   warps 4-11  thread = key and 64 of the rows: e^(x - lse) summed up in a register; at the unit's end one half hands its sums to the other, which writes the weight (or
 //               a part, where chunks of rows are joined by key_weights_join_kernel)
 // Waits are bounded; when one runs out the flag is raised, every later wait of any role fails at once, and a role whose wait failed is done.
@@ -26,9 +26,16 @@ constexpr int NK = 2, NS = 4;            // K tiles in shared memory, S^T buffer
 __host__ __device__ constexpr int q_buffers(int dh) { return dh == 64 ? 4 : 3; }
 constexpr int NU = 8;                    // units whose keys are described: none begins before the tile NS in front of its first has been read
 
-struct RowNote { float lse[RT]; int2 sees[RT]; };   // lse in the log2 domain, infinite: no weight; (place in the walk or -1, place behind which the window begins)
+struct alignas(16) RowNote { float lse[RT]; int2 sees[RT]; uint32_t flags; };   // lse in the log2 domain, infinite: no weight; (place in the walk or -1, place behind which the window begins)
 struct KeyNote { int x, y, place, at; };            // span, place in the window's terms, word of the weights or -1: no key
-constexpr uint32_t ROWS_OF = 0xf, MASKED_AT = 4, LAST = 256, FINAL = 512;   // bits 0-3: the group has rows, 4-7: and some do not see some key
+constexpr uint32_t MASKED_AT = 4;                   // of RowNote.flags: bits 0-3 a row of the group sees a key, 4-7 some row does not see some key
+constexpr uint32_t LAST = 1, FINAL = 2, STOP = 4;   // of TileNote.flags: the unit's last tile, the block's; behind it
+struct TileNote { int tile, part; uint32_t flags; };   // part: the place of the unit's sums among the parts
+struct UnitNote {
+  int row0, tokens, cached, h;
+  int x_least, x_most, y_least, y_most, place_least, place_most;   // over its keys: what a row has to be to see any, or all of them
+  bool rows;                             // some row may see some key
+};
 
 template <int DH>
 struct KwSmem {
@@ -38,9 +45,9 @@ struct KwSmem {
   RowNote rows[NS];
   KeyNote keys[NU][KT];
   float half[NU][KT];
-  uint32_t flags[NS];
-  int part[NS];                          // of the tile's unit: the place of its sums among the parts
-  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], rows_full[NS], s_full[NS], s_empty[NS], half_full[NU];
+  TileNote tile[NS];
+  UnitNote unit[NU];
+  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], tile_known[NS], rows_full[NS], s_full[NS], s_empty[NS], half_full[NU];
   uint32_t tmem;
   TreePlan<KW_THREADS> plan;
 };
@@ -148,36 +155,6 @@ struct KwBlock {
         if (key0 > rq.cached) begin = max(begin, min(end, (key0 - rq.cached) / per_tile));
         if (key0 >= t.sinks) end = max(begin, (int)min((long long)end, ((long long)key0 + KT - 1 + t.window - rq.cached - 1 + per_tile) / per_tile));
       }
-      // rows 4 groups of 32: row r is token r / group, head r % group
-      struct Ask { float lse[4]; int pre[4], behind[4]; } ask;
-      auto ask_rows = [&](int tile) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int r = g * 32 + lane, token = tile * per_tile + r / group;
-          const bool valid = r < t.rows && token < rq.tokens;
-          ask.lse[g] = INFINITY; ask.pre[g] = -1; ask.behind[g] = 0;
-          if (valid) {
-            ask.lse[g] = t.lse[(long long)(rq.row0 + token) * t.a.num_q_heads + u.h * group + r % group];
-            ask.pre[g] = span_of(t, rq, token).x;
-            ask.behind[g] = place_of(t, rq, token) - t.window;
-          }
-        }
-      };
-      auto look = [&](int tile, uint32_t* flags) {           // of the rows asked for
-        uint32_t f = 0;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if (isinf(ask.lse[g])) ask.pre[g] = -1;
-          const bool live = ask.pre[g] >= 0;
-          if (!live) { ask.lse[g] = INFINITY; ask.pre[g] = -0x7fffffff - 1; }
-          const bool any = live && ask.pre[g] >= x_least && ask.pre[g] < y_most && place_most > ask.behind[g];
-          const bool all = live && x_most <= ask.pre[g] && ask.pre[g] < y_least && place_least > ask.behind[g];
-          if (__any_sync(0xffffffffu, any)) f |= 1u << g;
-          if (!__all_sync(0xffffffffu, all)) f |= 1u << (MASKED_AT + g);
-        }
-        *flags = f;
-        return (f & ROWS_OF) != 0;
-      };
       // the first tile from `tile` on with a token that may see new keys alone, by the tokens' places; 128 tokens a round trip
       const bool sparse = t.a.spans && key0 >= rq.cached;
       auto candidate = [&](int tile) {
@@ -194,53 +171,89 @@ struct KwBlock {
         }
         return end;
       };
-      uint32_t flags = 0, flags_next = 0;
-      int tile = begin;
-      bool found = false;
-      while (!found && (tile = candidate(tile)) < end) {
-        ask_rows(tile);
-        found = look(tile, &flags);
-        if (!found) ++tile;
-      }
-      if (!found) { tile = max(0, min(begin, tiles - 1)); flags = 0; }   // no row sees any: a tile without rows, which ends the unit all the same
+      int tile = candidate(begin);
+      const bool rows = tile < end;
+      if (!rows) tile = max(0, min(begin, tiles - 1));        // no row sees any: a tile without rows, which ends the unit all the same
       for (bool first = true;; first = false) {
-        const Ask now = ask;
-        int next = tile + 1;
-        if (found && next < end) ask_rows(next);             // on its way under what follows
+        const int next = rows ? candidate(tile + 1) : end;
+        const bool more = next < end;
         if (!wait(sm.q_empty[j % NQ], j / NQ - 1)) return;
         if (!wait(sm.s_empty[j % NS], j / NS - 1)) return;
-        __syncwarp();
-        if (elect_one()) {
-          mbar_expect_tx(smem_u32(&sm.q_full[j % NQ]), DCH * t.rows * 128);
-          for (int c = 0; c < DCH; ++c)
-            tma_load_3d(smem_u32(sm.q[j % NQ]) + c * RT * 128, &map_q, smem_u32(&sm.q_full[j % NQ]), c * 64, u.h * group, rq.row0 + tile * per_tile);
-        }
         __syncwarp();
         if (first) {
 #pragma unroll
           for (int i = 0; i < KT / 32; ++i) sm.keys[n % NU][i * 32 + lane] = mine[i];
         }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          sm.rows[j % NS].lse[g * 32 + lane] = found ? now.lse[g] * TREE_LOG2E : INFINITY;
-          sm.rows[j % NS].sees[g * 32 + lane] = make_int2(now.pre[g], now.behind[g]);
-        }
-        bool more = false;
-        if (found) {
-          for (bool asked = true; next < end; asked = false) {
-            if (!asked) { next = candidate(next); if (next >= end) break; ask_rows(next); }
-            if (look(next, &flags_next)) { more = true; break; }
-            ++next;
-          }
-        }
-        if (lane == 0) sm.flags[j % NS] = flags | (more ? 0u : LAST | (pos + gridDim.x < units ? 0u : FINAL));
-        if (lane == 0) sm.part[j % NS] = (int)(pos / chunks) * chunks + u.chunk;
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.rows_full[j % NS]));
+        if (elect_one()) {
+          mbar_expect_tx(smem_u32(&sm.q_full[j % NQ]), DCH * t.rows * 128);
+          for (int c = 0; c < DCH; ++c)
+            tma_load_3d(smem_u32(sm.q[j % NQ]) + c * RT * 128, &map_q, smem_u32(&sm.q_full[j % NQ]), c * 64, u.h * group, rq.row0 + tile * per_tile);
+          if (first) sm.unit[n % NU] = UnitNote{rq.row0, rq.tokens, rq.cached, u.h, x_least, x_most, y_least, y_most, place_least, place_most, rows};
+          sm.tile[j % NS] = TileNote{tile, (int)(pos / chunks) * chunks + u.chunk, more ? 0u : LAST | (pos + gridDim.x < units ? 0u : FINAL)};
+          mbar_arrive(smem_u32(&sm.tile_known[j % NS]));
+        }
+        __syncwarp();
         ++j;
         if (!more) break;
-        tile = next; flags = flags_next;
+        tile = next;
       }
+    }
+    if (!wait(sm.s_empty[j % NS], j / NS - 1)) return;       // the row warp whose turn it is not
+    if (lane == 0) { sm.tile[j % NS].flags = STOP; mbar_arrive(smem_u32(&sm.tile_known[j % NS])); }
+  }
+
+  // ---- the rows of every other tile (a whole warp) ----
+  __device__ __forceinline__ void describe(int turn) {
+    const int lane = threadIdx.x & 31, group = t.group, per_tile = t.rows / group;
+    // this lane's rows, 32 apart: row r of a tile is token r / group, head r % group; behind the last one no token is
+    int token_in[4], head_in[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int r = g * 32 + lane;
+      token_in[g] = r < t.rows ? r / group : 1 << 30; head_in[g] = r % group;
+    }
+    int n = 0;
+    for (int j = 0;; ++j) {
+      if (!wait(sm.tile_known[j % NS], j / NS)) return;
+      const TileNote note = sm.tile[j % NS];
+      if (note.flags & STOP) return;
+      if ((j & 1) == turn) {
+        const UnitNote u = sm.unit[n % NU];
+        CacheRequest rq;
+        rq.row0 = u.row0; rq.tokens = u.rows ? u.tokens : 0; rq.cached = u.cached;
+        const float* const lse0 = t.lse + (long long)rq.row0 * t.a.num_q_heads + u.h * group;
+        float lse[4];
+        int pre[4], behind[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int token = note.tile * per_tile + token_in[g];
+          lse[g] = INFINITY; pre[g] = -1; behind[g] = 0;
+          if (token < rq.tokens) {
+            lse[g] = lse0[(long long)token * t.a.num_q_heads + head_in[g]];
+            pre[g] = span_of(t, rq, token).x;
+            behind[g] = place_of(t, rq, token) - t.window;
+          }
+        }
+        uint32_t flags = 0;
+        RowNote& rows = sm.rows[j % NS];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const bool live = pre[g] >= 0 && !isinf(lse[g]);    // no row, padding, one that saw nothing or that the caller leaves out
+          const bool any = live && pre[g] >= u.x_least && pre[g] < u.y_most && u.place_most > behind[g];
+          const bool all = live && u.x_most <= pre[g] && pre[g] < u.y_least && u.place_least > behind[g];
+          if (__any_sync(0xffffffffu, any)) flags |= 1u << g;
+          if (!__all_sync(0xffffffffu, all)) flags |= 1u << (MASKED_AT + g);
+          rows.lse[g * 32 + lane] = live ? lse[g] * TREE_LOG2E : INFINITY;
+          rows.sees[g * 32 + lane] = make_int2(live ? pre[g] : -0x7fffffff - 1, behind[g]);
+        }
+        if (lane == 0) rows.flags = flags;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.rows_full[j % NS]));
+      }
+      n += note.flags & LAST;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sm.s_empty[j % NS]));   // the note has been read, by the warp whose turn it is not, too
     }
   }
 
@@ -250,8 +263,8 @@ struct KwBlock {
     int n = 0;
     bool first = true;
     for (int j = 0;; ++j) {
-      if (!wait(sm.rows_full[j % NS], j / NS)) return;
-      const uint32_t flags = sm.flags[j % NS];
+      if (!wait(sm.tile_known[j % NS], j / NS)) return;
+      const uint32_t flags = sm.tile[j % NS].flags;
       if (first && !wait(sm.k_full[n % NK], n / NK)) return;
       if (!wait(sm.q_full[j % NQ], j / NQ)) return;         // (the producer has waited for the buffer of S^T)
       tc_fence_after();
@@ -282,8 +295,8 @@ struct KwBlock {
     for (int j = 0;; ++j) {
       if (!wait(sm.rows_full[j % NS], j / NS) || !wait(sm.s_full[j % NS], j / NS)) return;
       tc_fence_after();
-      const uint32_t flags = sm.flags[j % NS];
-      const int part = sm.part[j % NS];
+      const TileNote note = sm.tile[j % NS];
+      const uint32_t flags = sm.rows[j % NS].flags;
       if (first) { key = sm.keys[n % NU][in]; sum = 0.f; }
       const RowNote& rows = sm.rows[j % NS];
 #pragma unroll
@@ -328,7 +341,7 @@ struct KwBlock {
         sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
       }
       tc_fence_before();
-      const bool last = flags & LAST;
+      const bool last = note.flags & LAST;
       if (last && half == 1) { sm.half[n % NU][in] = sum; mbar_arrive(smem_u32(&sm.half_full[n % NU])); }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sm.s_empty[j % NS]));
@@ -336,8 +349,8 @@ struct KwBlock {
         if (!wait(sm.half_full[n % NU], n / NU)) return;
         sum += sm.half[n % NU][in];
         if (chunks > 1) {                                    // behind the places of the weights
-          t.part[((sm.plan.all(t) + part) * KT) + in] = sum;
-          if (part % chunks == 0) reinterpret_cast<int*>(t.part)[(long long)(part / chunks) * KT + in] = key.at;
+          t.part[((sm.plan.all(t) + note.part) * KT) + in] = sum;
+          if (note.part % chunks == 0) reinterpret_cast<int*>(t.part)[(long long)(note.part / chunks) * KT + in] = key.at;
         } else if (key.at != -1) {
           if (key.at >= 0) { float* const w = t.weights + key.at; *w = fmaf(*w, t.decay, sum); }
           else t.weights[-2 - key.at] = sum;
@@ -345,7 +358,7 @@ struct KwBlock {
       }
       first = last;
       n += last;
-      if (flags & FINAL) return;
+      if (note.flags & FINAL) return;
     }
   }
 };
@@ -360,7 +373,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __g
     prefetch_map(&map_q); prefetch_map(&map_k);
     for (int i = 0; i < NK; ++i) { mbar_init(smem_u32(&sm.k_full[i]), 1); mbar_init(smem_u32(&sm.k_empty[i]), 1); }
     for (int i = 0; i < q_buffers(DH); ++i) { mbar_init(smem_u32(&sm.q_full[i]), 1); mbar_init(smem_u32(&sm.q_empty[i]), 1); }
-    for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&sm.rows_full[i]), 1); mbar_init(smem_u32(&sm.s_full[i]), 1); mbar_init(smem_u32(&sm.s_empty[i]), KW_SUM); }
+    for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&sm.tile_known[i]), 1); mbar_init(smem_u32(&sm.rows_full[i]), 1); mbar_init(smem_u32(&sm.s_full[i]), 1); mbar_init(smem_u32(&sm.s_empty[i]), KW_SUM + 2); }
     for (int i = 0; i < NU; ++i) mbar_init(smem_u32(&sm.half_full[i]), KT);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -382,7 +395,8 @@ __global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __g
   if (blockIdx.x < units) {
     if (warp == 0) block.produce(units);
     else if (warp == 1) { if (elect_one()) block.issue(); }
-    else if (warp >= KW_FIRST) block.sum_up();
+    else if (warp < KW_FIRST) block.describe(warp - 2);
+    else block.sum_up();
   }
   settle();
   if (warp == 1) {
