@@ -2,7 +2,8 @@
 // key_weights.cu's.  S^T = K Q^T: 128 keys are the rows of the product and 128 query rows its columns, so that a key's sum over the queries is the sum along one thread's row of
 // tensor memory, and no thread needs another's.  A block (one an SM) takes unit after unit - a request, key head and tile of 128 keys, with all tiles of rows or a
 // chunk of them - K once, then the tiles of rows that see one of its keys:
-//   warp 0      producer: K (page by page) and Q tiles by TMA, and a note about each; what the unit's 128 keys are
+//   warp 12     planner, units ahead: where a unit's keys lie, what sees them, which tiles of rows
+//   warp 0      producer: K (page by page) and Q tiles by TMA, and a note about each
 //   warp 1      MMA issuer: S^T into one of four buffers of tensor memory
 //   warps 2, 3  every other tile of rows each: the rows' lse and what they see, which of the four groups of 32 rows see keys at all, and which not all
 //   warps 4-11  thread = key and 64 of the rows: e^(x - lse) summed up in a register; at the unit's end one half hands its sums to the other, which writes the weight (or
@@ -21,20 +22,24 @@ namespace {
 using namespace sm100;
 
 constexpr int KT = 128, RT = 128;        // keys and rows of a tile
-constexpr int KW_THREADS = 384, KW_FIRST = 4, KW_SUM = 8;   // warps 4 .. 11 sum
+constexpr int KW_THREADS = 416, KW_FIRST = 4, KW_SUM = 8;   // warps 4 .. 11 sum
 constexpr int NK = 2, NS = 4;            // K tiles in shared memory, S^T buffers in tensor memory
 __host__ __device__ constexpr int q_buffers(int dh) { return dh == 64 ? 4 : 3; }
-constexpr int NU = 8;                    // units whose keys are described: none begins before the tile NS in front of its first has been read
+constexpr int NU = 8;                    // units that are planned or worked on
 
 struct alignas(16) RowNote { float lse[RT]; int2 sees[RT]; uint32_t flags; };   // lse in the log2 domain, infinite: no weight; (place in the walk or -1, place behind which the window begins)
 struct KeyNote { int x, y, place, at; };            // span, place in the window's terms, word of the weights or -1: no key
 constexpr uint32_t MASKED_AT = 4;                   // of RowNote.flags: bits 0-3 a row of the group sees a key, 4-7 some row does not see some key
 constexpr uint32_t LAST = 1, FINAL = 2, STOP = 4;   // of TileNote.flags: the unit's last tile, the block's; behind it
-struct TileNote { int tile, part; uint32_t flags; };   // part: the place of the unit's sums among the parts
+struct TileNote { int tile; uint32_t flags; };
 struct UnitNote {
   int row0, tokens, cached, h;
   int x_least, x_most, y_least, y_most, place_least, place_most;   // over its keys: what a row has to be to see any, or all of them
-  bool rows;                             // some row may see some key
+  int begin, end;                        // tiles of rows that may see some
+  int part;                              // the place of its sums among the parts
+  uint32_t flags;                        // FINAL: the block's last
+  bool sparse;                           // new keys alone, seen by their spans
+  int k_row[KT / 16];                    // rows of the pool that its boxes begin at
 };
 
 template <int DH>
@@ -47,7 +52,7 @@ struct KwSmem {
   float half[NU][KT];
   TileNote tile[NS];
   UnitNote unit[NU];
-  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], tile_known[NS], rows_full[NS], s_full[NS], s_empty[NS], half_full[NU];
+  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], tile_known[NS], rows_full[NS], s_full[NS], s_empty[NS], half_full[NU], u_full[NU], u_empty[NU];
   uint32_t tmem;
   TreePlan<KW_THREADS> plan;
 };
@@ -95,77 +100,111 @@ struct KwBlock {
     return u;
   }
 
-  // ---- producer (a whole warp; one lane issues) ----
-  __device__ __forceinline__ void produce(long long units) {
+  // ---- planner (a whole warp) ----
+  // A unit's chain - its place, the request's offsets, its pages, its keys' spans - is some 3 us of round trips, as long as four tiles: lanes look units up side by side, and a
+  // unit's pages are asked for while the one in front of it is written down.  (In the producer that chain was what the block waited for: 32 x 512 candidates 94 us.)
+  __device__ __forceinline__ void plan_units(long long units) {
     const int lane = threadIdx.x & 31, boxes = KT / box, page_size = t.c.page_size, page_rows = 2 * t.c.num_kv_heads * page_size;
-    const int no_row = (int)(t.c.num_pages * page_rows), group = t.group, per_tile = t.rows / group;   // tokens of a tile
-    int j = 0, n = 0;                                       // tiles and units so far
-    for (long long pos = blockIdx.x; pos < units; pos += gridDim.x, ++n) {
-      const KwUnit u = unit_at(pos);
-      const KeyRange kr = key_range(t.c, u.b);
-      const CacheRequest& rq = kr.rq;
-      const int key0 = u.key_tile * KT, tiles = (rq.tokens + per_tile - 1) / per_tile, per = (tiles + chunks - 1) / chunks;
-      int begin = min(u.chunk * per, tiles), end = min(begin + per, tiles);
-      if (lane == 0 && u.key_tile == 0 && u.h == 0 && u.chunk == 0 && kr.keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
-      // ---- K, box by box
-      if (!wait(sm.k_empty[n % NK], n / NK - 1)) return;    // the first wait passes
-      int page = -1;
-      bool there = false;
-      if (lane < boxes && key0 + lane * box < kr.keys) {
-        const int key = key0 + lane * box, col = key / page_size;
-        page = kr.table[col];
-        there = (unsigned)page < (unsigned)t.c.num_pages;
-        if (!there) cache_report(t.c, CACHE_BAD_PAGE);
-      }
-      const int row = there ? page * page_rows + u.h * page_size + (key0 + lane * box) % page_size : no_row;
-      __syncwarp();
-      if (elect_one()) mbar_expect_tx(smem_u32(&sm.k_full[n % NK]), BLK);
-      __syncwarp();
-      for (int p = 0; p < boxes; ++p) {
-        const int at = __shfl_sync(0xffffffffu, row, p);
-        if (elect_one())
-          for (int c = 0; c < DCH; ++c) tma_load_2d(smem_u32(sm.k[n % NK]) + c * KT * 128 + p * box * 128, &map_k, smem_u32(&sm.k_full[n % NK]), c * 64, at);
-        __syncwarp();
-      }
-      // ---- this lane's four keys: what a row has to be to see all of them, or any
-      KeyNote mine[KT / 32];
-      int x_most = -1, y_least = 0x7fffffff, place_least = 0x7fffffff, x_least = 0x7fffffff, y_most = -1, place_most = -1;
+    const int no_row = (int)(t.c.num_pages * page_rows), per_tile = t.rows / t.group;   // tokens of a tile
+    int n = 0;
+    for (long long base = blockIdx.x; base < units; base += 32ll * gridDim.x) {
+      const long long of_lane = base + (long long)lane * gridDim.x;
+      KwUnit unit{0, 0, 0, 0};
+      KeyRange range;
+      range.keys = 0; range.rq.row0 = range.rq.tokens = range.rq.cached = 0;
+      if (of_lane < units) { unit = unit_at(of_lane); range = key_range(t.c, unit.b); }
+      auto from = [&](int v, int i) { return __shfl_sync(0xffffffffu, v, i); };
+      auto ask = [&](int i) {                               // this lane's box of unit i: its page, -2 behind the keys
+        const int key = from(unit.key_tile, i) * KT + lane * box, keys = from(range.keys, i), b = from(unit.b, i);
+        return lane < boxes && key < keys ? t.c.block_table[(long long)b * t.c.table_stride + key / page_size] : -2;
+      };
+      int page_after = ask(0);
+      const int count = (int)min(32ll, (units - base + gridDim.x - 1) / gridDim.x);
+      for (int i = 0; i < count; ++i, ++n) {
+        const int page = page_after;
+        if (i + 1 < count) page_after = ask(i + 1);
+        const int b = from(unit.b, i), h = from(unit.h, i), key0 = from(unit.key_tile, i) * KT, chunk = from(unit.chunk, i), keys = from(range.keys, i);
+        CacheRequest rq;
+        rq.row0 = from(range.rq.row0, i); rq.tokens = from(range.rq.tokens, i); rq.cached = from(range.rq.cached, i);
+        const long long pos = base + (long long)i * gridDim.x;
+        const bool there = (unsigned)page < (unsigned)t.c.num_pages;
+        if (page != -2 && !there) cache_report(t.c, CACHE_BAD_PAGE);
+        if (lane == 0 && key0 == 0 && h == 0 && chunk == 0 && keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
+        const int row = there ? page * page_rows + h * page_size + (key0 + lane * box) % page_size : no_row;
+        // this lane's four keys: what a row has to be to see all of them, or any
+        KeyNote mine[KT / 32];
+        int x_most = -1, y_least = 0x7fffffff, place_least = 0x7fffffff, x_least = 0x7fffffff, y_most = -1, place_most = -1;
 #pragma unroll
-      for (int i = 0; i < KT / 32; ++i) {
-        const int in = i * 32 + lane, key = key0 + in;
-        const int owner = in / box, of = __shfl_sync(0xffffffffu, page, owner);
-        const bool ok = __shfl_sync(0xffffffffu, (int)there, owner) && key < kr.keys;
-        KeyNote m{0x7fffffff, -1, 0, -1};
-        if (ok) {
-          m.x = 0; m.y = 0x7fffffff;
-          if (key >= rq.cached) { const int2 s = span_of(t, rq, key - rq.cached); m.x = s.x; m.y = s.y; }
-          m.place = key_place(t, rq, key);
-          m.at = (of * t.c.num_kv_heads + u.h) * page_size + key % page_size;
-          if (key >= rq.cached) m.at = -2 - m.at;           // a new key: no weight before
-          x_least = min(x_least, m.x); y_most = max(y_most, m.y); place_most = max(place_most, m.place);
+        for (int g = 0; g < KT / 32; ++g) {
+          const int in = g * 32 + lane, key = key0 + in;
+          const int owner = in / box, of = __shfl_sync(0xffffffffu, page, owner);
+          const bool ok = (unsigned)of < (unsigned)t.c.num_pages && key < keys;
+          KeyNote m{0x7fffffff, -1, 0, -1};
+          if (ok) {
+            m.x = 0; m.y = 0x7fffffff;
+            if (key >= rq.cached) { const int2 s = span_of(t, rq, key - rq.cached); m.x = s.x; m.y = s.y; }
+            m.place = key_place(t, rq, key);
+            m.at = (of * t.c.num_kv_heads + h) * page_size + key % page_size;
+            if (key >= rq.cached) m.at = -2 - m.at;         // a new key: no weight before
+            x_least = min(x_least, m.x); y_most = max(y_most, m.y); place_most = max(place_most, m.place);
+          }
+          x_most = max(x_most, m.x); y_least = min(y_least, m.y); place_least = min(place_least, ok ? m.place : -1);
+          mine[g] = m;
         }
-        x_most = max(x_most, m.x); y_least = min(y_least, m.y); place_least = min(place_least, ok ? m.place : -1);
-        mine[i] = m;
+        x_most = __reduce_max_sync(0xffffffffu, x_most); y_least = __reduce_min_sync(0xffffffffu, y_least); place_least = __reduce_min_sync(0xffffffffu, place_least);
+        x_least = __reduce_min_sync(0xffffffffu, x_least); y_most = __reduce_max_sync(0xffffffffu, y_most); place_most = __reduce_max_sync(0xffffffffu, place_most);
+        // its tiles of rows.  In a chain those in front of the keys, and those whose windows lie behind them, are not looked at.
+        const int tiles = (rq.tokens + per_tile - 1) / per_tile, per = (tiles + chunks - 1) / chunks;
+        int begin = min(chunk * per, tiles), end = min(begin + per, tiles);
+        if (is_chain(t)) {
+          if (key0 > rq.cached) begin = max(begin, min(end, (key0 - rq.cached) / per_tile));
+          if (key0 >= t.sinks) end = max(begin, (int)min((long long)end, ((long long)key0 + KT - 1 + t.window - rq.cached - 1 + per_tile) / per_tile));
+        }
+        if (!wait(sm.u_empty[n % NU], n / NU - 1)) return;
+        UnitNote& note = sm.unit[n % NU];
+#pragma unroll
+        for (int g = 0; g < KT / 32; ++g) sm.keys[n % NU][g * 32 + lane] = mine[g];
+        if (lane < boxes) note.k_row[lane] = row;
+        if (lane == 0) {
+          note.row0 = rq.row0; note.tokens = rq.tokens; note.cached = rq.cached; note.h = h;
+          note.x_least = x_least; note.x_most = x_most; note.y_least = y_least; note.y_most = y_most; note.place_least = place_least; note.place_most = place_most;
+          note.begin = begin; note.end = end; note.part = (int)(pos / chunks) * chunks + chunk;
+          note.flags = pos + gridDim.x < units ? 0u : FINAL;
+          note.sparse = t.a.spans && key0 >= rq.cached;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.u_full[n % NU]));
       }
-      x_most = __reduce_max_sync(0xffffffffu, x_most); y_least = __reduce_min_sync(0xffffffffu, y_least); place_least = __reduce_min_sync(0xffffffffu, place_least);
-      x_least = __reduce_min_sync(0xffffffffu, x_least); y_most = __reduce_max_sync(0xffffffffu, y_most); place_most = __reduce_max_sync(0xffffffffu, place_most);
+    }
+  }
 
-      // ---- tiles of rows.  In a chain those in front of the keys, and those whose windows lie behind them, are not looked at.
-      if (is_chain(t)) {
-        if (key0 > rq.cached) begin = max(begin, min(end, (key0 - rq.cached) / per_tile));
-        if (key0 >= t.sinks) end = max(begin, (int)min((long long)end, ((long long)key0 + KT - 1 + t.window - rq.cached - 1 + per_tile) / per_tile));
+  // ---- producer (a whole warp; one lane issues) ----
+  __device__ __forceinline__ void produce() {
+    const int lane = threadIdx.x & 31, boxes = KT / box, group = t.group, per_tile = t.rows / group;
+    int j = 0;                                              // tiles so far
+    for (int n = 0;; ++n) {
+      if (!wait(sm.u_full[n % NU], n / NU)) return;
+      const UnitNote& u = sm.unit[n % NU];
+      const int row0 = u.row0, tokens = u.tokens, h = u.h, begin = u.begin, end = u.end, x_least = u.x_least, y_most = u.y_most;
+      const bool sparse = u.sparse, final = u.flags & FINAL;
+      if (!wait(sm.k_empty[n % NK], n / NK - 1)) return;    // the first wait passes
+      __syncwarp();
+      if (elect_one()) {
+        mbar_expect_tx(smem_u32(&sm.k_full[n % NK]), BLK);
+        for (int p = 0; p < boxes; ++p)
+          for (int c = 0; c < DCH; ++c) tma_load_2d(smem_u32(sm.k[n % NK]) + c * KT * 128 + p * box * 128, &map_k, smem_u32(&sm.k_full[n % NK]), c * 64, u.k_row[p]);
       }
+      __syncwarp();
       // the first tile from `tile` on with a token that may see new keys alone, by the tokens' places; 128 tokens a round trip
-      const bool sparse = t.a.spans && key0 >= rq.cached;
       auto candidate = [&](int tile) {
         if (!sparse) return tile;
-        for (int tok = tile * per_tile; tok < min(end * per_tile, rq.tokens); tok += 128) {
+        for (int tok = tile * per_tile; tok < min(end * per_tile, tokens); tok += 128) {
           int pre[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) pre[i] = span_of(t, rq, min(tok + i * 32 + lane, rq.tokens - 1)).x;
+          for (int i = 0; i < 4; ++i) pre[i] = t.a.spans[2ll * (row0 + min(tok + i * 32 + lane, tokens - 1))];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t hit = __ballot_sync(0xffffffffu, tok + i * 32 + lane < rq.tokens && pre[i] >= x_least && pre[i] < y_most);
+            const uint32_t hit = __ballot_sync(0xffffffffu, tok + i * 32 + lane < tokens && pre[i] >= x_least && pre[i] < y_most);
             if (hit) return (tok + i * 32 + __ffs(hit) - 1) / per_tile;
           }
         }
@@ -173,24 +212,18 @@ struct KwBlock {
       };
       int tile = candidate(begin);
       const bool rows = tile < end;
-      if (!rows) tile = max(0, min(begin, tiles - 1));        // no row sees any: a tile without rows, which ends the unit all the same
-      for (bool first = true;; first = false) {
+      if (!rows) tile = -1;                                   // no row sees any: a tile without rows, which ends the unit all the same
+      for (;;) {
         const int next = rows ? candidate(tile + 1) : end;
         const bool more = next < end;
         if (!wait(sm.q_empty[j % NQ], j / NQ - 1)) return;
         if (!wait(sm.s_empty[j % NS], j / NS - 1)) return;
         __syncwarp();
-        if (first) {
-#pragma unroll
-          for (int i = 0; i < KT / 32; ++i) sm.keys[n % NU][i * 32 + lane] = mine[i];
-        }
-        __syncwarp();
         if (elect_one()) {
           mbar_expect_tx(smem_u32(&sm.q_full[j % NQ]), DCH * t.rows * 128);
           for (int c = 0; c < DCH; ++c)
-            tma_load_3d(smem_u32(sm.q[j % NQ]) + c * RT * 128, &map_q, smem_u32(&sm.q_full[j % NQ]), c * 64, u.h * group, rq.row0 + tile * per_tile);
-          if (first) sm.unit[n % NU] = UnitNote{rq.row0, rq.tokens, rq.cached, u.h, x_least, x_most, y_least, y_most, place_least, place_most, rows};
-          sm.tile[j % NS] = TileNote{tile, (int)(pos / chunks) * chunks + u.chunk, more ? 0u : LAST | (pos + gridDim.x < units ? 0u : FINAL)};
+            tma_load_3d(smem_u32(sm.q[j % NQ]) + c * RT * 128, &map_q, smem_u32(&sm.q_full[j % NQ]), c * 64, h * group, row0 + max(tile, 0) * per_tile);
+          sm.tile[j % NS] = TileNote{tile, more ? 0u : LAST | (final ? FINAL : 0u)};
           mbar_arrive(smem_u32(&sm.tile_known[j % NS]));
         }
         __syncwarp();
@@ -198,6 +231,7 @@ struct KwBlock {
         if (!more) break;
         tile = next;
       }
+      if (final) break;
     }
     if (!wait(sm.s_empty[j % NS], j / NS - 1)) return;       // the row warp whose turn it is not
     if (lane == 0) { sm.tile[j % NS].flags = STOP; mbar_arrive(smem_u32(&sm.tile_known[j % NS])); }
@@ -219,15 +253,15 @@ struct KwBlock {
       const TileNote note = sm.tile[j % NS];
       if (note.flags & STOP) return;
       if ((j & 1) == turn) {
-        const UnitNote u = sm.unit[n % NU];
+        const UnitNote& u = sm.unit[n % NU];
         CacheRequest rq;
-        rq.row0 = u.row0; rq.tokens = u.rows ? u.tokens : 0; rq.cached = u.cached;
+        rq.row0 = u.row0; rq.tokens = note.tile >= 0 ? u.tokens : 0; rq.cached = u.cached;
         const float* const lse0 = t.lse + (long long)rq.row0 * t.a.num_q_heads + u.h * group;
         float lse[4];
         int pre[4], behind[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int token = note.tile * per_tile + token_in[g];
+          const int token = max(note.tile, 0) * per_tile + token_in[g];
           lse[g] = INFINITY; pre[g] = -1; behind[g] = 0;
           if (token < rq.tokens) {
             lse[g] = lse0[(long long)token * t.a.num_q_heads + head_in[g]];
@@ -291,13 +325,14 @@ struct KwBlock {
     int n = 0;
     KeyNote key{0, 0, 0, -1};
     float sum = 0.f;
+    int part = 0;
     bool first = true;
     for (int j = 0;; ++j) {
       if (!wait(sm.rows_full[j % NS], j / NS) || !wait(sm.s_full[j % NS], j / NS)) return;
       tc_fence_after();
       const TileNote note = sm.tile[j % NS];
       const uint32_t flags = sm.rows[j % NS].flags;
-      if (first) { key = sm.keys[n % NU][in]; sum = 0.f; }
+      if (first) { key = sm.keys[n % NU][in]; part = sm.unit[n % NU].part; sum = 0.f; }
       const RowNote& rows = sm.rows[j % NS];
 #pragma unroll
       for (int g2 = 0; g2 < 2; ++g2) {
@@ -344,13 +379,16 @@ struct KwBlock {
       const bool last = note.flags & LAST;
       if (last && half == 1) { sm.half[n % NU][in] = sum; mbar_arrive(smem_u32(&sm.half_full[n % NU])); }
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sm.s_empty[j % NS]));
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&sm.s_empty[j % NS]));
+        if (last) mbar_arrive(smem_u32(&sm.u_empty[n % NU]));
+      }
       if (last && half == 0) {
         if (!wait(sm.half_full[n % NU], n / NU)) return;
         sum += sm.half[n % NU][in];
         if (chunks > 1) {                                    // behind the places of the weights
-          t.part[((sm.plan.all(t) + note.part) * KT) + in] = sum;
-          if (note.part % chunks == 0) reinterpret_cast<int*>(t.part)[(long long)(note.part / chunks) * KT + in] = key.at;
+          t.part[((sm.plan.all(t) + part) * KT) + in] = sum;
+          if (part % chunks == 0) reinterpret_cast<int*>(t.part)[(long long)(part / chunks) * KT + in] = key.at;
         } else if (key.at != -1) {
           if (key.at >= 0) { float* const w = t.weights + key.at; *w = fmaf(*w, t.decay, sum); }
           else t.weights[-2 - key.at] = sum;
@@ -374,7 +412,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __g
     for (int i = 0; i < NK; ++i) { mbar_init(smem_u32(&sm.k_full[i]), 1); mbar_init(smem_u32(&sm.k_empty[i]), 1); }
     for (int i = 0; i < q_buffers(DH); ++i) { mbar_init(smem_u32(&sm.q_full[i]), 1); mbar_init(smem_u32(&sm.q_empty[i]), 1); }
     for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&sm.tile_known[i]), 1); mbar_init(smem_u32(&sm.rows_full[i]), 1); mbar_init(smem_u32(&sm.s_full[i]), 1); mbar_init(smem_u32(&sm.s_empty[i]), KW_SUM + 2); }
-    for (int i = 0; i < NU; ++i) mbar_init(smem_u32(&sm.half_full[i]), KT);
+    for (int i = 0; i < NU; ++i) { mbar_init(smem_u32(&sm.half_full[i]), KT); mbar_init(smem_u32(&sm.u_full[i]), 1); mbar_init(smem_u32(&sm.u_empty[i]), KW_SUM); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(smem_u32(&sm.tmem), NS * RT);
@@ -393,10 +431,11 @@ __global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __g
       if (!cache_request(t.c, b).ok) cache_report(t.c, CACHE_BAD_OFFSETS);
   KwBlock<DH, CAP> block{t, map_q, map_k, sm, box, chunks, sm.tmem};
   if (blockIdx.x < units) {
-    if (warp == 0) block.produce(units);
+    if (warp == 0) block.produce();
     else if (warp == 1) { if (elect_one()) block.issue(); }
     else if (warp < KW_FIRST) block.describe(warp - 2);
-    else block.sum_up();
+    else if (warp < KW_FIRST + KW_SUM) block.sum_up();
+    else block.plan_units(units);
   }
   settle();
   if (warp == 1) {
