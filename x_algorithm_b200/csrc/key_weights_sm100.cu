@@ -2,12 +2,12 @@
 // key_weights.cu's.  S^T = K Q^T: 128 keys are the rows of the product and 128 query rows its columns, so that a key's sum over the queries is the sum along one thread's row of
 // tensor memory, and no thread needs another's.  A block (one an SM) takes unit after unit - a request, key head and tile of 128 keys, with all tiles of rows or a
 // chunk of them - K once, then the tiles of rows that see one of its keys:
-//   warp 12     planner, units ahead: where a unit's keys lie, what sees them, which tiles of rows
 //   warp 0      producer: K (page by page) and Q tiles by TMA, and a note about each
 //   warp 1      MMA issuer: S^T into one of four buffers of tensor memory
-//   warps 2, 3  every other tile of rows each: the rows' lse and what they see, which of the four groups of 32 rows see keys at all, and which not all
-//   warps 4-11  thread = key and 64 of the rows: e^(x - lse) summed up in a register; at the unit's end one half hands its sums to the other, which writes the weight (or
-//               a part, where chunks of rows are joined by key_weights_join_kernel)
+//   warp 2      planner, units ahead: where a unit's keys lie, what sees them, which tiles of rows
+//   warps 3, 20 .. 22   every fourth tile of rows each: the rows' lse and what they see, which of the four groups of 32 rows see keys at all, and which not all
+//   warps 4-19  thread = key and a group of the rows: e^(x - lse) summed up in a register; at the unit's end the groups hand their sums to the first, which writes the weight
+//               (or a part, where chunks of rows are joined by key_weights_join_kernel)
 // Waits are bounded; when one runs out the flag is raised, every later wait of any role fails at once, and a role whose wait failed is done.
 #include <string.h>
 
@@ -22,12 +22,13 @@ namespace {
 using namespace sm100;
 
 constexpr int KT = 128, RT = 128;        // keys and rows of a tile
-constexpr int KW_THREADS = 416, KW_FIRST = 4, KW_SUM = 8;   // warps 4 .. 11 sum
-constexpr int NK = 2, NS = 4;            // K tiles in shared memory, S^T buffers in tensor memory
+constexpr int KW_FIRST = 4, KW_SETS = 4, KW_SUM = 4 * KW_SETS;   // warps 4 .. 19 sum, four for each group of 32 rows
+constexpr int KW_ROWS = 4, KW_THREADS = 32 * (KW_FIRST + KW_SUM + KW_ROWS - 1);
+constexpr int NK = 2, NS = 4, NR = 8;    // K tiles in shared memory, S^T buffers in tensor memory, tiles of rows that are described ahead
 __host__ __device__ constexpr int q_buffers(int dh) { return dh == 64 ? 4 : 3; }
 constexpr int NU = 8;                    // units that are planned or worked on
 
-struct alignas(16) RowNote { float lse[RT]; int2 sees[RT]; uint32_t flags; };   // lse in the log2 domain, infinite: no weight; (place in the walk or -1, place behind which the window begins)
+struct alignas(16) RowNote { float less[RT]; int2 sees[RT]; uint32_t flags; };   // -lse in the log2 domain, -inf: no weight; (place in the walk or -1, place behind which the window begins)
 struct KeyNote { int x, y, place, at; };            // span, place in the window's terms, word of the weights or -1: no key
 constexpr uint32_t MASKED_AT = 4;                   // of RowNote.flags: bits 0-3 a row of the group sees a key, 4-7 some row does not see some key
 constexpr uint32_t LAST = 1, FINAL = 2, STOP = 4;   // of TileNote.flags: the unit's last tile, the block's; behind it
@@ -47,12 +48,12 @@ struct KwSmem {
   static constexpr int DCH = DH / 64, NQ = q_buffers(DH);
   uint8_t k[NK][DCH * KT * 128];
   uint8_t q[NQ][DCH * RT * 128];
-  RowNote rows[NS];
+  RowNote rows[NR];
   KeyNote keys[NU][KT];
-  float half[NU][KT];
-  TileNote tile[NS];
+  float sums[NU][KW_SETS - 1][KT];
+  TileNote tile[NR];
   UnitNote unit[NU];
-  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], tile_known[NS], rows_full[NS], s_full[NS], s_empty[NS], half_full[NU], u_full[NU], u_empty[NU];
+  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], tile_known[NR], rows_full[NR], rows_empty[NR], s_full[NS], s_empty[NS], sums_full[NU], u_full[NU], u_empty[NU];
   uint32_t tmem;
   TreePlan<KW_THREADS> plan;
 };
@@ -217,14 +218,14 @@ struct KwBlock {
         const int next = rows ? candidate(tile + 1) : end;
         const bool more = next < end;
         if (!wait(sm.q_empty[j % NQ], j / NQ - 1)) return;
-        if (!wait(sm.s_empty[j % NS], j / NS - 1)) return;
+        if (!wait(sm.rows_empty[j % NR], j / NR - 1)) return;
         __syncwarp();
         if (elect_one()) {
           mbar_expect_tx(smem_u32(&sm.q_full[j % NQ]), DCH * t.rows * 128);
           for (int c = 0; c < DCH; ++c)
             tma_load_3d(smem_u32(sm.q[j % NQ]) + c * RT * 128, &map_q, smem_u32(&sm.q_full[j % NQ]), c * 64, h * group, row0 + max(tile, 0) * per_tile);
-          sm.tile[j % NS] = TileNote{tile, more ? 0u : LAST | (final ? FINAL : 0u)};
-          mbar_arrive(smem_u32(&sm.tile_known[j % NS]));
+          sm.tile[j % NR] = TileNote{tile, more ? 0u : LAST | (final ? FINAL : 0u)};
+          mbar_arrive(smem_u32(&sm.tile_known[j % NR]));
         }
         __syncwarp();
         ++j;
@@ -233,11 +234,11 @@ struct KwBlock {
       }
       if (final) break;
     }
-    if (!wait(sm.s_empty[j % NS], j / NS - 1)) return;       // the row warp whose turn it is not
-    if (lane == 0) { sm.tile[j % NS].flags = STOP; mbar_arrive(smem_u32(&sm.tile_known[j % NS])); }
+    if (!wait(sm.rows_empty[j % NR], j / NR - 1)) return;       // the row warp whose turn it is not
+    if (lane == 0) { sm.tile[j % NR].flags = STOP; mbar_arrive(smem_u32(&sm.tile_known[j % NR])); }
   }
 
-  // ---- the rows of every other tile (a whole warp) ----
+  // ---- the rows of every fourth tile (a whole warp) ----
   __device__ __forceinline__ void describe(int turn) {
     const int lane = threadIdx.x & 31, group = t.group, per_tile = t.rows / group;
     // this lane's rows, 32 apart: row r of a tile is token r / group, head r % group; behind the last one no token is
@@ -249,45 +250,44 @@ struct KwBlock {
     }
     int n = 0;
     for (int j = 0;; ++j) {
-      if (!wait(sm.tile_known[j % NS], j / NS)) return;
-      const TileNote note = sm.tile[j % NS];
+      if (!wait(sm.tile_known[j % NR], j / NR)) return;
+      const TileNote note = sm.tile[j % NR];
       if (note.flags & STOP) return;
-      if ((j & 1) == turn) {
+      if (j % KW_ROWS == turn) {
         const UnitNote& u = sm.unit[n % NU];
         CacheRequest rq;
-        rq.row0 = u.row0; rq.tokens = note.tile >= 0 ? u.tokens : 0; rq.cached = u.cached;
+        rq.row0 = u.row0; rq.cached = u.cached;
         const float* const lse0 = t.lse + (long long)rq.row0 * t.a.num_q_heads + u.h * group;
         float lse[4];
         int pre[4], behind[4];
+        bool valid[4];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int token = max(note.tile, 0) * per_tile + token_in[g];
-          lse[g] = INFINITY; pre[g] = -1; behind[g] = 0;
-          if (token < rq.tokens) {
-            lse[g] = lse0[(long long)token * t.a.num_q_heads + head_in[g]];
-            pre[g] = span_of(t, rq, token).x;
-            behind[g] = place_of(t, rq, token) - t.window;
-          }
+        for (int g = 0; g < 4; ++g) {                         // loads without a condition: all on their way at once
+          const int token = max(note.tile, 0) * per_tile + token_in[g], at = max(0, min(token, u.tokens - 1));
+          valid[g] = note.tile >= 0 && token < u.tokens;
+          lse[g] = u.tokens > 0 ? lse0[(long long)at * t.a.num_q_heads + head_in[g]] : 0.f;
+          pre[g] = t.a.spans && u.tokens > 0 ? t.a.spans[2ll * (rq.row0 + at)] : at;
+          behind[g] = (t.positions && u.tokens > 0 ? max(rq.cached, t.positions[rq.row0 + at]) : t.a.spans ? rq.cached : rq.cached + at) - t.window;
         }
         uint32_t flags = 0;
-        RowNote& rows = sm.rows[j % NS];
+        RowNote& rows = sm.rows[j % NR];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const bool live = pre[g] >= 0 && !isinf(lse[g]);    // no row, padding, one that saw nothing or that the caller leaves out
+          const bool live = valid[g] && pre[g] >= 0 && !isinf(lse[g]);    // no row, padding, one that saw nothing or that the caller leaves out
           const bool any = live && pre[g] >= u.x_least && pre[g] < u.y_most && u.place_most > behind[g];
           const bool all = live && u.x_most <= pre[g] && pre[g] < u.y_least && u.place_least > behind[g];
           if (__any_sync(0xffffffffu, any)) flags |= 1u << g;
           if (!__all_sync(0xffffffffu, all)) flags |= 1u << (MASKED_AT + g);
-          rows.lse[g * 32 + lane] = live ? lse[g] * TREE_LOG2E : INFINITY;
+          rows.less[g * 32 + lane] = live ? lse[g] * -TREE_LOG2E : -INFINITY;
           rows.sees[g * 32 + lane] = make_int2(live ? pre[g] : -0x7fffffff - 1, behind[g]);
         }
         if (lane == 0) rows.flags = flags;
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.rows_full[j % NS]));
+        if (lane == 0) mbar_arrive(smem_u32(&sm.rows_full[j % NR]));
       }
       n += note.flags & LAST;
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sm.s_empty[j % NS]));   // the note has been read, by the warp whose turn it is not, too
+      if (lane == 0) mbar_arrive(smem_u32(&sm.rows_empty[j % NR]));   // the note has been read, by the warps whose turn it is not, too
     }
   }
 
@@ -297,10 +297,10 @@ struct KwBlock {
     int n = 0;
     bool first = true;
     for (int j = 0;; ++j) {
-      if (!wait(sm.tile_known[j % NS], j / NS)) return;
-      const uint32_t flags = sm.tile[j % NS].flags;
+      if (!wait(sm.tile_known[j % NR], j / NR)) return;
+      const uint32_t flags = sm.tile[j % NR].flags;
       if (first && !wait(sm.k_full[n % NK], n / NK)) return;
-      if (!wait(sm.q_full[j % NQ], j / NQ)) return;         // (the producer has waited for the buffer of S^T)
+      if (!wait(sm.s_empty[j % NS], j / NS - 1) || !wait(sm.q_full[j % NQ], j / NQ)) return;
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < DCH; ++c) {
@@ -318,8 +318,8 @@ struct KwBlock {
 
   // ---- sums ----
   __device__ __forceinline__ void sum_up() {
-    const int warp = warp_index() - KW_FIRST, lane = threadIdx.x & 31, half = warp >> 2, in = (warp & 3) * 32 + lane;
-    const uint32_t column = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 64;
+    const int warp = warp_index() - KW_FIRST, lane = threadIdx.x & 31, g = warp >> 2, in = (warp & 3) * 32 + lane;
+    const uint32_t column = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * 32;
     const WeightCap cap(t);
     const float csc = CAP ? 1.0f : t.csc;
     int n = 0;
@@ -328,18 +328,15 @@ struct KwBlock {
     int part = 0;
     bool first = true;
     for (int j = 0;; ++j) {
-      if (!wait(sm.rows_full[j % NS], j / NS) || !wait(sm.s_full[j % NS], j / NS)) return;
+      if (!wait(sm.rows_full[j % NR], j / NR) || !wait(sm.s_full[j % NS], j / NS)) return;
       tc_fence_after();
-      const TileNote note = sm.tile[j % NS];
-      const uint32_t flags = sm.rows[j % NS].flags;
+      const TileNote note = sm.tile[j % NR];
+      const uint32_t flags = sm.rows[j % NR].flags;
       if (first) { key = sm.keys[n % NU][in]; part = sm.unit[n % NU].part; sum = 0.f; }
-      const RowNote& rows = sm.rows[j % NS];
-#pragma unroll
-      for (int g2 = 0; g2 < 2; ++g2) {
-        const int g = half * 2 + g2;
-        if (!((flags >> g) & 1)) continue;
+      const RowNote& rows = sm.rows[j % NR];
+      if ((flags >> g) & 1) {
         float s[32];
-        tmem_ld32_nowait(column + (j % NS) * RT + g2 * 32, reinterpret_cast<uint32_t*>(s));
+        tmem_ld32_nowait(column + (j % NS) * RT, reinterpret_cast<uint32_t*>(s));
         tmem_ld_wait_on(s);
         if (CAP == 1) {
 #pragma unroll
@@ -356,36 +353,44 @@ struct KwBlock {
             for (int k = 0; k < 32; k += 2) cap.of_any(s[k], s[k + 1]);
           }
         }
-        const float4* const lse = reinterpret_cast<const float4*>(rows.lse + g * 32);
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        if (!((flags >> (MASKED_AT + g)) & 1)) {
+        const float4* const less = reinterpret_cast<const float4*>(rows.less + g * 32);
+        const float2 scale = make_float2(csc, csc);
+        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const bool masked = (flags >> (MASKED_AT + g)) & 1;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float4 l = lse[k];
-            acc[0] += tree_ex2(fmaf(s[4 * k], csc, -l.x)); acc[1] += tree_ex2(fmaf(s[4 * k + 1], csc, -l.y));
-            acc[2] += tree_ex2(fmaf(s[4 * k + 2], csc, -l.z)); acc[3] += tree_ex2(fmaf(s[4 * k + 3], csc, -l.w));
+        for (int k = 0; k < 32; k += 4) {
+          const float4 l = less[k / 4];
+          const float2 e0 = __ffma2_rn(make_float2(s[k], s[k + 1]), scale, make_float2(l.x, l.y)), e1 = __ffma2_rn(make_float2(s[k + 2], s[k + 3]), scale, make_float2(l.z, l.w));
+          s[k] = tree_ex2(e0.x); s[k + 1] = tree_ex2(e0.y); s[k + 2] = tree_ex2(e1.x); s[k + 3] = tree_ex2(e1.y);
+          if (!masked) {
+            acc[0] = __fadd2_rn(acc[0], make_float2(s[k], s[k + 1]));
+            acc[1] = __fadd2_rn(acc[1], make_float2(s[k + 2], s[k + 3]));
           }
-        } else {
+        }
+        if (masked) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
             const int2 see = rows.sees[g * 32 + k];
-            const float p = tree_ex2(fmaf(s[k], csc, -rows.lse[g * 32 + k]));
-            acc[k & 3] += key.x <= see.x && see.x < key.y && key.place > see.y ? p : 0.f;
+            const bool sees = key.x <= see.x && see.x < key.y && key.place > see.y;
+            if (k & 1) acc[0].y += sees ? s[k] : 0.f;
+            else acc[0].x += sees ? s[k] : 0.f;
           }
         }
-        sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+        sum += (acc[0].x + acc[1].x) + (acc[0].y + acc[1].y);
       }
       tc_fence_before();
       const bool last = note.flags & LAST;
-      if (last && half == 1) { sm.half[n % NU][in] = sum; mbar_arrive(smem_u32(&sm.half_full[n % NU])); }
+      if (last && g > 0) { sm.sums[n % NU][g - 1][in] = sum; mbar_arrive(smem_u32(&sm.sums_full[n % NU])); }
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(smem_u32(&sm.s_empty[j % NS]));
+        mbar_arrive(smem_u32(&sm.rows_empty[j % NR]));
         if (last) mbar_arrive(smem_u32(&sm.u_empty[n % NU]));
       }
-      if (last && half == 0) {
-        if (!wait(sm.half_full[n % NU], n / NU)) return;
-        sum += sm.half[n % NU][in];
+      if (last && g == 0) {
+        if (!wait(sm.sums_full[n % NU], n / NU)) return;
+#pragma unroll
+        for (int k = 0; k < KW_SETS - 1; ++k) sum += sm.sums[n % NU][k][in];
         if (chunks > 1) {                                    // behind the places of the weights
           t.part[((sm.plan.all(t) + part) * KT) + in] = sum;
           if (part % chunks == 0) reinterpret_cast<int*>(t.part)[(long long)(part / chunks) * KT + in] = key.at;
@@ -411,8 +416,9 @@ __global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __g
     prefetch_map(&map_q); prefetch_map(&map_k);
     for (int i = 0; i < NK; ++i) { mbar_init(smem_u32(&sm.k_full[i]), 1); mbar_init(smem_u32(&sm.k_empty[i]), 1); }
     for (int i = 0; i < q_buffers(DH); ++i) { mbar_init(smem_u32(&sm.q_full[i]), 1); mbar_init(smem_u32(&sm.q_empty[i]), 1); }
-    for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&sm.tile_known[i]), 1); mbar_init(smem_u32(&sm.rows_full[i]), 1); mbar_init(smem_u32(&sm.s_full[i]), 1); mbar_init(smem_u32(&sm.s_empty[i]), KW_SUM + 2); }
-    for (int i = 0; i < NU; ++i) { mbar_init(smem_u32(&sm.half_full[i]), KT); mbar_init(smem_u32(&sm.u_full[i]), 1); mbar_init(smem_u32(&sm.u_empty[i]), KW_SUM); }
+    for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&sm.s_full[i]), 1); mbar_init(smem_u32(&sm.s_empty[i]), KW_SUM); }
+    for (int i = 0; i < NR; ++i) { mbar_init(smem_u32(&sm.tile_known[i]), 1); mbar_init(smem_u32(&sm.rows_full[i]), 1); mbar_init(smem_u32(&sm.rows_empty[i]), KW_SUM + KW_ROWS); }
+    for (int i = 0; i < NU; ++i) { mbar_init(smem_u32(&sm.sums_full[i]), KT * (KW_SETS - 1)); mbar_init(smem_u32(&sm.u_full[i]), 1); mbar_init(smem_u32(&sm.u_empty[i]), KW_SUM); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(smem_u32(&sm.tmem), NS * RT);
@@ -433,9 +439,9 @@ __global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __g
   if (blockIdx.x < units) {
     if (warp == 0) block.produce();
     else if (warp == 1) { if (elect_one()) block.issue(); }
-    else if (warp < KW_FIRST) block.describe(warp - 2);
-    else if (warp < KW_FIRST + KW_SUM) block.sum_up();
-    else block.plan_units(units);
+    else if (warp == 2) block.plan_units(units);
+    else if (warp >= KW_FIRST && warp < KW_FIRST + KW_SUM) block.sum_up();
+    else block.describe(warp == 3 ? 0 : warp - (KW_FIRST + KW_SUM) + 1);
   }
   settle();
   if (warp == 1) {
