@@ -1,9 +1,10 @@
 // The attention weight that cached keys receive, on Blackwell tensor cores (tcgen05 + TMEM + TMA), for requests of more than 16 query rows a key head; the semantics are
-// key_weights.cu's.  S^T = K Q^T: 128 keys are the rows of the product and 128 query rows its columns, so that a key's sum over the queries is the sum along one thread's row of
+// key_weights.cu's.  S^T = K Q^T: 128 keys are the rows of the product and 256 query rows its columns, so that a key's sum over the queries is the sum along one thread's row of
 // tensor memory, and no thread needs another's.  A block (one an SM) takes unit after unit - a request, key head and tile of 128 keys, with all tiles of rows or a
-// chunk of them - K once, then the tiles of rows that see one of its keys:
-//   warp 0      producer: K (page by page) and Q tiles by TMA, and a note about each
-//   warp 1      MMA issuer: S^T into one of four buffers of tensor memory
+// chunk of them - K once, then the rows that see one of its keys, two tiles of 128 at a time (each role's own instructions a time, 1000 to 2700 cycles of a warp that is alone in its
+// code, were what the block waited for at one: 8 x 1022 tokens that see themselves, 16 heads of 128, 76 us):
+//   warp 0      producer: K (page by page) and Q tiles by TMA, and a note about each pair
+//   warp 1      MMA issuer: S^T into one of two buffers of tensor memory
 //   warp 2      planner, units ahead: where a unit's keys lie, what sees them, which tiles of rows
 //   warps 3, 20 .. 22   every fourth tile of rows each: the rows' lse and what they see, which of the four groups of 32 rows see keys at all, and which not all
 //   warps 4-19  thread = key and a group of the rows: e^(x - lse) summed up in a register; at the unit's end the groups hand their sums to the first, which writes the weight
@@ -21,44 +22,45 @@ namespace {
 
 using namespace sm100;
 
-constexpr int KT = 128, RT = 128;        // keys and rows of a tile
+constexpr int KT = 128, HT = 128, RT = 2 * HT;   // keys of a tile, rows of a tile, of a pair
 constexpr int KW_FIRST = 4, KW_SETS = 4, KW_SUM = 4 * KW_SETS;   // warps 4 .. 19 sum, four for each group of 32 rows
 constexpr int KW_ROWS = 4, KW_THREADS = 32 * (KW_FIRST + KW_SUM + KW_ROWS - 1);
-constexpr int NK = 2, NS = 4, NR = 8;    // K tiles in shared memory, S^T buffers in tensor memory, tiles of rows that are described ahead
-__host__ __device__ constexpr int q_buffers(int dh) { return dh == 64 ? 4 : 3; }
-constexpr int NU = 8;                    // units that are planned or worked on
+constexpr int NK = 2, NS = 2;            // K tiles in shared memory, S^T buffers in tensor memory
+__host__ __device__ constexpr int q_buffers(int dh) { return dh == 64 ? 3 : 2; }      // pairs of Q tiles
+__host__ __device__ constexpr int row_buffers(int dh) { return dh == 64 ? 4 : 3; }    // pairs that are described
+constexpr int NU = 4;                    // units that are planned or worked on
 
-struct alignas(16) RowNote { float less[RT]; int2 sees[RT]; uint32_t flags; };   // -lse in the log2 domain, -inf: no weight; (place in the walk or -1, place behind which the window begins)
+struct alignas(16) RowNote { float less[RT]; int2 sees[RT]; uint32_t flags[2]; };   // -lse in the log2 domain, -inf: no weight; (place in the walk or -1, place behind which the window begins)
 struct KeyNote { int x, y, place, at; };            // span, place in the window's terms, word of the weights or -1: no key
-constexpr uint32_t MASKED_AT = 4;                   // of RowNote.flags: bits 0-3 a row of the group sees a key, 4-7 some row does not see some key
-constexpr uint32_t LAST = 1, FINAL = 2, STOP = 4;   // of TileNote.flags: the unit's last tile, the block's; behind it
-struct TileNote { int tile; uint32_t flags; };
+constexpr uint32_t MASKED_AT = 4;                   // of RowNote.flags of a tile: bits 0-3 a row of the group sees a key, 4-7 some row does not see some key
+constexpr uint32_t LAST = 1, FINAL = 2, STOP = 4;   // of PairNote.flags: the unit's last pair, the block's; behind it
+struct PairNote { int tile, tiles; uint32_t flags; };   // its first tile, how many it has (0: a unit without rows)
 struct UnitNote {
   int row0, tokens, cached, h;
   int x_least, x_most, y_least, y_most, place_least, place_most;   // over its keys: what a row has to be to see any, or all of them
   int begin, end;                        // tiles of rows that may see some
   int part;                              // the place of its sums among the parts
   uint32_t flags;                        // FINAL: the block's last
-  bool sparse;                           // new keys alone, seen by their spans
+  uint32_t seen[2];                      // which of the first 64 of them do; those behind are looked at whether or not
   int k_row[KT / 16];                    // rows of the pool that its boxes begin at
 };
 
 template <int DH>
 struct KwSmem {
-  static constexpr int DCH = DH / 64, NQ = q_buffers(DH);
+  static constexpr int DCH = DH / 64, NQ = q_buffers(DH), NR = row_buffers(DH);
   uint8_t k[NK][DCH * KT * 128];
   uint8_t q[NQ][DCH * RT * 128];
   RowNote rows[NR];
   KeyNote keys[NU][KT];
   float sums[NU][KW_SETS - 1][KT];
-  TileNote tile[NR];
+  PairNote pair[NR];
   UnitNote unit[NU];
-  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], tile_known[NR], rows_full[NR], rows_empty[NR], s_full[NS], s_empty[NS], sums_full[NU], u_full[NU], u_empty[NU];
+  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], pair_known[NR], rows_full[NR], rows_empty[NR], s_full[NS], s_empty[NS], sums_full[NU], u_full[NU], u_empty[NU];
   uint32_t tmem;
   TreePlan<KW_THREADS> plan;
 };
 
-struct KwUnit { int b, h, key_tile, chunk; };
+struct KwUnit { int b, h, key_tile, chunk, part; };
 
 // The tiles of keys that rows may see; all of them where weights fade
 __device__ __forceinline__ TileRange key_tiles(const WeightsView& t, const KeyRange& k) {
@@ -78,7 +80,7 @@ __host__ __device__ constexpr long long parts_bytes(long long units, int chunks)
 
 template <int DH, int CAP>
 struct KwBlock {
-  static constexpr int DCH = DH / 64, NQ = q_buffers(DH);
+  static constexpr int DCH = DH / 64, NQ = q_buffers(DH), NR = row_buffers(DH);
   static constexpr uint32_t BLK = DCH * KT * 128;
   const WeightsView& t;
   const CUtensorMap& map_q;
@@ -90,76 +92,107 @@ struct KwBlock {
   __device__ __forceinline__ bool wait(const uint64_t& bar, int phase) const { return mbar_wait(smem_u32(&bar), (uint32_t)(phase & 1), t.c.status_dev); }
 
   // unit `pos` of the call
-  __device__ __forceinline__ KwUnit unit_at(long long pos) const {
+  __device__ __forceinline__ KwUnit unit_at(int pos) const {
     KwUnit u;
-    u.b = sm.plan.request_at(t, pos / chunks);
+    const int unit = chunks == 1 ? pos : pos / chunks;
+    u.chunk = pos - unit * chunks;
+    u.part = unit * chunks + u.chunk;
+    u.b = sm.plan.request_at(t, unit);
     const KeyRange k = key_range(t.c, u.b);
-    long long in = pos - sm.plan.before[u.b] * chunks;
-    u.chunk = (int)(in % chunks); in /= chunks;
-    u.h = (int)(in % t.c.num_kv_heads);
-    u.key_tile = key_tiles(t, k).at((int)(in / t.c.num_kv_heads));
+    const int in = unit - (int)sm.plan.before[u.b], tile = in / t.c.num_kv_heads;
+    u.h = in - tile * t.c.num_kv_heads;
+    u.key_tile = key_tiles(t, k).at(tile);
     return u;
   }
 
   // ---- planner (a whole warp) ----
   // A unit's chain - its place, the request's offsets, its pages, its keys' spans - is some 3 us of round trips, as long as four tiles: lanes look units up side by side, and a
   // unit's pages are asked for while the one in front of it is written down.  (In the producer that chain was what the block waited for: 32 x 512 candidates 94 us.)
-  __device__ __forceinline__ void plan_units(long long units) {
+  __device__ __forceinline__ void plan_units(int units) {
     const int lane = threadIdx.x & 31, boxes = KT / box, page_size = t.c.page_size, page_rows = 2 * t.c.num_kv_heads * page_size;
     const int no_row = (int)(t.c.num_pages * page_rows), per_tile = t.rows / t.group;   // tokens of a tile
-    int n = 0;
-    for (long long base = blockIdx.x; base < units; base += 32ll * gridDim.x) {
+    int before = 0;
+    for (long long base = blockIdx.x; base < units; base += 32ll * gridDim.x, before += 32) {
       const long long of_lane = base + (long long)lane * gridDim.x;
-      KwUnit unit{0, 0, 0, 0};
+      KwUnit unit{0, 0, 0, 0, 0};
       KeyRange range;
       range.keys = 0; range.rq.row0 = range.rq.tokens = range.rq.cached = 0;
-      if (of_lane < units) { unit = unit_at(of_lane); range = key_range(t.c, unit.b); }
+      if (of_lane < units) { unit = unit_at((int)of_lane); range = key_range(t.c, unit.b); }
       auto from = [&](int v, int i) { return __shfl_sync(0xffffffffu, v, i); };
       auto ask = [&](int i) {                               // this lane's box of unit i: its page, -2 behind the keys
         const int key = from(unit.key_tile, i) * KT + lane * box, keys = from(range.keys, i), b = from(unit.b, i);
         return lane < boxes && key < keys ? t.c.block_table[(long long)b * t.c.table_stride + key / page_size] : -2;
       };
       int page_after = ask(0);
-      const int count = (int)min(32ll, (units - base + gridDim.x - 1) / gridDim.x);
-      for (int i = 0; i < count; ++i, ++n) {
-        const int page = page_after;
+      const int count = __popc(__ballot_sync(0xffffffffu, of_lane < units));
+      for (int i = 0; i < count; ++i) {
+        const int n = before + i, page = page_after;
         if (i + 1 < count) page_after = ask(i + 1);
         const int b = from(unit.b, i), h = from(unit.h, i), key0 = from(unit.key_tile, i) * KT, chunk = from(unit.chunk, i), keys = from(range.keys, i);
         CacheRequest rq;
         rq.row0 = from(range.rq.row0, i); rq.tokens = from(range.rq.tokens, i); rq.cached = from(range.rq.cached, i);
-        const long long pos = base + (long long)i * gridDim.x;
+        const int part = from(unit.part, i);
+        const bool final = __shfl_sync(0xffffffffu, (int)(of_lane + gridDim.x >= units), i);
         const bool there = (unsigned)page < (unsigned)t.c.num_pages;
         if (page != -2 && !there) cache_report(t.c, CACHE_BAD_PAGE);
         if (lane == 0 && key0 == 0 && h == 0 && chunk == 0 && keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
-        const int row = there ? page * page_rows + h * page_size + (key0 + lane * box) % page_size : no_row;
-        // this lane's four keys: what a row has to be to see all of them, or any
+        const int slot0 = (key0 + lane * box) % page_size, row = there ? page * page_rows + h * page_size + slot0 : no_row;
+        // this lane's four keys: what a row has to be to see all of them, or any.  What is asked for of new ones is asked for at once.
         KeyNote mine[KT / 32];
+        int2 span[KT / 32];
+        int new_place[KT / 32];
+        const bool fresh = key0 + KT > rq.cached && rq.tokens > 0;
+#pragma unroll
+        for (int g = 0; g < KT / 32; ++g) {
+          const int token = max(0, min(key0 + g * 32 + lane - rq.cached, rq.tokens - 1));
+          span[g] = make_int2(token, rq.tokens); new_place[g] = t.a.spans ? rq.cached : rq.cached + token;
+          if (fresh && t.a.spans) span[g] = reinterpret_cast<const int2*>(t.a.spans)[rq.row0 + token];
+          if (fresh && t.positions) new_place[g] = t.positions[rq.row0 + token];
+        }
         int x_most = -1, y_least = 0x7fffffff, place_least = 0x7fffffff, x_least = 0x7fffffff, y_most = -1, place_most = -1;
 #pragma unroll
         for (int g = 0; g < KT / 32; ++g) {
-          const int in = g * 32 + lane, key = key0 + in;
-          const int owner = in / box, of = __shfl_sync(0xffffffffu, page, owner);
-          const bool ok = (unsigned)of < (unsigned)t.c.num_pages && key < keys;
-          KeyNote m{0x7fffffff, -1, 0, -1};
-          if (ok) {
-            m.x = 0; m.y = 0x7fffffff;
-            if (key >= rq.cached) { const int2 s = span_of(t, rq, key - rq.cached); m.x = s.x; m.y = s.y; }
-            m.place = key_place(t, rq, key);
-            m.at = (of * t.c.num_kv_heads + h) * page_size + key % page_size;
-            if (key >= rq.cached) m.at = -2 - m.at;         // a new key: no weight before
-            x_least = min(x_least, m.x); y_most = max(y_most, m.y); place_most = max(place_most, m.place);
-          }
-          x_most = max(x_most, m.x); y_least = min(y_least, m.y); place_least = min(place_least, ok ? m.place : -1);
+          const int in = g * 32 + lane, key = key0 + in, owner = in / box;
+          const int of = __shfl_sync(0xffffffffu, page, owner), slot = __shfl_sync(0xffffffffu, slot0, owner) + in - owner * box;
+          const bool ok = (unsigned)of < (unsigned)t.c.num_pages && key < keys, cached = key < rq.cached;
+          const int place = cached ? key : max(rq.cached, new_place[g]), at = (of * t.c.num_kv_heads + h) * page_size + slot;
+          KeyNote m;
+          m.x = !ok ? 0x7fffffff : cached ? 0 : span[g].x; m.y = !ok ? -1 : cached ? 0x7fffffff : span[g].y;
+          m.place = !ok ? -1 : place < t.sinks ? 0x7fffffff : place;
+          m.at = !ok ? -1 : cached ? at : -2 - at;          // a new key: no weight before
+          x_least = min(x_least, m.x); y_most = max(y_most, m.y); place_most = max(place_most, m.place);
+          x_most = max(x_most, m.x); y_least = min(y_least, m.y); place_least = min(place_least, m.place);
           mine[g] = m;
         }
         x_most = __reduce_max_sync(0xffffffffu, x_most); y_least = __reduce_min_sync(0xffffffffu, y_least); place_least = __reduce_min_sync(0xffffffffu, place_least);
         x_least = __reduce_min_sync(0xffffffffu, x_least); y_most = __reduce_max_sync(0xffffffffu, y_most); place_most = __reduce_max_sync(0xffffffffu, place_most);
         // its tiles of rows.  In a chain those in front of the keys, and those whose windows lie behind them, are not looked at.
-        const int tiles = (rq.tokens + per_tile - 1) / per_tile, per = (tiles + chunks - 1) / chunks;
+        const int tiles = (rq.tokens + per_tile - 1) / per_tile, per = ((tiles + chunks - 1) / chunks + 1) & ~1;
         int begin = min(chunk * per, tiles), end = min(begin + per, tiles);
         if (is_chain(t)) {
           if (key0 > rq.cached) begin = max(begin, min(end, (key0 - rq.cached) / per_tile));
           if (key0 >= t.sinks) end = max(begin, (int)min((long long)end, ((long long)key0 + KT - 1 + t.window - rq.cached - 1 + per_tile) / per_tile));
+        }
+        // Which of them have a token that sees new keys alone, by the tokens' places.  (Looked up by the producer as it went, a round trip a tile, then some 800 cycles of one warp's
+        // instructions: 8 x 1022 tokens that see themselves, 16 heads of 128, 78 us.)
+        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+        if (t.a.spans && key0 >= rq.cached) {
+          seen[0] = seen[1] = 0;
+          const int first = begin * per_tile, last = min(min(end, begin + 64) * per_tile, rq.tokens);
+          const float inverse = 1.0f / (float)per_tile;       // exact enough for quotients below 64: 8192 tokens at most
+          for (int token = first + lane; token < last; token += 256) {
+            int pre[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) pre[k] = t.a.spans[2ll * (rq.row0 + min(token + k * 32, rq.tokens - 1))];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int at = token + k * 32 - first;
+              int tile = (int)((float)at * inverse);
+              tile += (tile + 1) * per_tile <= at ? 1 : tile * per_tile > at ? -1 : 0;
+              if (first + at < last && pre[k] >= x_least && pre[k] < y_most) seen[tile >> 5] |= 1u << (tile & 31);
+            }
+          }
+          seen[0] = __reduce_or_sync(0xffffffffu, seen[0]); seen[1] = __reduce_or_sync(0xffffffffu, seen[1]);
         }
         if (!wait(sm.u_empty[n % NU], n / NU - 1)) return;
         UnitNote& note = sm.unit[n % NU];
@@ -169,9 +202,8 @@ struct KwBlock {
         if (lane == 0) {
           note.row0 = rq.row0; note.tokens = rq.tokens; note.cached = rq.cached; note.h = h;
           note.x_least = x_least; note.x_most = x_most; note.y_least = y_least; note.y_most = y_most; note.place_least = place_least; note.place_most = place_most;
-          note.begin = begin; note.end = end; note.part = (int)(pos / chunks) * chunks + chunk;
-          note.flags = pos + gridDim.x < units ? 0u : FINAL;
-          note.sparse = t.a.spans && key0 >= rq.cached;
+          note.begin = begin; note.end = end; note.part = part; note.seen[0] = seen[0]; note.seen[1] = seen[1];
+          note.flags = final ? FINAL : 0u;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sm.u_full[n % NU]));
@@ -181,13 +213,14 @@ struct KwBlock {
 
   // ---- producer (a whole warp; one lane issues) ----
   __device__ __forceinline__ void produce() {
-    const int lane = threadIdx.x & 31, boxes = KT / box, group = t.group, per_tile = t.rows / group;
-    int j = 0;                                              // tiles so far
+    const int lane = threadIdx.x & 31, boxes = KT / box, group = t.group, per_tile = t.rows / group, q_bytes = DCH * t.rows * 128;
+    int j = 0;                                              // pairs so far
     for (int n = 0;; ++n) {
       if (!wait(sm.u_full[n % NU], n / NU)) return;
       const UnitNote& u = sm.unit[n % NU];
-      const int row0 = u.row0, tokens = u.tokens, h = u.h, begin = u.begin, end = u.end, x_least = u.x_least, y_most = u.y_most;
-      const bool sparse = u.sparse, final = u.flags & FINAL;
+      const int row0 = u.row0, h = u.h, end = u.end;
+      const uint64_t seen = (uint64_t)u.seen[1] << 32 | u.seen[0];
+      const bool final = u.flags & FINAL;
       if (!wait(sm.k_empty[n % NK], n / NK - 1)) return;    // the first wait passes
       __syncwarp();
       if (elect_one()) {
@@ -196,36 +229,30 @@ struct KwBlock {
           for (int c = 0; c < DCH; ++c) tma_load_2d(smem_u32(sm.k[n % NK]) + c * KT * 128 + p * box * 128, &map_k, smem_u32(&sm.k_full[n % NK]), c * 64, u.k_row[p]);
       }
       __syncwarp();
-      // the first tile from `tile` on with a token that may see new keys alone, by the tokens' places; 128 tokens a round trip
-      auto candidate = [&](int tile) {
-        if (!sparse) return tile;
-        for (int tok = tile * per_tile; tok < min(end * per_tile, tokens); tok += 128) {
-          int pre[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) pre[i] = t.a.spans[2ll * (row0 + min(tok + i * 32 + lane, tokens - 1))];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t hit = __ballot_sync(0xffffffffu, tok + i * 32 + lane < tokens && pre[i] >= x_least && pre[i] < y_most);
-            if (hit) return (tok + i * 32 + __ffs(hit) - 1) / per_tile;
-          }
-        }
-        return end;
+      const int first = u.begin;
+      auto candidate = [&](int tile) {                        // the first tile from `tile` on that may see some
+        const int in = tile - first;
+        if (in >= 64) return tile;
+        const uint64_t left = seen >> in;
+        return left ? tile + __ffsll(left) - 1 : first + 64;
       };
-      int tile = candidate(begin);
-      const bool rows = tile < end;
-      if (!rows) tile = -1;                                   // no row sees any: a tile without rows, which ends the unit all the same
+      int tile = candidate(first);
+      const bool rows = tile < end;                           // none: a pair without rows, which ends the unit all the same
       for (;;) {
-        const int next = rows ? candidate(tile + 1) : end;
+        int next = rows ? candidate(tile + 1) : end, count = rows ? 1 : 0;
+        if (rows && next == tile + 1 && next < end) { count = 2; next = candidate(tile + 2); }
         const bool more = next < end;
         if (!wait(sm.q_empty[j % NQ], j / NQ - 1)) return;
         if (!wait(sm.rows_empty[j % NR], j / NR - 1)) return;
         __syncwarp();
         if (elect_one()) {
-          mbar_expect_tx(smem_u32(&sm.q_full[j % NQ]), DCH * t.rows * 128);
-          for (int c = 0; c < DCH; ++c)
-            tma_load_3d(smem_u32(sm.q[j % NQ]) + c * RT * 128, &map_q, smem_u32(&sm.q_full[j % NQ]), c * 64, h * group, row0 + max(tile, 0) * per_tile);
-          sm.tile[j % NR] = TileNote{tile, more ? 0u : LAST | (final ? FINAL : 0u)};
-          mbar_arrive(smem_u32(&sm.tile_known[j % NR]));
+          const int copies = max(count, 1);
+          mbar_expect_tx(smem_u32(&sm.q_full[j % NQ]), copies * q_bytes);
+          for (int i = 0; i < copies; ++i)
+            for (int c = 0; c < DCH; ++c)
+              tma_load_3d(smem_u32(sm.q[j % NQ]) + (c * RT + i * HT) * 128, &map_q, smem_u32(&sm.q_full[j % NQ]), c * 64, h * group, row0 + (rows ? tile + i : 0) * per_tile);
+          sm.pair[j % NR] = PairNote{tile, count, more ? 0u : LAST | (final ? FINAL : 0u)};
+          mbar_arrive(smem_u32(&sm.pair_known[j % NR]));
         }
         __syncwarp();
         ++j;
@@ -235,7 +262,7 @@ struct KwBlock {
       if (final) break;
     }
     if (!wait(sm.rows_empty[j % NR], j / NR - 1)) return;       // the row warp whose turn it is not
-    if (lane == 0) { sm.tile[j % NR].flags = STOP; mbar_arrive(smem_u32(&sm.tile_known[j % NR])); }
+    if (lane == 0) { sm.pair[j % NR].flags = STOP; mbar_arrive(smem_u32(&sm.pair_known[j % NR])); }
   }
 
   // ---- the rows of every fourth tile (a whole warp) ----
@@ -250,10 +277,13 @@ struct KwBlock {
     }
     int n = 0;
     for (int j = 0;; ++j) {
-      if (!wait(sm.tile_known[j % NR], j / NR)) return;
-      const TileNote note = sm.tile[j % NR];
+      if (!wait(sm.pair_known[j % NR], j / NR)) return;
+      const PairNote note = sm.pair[j % NR];
       if (note.flags & STOP) return;
-      if (j % KW_ROWS == turn) {
+      const int which = (turn - 2 * j) & (KW_ROWS - 1);       // the pair's tile that is this warp's turn
+      if (which < 2) {
+        const int tile = note.tile + which;
+        const bool there = which < note.tiles;
         const UnitNote& u = sm.unit[n % NU];
         CacheRequest rq;
         rq.row0 = u.row0; rq.cached = u.cached;
@@ -263,8 +293,8 @@ struct KwBlock {
         bool valid[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {                         // loads without a condition: all on their way at once
-          const int token = max(note.tile, 0) * per_tile + token_in[g], at = max(0, min(token, u.tokens - 1));
-          valid[g] = note.tile >= 0 && token < u.tokens;
+          const int token = (there ? tile : 0) * per_tile + token_in[g], at = max(0, min(token, u.tokens - 1));
+          valid[g] = there && token < u.tokens;
           lse[g] = u.tokens > 0 ? lse0[(long long)at * t.a.num_q_heads + head_in[g]] : 0.f;
           pre[g] = t.a.spans && u.tokens > 0 ? t.a.spans[2ll * (rq.row0 + at)] : at;
           behind[g] = (t.positions && u.tokens > 0 ? max(rq.cached, t.positions[rq.row0 + at]) : t.a.spans ? rq.cached : rq.cached + at) - t.window;
@@ -278,10 +308,10 @@ struct KwBlock {
           const bool all = live && u.x_most <= pre[g] && pre[g] < u.y_least && u.place_least > behind[g];
           if (__any_sync(0xffffffffu, any)) flags |= 1u << g;
           if (!__all_sync(0xffffffffu, all)) flags |= 1u << (MASKED_AT + g);
-          rows.less[g * 32 + lane] = live ? lse[g] * -TREE_LOG2E : -INFINITY;
-          rows.sees[g * 32 + lane] = make_int2(live ? pre[g] : -0x7fffffff - 1, behind[g]);
+          rows.less[which * HT + g * 32 + lane] = live ? lse[g] * -TREE_LOG2E : -INFINITY;
+          rows.sees[which * HT + g * 32 + lane] = make_int2(live ? pre[g] : -0x7fffffff - 1, behind[g]);
         }
-        if (lane == 0) rows.flags = flags;
+        if (lane == 0) rows.flags[which] = flags;
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sm.rows_full[j % NR]));
       }
@@ -293,12 +323,12 @@ struct KwBlock {
 
   // ---- MMA issuer (one thread) ----
   __device__ __forceinline__ void issue() {
-    constexpr uint32_t idesc = make_idesc(KT, RT);
+    constexpr uint32_t idesc_pair = make_idesc(KT, RT), idesc_one = make_idesc(KT, HT);
     int n = 0;
     bool first = true;
     for (int j = 0;; ++j) {
-      if (!wait(sm.tile_known[j % NR], j / NR)) return;
-      const uint32_t flags = sm.tile[j % NR].flags;
+      if (!wait(sm.pair_known[j % NR], j / NR)) return;
+      const uint32_t flags = sm.pair[j % NR].flags, idesc = sm.pair[j % NR].tiles == 2 ? idesc_pair : idesc_one;
       if (first && !wait(sm.k_full[n % NK], n / NK)) return;
       if (!wait(sm.s_empty[j % NS], j / NS - 1) || !wait(sm.q_full[j % NQ], j / NQ)) return;
       tc_fence_after();
@@ -318,7 +348,7 @@ struct KwBlock {
 
   // ---- sums ----
   __device__ __forceinline__ void sum_up() {
-    const int warp = warp_index() - KW_FIRST, lane = threadIdx.x & 31, g = warp >> 2, in = (warp & 3) * 32 + lane;
+    const int warp = warp_index() - KW_FIRST, lane = threadIdx.x & 31, g = warp >> 2, in = (warp & 3) * 32 + lane;   // group g of both tiles
     const uint32_t column = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * 32;
     const WeightCap cap(t);
     const float csc = CAP ? 1.0f : t.csc;
@@ -330,13 +360,15 @@ struct KwBlock {
     for (int j = 0;; ++j) {
       if (!wait(sm.rows_full[j % NR], j / NR) || !wait(sm.s_full[j % NS], j / NS)) return;
       tc_fence_after();
-      const TileNote note = sm.tile[j % NR];
-      const uint32_t flags = sm.rows[j % NR].flags;
+      const PairNote note = sm.pair[j % NR];
       if (first) { key = sm.keys[n % NU][in]; part = sm.unit[n % NU].part; sum = 0.f; }
       const RowNote& rows = sm.rows[j % NR];
-      if ((flags >> g) & 1) {
+#pragma unroll 1
+      for (int i = 0; i < note.tiles; ++i) {
+        const uint32_t flags = rows.flags[i];
+        if (!((flags >> g) & 1)) continue;
         float s[32];
-        tmem_ld32_nowait(column + (j % NS) * RT, reinterpret_cast<uint32_t*>(s));
+        tmem_ld32_nowait(column + (j % NS) * RT + i * HT, reinterpret_cast<uint32_t*>(s));
         tmem_ld_wait_on(s);
         if (CAP == 1) {
 #pragma unroll
@@ -353,7 +385,7 @@ struct KwBlock {
             for (int k = 0; k < 32; k += 2) cap.of_any(s[k], s[k + 1]);
           }
         }
-        const float4* const less = reinterpret_cast<const float4*>(rows.less + g * 32);
+        const float4* const less = reinterpret_cast<const float4*>(rows.less + i * HT + g * 32);
         const float2 scale = make_float2(csc, csc);
         float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         const bool masked = (flags >> (MASKED_AT + g)) & 1;
@@ -368,12 +400,11 @@ struct KwBlock {
           }
         }
         if (masked) {
+          const int4* const sees = reinterpret_cast<const int4*>(rows.sees + i * HT + g * 32);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const int2 see = rows.sees[g * 32 + k];
-            const bool sees = key.x <= see.x && see.x < key.y && key.place > see.y;
-            if (k & 1) acc[0].y += sees ? s[k] : 0.f;
-            else acc[0].x += sees ? s[k] : 0.f;
+          for (int k = 0; k < 32; k += 2) {
+            const int4 see = sees[k / 2];
+            acc[0] = __fadd2_rn(acc[0], make_float2(key.x <= see.x && see.x < key.y && key.place > see.y ? s[k] : 0.f, key.x <= see.z && see.z < key.y && key.place > see.w ? s[k + 1] : 0.f));
           }
         }
         sum += (acc[0].x + acc[1].x) + (acc[0].y + acc[1].y);
@@ -417,7 +448,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __g
     for (int i = 0; i < NK; ++i) { mbar_init(smem_u32(&sm.k_full[i]), 1); mbar_init(smem_u32(&sm.k_empty[i]), 1); }
     for (int i = 0; i < q_buffers(DH); ++i) { mbar_init(smem_u32(&sm.q_full[i]), 1); mbar_init(smem_u32(&sm.q_empty[i]), 1); }
     for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&sm.s_full[i]), 1); mbar_init(smem_u32(&sm.s_empty[i]), KW_SUM); }
-    for (int i = 0; i < NR; ++i) { mbar_init(smem_u32(&sm.tile_known[i]), 1); mbar_init(smem_u32(&sm.rows_full[i]), 1); mbar_init(smem_u32(&sm.rows_empty[i]), KW_SUM + KW_ROWS); }
+    for (int i = 0; i < row_buffers(DH); ++i) { mbar_init(smem_u32(&sm.pair_known[i]), 1); mbar_init(smem_u32(&sm.rows_full[i]), 2); mbar_init(smem_u32(&sm.rows_empty[i]), KW_SUM + KW_ROWS); }
     for (int i = 0; i < NU; ++i) { mbar_init(smem_u32(&sm.sums_full[i]), KT * (KW_SETS - 1)); mbar_init(smem_u32(&sm.u_full[i]), 1); mbar_init(smem_u32(&sm.u_empty[i]), KW_SUM); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -427,7 +458,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __g
   tc_fence_after();
   sm.plan.make_of(t, [&](const KeyRange& k) { return key_tiles_of(t, k) * t.c.num_kv_heads; });
   const int chunks = parts_bytes(sm.plan.all(t), t.chunks) <= t.a.workspace_bytes ? t.chunks : 1;   // more keys than the caller said: no room for parts
-  const long long units = sm.plan.all(t) * chunks;
+  const int units = (int)sm.plan.all(t) * chunks;
   if (t.chunks > 1) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (blockIdx.x == 0 && threadIdx.x == 0) *static_cast<PartsHead*>(t.a.workspace) = PartsHead{sm.plan.all(t), chunks, 0};
@@ -488,21 +519,23 @@ phx_status launch(const WeightsView& t, const CUtensorMap& map_q, const CUtensor
 
 }  // namespace
 
-bool weights_tc_supported(const WeightsView& t) { return (t.c.key_size == 64 || t.c.key_size == 128) && t.group <= RT && (long long)t.a.max_tokens * t.group > 16; }
+bool weights_tc_supported(const WeightsView& t) { return (t.c.key_size == 64 || t.c.key_size == 128) && t.group <= HT && (long long)t.a.max_tokens * t.group > 16; }
 
 phx_status weights_tc_launch(WeightsView& t, cudaStream_t stream, std::string& err) {
-  t.rows = RT / t.group * t.group; t.keys = KT;
+  t.rows = HT / t.group * t.group; t.keys = KT;
   int box = KT;                                    // the largest power of two that a page is a multiple of, at most a tile
   while (t.c.page_size % box != 0) box /= 2;
   CUtensorMap map_q, map_k;
   phx_status s = tree_query_map(&map_q, t, err);
   if (s == PHX_OK) s = tree_pool_map(&map_k, t, box, err);
-  // Tiles of rows in chunks where units alone leave blocks idle in a last round: about eight rounds then, of four tiles at least
+  // Tiles of rows in chunks where units alone leave blocks idle in a last round: about six rounds then, of two pairs at least
   const WeightsView whole = t;
   const int per_tile = t.rows / t.group, sms = device_sms();
-  for (int b0 = 0; s == PHX_OK && b0 < whole.c.batch; b0 += TREE_MAX_SPLIT_BATCH) {   // as many requests as a block plans
+  const long long most_units = ((long long)t.c.table_cols * t.c.page_size + KT - 1) / KT * t.c.num_kv_heads;   // of a request
+  const int slice = (int)(most_units * TREE_MAX_SPLIT_BATCH <= (1 << 27) ? TREE_MAX_SPLIT_BATCH : most_units < (1 << 27) ? (1 << 27) / most_units : 1);
+  for (int b0 = 0; s == PHX_OK && b0 < whole.c.batch; b0 += slice) {   // as many requests as a block plans, whose units a number of 32 bits counts
     t = whole;
-    t.c.batch = whole.c.batch - b0 < TREE_MAX_SPLIT_BATCH ? whole.c.batch - b0 : TREE_MAX_SPLIT_BATCH;
+    t.c.batch = whole.c.batch - b0 < slice ? whole.c.batch - b0 : slice;
     t.c.q_start += b0; t.c.lengths += b0; t.c.block_table += b0 * t.c.table_stride;
     long long tiles = (t.a.max_keys + KT - 1) / KT;
     if (t.decay == 1.0f) {
@@ -512,9 +545,10 @@ phx_status weights_tc_launch(WeightsView& t, cudaStream_t stream, std::string& e
     const long long units = tiles * t.c.num_kv_heads * t.c.batch, row_tiles = (t.a.max_tokens + per_tile - 1) / per_tile;
     t.chunks = 1;
     if (units < 4 * sms) {
-      const long long want = (8ll * sms + units - 1) / units, most = row_tiles / 4;
-      t.chunks = (int)(want < most ? want : most);
-      if (t.chunks < 1) t.chunks = 1;
+      const long long pairs = (row_tiles + 1) / 2, want = (6ll * sms + units - 1) / units;
+      long long per = pairs / want > 2 ? pairs / want : 2;   // pairs of a chunk
+      if ((pairs + per - 1) / per > 15) per = (pairs + 14) / 15;
+      t.chunks = (int)((pairs + per - 1) / per);
       while (t.chunks > 1 && parts_bytes(units, t.chunks) > t.a.workspace_bytes) --t.chunks;
     }
     t.part = reinterpret_cast<float*>(static_cast<uint8_t*>(t.a.workspace) + sizeof(PartsHead));
