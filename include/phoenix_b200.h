@@ -892,12 +892,15 @@ phx_status phx_key_weights_device(int32_t device, const phx_cache_batch* cache, 
  * in its order, key, value and weight, in the request's own pages; places behind are left as they are, and the pages behind the budget are the caller's to
  * hand out.  A request with at most `budget` keys stays as it is.  kept_out [batch][num_kv_heads][budget]: the places that the kept keys had, ascending,
  * -1 behind a shorter request's last; lengths_out [batch]: keys per request now (may be `lengths` itself).  A page may belong to one request of the call only.
- * max_keys (the most that a request has) chooses launch sizes only.  Of the cache block q_start and num_tokens are not used.  Bad pages and lengths raise
+ * max_keys (the most that a request has) chooses launch sizes only.  workspace: phx_tree_workspace_bytes (of which batch x heads x budget / 16 bytes are used), not
+ * shared by calls that may overlap; nothing in it is kept.  Of the cache block q_start and num_tokens are not used.  Bad pages and lengths raise
  * status bits as above.  Asynchronous on `stream`. */
 typedef struct phx_evict_args {
   float* weights;              /* [num_pages][num_kv_heads][page_size] */
   int32_t* lengths_out;
   int32_t* kept_out;
+  void* workspace;
+  int64_t workspace_bytes;
   int64_t max_keys;
   int32_t budget;
   int32_t sinks;

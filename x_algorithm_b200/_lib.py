@@ -126,7 +126,7 @@ class KeyWeightsArgs(C.Structure):   # phx_key_weights_args
 
 
 class EvictArgs(C.Structure):   # phx_evict_args
-    _fields_ = [(n, C.c_void_p) for n in ("weights", "lengths_out", "kept_out")] + [("max_keys", C.c_int64)] + [
+    _fields_ = [(n, C.c_void_p) for n in ("weights", "lengths_out", "kept_out", "workspace")] + [("workspace_bytes", C.c_int64), ("max_keys", C.c_int64)] + [
         (n, C.c_int32) for n in ("budget", "sinks", "recent", "_pad")]
 
 

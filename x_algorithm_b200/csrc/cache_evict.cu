@@ -3,9 +3,10 @@
 //
 // Two launches.  evict_select_kernel finds what stays: a cluster of blocks shares a head's keys, each with its stretch of weights in shared memory as integers of the
 // same order, and the smallest weight that stays comes out of three histograms, of 11, 11 and 10 bits, summed over the cluster (fewer where a digit decides already);
-// the places that stay are then numbered by prefix sums, equal weights by their order.  evict_move_kernel moves rows: a block takes the keys or the values (or some of
-// their columns, or the weights) of one head from the front to the back.  A row only ever moves forward, so what a chunk of places receives lies in it or behind:
-// once a block has read a chunk and all before it, it may write there, and later chunks may be on their way meanwhile.  No block waits for another.
+// the places that stay are then numbered by prefix sums, equal weights by their order.  evict_move_kernel moves rows: a block takes what goes to one chunk of a head's places,
+// keys, values and weights, into shared memory, says so, and writes it once all chunks in front of it have been read.  That is enough: a row only ever moves to the front, so what
+// lies in a chunk's places is taken by that chunk or one before it.  Chunks are handed out in order, by a counter, so a block only waits for blocks that have begun, and whose reads
+// wait for nothing.  (Blocks that went through a head's places from front to back by themselves: 247 us for 2 x 4 heads of 100 k keys, 89 us for 64 x 4 of 4096.)
 #include <string>
 
 #include "cache_batch.cuh"
@@ -21,7 +22,10 @@ struct EvictView {
   phx_evict_args a;
   uint64_t page_magic;           // ceil(2^36 / (page_size / 16))
   int held;                      // weights that a block of the select keeps in shared memory
-  int slices;                    // blocks that share a head's rows by columns
+  int rows;                      // places of a chunk
+  int chunks;                    // of a head
+  int* ticket;                   // the next chunk to hand out
+  int* read;                     // [batch][heads][chunks] whether it has been read
 };
 // x / page_size for x below 2^31: exact, as x / 16 < 2^27 and page_size / 16 <= 256 (the product's error stays below 2^27 * 256 < 2^36)
 __device__ __forceinline__ int page_column(const EvictView& t, int x) { return (int)(((uint64_t)((uint32_t)x >> 4) * t.page_magic) >> 36); }
@@ -73,6 +77,11 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   const EvictRequest rq = evict_request(t, b);
   if (rank == 0 && h == 0 && tid == 0 && !rq.ok) cache_report(t.c, CACHE_BAD_OFFSETS);
   int* const kept = t.a.kept_out + ((long long)b * t.c.num_kv_heads + h) * t.a.budget;
+  if (rank == 0) {                                           // for the launch behind
+    int* const read = t.read + ((long long)b * t.c.num_kv_heads + h) * t.chunks;
+    for (int i = tid; i < t.chunks; i += SEL_THREADS) read[i] = 0;
+    if (b == 0 && h == 0 && tid == 0) *t.ticket = 0;
+  }
   if (rq.length <= t.a.budget) {                             // the same for the whole cluster
     for (int i = rank * SEL_THREADS + tid; i < t.a.budget; i += ranks * SEL_THREADS) kept[i] = i < rq.length ? i : -1;
     return;
@@ -87,7 +96,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   const bool in_smem = per <= t.held;
   for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) (&sm.hist[0][0])[i] = 0;
   if (in_smem) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = tid; i < count; i += SEL_THREADS) held[i] = weight_at(from + i);
   }
   __syncthreads();
@@ -109,9 +118,14 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
     const int bin0 = SEL_BINS - 4 - 4 * tid;
     uint4 sum = make_uint4(0, 0, 0, 0);
     const uint32_t addr = smem_u32(hist + bin0);
-    for (int r = 0; r < ranks; ++r) {
-      const uint4 v = ranks > 1 ? remote_u32x4(mapa_shared(addr, r)) : *reinterpret_cast<const uint4*>(hist + bin0);
-      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    if (ranks == 1) {
+      sum = *reinterpret_cast<const uint4*>(hist + bin0);
+    } else {
+      uint4 v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] = r < ranks ? remote_u32x4(mapa_shared(addr, r)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) { sum.x += v[r].x; sum.y += v[r].y; sum.z += v[r].z; sum.w += v[r].w; }
     }
     uint32_t mine = sum.x + sum.y + sum.z + sum.w, upto = mine;
 #pragma unroll
@@ -174,92 +188,84 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
 
 // ---- moving together ---------------------------------------------------------------------------------------------------------
 
-constexpr int MOVE_THREADS = 256, MOVE_ROWS = 4, MOVE_STAGES = 4;   // copies of a thread in a chunk, chunks on their way
+constexpr int MOVE_THREADS = 256, MOVE_BYTES = 32 * 1024;   // of a chunk's keys and values
 
-// Copies of BYTES (16 or 4): thread i has piece i % pieces of row i / pieces, and of the rows a chunk's quarter further on.  row(place) is the address of
-// a place's first byte of this block's columns, or null where its page is none of the pool's.
-template <int BYTES, class RowOf>
-__device__ __forceinline__ void move_rows(const EvictView& t, const int* kept, uint8_t* ring, int pieces, RowOf row) {
-  const int tid = threadIdx.x, piece = tid % pieces, row_in = tid / pieces, rows = MOVE_THREADS / pieces, chunk = rows * MOVE_ROWS;
-  const int chunks = (t.a.budget + chunk - 1) / chunk;
-  uint8_t* const mine = ring + tid * BYTES;
-  auto place_of = [&](int c, int k) { return c * chunk + k * rows + row_in; };
-  int src[MOVE_ROWS];                                        // of the chunk that is fetched next
-  auto ask = [&](int c) {
-#pragma unroll
-    for (int k = 0; k < MOVE_ROWS; ++k) { const int to = place_of(c, k); src[k] = to < t.a.budget ? kept[to] : -1; }
-  };
-  uint32_t moved = 0;                                        // which rows were fetched, of the chunks on their way
-  auto fetch = [&](int c) {
-    const int at = (c % MOVE_STAGES) * MOVE_ROWS;
-    const uint8_t* from[MOVE_ROWS];
-#pragma unroll
-    for (int k = 0; k < MOVE_ROWS; ++k) from[k] = src[k] >= 0 && src[k] != place_of(c, k) ? row(src[k]) : nullptr;
-#pragma unroll
-    for (int k = 0; k < MOVE_ROWS; ++k) {
-      moved = (moved & ~(1u << (at + k))) | (from[k] ? 1u << (at + k) : 0u);
-      if (!from[k]) continue;
-      const uint32_t to = smem_u32(mine + (at + k) * (MOVE_THREADS * BYTES));
-      if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from[k] + piece * BYTES) : "memory");
-      else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from[k] + piece * BYTES) : "memory");
+// Bounded wait until the n words at p are set, by all threads; false when the limit ran out or another wait's did.  Every thread comes out with the same answer.
+__device__ __forceinline__ bool wait_all_set(const int* p, int n, volatile int* status) {
+  unsigned long long t0 = 0;
+  for (uint32_t it = 0;; ++it) {
+    bool all = true, over = false;
+    for (int i = threadIdx.x; i < n; i += MOVE_THREADS) {
+      int v;
+      asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p + i) : "memory");
+      all &= v != 0;
     }
-  };
-  ask(0);
-  for (int c = 0; c < MOVE_STAGES - 1; ++c) {
-    if (c < chunks) { fetch(c); ask(c + 1); }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
-  for (int c = 0; c < chunks; ++c) {
-    const int ahead = c + MOVE_STAGES - 1;
-    if (ahead < chunks) { fetch(ahead); ask(ahead + 1); }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    asm volatile("cp.async.wait_group %0;" ::"n"(MOVE_STAGES - 1) : "memory");
-    __syncthreads();                                         // all of this chunk and of those before has been read
-    const int at = (c % MOVE_STAGES) * MOVE_ROWS;
-#pragma unroll
-    for (int k = 0; k < MOVE_ROWS; ++k)
-      if ((moved >> (at + k)) & 1) {
-        const uint8_t* const from = mine + (at + k) * (MOVE_THREADS * BYTES);
-        uint8_t* const to = row(place_of(c, k));
-        if (to) {
-          if (BYTES == 16) *reinterpret_cast<uint4*>(to + piece * BYTES) = *reinterpret_cast<const uint4*>(from);
-          else *reinterpret_cast<uint32_t*>(to + piece * BYTES) = *reinterpret_cast<const uint32_t*>(from);
-        }
-      }
+    if ((it & 0xff) == 0xff && threadIdx.x == 0) {
+      const unsigned long long now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      const unsigned us = (unsigned)status[1];
+      over = status[0] != 0 || now - t0 > (us ? 1000ull * us : WAIT_LIMIT_NS);
+    }
+    if (__syncthreads_and(all)) return true;
+    if (__syncthreads_or(over)) { if (threadIdx.x == 0) status[0] = 1; return false; }
   }
 }
 
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictView t) {
-  extern __shared__ __align__(16) uint8_t smem_bytes[];
+  __shared__ __align__(16) uint8_t data[MOVE_BYTES];
+  __shared__ int ticket;
+  __shared__ int to_page[MOVE_BYTES / 128], from[MOVE_BYTES / 128];   // of each place of the chunk: its page, the place that it receives (or -1)
+  __shared__ int from_page[MOVE_BYTES / 128];
+  __shared__ float weight[MOVE_BYTES / 128];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int h = blockIdx.y, b = blockIdx.z, stream = blockIdx.x;
-  const int* const kept = t.a.kept_out + ((long long)b * t.c.num_kv_heads + h) * t.a.budget;
-  const bool weights = stream == 2 * t.slices;
+  const int tid = threadIdx.x, heads = t.c.batch * t.c.num_kv_heads;
+  if (tid == 0) ticket = atomicAdd(t.ticket, 1);
+  __syncthreads();
+  const int chunk = ticket / heads, of = ticket - chunk * heads, b = of / t.c.num_kv_heads, h = of - b * t.c.num_kv_heads;
+  const int* const kept = t.a.kept_out + (long long)of * t.a.budget;
   // the one reader of this request's length in this launch, so that lengths_out may be lengths
-  if (weights && h == 0 && threadIdx.x == 0) t.a.lengths_out[b] = min(evict_request(t, b).length, t.a.budget);
+  if (chunk == 0 && h == 0 && tid == 0) t.a.lengths_out[b] = min(evict_request(t, b).length, t.a.budget);
   if (kept[t.a.budget - 1] < t.a.budget) return;             // at most `budget` keys: all where they are
+  const int first = chunk * t.rows, count = min(t.rows, t.a.budget - first);
   const int* const table = t.c.block_table + (long long)b * t.c.table_stride;
-  auto page_of = [&](int place, int* slot) {
-    const int col = page_column(t, place), page = table[col];
-    *slot = place - col * t.c.page_size;
+  auto page_at = [&](int place) {                            // -1: none of the pool's
+    const int page = table[page_column(t, place)];
     if ((unsigned)page < (unsigned)t.c.num_pages) return page;
     cache_report(t.c, CACHE_BAD_PAGE);
     return -1;
   };
-  if (weights) {
-    move_rows<4>(t, kept, smem_bytes, 1, [&](int place) -> uint8_t* {
-      int slot;
-      const int page = page_of(place, &slot);
-      return page < 0 ? nullptr : reinterpret_cast<uint8_t*>(t.a.weights + ((long long)page * t.c.num_kv_heads + h) * t.c.page_size + slot);
-    });
-  } else {
-    const int which = stream / t.slices, row_bytes = t.c.key_size * 2, bytes = row_bytes / t.slices, column = (stream % t.slices) * bytes;
-    move_rows<16>(t, kept, smem_bytes, bytes / 16, [&](int place) -> uint8_t* {
-      int slot;
-      const int page = page_of(place, &slot);
-      return page < 0 ? nullptr : reinterpret_cast<uint8_t*>(t.c.pages) + (cache_row0(t.c, page, which, h) * 2 + (long long)slot * row_bytes + column);
-    });
+  for (int i = tid; i < count; i += MOVE_THREADS) {
+    const int src = kept[first + i], to = page_at(first + i), page = page_at(src);
+    const bool moves = src != first + i && to >= 0 && page >= 0;
+    from[i] = moves ? src - page_column(t, src) * t.c.page_size : -1;
+    from_page[i] = page; to_page[i] = to;
+    if (moves) weight[i] = t.a.weights[((long long)page * t.c.num_kv_heads + h) * t.c.page_size + from[i]];
   }
+  __syncthreads();
+  const int pieces = t.c.key_size / 8;                       // of 16 bytes of a row; the values' rows behind the keys'
+  const int row_of = tid / pieces, piece = tid - row_of * pieces, rows_on = MOVE_THREADS / pieces;
+  auto address = [&](int page, int which, int slot) { return reinterpret_cast<uint8_t*>(t.c.pages + cache_row0(t.c, page, which, h) + (long long)slot * t.c.key_size) + piece * 16; };
+  for (int r = row_of; r < 2 * count; r += rows_on) {
+    const int which = r >= count, i = r - which * count;
+    if (from[i] < 0) continue;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(data + (r * pieces + piece) * 16)), "l"(address(from_page[i], which, from[i])) : "memory");
+  }
+  asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  int* const read = t.read + (long long)of * t.chunks;
+  if (tid == 0) asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(read + chunk), "r"(1) : "memory");
+  if (!wait_all_set(read, chunk, t.c.status_dev)) return;
+  for (int r = row_of; r < 2 * count; r += rows_on) {
+    const int which = r >= count, i = r - which * count;
+    if (from[i] < 0) continue;
+    const int place = first + i, slot = place - page_column(t, place) * t.c.page_size;
+    *reinterpret_cast<uint4*>(address(to_page[i], which, slot)) = *reinterpret_cast<const uint4*>(data + (r * pieces + piece) * 16);
+  }
+  for (int i = tid; i < count; i += MOVE_THREADS)
+    if (from[i] >= 0) {
+      const int place = first + i, slot = place - page_column(t, place) * t.c.page_size;
+      t.a.weights[((long long)to_page[i] * t.c.num_kv_heads + h) * t.c.page_size + slot] = weight[i];
+    }
 }
 
 }  // namespace
@@ -295,15 +301,18 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
   constexpr int MOST_HELD = 48 * 1024;                        // weights: 192 KB beside the histograms; longer stretches are read from memory at each pass
   const long long per = (t.a.max_keys + ranks - 1) / ranks;
   t.held = (int)(per < MOST_HELD ? per : MOST_HELD);
-  // Columns of a head's rows are shared between blocks until the device has two blocks an SM; a block copies 64 bytes of a row at least
-  t.slices = 1;
-  while (heads * 2 * t.slices < 2ll * device_sms() && t.c.key_size * 2 / (2 * t.slices) >= 64) t.slices *= 2;
-  const int select_smem = (int)sizeof(SelectSmem) + t.held * 4, move_smem = MOVE_STAGES * MOVE_ROWS * MOVE_THREADS * 16;
-  static SmemLimit select_limit, move_limit;
+  t.rows = MOVE_BYTES / (4 * t.c.key_size);                   // 64 to 256
+  t.chunks = (t.a.budget + t.rows - 1) / t.rows;
+  if (heads * t.chunks > 2147483647ll) return bad("budget x heads x batch is too large");
+  if (t.a.workspace_bytes < 16 + heads * t.chunks * 4) return bad("workspace is smaller than phx_tree_workspace_bytes or too small for this many heads and budget");
+  if (!t.a.workspace || !aligned16(t.a.workspace)) return bad("workspace must be a 16-byte aligned buffer");
+  t.ticket = static_cast<int*>(t.a.workspace);
+  t.read = t.ticket + 4;
+  const int select_smem = (int)sizeof(SelectSmem) + t.held * 4;
+  static SmemLimit select_limit;
   std::string err;
   auto launch = [&]() -> phx_status {
     PHX_CUDA_TRY(select_limit.raise(evict_select_kernel, (int)sizeof(SelectSmem) + MOST_HELD * 4), err);
-    PHX_CUDA_TRY(move_limit.raise(evict_move_kernel, move_smem), err);
     cudaLaunchConfig_t lc;
     memset(&lc, 0, sizeof(lc));
     lc.gridDim = dim3(ranks, t.c.num_kv_heads, t.c.batch); lc.blockDim = dim3(SEL_THREADS); lc.dynamicSmemBytes = select_smem; lc.stream = st;
@@ -312,7 +321,7 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
     at[0].val.clusterDim.x = ranks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     lc.attrs = at; lc.numAttrs = 1;
     PHX_CUDA_TRY(cudaLaunchKernelEx(&lc, evict_select_kernel, t), err);
-    PHX_CUDA_TRY(launch_programmatic(evict_move_kernel, dim3(2 * t.slices + 1, t.c.num_kv_heads, t.c.batch), dim3(MOVE_THREADS), move_smem, st, t), err);
+    PHX_CUDA_TRY(launch_programmatic(evict_move_kernel, dim3((unsigned)(heads * t.chunks)), dim3(MOVE_THREADS), 0, st, t), err);
     dispatch_note(DK_CACHE_EVICT);
     return PHX_OK;
   };

@@ -79,7 +79,7 @@ class _Structs(threading.local):
 
 _structs = _Structs()
 _BATCH, _APPEND, _TREE, _LOGPROBS = (struct.Struct(f).pack_into for f in ("=7q6i", "=8q2ifi", "=7q2i2f2i", "=7q5i2fi"))   # the blocks' fields, in order
-_WINDOW, _WEIGHTS, _EVICT = (struct.Struct(f).pack_into for f in ("=7q2i2f2i2q2i", "=9q4i2fif", "=4q4i"))
+_WINDOW, _WEIGHTS, _EVICT = (struct.Struct(f).pack_into for f in ("=7q2i2f2i2q2i", "=9q4i2fif", "=6q4i"))
 _BF16, _F32, _I32, _I64, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.int64, torch.uint8
 
 
@@ -342,7 +342,7 @@ def key_weights(q, pages, q_start, lengths, block_table, lse, weights, spans=Non
 
 
 def evict(weights, pages, lengths, block_table, *, budget: int, sinks: int = 0, recent: int = 0, max_keys: Optional[int] = None, lengths_out=None, kept=None,
-          stream: Optional[int] = None):
+          workspace=None, stream: Optional[int] = None):
     """Requests with more than `budget` keys keep, in each key head, the first `sinks`, the last `recent`, and of the others the ones with the largest weights (ties: the
     earlier); keys, values and weights move together in their order, in place, to the front of the request's own pages.  Returns (lengths int32 [B] now, the
     places that the kept keys had, ascending, int32 [B, kv heads, budget], -1 behind the last of a shorter request).  lengths_out may be `lengths`.  A page may belong
@@ -350,10 +350,10 @@ def evict(weights, pages, lengths, block_table, *, budget: int, sinks: int = 0, 
     device = _rows(weights, "weights", _F32, 3)
     if _elsewhere(device, stream):
         with _under(device, stream):
-            return evict(weights, pages, lengths, block_table, budget=budget, sinks=sinks, recent=recent, max_keys=max_keys, lengths_out=lengths_out, kept=kept)
+            return evict(weights, pages, lengths, block_table, budget=budget, sinks=sinks, recent=recent, max_keys=max_keys, lengths_out=lengths_out, kept=kept, workspace=workspace)
     stream = _stream(device, stream)
-    mine = _structs
-    kv_heads, page_size, _, cols = _batch(mine.batch, pages, _NO_ROWS, lengths, block_table, 0, device, _keep(device, stream))
+    state, mine = _keep(device, stream), _structs
+    kv_heads, page_size, _, cols = _batch(mine.batch, pages, _NO_ROWS, lengths, block_table, 0, device, state)
     _need(weights, "weights", _F32, (pages.shape[0], kv_heads, page_size), device)
     if not (1 <= budget <= 2**31 - 1 and sinks >= 0 and recent >= 0 and sinks + recent <= budget):
         raise ValueError("budget must be at least 1 and hold sinks + recent keys")
@@ -367,7 +367,8 @@ def evict(weights, pages, lengths, block_table, *, budget: int, sinks: int = 0, 
         kept = torch.empty_strided(shape, (kv_heads * budget, budget, 1), dtype=_I32, device=weights.device)
     else:
         _need(kept, "kept", _I32, shape, device)
-    _EVICT(mine.evict, 0, weights.data_ptr(), lengths_out.data_ptr(), kept.data_ptr(), cols * page_size if max_keys is None else max_keys, budget, sinks, recent, 0)
+    space, size = _space(workspace, state, device, stream)
+    _EVICT(mine.evict, 0, weights.data_ptr(), lengths_out.data_ptr(), kept.data_ptr(), space, size, cols * page_size if max_keys is None else max_keys, budget, sinks, recent, 0)
     _ok(lib.phx_evict_device(device, mine.batch_ref, mine.evict_ref, stream))
     return lengths_out, kept
 
