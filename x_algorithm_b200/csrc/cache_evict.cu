@@ -4,9 +4,10 @@
 // Two launches.  evict_select_kernel finds what stays: a cluster of blocks shares a head's keys, each with its stretch of weights in shared memory as integers of the
 // same order, and the smallest weight that stays comes out of three histograms, of 11, 11 and 10 bits, summed over the cluster (fewer where a digit decides already);
 // the places that stay are then numbered by prefix sums, equal weights by their order.  evict_move_kernel moves rows: a block takes what goes to one chunk of a head's places,
-// keys, values and weights, into shared memory, says so, and writes it once all chunks in front of it have been read.  That is enough: a row only ever moves to the front, so what
-// lies in a chunk's places is taken by that chunk or one before it.  Chunks are handed out in order, by a counter, so a block only waits for blocks that have begun, and whose reads
-// wait for nothing.  (Blocks that went through a head's places from front to back by themselves: 247 us for 2 x 4 heads of 100 k keys, 89 us for 64 x 4 of 4096.)
+// keys, values and weights, into shared memory, says so, and writes it once what it writes over has been read.  A row only ever moves to the front, so what lies in a chunk's
+// places is taken by that chunk or one before it, by two at most: it is no more than fills one.  Chunks are handed out in order, by a counter, so a block only waits for blocks that
+// have begun, and whose reads wait for nothing.  (Waiting for all chunks in front, 2 x 4 heads of 100 k keys took 71 us.)
+//  (Blocks that went through a head's places from front to back by themselves: 247 us for 2 x 4 heads of 100 k keys, 89 us for 64 x 4 of 4096.)
 #include <string>
 
 #include "cache_batch.cuh"
@@ -42,11 +43,12 @@ __device__ __forceinline__ EvictRequest evict_request(const EvictView& t, int b)
 
 // ---- what stays ------------------------------------------------------------------------------------------------------------
 
-constexpr int SEL_THREADS = 512, SEL_BINS = 2048;
+constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, SEL_BINS = 2048, SEL_COARSE = SEL_BINS / 32, SEL_RANKS = 8;
 struct SelectSmem {
   uint32_t hist[3][SEL_BINS];
-  uint32_t warp_sum[2][SEL_THREADS / 32];
-  uint32_t taken[2];             // this block's heavier weights, and those equal to the smallest that stays
+  uint32_t coarse[3][SEL_COARSE];        // sums of 32 bins
+  uint32_t warp_more[SEL_WARPS], warp_same[SEL_WARPS];
+  uint32_t taken[2];                     // this block's heavier weights, and those equal to the smallest that stays
   uint32_t bin, above, in_bin;
 };
 
@@ -62,12 +64,6 @@ __device__ __forceinline__ uint32_t remote_u32(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ uint4 remote_u32x4(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-
 __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictView t) {
   extern __shared__ __align__(16) uint8_t smem_bytes[];
   SelectSmem& sm = *reinterpret_cast<SelectSmem*>(smem_bytes);
@@ -113,34 +109,37 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
       const uint32_t v = order_at(i);
       if (pass == 0 || (v >> (shift + bits)) == prefix) atomicAdd(&hist[(v >> shift) & ((1u << bits) - 1)], 1u);
     }
-    if (ranks > 1) cluster_sync_all(); else __syncthreads();
-    // bins 4 tid' .. 4 tid' + 3, from the top: tid 0 has the highest
-    const int bin0 = SEL_BINS - 4 - 4 * tid;
-    uint4 sum = make_uint4(0, 0, 0, 0);
-    const uint32_t addr = smem_u32(hist + bin0);
-    if (ranks == 1) {
-      sum = *reinterpret_cast<const uint4*>(hist + bin0);
-    } else {
-      uint4 v[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) v[r] = r < ranks ? remote_u32x4(mapa_shared(addr, r)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int r = 0; r < 8; ++r) { sum.x += v[r].x; sum.y += v[r].y; sum.z += v[r].z; sum.w += v[r].w; }
-    }
-    uint32_t mine = sum.x + sum.y + sum.z + sum.w, upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o); upto += lane >= o ? x : 0; }
-    if (lane == 31) sm.warp_sum[0][warp] = upto;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) upto += sm.warp_sum[0][w];
-    if (upto >= want && upto - mine < want) {                // the bin is one of this thread's
-      uint32_t above = upto - mine;
-      const uint32_t of[4] = {sum.w, sum.z, sum.y, sum.x};
+    for (int c = warp; c < SEL_COARSE; c += SEL_WARPS) {
+      const uint32_t sum = __reduce_add_sync(0xffffffffu, hist[c * 32 + lane]);
+      if (lane == 0) sm.coarse[pass][c] = sum;
+    }
+    if (ranks > 1) cluster_sync_all(); else __syncthreads();
+    if (warp == 0) {                                         // the bin of the last that stays, from the top: among the coarse ones first
+      auto sum_of = [&](const uint32_t* p) {
+        if (ranks == 1) return *p;
+        uint32_t v[SEL_RANKS], sum = 0;
+        const uint32_t addr = smem_u32(p);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (above < want && above + of[k] >= want) { sm.bin = (uint32_t)(bin0 + 3 - k); sm.above = above; sm.in_bin = of[k]; }
-        above += of[k];
-      }
+        for (int r = 0; r < SEL_RANKS; ++r) v[r] = r < ranks ? remote_u32(mapa_shared(addr, r)) : 0;
+#pragma unroll
+        for (int r = 0; r < SEL_RANKS; ++r) sum += v[r];
+        return sum;
+      };
+      auto upto = [&](uint32_t v) {                          // with those of the lanes in front
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(0xffffffffu, v, o); v += lane >= o ? x : 0; }
+        return v;
+      };
+      const int c0 = SEL_COARSE - 1 - 2 * lane;              // this lane's coarse bins: c0, c0 - 1
+      const uint32_t s0 = sum_of(&sm.coarse[pass][c0]), s1 = sum_of(&sm.coarse[pass][c0 - 1]), with = upto(s0 + s1), front = with - s0 - s1;
+      const int owner = __ffs(__ballot_sync(0xffffffffu, with >= want)) - 1;
+      const bool second = front + s0 < want;
+      const int coarse = __shfl_sync(0xffffffffu, second ? c0 - 1 : c0, owner);
+      const uint32_t above = __shfl_sync(0xffffffffu, second ? front + s0 : front, owner);
+      const uint32_t mine = sum_of(&hist[coarse * 32 + 31 - lane]), to = above + upto(mine);
+      const int at = __ffs(__ballot_sync(0xffffffffu, to >= want)) - 1;
+      if (lane == at) { sm.bin = (uint32_t)(coarse * 32 + 31 - lane); sm.above = to - mine; sm.in_bin = mine; }
     }
     __syncthreads();
     prefix = (prefix << bits) | sm.bin;
@@ -150,34 +149,30 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
     __syncthreads();
   }
 
-  // numbers of what stays: a thread's keys lie one behind the other (an odd number of them: no two of a warp in one bank)
-  const int seg = ((count + SEL_THREADS - 1) / SEL_THREADS) | 1, i0 = min(tid * seg, count), i1 = min(i0 + seg, count);
+  // numbers of what stays: a warp's keys lie one behind the other, 32 at a time
+  const int seg = ((count + SEL_WARPS - 1) / SEL_WARPS + 31) & ~31, i0 = min(warp * seg, count), i1 = min(i0 + seg, count);
   uint32_t more = 0, same = 0;
-  for (int i = i0; i < i1; ++i) { const uint32_t v = order_at(i); more += v > least; same += v == least; }
-  uint32_t more_upto = more, same_upto = same;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t x = __shfl_up_sync(0xffffffffu, more_upto, o), y = __shfl_up_sync(0xffffffffu, same_upto, o);
-    more_upto += lane >= o ? x : 0; same_upto += lane >= o ? y : 0;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const uint32_t v = i < i1 ? order_at(i) : 0;
+    more += __popc(__ballot_sync(0xffffffffu, i < i1 && v > least)); same += __popc(__ballot_sync(0xffffffffu, i < i1 && v == least));
   }
+  if (lane == 0) { sm.warp_more[warp] = more; sm.warp_same[warp] = same; }
   __syncthreads();
-  if (lane == 31) { sm.warp_sum[0][warp] = more_upto; sm.warp_sum[1][warp] = same_upto; }
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) { more_upto += sm.warp_sum[0][w]; same_upto += sm.warp_sum[1][w]; }
-  if (tid == SEL_THREADS - 1) { sm.taken[0] = more_upto; sm.taken[1] = same_upto; }
-  uint32_t more_before = more_upto - more, same_before = same_upto - same;
+  uint32_t more_before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_more[lane] : 0), same_before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_same[lane] : 0);
   if (ranks > 1) {
+    if (tid == SEL_THREADS - 32) { sm.taken[0] = more_before + more; sm.taken[1] = same_before + same; }   // the last warp
     cluster_sync_all();
-    for (int r = 0; r < rank; ++r) {
-      more_before += remote_u32(mapa_shared(smem_u32(&sm.taken[0]), r));
-      same_before += remote_u32(mapa_shared(smem_u32(&sm.taken[1]), r));
-    }
+    const bool in_front = lane < rank;
+    more_before += __reduce_add_sync(0xffffffffu, in_front ? remote_u32(mapa_shared(smem_u32(&sm.taken[0]), in_front ? lane : 0)) : 0);
+    same_before += __reduce_add_sync(0xffffffffu, in_front ? remote_u32(mapa_shared(smem_u32(&sm.taken[1]), in_front ? lane : 0)) : 0);
   }
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t v = order_at(i);
-    const uint32_t to = rq.sinks + more_before + min(same_before, equal);
-    if ((v > least || (v == least && same_before < equal)) && to < (uint32_t)t.a.budget) kept[to] = from + i;
-    more_before += v > least; same_before += v == least;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const uint32_t v = i < i1 ? order_at(i) : 0, in_front = (1u << lane) - 1;
+    const bool heavier = i < i1 && v > least, like = i < i1 && v == least;
+    const uint32_t heavier_of = __ballot_sync(0xffffffffu, heavier), like_of = __ballot_sync(0xffffffffu, like);
+    const uint32_t likes = same_before + __popc(like_of & in_front), to = rq.sinks + more_before + __popc(heavier_of & in_front) + min(likes, equal);
+    if ((heavier || (like && likes < equal)) && to < (uint32_t)t.a.budget) kept[to] = from + i;
+    more_before += __popc(heavier_of); same_before += __popc(like_of);
   }
   // the first keys and the last ones
   const int recent = rq.length - rq.behind;
@@ -225,21 +220,29 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictVie
   const int* const kept = t.a.kept_out + (long long)of * t.a.budget;
   // the one reader of this request's length in this launch, so that lengths_out may be lengths
   if (chunk == 0 && h == 0 && tid == 0) t.a.lengths_out[b] = min(evict_request(t, b).length, t.a.budget);
-  if (kept[t.a.budget - 1] < t.a.budget) return;             // at most `budget` keys: all where they are
   const int first = chunk * t.rows, count = min(t.rows, t.a.budget - first);
   const int* const table = t.c.block_table + (long long)b * t.c.table_stride;
-  auto page_at = [&](int place) {                            // -1: none of the pool's
-    const int page = table[page_column(t, place)];
-    if ((unsigned)page < (unsigned)t.c.num_pages) return page;
+  auto good = [&](int page) {
+    if ((unsigned)page < (unsigned)t.c.num_pages) return true;
     cache_report(t.c, CACHE_BAD_PAGE);
-    return -1;
+    return false;
   };
-  for (int i = tid; i < count; i += MOVE_THREADS) {
-    const int src = kept[first + i], to = page_at(first + i), page = page_at(src);
-    const bool moves = src != first + i && to >= 0 && page >= 0;
-    from[i] = moves ? src - page_column(t, src) * t.c.page_size : -1;
-    from_page[i] = page; to_page[i] = to;
-    if (moves) weight[i] = t.a.weights[((long long)page * t.c.num_kv_heads + h) * t.c.page_size + from[i]];
+  // Round trips: the place that this thread's place receives and its page at once (the first `budget` places have columns where a request is over its budget), that one's page, its rows.
+  const int last = kept[t.a.budget - 1];
+  int src = -1, to = -1;
+  const int place = first + tid, col = page_column(t, place);
+  if (tid < count) {
+    src = kept[place];
+    if (col < t.c.table_cols) to = table[col];
+  }
+  if (last < t.a.budget) return;                             // at most `budget` keys: all where they are
+  if (tid < count) {
+    const int src_col = page_column(t, src), page = table[src_col], slot = src - src_col * t.c.page_size;
+    const bool there = good(to), moves = good(page) && there && src != place;
+    from[tid] = moves ? slot : -1;
+    from_page[tid] = page; to_page[tid] = to;
+    if (moves)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(weight + tid)), "l"(t.a.weights + ((long long)page * t.c.num_kv_heads + h) * t.c.page_size + slot) : "memory");
   }
   __syncthreads();
   const int pieces = t.c.key_size / 8;                       // of 16 bytes of a row; the values' rows behind the keys'
@@ -250,11 +253,22 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictVie
     if (from[i] < 0) continue;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(data + (r * pieces + piece) * 16)), "l"(address(from_page[i], which, from[i])) : "memory");
   }
-  asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  // under the copies: the first of the kept rows that lies in this chunk's places (or behind), 256 looked at at a time
+  int reader = 0;
+  for (int left = first + 1; left > 0;) {                    // it is not behind place `first` of the kept ones
+    const int step = (left + MOVE_THREADS - 1) / MOVE_THREADS, at = tid * step;
+    const int before = __syncthreads_count(at < left && kept[reader + min(at, left - 1)] < first);
+    if (before == 0) break;
+    reader += (before - 1) * step + 1;
+    left = min(step - 1, left - (before - 1) * step - 1);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   int* const read = t.read + (long long)of * t.chunks;
   if (tid == 0) asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(read + chunk), "r"(1) : "memory");
-  if (!wait_all_set(read, chunk, t.c.status_dev)) return;
+  const int from_chunk = reader / t.rows, to_chunk = min(chunk, (reader + t.rows - 1) / t.rows + 1);   // in front of this one: whose sources may lie here
+  if (!wait_all_set(read + from_chunk, to_chunk - from_chunk, t.c.status_dev)) return;
   for (int r = row_of; r < 2 * count; r += rows_on) {
     const int which = r >= count, i = r - which * count;
     if (from[i] < 0) continue;
@@ -297,7 +311,7 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
 
   // Blocks of a cluster: as long as the heads' clusters fit the device twice over and a block keeps 1024 weights
   int ranks = 1;
-  while (ranks < 8 && heads * ranks * 2 <= 2ll * device_sms() && t.a.max_keys / ranks > 1024) ranks *= 2;
+  while (ranks < SEL_RANKS && heads * ranks * 2 <= 2ll * device_sms() && t.a.max_keys / ranks > 1024) ranks *= 2;
   constexpr int MOST_HELD = 48 * 1024;                        // weights: 192 KB beside the histograms; longer stretches are read from memory at each pass
   const long long per = (t.a.max_keys + ranks - 1) / ranks;
   t.held = (int)(per < MOST_HELD ? per : MOST_HELD);
