@@ -259,6 +259,10 @@ EVICT = [
     (2, 20011, 2, 64, 128, 10000, 0, 1000),
     (1, 70001, 1, 64, 128, 30000, 4, 64),
     (40, 500, 8, 64, 32, 250, 4, 64),
+    (3, 30000, 2, 64, 16, 200, 4, 64),
+    (2, 900, 2, 32, 128, 256, 0, 0),
+    (2, 900, 2, 128, 16, 128, 4, 100),
+    (2, 900, 2, 128, 16, 129, 4, 100),
 ]
 
 
@@ -282,7 +286,11 @@ def test_evict(case, values):
             w = torch.where(pick == i, x, w)
     c["weights"] = w
     want = evict_plain(c, c["n_old"], budget, sinks, recent)
+    copies = [c[k].clone() for k in ("weights", "pages", "lengths")]
     lengths, kept = decoding.evict(c["weights"], c["pages"], c["lengths"], c["table"], budget=budget, sinks=sinks, recent=recent)
+    in_place, again = decoding.evict(*copies, c["table"], budget=budget, sinks=sinks, recent=recent, lengths_out=copies[2], max_keys=1)   # lengths written over, a hint too small
+    assert in_place is copies[2] and torch.equal(in_place, lengths) and torch.equal(again, kept)
+    assert torch.equal(copies[1].view(torch.int16), c["pages"].view(torch.int16)) and torch.equal(copies[0].view(torch.int32), c["weights"].view(torch.int32))
     decoding.check_status()
     assert torch.equal(lengths, want[2]) and torch.equal(kept, want[3])
     assert torch.equal(c["pages"].view(torch.int16), want[0].view(torch.int16))

@@ -25,6 +25,7 @@ struct EvictView {
   int held;                      // weights that a block of the select keeps in shared memory
   int rows;                      // places of a chunk
   int chunks;                    // of a head
+  int alone;                     // few rows: the select's blocks move them, too
   int* ticket;                   // the next chunk to hand out
   int* read;                     // [batch][heads][chunks] whether it has been read
 };
@@ -41,16 +42,70 @@ __device__ __forceinline__ EvictRequest evict_request(const EvictView& t, int b)
   return r;
 }
 
+// ---- a chunk of a head's places, moved by a block ------------------------------------------------------------------------------
+
+struct ChunkPlaces { int to_page[256], from[256], from_page[256]; float weight[256]; };   // of each place: its page, the slot and page of what it receives (slot -1: nothing)
+template <int THREADS>
+struct ChunkMove {
+  const EvictView& t;
+  ChunkPlaces& at;
+  uint8_t* data;                                             // rows of keys, behind them rows of values
+  int b, h, first, count, pieces;                            // pieces of 16 bytes in a row
+  __device__ __forceinline__ bool good(int page) const {
+    if ((unsigned)page < (unsigned)t.c.num_pages) return true;
+    cache_report(t.c, CACHE_BAD_PAGE);
+    return false;
+  }
+  __device__ __forceinline__ uint8_t* address(int page, int which, int slot, int piece) const {
+    return reinterpret_cast<uint8_t*>(t.c.pages + cache_row0(t.c, page, which, h) + (long long)slot * t.c.key_size) + piece * 16;
+  }
+  __device__ __forceinline__ const int* table() const { return t.c.block_table + (long long)b * t.c.table_stride; }
+  // place `i` of the chunk, in page `to`, receives place `src`
+  __device__ __forceinline__ void place(int i, int src, int to) {
+    const int src_col = page_column(t, src), page = table()[src_col], slot = src - src_col * t.c.page_size;
+    const bool there = good(to), moves = good(page) && there && src != first + i;
+    at.from[i] = moves ? slot : -1;
+    at.from_page[i] = page; at.to_page[i] = to;
+    if (moves)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(at.weight + i)), "l"(t.a.weights + ((long long)page * t.c.num_kv_heads + h) * t.c.page_size + slot) : "memory");
+  }
+  __device__ __forceinline__ void fetch() {                  // behind a barrier behind place()
+    const int row_of = threadIdx.x / pieces, piece = threadIdx.x - row_of * pieces;
+    for (int r = row_of; r < 2 * count; r += THREADS / pieces) {
+      const int which = r >= count, i = r - which * count;
+      if (at.from[i] < 0) continue;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(data + (r * pieces + piece) * 16)), "l"(address(at.from_page[i], which, at.from[i], piece)) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ void store() const {            // once nothing reads what it writes over
+    const int row_of = threadIdx.x / pieces, piece = threadIdx.x - row_of * pieces;
+    for (int r = row_of; r < 2 * count; r += THREADS / pieces) {
+      const int which = r >= count, i = r - which * count;
+      if (at.from[i] < 0) continue;
+      const int to = first + i, slot = to - page_column(t, to) * t.c.page_size;
+      *reinterpret_cast<uint4*>(address(at.to_page[i], which, slot, piece)) = *reinterpret_cast<const uint4*>(data + (r * pieces + piece) * 16);
+    }
+    for (int i = threadIdx.x; i < count; i += THREADS)
+      if (at.from[i] >= 0) {
+        const int to = first + i, slot = to - page_column(t, to) * t.c.page_size;
+        t.a.weights[((long long)at.to_page[i] * t.c.num_kv_heads + h) * t.c.page_size + slot] = at.weight[i];
+      }
+  }
+};
+
 // ---- what stays ------------------------------------------------------------------------------------------------------------
 
 constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, SEL_BINS = 2048, SEL_COARSE = SEL_BINS / 32, SEL_RANKS = 8;
-struct SelectSmem {
+struct alignas(16) SelectSmem {
   uint32_t hist[3][SEL_BINS];
   uint32_t coarse[3][SEL_COARSE];        // sums of 32 bins
   uint32_t warp_more[SEL_WARPS], warp_same[SEL_WARPS];
   uint32_t taken[2];                     // this block's heavier weights, and those equal to the smallest that stays
   uint32_t bin, above, in_bin;
 };
+
+static_assert(sizeof(SelectSmem) % 16 == 0 && sizeof(ChunkPlaces) % 16 == 0, "what lies behind them is copied to in pieces of 16 bytes");
 
 // the order of weights as that of unsigned integers: NaN above all, zeros alike
 __device__ __forceinline__ uint32_t weight_order(float w) {
@@ -73,7 +128,8 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   const EvictRequest rq = evict_request(t, b);
   if (rank == 0 && h == 0 && tid == 0 && !rq.ok) cache_report(t.c, CACHE_BAD_OFFSETS);
   int* const kept = t.a.kept_out + ((long long)b * t.c.num_kv_heads + h) * t.a.budget;
-  if (rank == 0) {                                           // for the launch behind
+  if (t.alone && rank == 0 && h == 0 && tid == 0) t.a.lengths_out[b] = min(rq.length, t.a.budget);
+  if (!t.alone && rank == 0) {                               // for the launch behind
     int* const read = t.read + ((long long)b * t.c.num_kv_heads + h) * t.chunks;
     for (int i = tid; i < t.chunks; i += SEL_THREADS) read[i] = 0;
     if (b == 0 && h == 0 && tid == 0) *t.ticket = 0;
@@ -91,9 +147,28 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   };
   const bool in_smem = per <= t.held;
   for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) (&sm.hist[0][0])[i] = 0;
-  if (in_smem) {
-#pragma unroll 8
-    for (int i = tid; i < count; i += SEL_THREADS) held[i] = weight_at(from + i);
+  if (in_smem) {                                             // loads without a condition: a batch of pages, then of weights, on their way at once
+    constexpr int BATCH = 4;
+    for (int i0 = tid; i0 < count; i0 += BATCH * SEL_THREADS) {
+      int page[BATCH], slot[BATCH];
+      float w[BATCH];
+      bool bad = false;
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int key = from + min(i0 + k * SEL_THREADS, count - 1), col = page_column(t, key);
+        page[k] = table[col]; slot[k] = key - col * t.c.page_size;
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const bool good = (unsigned)page[k] < (unsigned)t.c.num_pages;
+        bad |= !good;
+        w[k] = t.a.weights[((long long)(good ? page[k] : 0) * t.c.num_kv_heads + h) * t.c.page_size + slot[k]];
+        page[k] = good;
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) if (i0 + k * SEL_THREADS < count) held[i0 + k * SEL_THREADS] = page[k] ? weight_order(w[k]) : 0u;
+      if (bad) cache_report(t.c, CACHE_BAD_PAGE);
+    }
   }
   __syncthreads();
   auto order_at = [&](int i) { return in_smem ? held[i] : weight_at(from + i); };
@@ -178,7 +253,17 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   const int recent = rq.length - rq.behind;
   for (int i = rank * SEL_THREADS + tid; i < rq.sinks; i += ranks * SEL_THREADS) kept[i] = i;
   for (int i = rank * SEL_THREADS + tid; i < recent; i += ranks * SEL_THREADS) kept[t.a.budget - recent + i] = rq.behind + i;
-  if (ranks > 1) cluster_sync_all();                         // the others may still be reading this block's counts
+  if (ranks > 1) cluster_sync_all();                         // the others may still be reading this block's counts; the places that they wrote are there
+  if (!t.alone || rank > 0) return;
+  __syncthreads();
+  if (kept[t.a.budget - 1] < t.a.budget) return;
+  ChunkMove<SEL_THREADS> move{t, *reinterpret_cast<ChunkPlaces*>(held), reinterpret_cast<uint8_t*>(held) + sizeof(ChunkPlaces), b, h, 0, t.a.budget, t.c.key_size / 8};
+  for (int i = tid; i < t.a.budget; i += SEL_THREADS) move.place(i, kept[i], table[page_column(t, i)]);
+  __syncthreads();
+  move.fetch();
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  move.store();
 }
 
 // ---- moving together ---------------------------------------------------------------------------------------------------------
@@ -208,10 +293,8 @@ __device__ __forceinline__ bool wait_all_set(const int* p, int n, volatile int* 
 
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictView t) {
   __shared__ __align__(16) uint8_t data[MOVE_BYTES];
+  __shared__ ChunkPlaces places;
   __shared__ int ticket;
-  __shared__ int to_page[MOVE_BYTES / 128], from[MOVE_BYTES / 128];   // of each place of the chunk: its page, the place that it receives (or -1)
-  __shared__ int from_page[MOVE_BYTES / 128];
-  __shared__ float weight[MOVE_BYTES / 128];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, heads = t.c.batch * t.c.num_kv_heads;
   if (tid == 0) ticket = atomicAdd(t.ticket, 1);
@@ -221,39 +304,19 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictVie
   // the one reader of this request's length in this launch, so that lengths_out may be lengths
   if (chunk == 0 && h == 0 && tid == 0) t.a.lengths_out[b] = min(evict_request(t, b).length, t.a.budget);
   const int first = chunk * t.rows, count = min(t.rows, t.a.budget - first);
-  const int* const table = t.c.block_table + (long long)b * t.c.table_stride;
-  auto good = [&](int page) {
-    if ((unsigned)page < (unsigned)t.c.num_pages) return true;
-    cache_report(t.c, CACHE_BAD_PAGE);
-    return false;
-  };
+  ChunkMove<MOVE_THREADS> move{t, places, data, b, h, first, count, t.c.key_size / 8};
   // Round trips: the place that this thread's place receives and its page at once (the first `budget` places have columns where a request is over its budget), that one's page, its rows.
   const int last = kept[t.a.budget - 1];
   int src = -1, to = -1;
-  const int place = first + tid, col = page_column(t, place);
+  const int col = page_column(t, first + tid);
   if (tid < count) {
-    src = kept[place];
-    if (col < t.c.table_cols) to = table[col];
+    src = kept[first + tid];
+    if (col < t.c.table_cols) to = move.table()[col];
   }
   if (last < t.a.budget) return;                             // at most `budget` keys: all where they are
-  if (tid < count) {
-    const int src_col = page_column(t, src), page = table[src_col], slot = src - src_col * t.c.page_size;
-    const bool there = good(to), moves = good(page) && there && src != place;
-    from[tid] = moves ? slot : -1;
-    from_page[tid] = page; to_page[tid] = to;
-    if (moves)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(weight + tid)), "l"(t.a.weights + ((long long)page * t.c.num_kv_heads + h) * t.c.page_size + slot) : "memory");
-  }
+  if (tid < count) move.place(tid, src, to);
   __syncthreads();
-  const int pieces = t.c.key_size / 8;                       // of 16 bytes of a row; the values' rows behind the keys'
-  const int row_of = tid / pieces, piece = tid - row_of * pieces, rows_on = MOVE_THREADS / pieces;
-  auto address = [&](int page, int which, int slot) { return reinterpret_cast<uint8_t*>(t.c.pages + cache_row0(t.c, page, which, h) + (long long)slot * t.c.key_size) + piece * 16; };
-  for (int r = row_of; r < 2 * count; r += rows_on) {
-    const int which = r >= count, i = r - which * count;
-    if (from[i] < 0) continue;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(data + (r * pieces + piece) * 16)), "l"(address(from_page[i], which, from[i])) : "memory");
-  }
-  asm volatile("cp.async.commit_group;" ::: "memory");
+  move.fetch();
   // under the copies: the first of the kept rows that lies in this chunk's places (or behind), 256 looked at at a time
   int reader = 0;
   for (int left = first + 1; left > 0;) {                    // it is not behind place `first` of the kept ones
@@ -269,17 +332,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictVie
   if (tid == 0) asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(read + chunk), "r"(1) : "memory");
   const int from_chunk = reader / t.rows, to_chunk = min(chunk, (reader + t.rows - 1) / t.rows + 1);   // in front of this one: whose sources may lie here
   if (!wait_all_set(read + from_chunk, to_chunk - from_chunk, t.c.status_dev)) return;
-  for (int r = row_of; r < 2 * count; r += rows_on) {
-    const int which = r >= count, i = r - which * count;
-    if (from[i] < 0) continue;
-    const int place = first + i, slot = place - page_column(t, place) * t.c.page_size;
-    *reinterpret_cast<uint4*>(address(to_page[i], which, slot)) = *reinterpret_cast<const uint4*>(data + (r * pieces + piece) * 16);
-  }
-  for (int i = tid; i < count; i += MOVE_THREADS)
-    if (from[i] >= 0) {
-      const int place = first + i, slot = place - page_column(t, place) * t.c.page_size;
-      t.a.weights[((long long)to_page[i] * t.c.num_kv_heads + h) * t.c.page_size + slot] = weight[i];
-    }
+  move.store();
 }
 
 }  // namespace
@@ -299,6 +352,7 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
   if (t.a.budget < 1 || t.a.sinks < 0 || t.a.recent < 0 || (long long)t.a.sinks + t.a.recent > t.a.budget) return bad("budget must be at least 1 and hold sinks + recent keys");
   if (t.a.max_keys < 0) return bad("negative size");
   if (t.c.batch == 0) return PHX_OK;
+  if (t.c.num_pages == 0) return bad("an empty pool has no keys");
   if (!t.a.weights || !t.a.lengths_out || !t.a.kept_out) return bad("weights, lengths_out and kept_out are required");
   const long long columns = (long long)t.c.table_cols * t.c.page_size;
   if (t.a.max_keys > columns) t.a.max_keys = columns;
@@ -315,6 +369,11 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
   constexpr int MOST_HELD = 48 * 1024;                        // weights: 192 KB beside the histograms; longer stretches are read from memory at each pass
   const long long per = (t.a.max_keys + ranks - 1) / ranks;
   t.held = (int)(per < MOST_HELD ? per : MOST_HELD);
+  // Up to 256 rows and 64 KB of keys and values a head, the select's block moves them itself, in shared memory that the weights were in: a launch less.  Its heads may not all have read
+  // a length that is written over, so lengths_out must not be lengths.
+  const long long move_bytes = (long long)sizeof(ChunkPlaces) + (long long)t.a.budget * 4 * t.c.key_size;
+  t.alone = t.a.budget <= 256 && move_bytes <= 68 * 1024 && (t.a.lengths_out + t.c.batch <= t.c.lengths || t.c.lengths + t.c.batch <= t.a.lengths_out);
+  if (t.alone && t.held * 4 < move_bytes) t.held = (int)((move_bytes + 3) / 4);
   t.rows = MOVE_BYTES / (4 * t.c.key_size);                   // 64 to 256
   t.chunks = (t.a.budget + t.rows - 1) / t.rows;
   if (heads * t.chunks > 2147483647ll) return bad("budget x heads x batch is too large");
@@ -335,7 +394,7 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
     at[0].val.clusterDim.x = ranks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     lc.attrs = at; lc.numAttrs = 1;
     PHX_CUDA_TRY(cudaLaunchKernelEx(&lc, evict_select_kernel, t), err);
-    PHX_CUDA_TRY(launch_programmatic(evict_move_kernel, dim3((unsigned)(heads * t.chunks)), dim3(MOVE_THREADS), 0, st, t), err);
+    if (!t.alone) PHX_CUDA_TRY(launch_programmatic(evict_move_kernel, dim3((unsigned)(heads * t.chunks)), dim3(MOVE_THREADS), 0, st, t), err);
     dispatch_note(DK_CACHE_EVICT);
     return PHX_OK;
   };
