@@ -60,14 +60,15 @@ struct ChunkMove {
     return reinterpret_cast<uint8_t*>(t.c.pages + cache_row0(t.c, page, which, h) + (long long)slot * t.c.key_size) + piece * 16;
   }
   __device__ __forceinline__ const int* table() const { return t.c.block_table + (long long)b * t.c.table_stride; }
-  // place `i` of the chunk, in page `to`, receives place `src`
-  __device__ __forceinline__ void place(int i, int src, int to) {
+  // place `i` of the chunk, in page `to`, receives place `src`; whether it is another
+  __device__ __forceinline__ bool place(int i, int src, int to) {
     const int src_col = page_column(t, src), page = table()[src_col], slot = src - src_col * t.c.page_size;
     const bool there = good(to), moves = good(page) && there && src != first + i;
     at.from[i] = moves ? slot : -1;
     at.from_page[i] = page; at.to_page[i] = to;
     if (moves)
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(at.weight + i)), "l"(t.a.weights + ((long long)page * t.c.num_kv_heads + h) * t.c.page_size + slot) : "memory");
+    return moves;
   }
   __device__ __forceinline__ void fetch() {                  // behind a barrier behind place()
     const int row_of = threadIdx.x / pieces, piece = threadIdx.x - row_of * pieces;
@@ -314,8 +315,11 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictVie
     if (col < t.c.table_cols) to = move.table()[col];
   }
   if (last < t.a.budget) return;                             // at most `budget` keys: all where they are
-  if (tid < count) move.place(tid, src, to);
-  __syncthreads();
+  int* const read = t.read + (long long)of * t.chunks;
+  if (!__syncthreads_or(tid < count && move.place(tid, src, to))) {   // all stays where it is
+    if (tid == 0) asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(read + chunk), "r"(1) : "memory");
+    return;
+  }
   move.fetch();
   // under the copies: the first of the kept rows that lies in this chunk's places (or behind), 256 looked at at a time
   int reader = 0;
@@ -328,7 +332,6 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictVie
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  int* const read = t.read + (long long)of * t.chunks;
   if (tid == 0) asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(read + chunk), "r"(1) : "memory");
   const int from_chunk = reader / t.rows, to_chunk = min(chunk, (reader + t.rows - 1) / t.rows + 1);   // in front of this one: whose sources may lie here
   if (!wait_all_set(read + from_chunk, to_chunk - from_chunk, t.c.status_dev)) return;
