@@ -61,9 +61,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 // what the producer notes about a tile
 struct TileNote {
   int tile;
-  uint32_t flags;                       // bits 0 .. 3: boxes in pages of the pool; MASKED, LAST of the piece, FINAL of the block
+  uint32_t flags;                       // bits 0 .. 3: boxes in pages of the pool; MASKED, LAST of the piece, FINAL of the block; PLACES: new keys that some row's window leaves out
 };
-constexpr uint32_t MASKED = 16, LAST = 32, FINAL = 64, BOXES = 15;
+struct alignas(16) WindowNote : TileNote {
+  int cached, keys;                     // of the request
+};
+template <class View> using NoteOf = std::conditional_t<has_window<View>, WindowNote, TileNote>;
+constexpr uint32_t MASKED = 16, LAST = 32, FINAL = 64, PLACES = 128, BOXES = 15;
 
 template <int DH, class View>
 struct TcSmem {
@@ -71,9 +75,10 @@ struct TcSmem {
   uint8_t q[DCH * SLAB];
   uint8_t k[NB][DCH * KT * 128];
   uint8_t v[NB][DCH * KT * 128];
-  int2 span[2][KT];                     // of a masked tile's keys
-  int place[2][has_window<View> ? KT : 1];
-  TileNote note[8];
+  // (pre, end) of a masked tile's keys; with a window those of new keys alone, and their places, of as many tiles as notes
+  int2 span[has_window<View> ? 8 : 2][KT];
+  int place[has_window<View> ? 8 : 1][has_window<View> ? KT : 1];
+  NoteOf<View> note[8];
   uint64_t q_full, q_empty, k_full[NB], k_empty[NB], v_full[NB], v_empty[NB], s_full[2], p_ready, o_done, o_empty, together;
   uint32_t tmem;
   int odd[2];                           // the last piece (by its number's parity) with infinities or NaN in a masked tile, plus 1
@@ -256,13 +261,30 @@ struct TcBlock {
 #pragma unroll
         for (int p = 0; p < 4; ++p) rows[p] = __shfl_sync(0xffffffffu, row, p);
         if (!wait(sm.k_empty[j % NB], j / NB - 1)) return;
+        bool places = false;
+        if constexpr (WINDOW) {
+          const bool is_chain_call = is_chain(t);                             // what the softmax asks for of new keys, before the next tile's are asked for
+          if ((masked || there != (1u << boxes) - 1) && !is_chain_call && tile >= old_tiles) {
+#pragma unroll
+            for (int i = 0; i < KT / 32; ++i) {
+              const int key = tile * KT + i * 32 + lane;
+              const bool fresh = key >= rq.cached && key < keys;
+              sm.span[j & 7][i * 32 + lane] = fresh ? span_of(t, rq, key - rq.cached) : make_int2(0x7fffffff, -1);
+              const int place = fresh ? key_place(t, rq, key) : 0x7fffffff;
+              if (t.positions) sm.place[j & 7][i * 32 + lane] = place;
+              places |= place <= behind_last;
+            }
+            places = __any_sync(0xffffffffu, places);
+          }
+        }
         const int follows = next_tile(tile + 1, &masked_next);
         __syncwarp();
         if (elect_one()) {
           const int b = j % NB;
-          TileNote n;
+          NoteOf<View> n;
           n.tile = tile;
-          n.flags = there | (masked || there != (1u << boxes) - 1 ? MASKED : 0u) | (follows >= last ? LAST | (more ? 0u : FINAL) : 0u);
+          if constexpr (WINDOW) { n.cached = rq.cached; n.keys = keys; }
+          n.flags = there | (masked || there != (1u << boxes) - 1 ? MASKED : 0u) | (follows >= last ? LAST | (more ? 0u : FINAL) : 0u) | (places ? PLACES : 0u);
           sm.note[j & 7] = n;                              // in front of the arrival, which publishes it
           mbar_expect_tx(smem_u32(&sm.k_full[b]), BLK);
 #pragma unroll
@@ -336,19 +358,48 @@ struct TcBlock {
     }
   }
 
-  // whether the row at `pre`, whose window begins behind place `behind`, sees key k of the masked tile in buffer `at`
-  __device__ __forceinline__ bool sees(int at, int k, int pre, int behind) const {
-    const int2 sp = sm.span[at][k];
-    bool see = sp.x <= pre && pre < sp.y;
-    if constexpr (WINDOW) see &= sm.place[at][k] > behind;
-    return see;
+  // Which keys of a masked tile the row at `pre` sees, whose window begins behind place `behind`: of the cached ones and of a chain a stretch and the
+  // first keys, in a few instructions; of new ones with spans those whose span has it, and those of their places that some window leaves out compared, too.
+  __device__ __forceinline__ void window_seen(const WindowNote& note, bool all_there, int at, int pre, int behind, uint32_t* seen) const {
+    const int key0 = note.tile * KT, cached = note.cached - key0;
+    const bool chain = is_chain(t);                          // `pre` is a token's number then, and it sees up to itself
+    auto below = [](int n) { uint32_t m; asm("bmsk.clamp.b32 %0, 0, %1;" : "=r"(m) : "r"(max(n, 0))); return m; };   // the lowest n bits
+    const int end = min(note.keys - key0, chain ? cached + pre + 1 : cached), begin = behind + 1 - key0, first = t.sinks - key0;
+#pragma unroll
+    for (int w = 0; w < KT / 32; ++w) seen[w] = below(end - 32 * w) & (~below(begin - 32 * w) | below(first - 32 * w));
+    if (!chain && cached < KT) {
+#pragma unroll 1
+      for (int k = 0; k < KT; k += 16) {                    // short code: it runs seldom, and is fetched anew each time
+        uint32_t some = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const int4 s = *reinterpret_cast<const int4*>(&sm.span[at][k + i]);
+          if (s.x <= pre && pre < s.y) some |= 1u << i;
+          if (s.z <= pre && pre < s.w) some |= 2u << i;
+        }
+        some <<= k & 31;
+        if (k < 32) seen[0] |= some; else seen[1] |= some;
+      }
+      if (note.flags & PLACES) {
+#pragma unroll 1
+        for (int k = max(0, cached); k < KT; ++k)
+          if (sm.place[at][k] <= behind) { if (k < 32) seen[0] &= ~(1u << k); else seen[1] &= ~(1u << (k - 32)); }
+      }
+    }
+    if (!all_there) {                                       // keys in no page of the pool
+#pragma unroll 1
+      for (int p = 0; p < KT / box; ++p)
+        if (!((note.flags >> p) & 1))
+          for (int k = p * box; k < (p + 1) * box; k += 16) { if (k < 32) seen[0] &= ~(0xffffu << k); else seen[1] &= ~(0xffffu << (k - 32)); }
+    }
+    if (pre < 0) seen[0] = seen[1] = 0;
   }
 
   // The polynomial and the exponential form of tanh differ in their last bits, so a key that a row does not see must not choose between them.  In a masked tile a row
   // goes by the logits that it sees, 16 keys at a time, in tensor memory and in a loop of its own: beside the code for whole tiles, where a warp takes one form
   // for all, such choices made that code 3 to 20 % slower (registers).  24 trees of 32 over up to 8192 keys, 32 heads of 128: 106 us, 152 with logits around the cap; 110 and 151 when
   // masked tiles were capped there by the warp's choice; 32 x 512 candidates under a cap 97 and 132, were 111 and 128.
-  __device__ __forceinline__ void cap_masked(const TreeCap& cap, uint32_t s_col, int at, int pre, int behind) const {
+  __device__ __forceinline__ void cap_masked(const TreeCap& cap, uint32_t s_col, const int2* span, int pre, const uint32_t* all_seen) const {
     tmem_ld_wait();
 #pragma unroll 1
     for (int c = 0; c < KT / 16; ++c) {
@@ -359,7 +410,9 @@ struct TcBlock {
       float most = 0.f;
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
-        if (sees(at, c * 16 + k, pre, behind)) { seen |= 1u << k; most = fmaxf(most, fabsf(x[k])); }
+        bool see;
+        if constexpr (WINDOW) { see = ((c < 2 ? all_seen[0] : all_seen[1]) >> ((c & 1) * 16 + k)) & 1; } else { const int2 sp = span[c * 16 + k]; see = sp.x <= pre && pre < sp.y; }
+        if (see) { seen |= 1u << k; most = fmaxf(most, fabsf(x[k])); }
       }
       if (most * cap.small_scale <= TreeCap::SMALL) {
         if (seen != 0) {
@@ -417,20 +470,23 @@ struct TcBlock {
 #pragma unroll
           for (int c = 0; c < KT / 32; ++c) tmem_ld32_nowait(s_col + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
         }
-        const TileNote note = sm.note[j & 7];
+        const NoteOf<View> note = sm.note[j & 7];
         const bool masked = note.flags & MASKED;
-        if (masked) {                                       // the same for all 128 threads
-          if (r < KT) {
-            const int key = note.tile * KT + r;
-            int2 sp = make_int2(0, 0x7fffffff);             // cached: seen by all but padding
-            if (key >= kr.keys || !((note.flags >> (r / box)) & 1)) sp = make_int2(0x7fffffff, -1);
-            else if (key >= rq.cached) sp = span_of(t, rq, key - rq.cached);
-            sm.span[j & 1][r] = sp;
-            if constexpr (WINDOW) sm.place[j & 1][r] = key < kr.keys ? key_place(t, rq, key) : 0;
-          }
-          // infinities and NaN among the values: out of the product
-          if (!wait(sm.v_full[j % NB], j / NB)) return;
+        // Infinities and NaN among a masked tile's values: out of the product
+        auto take_out_odd = [&](bool look_first) {
+          if (!wait(sm.v_full[j % NB], j / NB)) return false;
           uint4* const v = reinterpret_cast<uint4*>(sm.v[j % NB]);
+          if (look_first) {                                  // the largest size of all: neither infinite nor NaN, as a rule
+            __nv_bfloat162 most = __float2bfloat162_rn(0.f);
+#pragma unroll
+            for (int i = 0; i < (int)BLK / 2048; ++i) {
+              const uint4 x = v[i * 128 + r];
+              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) most = __hmax2_nan(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[k])));
+            }
+            if (!odd_pair(*reinterpret_cast<const uint32_t*>(&most))) return true;
+          }
           bool odd = false;
           for (int i = r; i < (int)BLK / 16; i += 128) {
             uint4 x = v[i];
@@ -444,13 +500,28 @@ struct TcBlock {
           }
           if (odd) sm.odd[piece & 1] = piece + 1;
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          return true;
+        };
+        if (!WINDOW && masked) {                            // the same for all 128 threads
+          if (r < KT) {
+            const int key = note.tile * KT + r;
+            int2 sp = make_int2(0, 0x7fffffff);             // cached: seen by all but padding
+            if (key >= kr.keys || !((note.flags >> (r / box)) & 1)) sp = make_int2(0x7fffffff, -1);
+            else if (key >= rq.cached) sp = span_of(t, rq, key - rq.cached);
+            sm.span[j & 1][r] = sp;
+          }
+          if (!take_out_odd(false)) return;
           mbar_arrive(smem_u32(&sm.together));              // a barrier of the softmax threads whose wait is bounded, too
           if (!wait(sm.together, together++)) return;
+        }
+        uint32_t seen[KT / 32] = {0, 0};
+        if constexpr (WINDOW) {
+          if (masked) { window_seen(note, (note.flags & BOXES) == all_there, j & 7, pre, behind, seen); __syncwarp(); }
         }
         float alpha = 1.0f;
         if (busy) {
           if (CAP == 2 && masked) {
-            cap_masked(cap, s_col, j & 1, pre, behind);
+            cap_masked(cap, s_col, sm.span[j & 1], pre, seen);
 #pragma unroll
             for (int c = 0; c < KT / 32; ++c) tmem_ld32_nowait(s_col + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
           }
@@ -494,7 +565,10 @@ struct TcBlock {
           }
           if (masked && CAP != 2) {
 #pragma unroll
-            for (int k = 0; k < KT; ++k) if (!sees(j & 1, k, pre, behind)) s[k] = -INFINITY;
+            for (int k = 0; k < KT; ++k) {
+              if constexpr (WINDOW) { if (!((seen[k / 32] >> (k & 31)) & 1)) s[k] = -INFINITY; }
+              else { const int2 sp = sm.span[j & 1][k]; if (!(sp.x <= pre && pre < sp.y)) s[k] = -INFINITY; }
+            }
           }
           if (CAP != 2 || masked) bm = top_of();
           // The reference only has to bound the exponentials: it moves when the maximum has outgrown it by 2^8 (P stays below 256, as exact in bf16 as below
@@ -535,6 +609,7 @@ struct TcBlock {
           tc_fence_before();
           l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
         }
+        if (WINDOW && masked && !take_out_odd(true)) return;    // no other thread's stores are read here: they are there with the arrival below
         // S of this tile did not wait for P V of the one before: its barrier must not run two phases ahead of the issuer
         if (j > first && !wait(sm.o_done, j - 1)) return;
         mbar_arrive(smem_u32(&sm.p_ready));
