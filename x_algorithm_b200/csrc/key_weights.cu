@@ -18,7 +18,7 @@
 namespace phx {
 namespace {
 
-constexpr int KW_WARPS = 8, KW_KEYS = 16, KW_PER = 4;   // tiles of a warp
+constexpr int KW_WARPS = 8, KW_KEYS = 16, KW_PER = 8;   // tiles of a warp
 constexpr int KW_BLOCK_TILES = KW_WARPS * KW_PER;
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -93,20 +93,24 @@ __global__ void __launch_bounds__(32 * KW_WARPS, DH == 128 && NB == 2 ? 1 : 2) k
 
   uint4 k[2][2][CH];
   int tile_of[2], page_in[2];
+  float old[2];                                            // the weight of this lane's key, on its way with the keys
   int begin = blockIdx.x * KW_BLOCK_TILES + warp;
-  auto fetch = [&](int it, int to) {                       // the tile of turn `it`
-    const int i = begin + it * KW_WARPS;
-    tile_of[to] = i < count ? (i < sinks ? i : i - sinks + first) : -1;
+  auto tile_at = [&](int it) { const int i = begin + it * KW_WARPS; return i < count ? (i < sinks ? i : i - sinks + first) : -1; };   // of turn `it`
+  int pages = -1;                                          // lane i: the page of turn i, all of them asked for at once
+  auto ask_pages = [&]() { const int tile = lane < KW_PER ? tile_at(lane) : -1; if (tile >= 0) pages = kr.table[tile * KW_KEYS / t.c.page_size]; };
+  auto fetch = [&](int it, int to) {
+    tile_of[to] = tile_at(it);
     if (tile_of[to] < 0) return;
-    const int key = tile_of[to] * KW_KEYS, col = key / t.c.page_size;
-    const int page = kr.table[col];
+    const int key = tile_of[to] * KW_KEYS, page = __shfl_sync(0xffffffffu, pages, it);
     page_in[to] = page;
     if ((unsigned)page >= (unsigned)t.c.num_pages) return;
-    const uint16_t* src = t.c.pages + cache_row0(t.c, page, 0, h) + (long long)(key - col * t.c.page_size + quad) * DH + in * 8;
+    const uint16_t* src = t.c.pages + cache_row0(t.c, page, 0, h) + (long long)(key % t.c.page_size + quad) * DH + in * 8;
 #pragma unroll
     for (int c = 0; c < CH; ++c) { k[to][0][c] = load_once(src + c * 32); k[to][1][c] = load_once(src + 8 * DH + c * 32); }
+    old[to] = in < 2 ? t.weights[((long long)page * t.c.num_kv_heads + h) * t.c.page_size + key % t.c.page_size + quad + 8 * in] : 0.f;
   };
   if (begin >= count) return;
+  ask_pages();
   fetch(0, 0);
   if (!many && rows > 0) load_rows(0);
   for (;;) {
@@ -178,12 +182,12 @@ __global__ void __launch_bounds__(32 * KW_WARPS, DH == 128 && NB == 2 ? 1 : 2) k
     const int key = key0 + quad + 8 * in;
     if (in < 2 && key < kr.keys) {
       float* const w = t.weights + ((long long)page * t.c.num_kv_heads + h) * t.c.page_size + key % t.c.page_size;
-      const float old = key < rq.cached ? *w * t.decay : 0.f;
-      *w = old + (in == 0 ? sum[0] : sum[1]);
+      *w = (key < rq.cached ? old[cur] * t.decay : 0.f) + (in == 0 ? sum[0] : sum[1]);
     }
   }
   begin += gridDim.x * KW_BLOCK_TILES;                     // requests longer than the caller said
   if (begin >= count) return;
+  ask_pages();
   fetch(0, 0);
   }
 }

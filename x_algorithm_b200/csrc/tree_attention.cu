@@ -584,7 +584,10 @@ phx_status attend(int32_t device, const phx_cache_batch* cache, View& t, cudaStr
   }
   const long long blocks = per_sm * device_sms(), fed = units * (tiles + t.setup) / (tc ? 8 : 4);   // no block for fewer places: parts and joins take longer than that many
   const long long idle = (units + blocks - 1) / blocks * blocks - units;                  // blocks without a unit in the last round of whole ones
-  const bool few = tc ? tiles >= 8 && (units < 2 * blocks || idle * tiles > 3 * t.c.key_size / 8 * blocks) : tiles >= 4 && units < 8 * blocks;
+  // With a window the first keys have a tile of their own, mostly empty, and parts and join pay from 10 tiles on: one token, 16 heads on 4 key heads of 128, windows of 128, 256,
+  // 384, 512, 768, 1024 keys: shared 15.4, 16.2, 16.7, 17.1, 17.1, 17.5 us, whole 9.7, 12.1, 14.4, 16.8, 21.3, 26.0 (8 heads of 64: 12.6 to 14.6, whole 8.1 to 22.0; 8 requests alike).
+  const int least = has_window<View> ? 10 : 4;
+  const bool few = tc ? tiles >= 8 && (units < 2 * blocks || idle * tiles > 3 * t.c.key_size / 8 * blocks) : tiles >= least && units < 8 * blocks;
   t.split = few && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)(fed < blocks ? fed : blocks) : 0;
   if (t.split < 2) t.split = 0;                                                            // one block takes whole units: there is no bound between blocks, nothing to join
   t.turns = tc && !t.split && units > blocks && t.c.batch <= TREE_MAX_SPLIT_BATCH ? (int)blocks : 0;
