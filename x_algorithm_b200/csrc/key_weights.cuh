@@ -9,7 +9,6 @@ struct WeightsView : WindowView {   // lse is read here
   float* weights;                   // [num_pages][num_kv_heads][page_size]
   float decay;
   int chunks;                       // of a request's tiles of rows that different blocks take (tcgen05 kernel); above 1 their sums are joined behind
-  float* part;                      // [chunks][unit][keys of a tile] sums of a chunk
 };
 
 // cap(s * scale) in the log2 domain, two at a time.  A weight is an fp32 number that follows its logit one to one, so tanh is an odd polynomial with one coefficient more than

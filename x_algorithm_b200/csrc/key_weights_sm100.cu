@@ -1,14 +1,15 @@
 // The attention weight that cached keys receive, on Blackwell tensor cores (tcgen05 + TMEM + TMA), for requests of more than 16 query rows a key head; the semantics are
 // key_weights.cu's.  S^T = K Q^T: 128 keys are the rows of the product and 256 query rows its columns, so that a key's sum over the queries is the sum along one thread's row of
-// tensor memory, and no thread needs another's.  A block (one an SM) takes unit after unit - a request, key head and tile of 128 keys, with all tiles of rows or a
-// chunk of them - K once, then the rows that see one of its keys, two tiles of 128 at a time (each role's own instructions a time, 1000 to 2700 cycles of a warp that is alone in its
-// code, were what the block waited for at one: 8 x 1022 tokens that see themselves, 16 heads of 128, 76 us):
-//   warp 0      producer: K (page by page) and Q tiles by TMA, and a note about each pair
+// tensor memory, and no thread needs another's.
+//
+// key_weights_plan_kernel writes down, a warp for each, the units - a request, key head and tile of 128 keys, with all tiles of 128 rows that may see them or a chunk of those - and the tiles of
+// rows: their lse, what they see, and its bounds for each 32 of them.  key_weights_tc_kernel, a block an SM, takes unit after unit, K once, then its rows, two tiles at a time:
+//   warp 0      producer: K (page by page) and Q tiles by TMA, what is written down about them by bulk copies
 //   warp 1      MMA issuer: S^T into one of two buffers of tensor memory
-//   warp 2      planner, units ahead: where a unit's keys lie, what sees them, which tiles of rows
-//   warps 3, 20 .. 22   every fourth tile of rows each: the rows' lse and what they see, which of the four groups of 32 rows see keys at all, and which not all
-//   warps 4-19  thread = key and a group of the rows: e^(x - lse) summed up in a register; at the unit's end the groups hand their sums to the first, which writes the weight
-//               (or a part, where chunks of rows are joined by key_weights_join_kernel)
+//   warps 4-19  thread = key and a group of 32 rows of either tile: e^(x - lse) summed up in a register, masked where some key of the warp is not seen by some row of the group; at the
+//               unit's end the groups hand their sums to the first, which writes the weight (or a part, where chunks of rows are joined by key_weights_join_kernel)
+// (All of that in one kernel, by a planner warp and four that described rows, was slower: such code runs at 10 cycles an instruction, by one warp beside sixteen, and the block waited for it.
+// 32 x 512 candidates over up to 1022 keys, 8 heads of 64: 62 us; 8 x 1022 tokens that see themselves, 16 heads of 128: 66 us.)
 // Waits are bounded; when one runs out the flag is raised, every later wait of any role fails at once, and a role whose wait failed is done.
 #include <string.h>
 
@@ -24,43 +25,33 @@ using namespace sm100;
 
 constexpr int KT = 128, HT = 128, RT = 2 * HT;   // keys of a tile, rows of a tile, of a pair
 constexpr int KW_FIRST = 4, KW_SETS = 4, KW_SUM = 4 * KW_SETS;   // warps 4 .. 19 sum, four for each group of 32 rows
-constexpr int KW_ROWS = 4, KW_THREADS = 32 * (KW_FIRST + KW_SUM + KW_ROWS - 1);
-constexpr int NK = 2, NS = 2;            // K tiles in shared memory, S^T buffers in tensor memory
+constexpr int KW_THREADS = 32 * (KW_FIRST + KW_SUM);
+constexpr int PLAN_THREADS = 256;
+constexpr int NK = 2, NS = 2, NR = 4;    // K tiles in shared memory, S^T buffers in tensor memory, pairs whose rows are described
 __host__ __device__ constexpr int q_buffers(int dh) { return dh == 64 ? 3 : 2; }      // pairs of Q tiles
-__host__ __device__ constexpr int row_buffers(int dh) { return dh == 64 ? 4 : 3; }    // pairs that are described
-constexpr int NU = 4;                    // units that are planned or worked on
+constexpr int NU = 4;                    // units that are worked on
 
-struct alignas(16) RowNote { float less[RT]; int2 sees[RT]; uint32_t flags[2]; };   // -lse in the log2 domain, -inf: no weight; (place in the walk or -1, place behind which the window begins)
-struct KeyNote { int x, y, place, at; };            // span, place in the window's terms, word of the weights or -1: no key
-constexpr uint32_t MASKED_AT = 4;                   // of RowNote.flags of a tile: bits 0-3 a row of the group sees a key, 4-7 some row does not see some key
-constexpr uint32_t LAST = 1, FINAL = 2, STOP = 4;   // of PairNote.flags: the unit's last pair, the block's; behind it
-struct PairNote { int tile, tiles; uint32_t flags; };   // its first tile, how many it has (0: a unit without rows)
-struct UnitNote {
-  int row0, tokens, cached, h;
-  int x_least, x_most, y_least, y_most, place_least, place_most;   // over its keys: what a row has to be to see any, or all of them
-  int begin, end;                        // tiles of rows that may see some
+// What is written down in the workspace.  Rows: -lse in the log2 domain (-inf: no weight); (place in the walk, place behind which the window begins); for each 32 of them the least and the last
+// such place (the least is INT_MIN where one adds nothing), the least and the last beginning
+struct alignas(16) RowNote { float less[HT]; int2 sees[HT]; int4 bound[HT / 32]; };
+struct alignas(16) UnitNote {
+  int row0, cached, keys, key0, h;       // of its request, its first key, its key head
+  int begin, end;                        // tiles of rows that may see some of its keys
   int part;                              // the place of its sums among the parts
-  uint32_t flags;                        // FINAL: the block's last
-  uint32_t seen[2];                      // which of the first 64 of them do; those behind are looked at whether or not
+  int rows;                              // the RowNote of the request's and head's first tile
+  uint32_t seen[2];                      // which of its first 64 tiles do; those behind are looked at whether or not
+  int pad[5];
   int k_row[KT / 16];                    // rows of the pool that its boxes begin at
+  int at[KT / 16];                       // words of the weights that they begin at, -1: in no page of the pool
 };
+static_assert(sizeof(UnitNote) == 128 && sizeof(RowNote) % 16 == 0, "a lane a word; pieces of 16 bytes");
+struct alignas(16) Head { long long units, rows_at, parts_at; int chunks, pad; };   // units without chunks; bytes from the workspace's begin to the RowNotes and the parts
+constexpr long long UNITS_AT = sizeof(Head);
+__host__ __device__ constexpr long long parts_bytes(long long units, int chunks) { return chunks > 1 ? units * KT * 4 * (chunks + 1) : 0; }
 
-template <int DH>
-struct KwSmem {
-  static constexpr int DCH = DH / 64, NQ = q_buffers(DH), NR = row_buffers(DH);
-  uint8_t k[NK][DCH * KT * 128];
-  uint8_t q[NQ][DCH * RT * 128];
-  RowNote rows[NR];
-  KeyNote keys[NU][KT];
-  float sums[NU][KW_SETS - 1][KT];
-  PairNote pair[NR];
-  UnitNote unit[NU];
-  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], pair_known[NR], rows_full[NR], rows_empty[NR], s_full[NS], s_empty[NS], sums_full[NU], u_full[NU], u_empty[NU];
-  uint32_t tmem;
-  TreePlan<KW_THREADS> plan;
-};
-
-struct KwUnit { int b, h, key_tile, chunk, part; };
+constexpr uint32_t LAST = 1, FINAL = 2;  // of PairNote.flags: the unit's last pair, the block's
+struct PairNote { int tiles; uint32_t flags; };      // how many tiles it has (0: a unit without rows)
+struct KeyNote { int x, y, place, at; };             // span, place in the window's terms, word of the weights: a new key's as -2 - word, -1: no key
 
 // The tiles of keys that rows may see; all of them where weights fade
 __device__ __forceinline__ TileRange key_tiles(const WeightsView& t, const KeyRange& k) {
@@ -68,160 +59,152 @@ __device__ __forceinline__ TileRange key_tiles(const WeightsView& t, const KeyRa
   if (t.decay != 1.0f || all == 0) return TileRange{all, all, all};
   return tile_range(t, k, 0, k.rq.tokens - 1);
 }
-__device__ __forceinline__ long long key_tiles_of(const WeightsView& t, const KeyRange& k) {
+__device__ __forceinline__ int key_tiles_of(const WeightsView& t, const KeyRange& k) {
   if (k.rq.tokens == 0 && t.decay == 1.0f) return 0;
   const TileRange r = key_tiles(t, k);
   return r.sinks + max(0, r.end - r.first);
 }
+__device__ __forceinline__ int row_tiles_of(const WeightsView& t, const KeyRange& k) { const int per = t.rows / t.group; return (k.rq.tokens + per - 1) / per; }
 
-// What the join finds in front of the parts
-struct PartsHead { long long units; int chunks, pad; };
-__host__ __device__ constexpr long long parts_bytes(long long units, int chunks) { return (long long)sizeof(PartsHead) + units * KT * 4 * (chunks + 1); }
+// A unit, by a warp
+__device__ void plan_unit(const WeightsView& t, int box, int chunks, int pos, const TreePlan<PLAN_THREADS>& units, const TreePlan<PLAN_THREADS>& tiles_of, UnitNote* out) {
+  const int lane = threadIdx.x & 31, boxes = KT / box, page_size = t.c.page_size, per_tile = t.rows / t.group, heads = t.c.num_kv_heads;
+  const int unit = pos / chunks, chunk = pos - unit * chunks, b = units.request_at(t, unit);
+  const KeyRange k = key_range(t.c, b);
+  const CacheRequest& rq = k.rq;
+  const int in = unit - (int)units.before[b], at_tile = in / heads, h = in - at_tile * heads, key0 = key_tiles(t, k).at(at_tile) * KT;
+  // its boxes: lane i has box i
+  const int key = key0 + lane * box, col = key / page_size, slot0 = key - col * page_size;
+  int page = -2;
+  if (lane < boxes && key < k.keys) page = k.table[col];
+  const bool there = (unsigned)page < (unsigned)t.c.num_pages;
+  if (page != -2 && !there) cache_report(t.c, CACHE_BAD_PAGE);
+  if (lane == 0 && key0 == 0 && h == 0 && chunk == 0 && k.keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
+  // its tiles of rows.  In a chain those in front of the keys, and those whose windows lie behind them, are not looked at.
+  const int tiles = row_tiles_of(t, k), per = ((tiles + chunks - 1) / chunks + 1) & ~1;
+  int begin = min(chunk * per, tiles), end = min(begin + per, tiles);
+  if (is_chain(t)) {
+    if (key0 > rq.cached) begin = max(begin, min(end, (key0 - rq.cached) / per_tile));
+    if (key0 >= t.sinks) end = max(begin, (int)min((long long)end, ((long long)key0 + KT - 1 + t.window - rq.cached - 1 + per_tile) / per_tile));
+  }
+  // Which of them have a token that sees new keys alone, by the tokens' places
+  uint32_t seen0 = 0xffffffffu, seen1 = 0xffffffffu;
+  if (t.a.spans && key0 >= rq.cached && rq.tokens > 0) {
+    int x_least = 0x7fffffff, y_most = -1;
+    for (int i = lane; i < KT; i += 32)
+      if (key0 + i < k.keys) { const int2 s = span_of(t, rq, key0 + i - rq.cached); x_least = min(x_least, s.x); y_most = max(y_most, s.y); }
+    x_least = __reduce_min_sync(0xffffffffu, x_least); y_most = __reduce_max_sync(0xffffffffu, y_most);
+    seen0 = seen1 = 0;
+    const int first = begin * per_tile, last = min(min(end, begin + 64) * per_tile, rq.tokens);
+    for (int token = first + lane; token < last; token += 32) {
+      const int pre = t.a.spans[2ll * (rq.row0 + token)], tile = (token - first) / per_tile;
+      if (pre >= x_least && pre < y_most) { if (tile < 32) seen0 |= 1u << tile; else seen1 |= 1u << (tile - 32); }
+    }
+    seen0 = __reduce_or_sync(0xffffffffu, seen0); seen1 = __reduce_or_sync(0xffffffffu, seen1);
+  }
+  if (lane == 0) {
+    out->row0 = rq.row0; out->cached = rq.cached; out->keys = k.keys; out->key0 = key0; out->h = h;
+    out->begin = begin; out->end = end; out->part = unit * chunks + chunk; out->rows = (int)tiles_of.before[b] + h * tiles;
+    out->seen[0] = seen0; out->seen[1] = seen1;
+  }
+  if (lane < KT / 16) {
+    out->k_row[lane] = there ? (page * 2 * heads + h) * page_size + slot0 : (int)(t.c.num_pages * 2 * heads * page_size);   // behind the pool: zeros
+    out->at[lane] = there ? (page * heads + h) * page_size + slot0 : -1;
+  }
+}
+
+// A tile of rows, by a warp: 32 at a time
+__device__ void plan_rows(const WeightsView& t, int pos, const TreePlan<PLAN_THREADS>& tiles_of, RowNote* out) {
+  const int lane = threadIdx.x & 31, per_tile = t.rows / t.group, b = tiles_of.request_at(t, pos);
+  const CacheRequest rq = cache_request(t.c, b);
+  const int in = pos - (int)tiles_of.before[b], tiles = (rq.tokens + per_tile - 1) / per_tile, h = in / tiles, tile = in - h * tiles;
+#pragma unroll
+  for (int g = 0; g < HT / 32; ++g) {
+    const int r = g * 32 + lane, token = tile * per_tile + r / t.group, at = min(token, rq.tokens - 1);
+    const float lse = t.lse[(long long)(rq.row0 + at) * t.a.num_q_heads + h * t.group + r % t.group];
+    const int pre = span_of(t, rq, at).x, behind = place_of(t, rq, at) - t.window;
+    const bool live = r < t.rows && token < rq.tokens && pre >= 0 && !isinf(lse);   // no row, padding, one that saw nothing or that the caller leaves out
+    constexpr int NONE = -0x7fffffff - 1;
+    out->less[r] = live ? lse * -TREE_LOG2E : -INFINITY;
+    out->sees[r] = make_int2(live ? pre : NONE, behind);
+    const int4 bound = make_int4(__reduce_min_sync(0xffffffffu, live ? pre : NONE), __reduce_max_sync(0xffffffffu, live ? pre : NONE),
+                                 __reduce_min_sync(0xffffffffu, live ? behind : 0x7fffffff), __reduce_max_sync(0xffffffffu, live ? behind : NONE));
+    if (lane == 0) out->bound[g] = bound;
+  }
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) key_weights_plan_kernel(const WeightsView t, int box) {
+  __shared__ TreePlan<PLAN_THREADS> units, tiles;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  units.make_of(t, [&](const KeyRange& k) { return (long long)key_tiles_of(t, k) * t.c.num_kv_heads; });
+  tiles.make_of(t, [&](const KeyRange& k) { return (long long)row_tiles_of(t, k) * t.c.num_kv_heads; });
+  const long long all_units = units.all(t), all_tiles = tiles.all(t);
+  // more keys than the caller said: no room for parts
+  auto bytes = [&](int chunks) { return UNITS_AT + all_units * chunks * (long long)sizeof(UnitNote) + all_tiles * (long long)sizeof(RowNote) + parts_bytes(all_units, chunks); };
+  const int chunks = bytes(t.chunks) <= t.a.workspace_bytes ? t.chunks : 1;
+  uint8_t* const space = static_cast<uint8_t*>(t.a.workspace);
+  if (bytes(chunks) > t.a.workspace_bytes) {                 // only offsets that name rows twice get here
+    if (blockIdx.x == 0 && threadIdx.x == 0) { *reinterpret_cast<Head*>(space) = Head{0, 0, 0, 1, 0}; cache_report(t.c, CACHE_BAD_OFFSETS); }
+    return;
+  }
+  const long long rows_at = UNITS_AT + all_units * chunks * (long long)sizeof(UnitNote), notes = all_units * chunks + all_tiles;
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *reinterpret_cast<Head*>(space) = Head{all_units, rows_at, rows_at + all_tiles * (long long)sizeof(RowNote), chunks, 0};
+    for (int b = threadIdx.x; b < t.c.batch; b += PLAN_THREADS)
+      if (!cache_request(t.c, b).ok) cache_report(t.c, CACHE_BAD_OFFSETS);
+  }
+  for (long long i = blockIdx.x * (PLAN_THREADS / 32) + (threadIdx.x >> 5); i < notes; i += (long long)gridDim.x * (PLAN_THREADS / 32)) {
+    if (i < all_tiles) plan_rows(t, (int)i, tiles, reinterpret_cast<RowNote*>(space + rows_at) + i);
+    else plan_unit(t, box, chunks, (int)(i - all_tiles), units, tiles, reinterpret_cast<UnitNote*>(space + UNITS_AT) + (i - all_tiles));
+  }
+}
+
+template <int DH>
+struct KwSmem {
+  static constexpr int DCH = DH / 64, NQ = q_buffers(DH);
+  uint8_t k[NK][DCH * KT * 128];
+  uint8_t q[NQ][DCH * RT * 128];
+  RowNote rows[NR][2];
+  UnitNote unit[NU];
+  float sums[NU][KW_SETS - 1][KT];
+  PairNote pair[NR];
+  uint64_t k_full[NK], k_empty[NK], q_full[NQ], q_empty[NQ], r_full[NR], r_empty[NR], s_full[NS], s_empty[NS], sums_full[NU], u_empty[NU];
+  uint32_t tmem;
+};
 
 template <int DH, int CAP>
 struct KwBlock {
-  static constexpr int DCH = DH / 64, NQ = q_buffers(DH), NR = row_buffers(DH);
+  static constexpr int DCH = DH / 64, NQ = q_buffers(DH);
   static constexpr uint32_t BLK = DCH * KT * 128;
   const WeightsView& t;
   const CUtensorMap& map_q;
   const CUtensorMap& map_k;
   KwSmem<DH>& sm;
-  int box, chunks;                       // chunks that a request's tiles of rows are taken in
+  int box, units, chunks;
+  const uint8_t* space;
+  long long rows_at;
+  float* parts;
   uint32_t tmem;
 
   __device__ __forceinline__ bool wait(const uint64_t& bar, int phase) const { return mbar_wait(smem_u32(&bar), (uint32_t)(phase & 1), t.c.status_dev); }
 
-  // unit `pos` of the call
-  __device__ __forceinline__ KwUnit unit_at(int pos) const {
-    KwUnit u;
-    const int unit = chunks == 1 ? pos : pos / chunks;
-    u.chunk = pos - unit * chunks;
-    u.part = unit * chunks + u.chunk;
-    u.b = sm.plan.request_at(t, unit);
-    const KeyRange k = key_range(t.c, u.b);
-    const int in = unit - (int)sm.plan.before[u.b], tile = in / t.c.num_kv_heads;
-    u.h = in - tile * t.c.num_kv_heads;
-    u.key_tile = key_tiles(t, k).at(tile);
-    return u;
-  }
-
-  // ---- planner (a whole warp) ----
-  // A unit's chain - its place, the request's offsets, its pages, its keys' spans - is some 3 us of round trips, as long as four tiles: lanes look units up side by side, and a
-  // unit's pages are asked for while the one in front of it is written down.  (In the producer that chain was what the block waited for: 32 x 512 candidates 94 us.)
-  __device__ __forceinline__ void plan_units(int units) {
-    const int lane = threadIdx.x & 31, boxes = KT / box, page_size = t.c.page_size, page_rows = 2 * t.c.num_kv_heads * page_size;
-    const int no_row = (int)(t.c.num_pages * page_rows), per_tile = t.rows / t.group;   // tokens of a tile
-    int before = 0;
-    for (long long base = blockIdx.x; base < units; base += 32ll * gridDim.x, before += 32) {
-      const long long of_lane = base + (long long)lane * gridDim.x;
-      KwUnit unit{0, 0, 0, 0, 0};
-      KeyRange range;
-      range.keys = 0; range.rq.row0 = range.rq.tokens = range.rq.cached = 0;
-      if (of_lane < units) { unit = unit_at((int)of_lane); range = key_range(t.c, unit.b); }
-      auto from = [&](int v, int i) { return __shfl_sync(0xffffffffu, v, i); };
-      auto ask = [&](int i) {                               // this lane's box of unit i: its page, -2 behind the keys
-        const int key = from(unit.key_tile, i) * KT + lane * box, keys = from(range.keys, i), b = from(unit.b, i);
-        return lane < boxes && key < keys ? t.c.block_table[(long long)b * t.c.table_stride + key / page_size] : -2;
-      };
-      int page_after = ask(0);
-      const int count = __popc(__ballot_sync(0xffffffffu, of_lane < units));
-      for (int i = 0; i < count; ++i) {
-        const int n = before + i, page = page_after;
-        if (i + 1 < count) page_after = ask(i + 1);
-        const int b = from(unit.b, i), h = from(unit.h, i), key0 = from(unit.key_tile, i) * KT, chunk = from(unit.chunk, i), keys = from(range.keys, i);
-        CacheRequest rq;
-        rq.row0 = from(range.rq.row0, i); rq.tokens = from(range.rq.tokens, i); rq.cached = from(range.rq.cached, i);
-        const int part = from(unit.part, i);
-        const bool final = __shfl_sync(0xffffffffu, (int)(of_lane + gridDim.x >= units), i);
-        const bool there = (unsigned)page < (unsigned)t.c.num_pages;
-        if (page != -2 && !there) cache_report(t.c, CACHE_BAD_PAGE);
-        if (lane == 0 && key0 == 0 && h == 0 && chunk == 0 && keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
-        const int slot0 = (key0 + lane * box) % page_size, row = there ? page * page_rows + h * page_size + slot0 : no_row;
-        // this lane's four keys: what a row has to be to see all of them, or any.  What is asked for of new ones is asked for at once.
-        KeyNote mine[KT / 32];
-        int2 span[KT / 32];
-        int new_place[KT / 32];
-        const bool fresh = key0 + KT > rq.cached && rq.tokens > 0;
-#pragma unroll
-        for (int g = 0; g < KT / 32; ++g) {
-          const int token = max(0, min(key0 + g * 32 + lane - rq.cached, rq.tokens - 1));
-          span[g] = make_int2(token, rq.tokens); new_place[g] = t.a.spans ? rq.cached : rq.cached + token;
-          if (fresh && t.a.spans) span[g] = reinterpret_cast<const int2*>(t.a.spans)[rq.row0 + token];
-          if (fresh && t.positions) new_place[g] = t.positions[rq.row0 + token];
-        }
-        int x_most = -1, y_least = 0x7fffffff, place_least = 0x7fffffff, x_least = 0x7fffffff, y_most = -1, place_most = -1;
-#pragma unroll
-        for (int g = 0; g < KT / 32; ++g) {
-          const int in = g * 32 + lane, key = key0 + in, owner = in / box;
-          const int of = __shfl_sync(0xffffffffu, page, owner), slot = __shfl_sync(0xffffffffu, slot0, owner) + in - owner * box;
-          const bool ok = (unsigned)of < (unsigned)t.c.num_pages && key < keys, cached = key < rq.cached;
-          const int place = cached ? key : max(rq.cached, new_place[g]), at = (of * t.c.num_kv_heads + h) * page_size + slot;
-          KeyNote m;
-          m.x = !ok ? 0x7fffffff : cached ? 0 : span[g].x; m.y = !ok ? -1 : cached ? 0x7fffffff : span[g].y;
-          m.place = !ok ? -1 : place < t.sinks ? 0x7fffffff : place;
-          m.at = !ok ? -1 : cached ? at : -2 - at;          // a new key: no weight before
-          x_least = min(x_least, m.x); y_most = max(y_most, m.y); place_most = max(place_most, m.place);
-          x_most = max(x_most, m.x); y_least = min(y_least, m.y); place_least = min(place_least, m.place);
-          mine[g] = m;
-        }
-        x_most = __reduce_max_sync(0xffffffffu, x_most); y_least = __reduce_min_sync(0xffffffffu, y_least); place_least = __reduce_min_sync(0xffffffffu, place_least);
-        x_least = __reduce_min_sync(0xffffffffu, x_least); y_most = __reduce_max_sync(0xffffffffu, y_most); place_most = __reduce_max_sync(0xffffffffu, place_most);
-        // its tiles of rows.  In a chain those in front of the keys, and those whose windows lie behind them, are not looked at.
-        const int tiles = (rq.tokens + per_tile - 1) / per_tile, per = ((tiles + chunks - 1) / chunks + 1) & ~1;
-        int begin = min(chunk * per, tiles), end = min(begin + per, tiles);
-        if (is_chain(t)) {
-          if (key0 > rq.cached) begin = max(begin, min(end, (key0 - rq.cached) / per_tile));
-          if (key0 >= t.sinks) end = max(begin, (int)min((long long)end, ((long long)key0 + KT - 1 + t.window - rq.cached - 1 + per_tile) / per_tile));
-        }
-        // Which of them have a token that sees new keys alone, by the tokens' places.  (Looked up by the producer as it went, a round trip a tile, then some 800 cycles of one warp's
-        // instructions: 8 x 1022 tokens that see themselves, 16 heads of 128, 78 us.)
-        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-        if (t.a.spans && key0 >= rq.cached) {
-          seen[0] = seen[1] = 0;
-          const int first = begin * per_tile, last = min(min(end, begin + 64) * per_tile, rq.tokens);
-          const float inverse = 1.0f / (float)per_tile;       // exact enough for quotients below 64: 8192 tokens at most
-          for (int token = first + lane; token < last; token += 256) {
-            int pre[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) pre[k] = t.a.spans[2ll * (rq.row0 + min(token + k * 32, rq.tokens - 1))];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int at = token + k * 32 - first;
-              int tile = (int)((float)at * inverse);
-              tile += (tile + 1) * per_tile <= at ? 1 : tile * per_tile > at ? -1 : 0;
-              if (first + at < last && pre[k] >= x_least && pre[k] < y_most) seen[tile >> 5] |= 1u << (tile & 31);
-            }
-          }
-          seen[0] = __reduce_or_sync(0xffffffffu, seen[0]); seen[1] = __reduce_or_sync(0xffffffffu, seen[1]);
-        }
-        if (!wait(sm.u_empty[n % NU], n / NU - 1)) return;
-        UnitNote& note = sm.unit[n % NU];
-#pragma unroll
-        for (int g = 0; g < KT / 32; ++g) sm.keys[n % NU][g * 32 + lane] = mine[g];
-        if (lane < boxes) note.k_row[lane] = row;
-        if (lane == 0) {
-          note.row0 = rq.row0; note.tokens = rq.tokens; note.cached = rq.cached; note.h = h;
-          note.x_least = x_least; note.x_most = x_most; note.y_least = y_least; note.y_most = y_most; note.place_least = place_least; note.place_most = place_most;
-          note.begin = begin; note.end = end; note.part = part; note.seen[0] = seen[0]; note.seen[1] = seen[1];
-          note.flags = final ? FINAL : 0u;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.u_full[n % NU]));
-      }
-    }
-  }
-
   // ---- producer (a whole warp; one lane issues) ----
   __device__ __forceinline__ void produce() {
     const int lane = threadIdx.x & 31, boxes = KT / box, group = t.group, per_tile = t.rows / group, q_bytes = DCH * t.rows * 128;
-    int j = 0;                                              // pairs so far
-    for (int n = 0;; ++n) {
-      if (!wait(sm.u_full[n % NU], n / NU)) return;
+    const RowNote* const notes = reinterpret_cast<const RowNote*>(space + rows_at);
+    const uint32_t* const words = reinterpret_cast<const uint32_t*>(space + UNITS_AT) + lane;   // a lane a word of a unit's note, the next one's on its way
+    uint32_t word = words[(long long)blockIdx.x * 32];
+    int j = 0, n = 0;                                       // pairs and units so far
+    for (int pos = blockIdx.x; pos < units; pos += gridDim.x, ++n) {
+      if (!wait(sm.u_empty[n % NU], n / NU - 1)) return;    // the first wait passes
+      reinterpret_cast<uint32_t*>(&sm.unit[n % NU])[lane] = word;
+      const bool final = pos + (int)gridDim.x >= units;
+      if (!final) word = words[(long long)(pos + gridDim.x) * 32];
+      __syncwarp();
       const UnitNote& u = sm.unit[n % NU];
-      const int row0 = u.row0, h = u.h, end = u.end;
+      const int row0 = u.row0, h = u.h, first = u.begin, end = u.end, rows = u.rows;
       const uint64_t seen = (uint64_t)u.seen[1] << 32 | u.seen[0];
-      const bool final = u.flags & FINAL;
-      if (!wait(sm.k_empty[n % NK], n / NK - 1)) return;    // the first wait passes
+      if (!wait(sm.k_empty[n % NK], n / NK - 1)) return;
       __syncwarp();
       if (elect_one()) {
         mbar_expect_tx(smem_u32(&sm.k_full[n % NK]), BLK);
@@ -229,7 +212,6 @@ struct KwBlock {
           for (int c = 0; c < DCH; ++c) tma_load_2d(smem_u32(sm.k[n % NK]) + c * KT * 128 + p * box * 128, &map_k, smem_u32(&sm.k_full[n % NK]), c * 64, u.k_row[p]);
       }
       __syncwarp();
-      const int first = u.begin;
       auto candidate = [&](int tile) {                        // the first tile from `tile` on that may see some
         const int in = tile - first;
         if (in >= 64) return tile;
@@ -237,87 +219,31 @@ struct KwBlock {
         return left ? tile + __ffsll(left) - 1 : first + 64;
       };
       int tile = candidate(first);
-      const bool rows = tile < end;                           // none: a pair without rows, which ends the unit all the same
+      const bool some = tile < end;                           // none: a pair without rows, which ends the unit all the same
       for (;;) {
-        int next = rows ? candidate(tile + 1) : end, count = rows ? 1 : 0;
-        if (rows && next == tile + 1 && next < end) { count = 2; next = candidate(tile + 2); }
+        int next = some ? candidate(tile + 1) : end, count = some ? 1 : 0;
+        if (some && next == tile + 1 && next < end) { count = 2; next = candidate(tile + 2); }
         const bool more = next < end;
         if (!wait(sm.q_empty[j % NQ], j / NQ - 1)) return;
-        if (!wait(sm.rows_empty[j % NR], j / NR - 1)) return;
+        if (!wait(sm.r_empty[j % NR], j / NR - 1)) return;
         __syncwarp();
         if (elect_one()) {
+          sm.pair[j % NR] = PairNote{count, more ? 0u : LAST | (final ? FINAL : 0u)};   // in front of the arrivals, which publish it
+          const uint32_t q_bar = smem_u32(&sm.q_full[j % NQ]), r_bar = smem_u32(&sm.r_full[j % NR]);
           const int copies = max(count, 1);
-          mbar_expect_tx(smem_u32(&sm.q_full[j % NQ]), copies * q_bytes);
+          mbar_expect_tx(q_bar, copies * q_bytes);
           for (int i = 0; i < copies; ++i)
-            for (int c = 0; c < DCH; ++c)
-              tma_load_3d(smem_u32(sm.q[j % NQ]) + (c * RT + i * HT) * 128, &map_q, smem_u32(&sm.q_full[j % NQ]), c * 64, h * group, row0 + (rows ? tile + i : 0) * per_tile);
-          sm.pair[j % NR] = PairNote{tile, count, more ? 0u : LAST | (final ? FINAL : 0u)};
-          mbar_arrive(smem_u32(&sm.pair_known[j % NR]));
+            for (int c = 0; c < DCH; ++c) tma_load_3d(smem_u32(sm.q[j % NQ]) + (c * RT + i * HT) * 128, &map_q, q_bar, c * 64, h * group, row0 + (some ? tile + i : 0) * per_tile);
+          mbar_expect_tx(r_bar, count * (int)sizeof(RowNote));
+          for (int i = 0; i < count; ++i)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(smem_u32(&sm.rows[j % NR][i])), "l"(notes + rows + tile + i), "r"((uint32_t)sizeof(RowNote)), "r"(r_bar) : "memory");
         }
         __syncwarp();
         ++j;
         if (!more) break;
         tile = next;
       }
-      if (final) break;
-    }
-    if (!wait(sm.rows_empty[j % NR], j / NR - 1)) return;       // the row warp whose turn it is not
-    if (lane == 0) { sm.pair[j % NR].flags = STOP; mbar_arrive(smem_u32(&sm.pair_known[j % NR])); }
-  }
-
-  // ---- the rows of every fourth tile (a whole warp) ----
-  __device__ __forceinline__ void describe(int turn) {
-    const int lane = threadIdx.x & 31, group = t.group, per_tile = t.rows / group;
-    // this lane's rows, 32 apart: row r of a tile is token r / group, head r % group; behind the last one no token is
-    int token_in[4], head_in[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int r = g * 32 + lane;
-      token_in[g] = r < t.rows ? r / group : 1 << 30; head_in[g] = r % group;
-    }
-    int n = 0;
-    for (int j = 0;; ++j) {
-      if (!wait(sm.pair_known[j % NR], j / NR)) return;
-      const PairNote note = sm.pair[j % NR];
-      if (note.flags & STOP) return;
-      const int which = (turn - 2 * j) & (KW_ROWS - 1);       // the pair's tile that is this warp's turn
-      if (which < 2) {
-        const int tile = note.tile + which;
-        const bool there = which < note.tiles;
-        const UnitNote& u = sm.unit[n % NU];
-        CacheRequest rq;
-        rq.row0 = u.row0; rq.cached = u.cached;
-        const float* const lse0 = t.lse + (long long)rq.row0 * t.a.num_q_heads + u.h * group;
-        float lse[4];
-        int pre[4], behind[4];
-        bool valid[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {                         // loads without a condition: all on their way at once
-          const int token = (there ? tile : 0) * per_tile + token_in[g], at = max(0, min(token, u.tokens - 1));
-          valid[g] = there && token < u.tokens;
-          lse[g] = u.tokens > 0 ? lse0[(long long)at * t.a.num_q_heads + head_in[g]] : 0.f;
-          pre[g] = t.a.spans && u.tokens > 0 ? t.a.spans[2ll * (rq.row0 + at)] : at;
-          behind[g] = (t.positions && u.tokens > 0 ? max(rq.cached, t.positions[rq.row0 + at]) : t.a.spans ? rq.cached : rq.cached + at) - t.window;
-        }
-        uint32_t flags = 0;
-        RowNote& rows = sm.rows[j % NR];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const bool live = valid[g] && pre[g] >= 0 && !isinf(lse[g]);    // no row, padding, one that saw nothing or that the caller leaves out
-          const bool any = live && pre[g] >= u.x_least && pre[g] < u.y_most && u.place_most > behind[g];
-          const bool all = live && u.x_most <= pre[g] && pre[g] < u.y_least && u.place_least > behind[g];
-          if (__any_sync(0xffffffffu, any)) flags |= 1u << g;
-          if (!__all_sync(0xffffffffu, all)) flags |= 1u << (MASKED_AT + g);
-          rows.less[which * HT + g * 32 + lane] = live ? lse[g] * -TREE_LOG2E : -INFINITY;
-          rows.sees[which * HT + g * 32 + lane] = make_int2(live ? pre[g] : -0x7fffffff - 1, behind[g]);
-        }
-        if (lane == 0) rows.flags[which] = flags;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.rows_full[j % NR]));
-      }
-      n += note.flags & LAST;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sm.rows_empty[j % NR]));   // the note has been read, by the warps whose turn it is not, too
     }
   }
 
@@ -327,10 +253,11 @@ struct KwBlock {
     int n = 0;
     bool first = true;
     for (int j = 0;; ++j) {
-      if (!wait(sm.pair_known[j % NR], j / NR)) return;
-      const uint32_t flags = sm.pair[j % NR].flags, idesc = sm.pair[j % NR].tiles == 2 ? idesc_pair : idesc_one;
+      if (!wait(sm.q_full[j % NQ], j / NQ)) return;
+      const PairNote note = sm.pair[j % NR];
+      const uint32_t idesc = note.tiles == 2 ? idesc_pair : idesc_one;
       if (first && !wait(sm.k_full[n % NK], n / NK)) return;
-      if (!wait(sm.s_empty[j % NS], j / NS - 1) || !wait(sm.q_full[j % NQ], j / NQ)) return;
+      if (!wait(sm.s_empty[j % NS], j / NS - 1)) return;
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < DCH; ++c) {
@@ -340,13 +267,29 @@ struct KwBlock {
       }
       umma_commit(smem_u32(&sm.q_empty[j % NQ]));
       umma_commit(smem_u32(&sm.s_full[j % NS]));
-      first = flags & LAST;
+      first = note.flags & LAST;
       if (first) { umma_commit(smem_u32(&sm.k_empty[n % NK])); ++n; }
-      if (flags & FINAL) return;
+      if (note.flags & FINAL) return;
     }
   }
 
   // ---- sums ----
+  // key `in` of a unit
+  __device__ __forceinline__ KeyNote key_of(const UnitNote& u, int in) const {
+    const int key = u.key0 + in, at0 = u.at[in / box], at = at0 + in % box;
+    KeyNote m{0x7fffffff, -1, -1, -1};
+    if (at0 < 0 || key >= u.keys) return m;
+    m.x = 0; m.y = 0x7fffffff; m.place = key; m.at = at;
+    if (key >= u.cached) {
+      const int token = key - u.cached;
+      m.at = -2 - at;
+      if (t.a.spans) { const int2 s = reinterpret_cast<const int2*>(t.a.spans)[u.row0 + token]; m.x = s.x; m.y = s.y; }
+      else m.x = token;
+      m.place = t.positions ? max(u.cached, t.positions[u.row0 + token]) : t.a.spans ? u.cached : key;
+    }
+    if (m.place < t.sinks) m.place = 0x7fffffff;
+    return m;
+  }
   __device__ __forceinline__ void sum_up() {
     const int warp = warp_index() - KW_FIRST, lane = threadIdx.x & 31, g = warp >> 2, in = (warp & 3) * 32 + lane;   // group g of both tiles
     const uint32_t column = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * 32;
@@ -358,15 +301,17 @@ struct KwBlock {
     int part = 0;
     bool first = true;
     for (int j = 0;; ++j) {
-      if (!wait(sm.rows_full[j % NR], j / NR) || !wait(sm.s_full[j % NS], j / NS)) return;
-      tc_fence_after();
+      if (!wait(sm.r_full[j % NR], j / NR)) return;
       const PairNote note = sm.pair[j % NR];
-      if (first) { key = sm.keys[n % NU][in]; part = sm.unit[n % NU].part; sum = 0.f; }
-      const RowNote& rows = sm.rows[j % NR];
+      if (first) { key = key_of(sm.unit[n % NU], in); part = sm.unit[n % NU].part; sum = 0.f; }
+      if (!wait(sm.s_full[j % NS], j / NS)) return;
+      tc_fence_after();
 #pragma unroll 1
       for (int i = 0; i < note.tiles; ++i) {
-        const uint32_t flags = rows.flags[i];
-        if (!((flags >> g) & 1)) continue;
+        const RowNote& rows = sm.rows[j % NR][i];
+        const int4 bound = rows.bound[g];
+        if (!__any_sync(0xffffffffu, key.x <= bound.y && key.y > bound.x && key.place > bound.z)) continue;
+        const bool masked = !__all_sync(0xffffffffu, key.x <= bound.x && key.y > bound.y && key.place > bound.w);
         float s[32];
         tmem_ld32_nowait(column + (j % NS) * RT + i * HT, reinterpret_cast<uint32_t*>(s));
         tmem_ld_wait_on(s);
@@ -385,10 +330,9 @@ struct KwBlock {
             for (int k = 0; k < 32; k += 2) cap.of_any(s[k], s[k + 1]);
           }
         }
-        const float4* const less = reinterpret_cast<const float4*>(rows.less + i * HT + g * 32);
+        const float4* const less = reinterpret_cast<const float4*>(rows.less + g * 32);
         const float2 scale = make_float2(csc, csc);
         float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        const bool masked = (flags >> (MASKED_AT + g)) & 1;
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
           const float4 l = less[k / 4];
@@ -400,7 +344,7 @@ struct KwBlock {
           }
         }
         if (masked) {
-          const int4* const sees = reinterpret_cast<const int4*>(rows.sees + i * HT + g * 32);
+          const int4* const sees = reinterpret_cast<const int4*>(rows.sees + g * 32);
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             const int4 see = sees[k / 2];
@@ -415,7 +359,7 @@ struct KwBlock {
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(smem_u32(&sm.s_empty[j % NS]));
-        mbar_arrive(smem_u32(&sm.rows_empty[j % NR]));
+        mbar_arrive(smem_u32(&sm.r_empty[j % NR]));
         if (last) mbar_arrive(smem_u32(&sm.u_empty[n % NU]));
       }
       if (last && g == 0) {
@@ -423,8 +367,8 @@ struct KwBlock {
 #pragma unroll
         for (int k = 0; k < KW_SETS - 1; ++k) sum += sm.sums[n % NU][k][in];
         if (chunks > 1) {                                    // behind the places of the weights
-          t.part[((sm.plan.all(t) + part) * KT) + in] = sum;
-          if (part % chunks == 0) reinterpret_cast<int*>(t.part)[(long long)(part / chunks) * KT + in] = key.at;
+          parts[(long long)(units / chunks + part) * KT + in] = sum;
+          if (part % chunks == 0) reinterpret_cast<int*>(parts)[(long long)(part / chunks) * KT + in] = key.at;
         } else if (key.at != -1) {
           if (key.at >= 0) { float* const w = t.weights + key.at; *w = fmaf(*w, t.decay, sum); }
           else t.weights[-2 - key.at] = sum;
@@ -448,31 +392,24 @@ __global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __g
     for (int i = 0; i < NK; ++i) { mbar_init(smem_u32(&sm.k_full[i]), 1); mbar_init(smem_u32(&sm.k_empty[i]), 1); }
     for (int i = 0; i < q_buffers(DH); ++i) { mbar_init(smem_u32(&sm.q_full[i]), 1); mbar_init(smem_u32(&sm.q_empty[i]), 1); }
     for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&sm.s_full[i]), 1); mbar_init(smem_u32(&sm.s_empty[i]), KW_SUM); }
-    for (int i = 0; i < row_buffers(DH); ++i) { mbar_init(smem_u32(&sm.pair_known[i]), 1); mbar_init(smem_u32(&sm.rows_full[i]), 2); mbar_init(smem_u32(&sm.rows_empty[i]), KW_SUM + KW_ROWS); }
-    for (int i = 0; i < NU; ++i) { mbar_init(smem_u32(&sm.sums_full[i]), KT * (KW_SETS - 1)); mbar_init(smem_u32(&sm.u_full[i]), 1); mbar_init(smem_u32(&sm.u_empty[i]), KW_SUM); }
+    for (int i = 0; i < NR; ++i) { mbar_init(smem_u32(&sm.r_full[i]), 1); mbar_init(smem_u32(&sm.r_empty[i]), KW_SUM); }
+    for (int i = 0; i < NU; ++i) { mbar_init(smem_u32(&sm.sums_full[i]), KT * (KW_SETS - 1)); mbar_init(smem_u32(&sm.u_empty[i]), KW_SUM); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(smem_u32(&sm.tmem), NS * RT);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  sm.plan.make_of(t, [&](const KeyRange& k) { return key_tiles_of(t, k) * t.c.num_kv_heads; });
-  const int chunks = parts_bytes(sm.plan.all(t), t.chunks) <= t.a.workspace_bytes ? t.chunks : 1;   // more keys than the caller said: no room for parts
-  const int units = (int)sm.plan.all(t) * chunks;
-  if (t.chunks > 1) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (blockIdx.x == 0 && threadIdx.x == 0) *static_cast<PartsHead*>(t.a.workspace) = PartsHead{sm.plan.all(t), chunks, 0};
-  }
-  if (blockIdx.x == 0)
-    for (int b = threadIdx.x; b < t.c.batch; b += KW_THREADS)
-      if (!cache_request(t.c, b).ok) cache_report(t.c, CACHE_BAD_OFFSETS);
-  KwBlock<DH, CAP> block{t, map_q, map_k, sm, box, chunks, sm.tmem};
+  asm volatile("griddepcontrol.wait;" ::: "memory");         // what the plan kernel writes
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  uint8_t* const space = static_cast<uint8_t*>(t.a.workspace);
+  const Head head = *reinterpret_cast<const Head*>(space);
+  const int units = (int)head.units * head.chunks;
+  KwBlock<DH, CAP> block{t, map_q, map_k, sm, box, units, head.chunks, space, head.rows_at, reinterpret_cast<float*>(space + head.parts_at), sm.tmem};
   if (blockIdx.x < units) {
     if (warp == 0) block.produce();
     else if (warp == 1) { if (elect_one()) block.issue(); }
-    else if (warp == 2) block.plan_units(units);
-    else if (warp >= KW_FIRST && warp < KW_FIRST + KW_SUM) block.sum_up();
-    else block.describe(warp == 3 ? 0 : warp - (KW_FIRST + KW_SUM) + 1);
+    else if (warp >= KW_FIRST) block.sum_up();
   }
   settle();
   if (warp == 1) {
@@ -484,13 +421,15 @@ __global__ void __launch_bounds__(KW_THREADS, 1) key_weights_tc_kernel(const __g
 // Sums of a key's chunks of rows, in their order
 __global__ void __launch_bounds__(256) key_weights_join_kernel(const WeightsView t) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const PartsHead head = *static_cast<const PartsHead*>(t.a.workspace);
+  const uint8_t* const space = static_cast<const uint8_t*>(t.a.workspace);
+  const Head head = *reinterpret_cast<const Head*>(space);
   if (head.chunks == 1) return;
-  const int* const at_of = reinterpret_cast<const int*>(t.part);
+  const float* const parts = reinterpret_cast<const float*>(space + head.parts_at);
+  const int* const at_of = reinterpret_cast<const int*>(parts);
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < head.units * KT; i += (long long)gridDim.x * 256) {
     const int at = at_of[i];
     if (at == -1) continue;
-    const float* const part = t.part + (head.units + i / KT * head.chunks) * KT + i % KT;
+    const float* const part = parts + (head.units + i / KT * head.chunks) * KT + i % KT;
     float sum = 0.f;
 #pragma unroll 4
     for (int c = 0; c < head.chunks; ++c) sum += part[c * KT];
@@ -505,21 +444,28 @@ phx_status launch(const WeightsView& t, const CUtensorMap& map_q, const CUtensor
   static_assert(smem <= 227 * 1024, "a block's shared memory");
   static SmemLimit limit;
   PHX_CUDA_TRY(limit.raise(key_weights_tc_kernel<DH, CAP>, smem), err);
-  key_weights_tc_kernel<DH, CAP><<<blocks, KW_THREADS, smem, stream>>>(t, map_q, map_k, box);
-  PHX_CUDA_TRY(cudaGetLastError(), err);
+  PHX_CUDA_TRY(launch_programmatic(key_weights_tc_kernel<DH, CAP>, dim3(blocks), dim3(KW_THREADS), smem, stream, t, map_q, map_k, box), err);
   dispatch_note(DK_KEY_WEIGHTS_TC);
   return PHX_OK;
 }
-
 template <int DH>
 phx_status launch(const WeightsView& t, const CUtensorMap& map_q, const CUtensorMap& map_k, int box, int blocks, cudaStream_t stream, std::string& err) {
   return t.a.cap_method == 0 ? launch<DH, 0>(t, map_q, map_k, box, blocks, stream, err) : t.a.cap_method == 1 ? launch<DH, 1>(t, map_q, map_k, box, blocks, stream, err)
                                                                                                                : launch<DH, 2>(t, map_q, map_k, box, blocks, stream, err);
 }
 
+// Tiles of rows that a call may have, whatever its offsets are, and what is written down about them; the most units of a request
+long long row_tiles_bound(const WeightsView& t, int batch) { return ((long long)t.c.num_tokens / (HT / t.group) + batch) * t.c.num_kv_heads; }
+long long units_bound(const WeightsView& t) { return ((long long)t.c.table_cols * t.c.page_size + KT - 1) / KT * t.c.num_kv_heads; }
+
 }  // namespace
 
-bool weights_tc_supported(const WeightsView& t) { return (t.c.key_size == 64 || t.c.key_size == 128) && t.group <= HT && (long long)t.a.max_tokens * t.group > 16; }
+// Up to 16 rows a key head the mma.sync kernel reads the keys once, as fast as they come.  What is written down about rows (13 bytes each) and one request's keys has to fit three quarters of the
+// workspace, some two million rows and 100 thousand tiles of keys; calls beyond that, and heads of 32, stay with it, too.
+bool weights_tc_supported(const WeightsView& t) {
+  if ((t.c.key_size != 64 && t.c.key_size != 128) || t.group > HT || (long long)t.a.max_tokens * t.group <= 16) return false;
+  return UNITS_AT + row_tiles_bound(t, t.c.batch < TREE_MAX_SPLIT_BATCH ? t.c.batch : TREE_MAX_SPLIT_BATCH) * (long long)sizeof(RowNote) + units_bound(t) * (long long)sizeof(UnitNote) <= t.a.workspace_bytes / 4 * 3;
+}
 
 phx_status weights_tc_launch(WeightsView& t, cudaStream_t stream, std::string& err) {
   t.rows = HT / t.group * t.group; t.keys = KT;
@@ -528,12 +474,13 @@ phx_status weights_tc_launch(WeightsView& t, cudaStream_t stream, std::string& e
   CUtensorMap map_q, map_k;
   phx_status s = tree_query_map(&map_q, t, err);
   if (s == PHX_OK) s = tree_pool_map(&map_k, t, box, err);
-  // Tiles of rows in chunks where units alone leave blocks idle in a last round: about six rounds then, of two pairs at least
   const WeightsView whole = t;
   const int per_tile = t.rows / t.group, sms = device_sms();
-  const long long most_units = ((long long)t.c.table_cols * t.c.page_size + KT - 1) / KT * t.c.num_kv_heads;   // of a request
-  const int slice = (int)(most_units * TREE_MAX_SPLIT_BATCH <= (1 << 27) ? TREE_MAX_SPLIT_BATCH : most_units < (1 << 27) ? (1 << 27) / most_units : 1);
-  for (int b0 = 0; s == PHX_OK && b0 < whole.c.batch; b0 += slice) {   // as many requests as a block plans, whose units a number of 32 bits counts
+  // as many requests at a time as a block plans and whose notes fit
+  const long long room = t.a.workspace_bytes - UNITS_AT - row_tiles_bound(t, t.c.batch < TREE_MAX_SPLIT_BATCH ? t.c.batch : TREE_MAX_SPLIT_BATCH) * (long long)sizeof(RowNote);
+  const long long fit = room / (units_bound(t) * (long long)sizeof(UnitNote));
+  const int slice = (int)(fit < TREE_MAX_SPLIT_BATCH ? fit : TREE_MAX_SPLIT_BATCH);
+  for (int b0 = 0; s == PHX_OK && b0 < whole.c.batch; b0 += slice) {
     t = whole;
     t.c.batch = whole.c.batch - b0 < slice ? whole.c.batch - b0 : slice;
     t.c.q_start += b0; t.c.lengths += b0; t.c.block_table += b0 * t.c.table_stride;
@@ -542,6 +489,7 @@ phx_status weights_tc_launch(WeightsView& t, cudaStream_t stream, std::string& e
       const long long seen = ((long long)t.sinks + KT - 1) / KT + ((long long)t.window + t.a.max_tokens + KT - 3) / KT + 1;
       if (seen < tiles) tiles = seen;
     }
+    // Tiles of rows in chunks where units alone leave blocks idle in a last round: about six rounds then, of two pairs at least
     const long long units = tiles * t.c.num_kv_heads * t.c.batch, row_tiles = (t.a.max_tokens + per_tile - 1) / per_tile;
     t.chunks = 1;
     if (units < 4 * sms) {
@@ -549,9 +497,10 @@ phx_status weights_tc_launch(WeightsView& t, cudaStream_t stream, std::string& e
       long long per = pairs / want > 2 ? pairs / want : 2;   // pairs of a chunk
       if ((pairs + per - 1) / per > 15) per = (pairs + 14) / 15;
       t.chunks = (int)((pairs + per - 1) / per);
-      while (t.chunks > 1 && parts_bytes(units, t.chunks) > t.a.workspace_bytes) --t.chunks;
     }
-    t.part = reinterpret_cast<float*>(static_cast<uint8_t*>(t.a.workspace) + sizeof(PartsHead));
+    const long long notes = units * t.chunks + row_tiles * t.c.num_kv_heads * t.c.batch, plans = (notes + PLAN_THREADS / 32 - 1) / (PLAN_THREADS / 32);
+    key_weights_plan_kernel<<<(unsigned)(plans < 4 * sms ? plans : 4 * sms), PLAN_THREADS, 0, stream>>>(t, box);
+    PHX_CUDA_TRY(cudaGetLastError(), err);
     const int blocks = (int)(units * t.chunks < sms ? units * t.chunks : sms);
     s = t.c.key_size == 64 ? launch<64>(t, map_q, map_k, box, blocks, stream, err) : launch<128>(t, map_q, map_k, box, blocks, stream, err);
     if (s == PHX_OK && t.chunks > 1) {
