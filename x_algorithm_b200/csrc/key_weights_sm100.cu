@@ -6,8 +6,9 @@
 // rows: their lse, what they see, and its bounds for each 32 of them.  key_weights_tc_kernel, a block an SM, takes unit after unit, K once, then its rows, two tiles at a time:
 //   warp 0      producer: K (page by page) and Q tiles by TMA, what is written down about them by bulk copies
 //   warp 1      MMA issuer: S^T into one of two buffers of tensor memory
-//   warps 4-19  thread = key and a group of 32 rows of either tile: e^(x - lse) summed up in a register, masked where some key of the warp is not seen by some row of the group; at the
-//               unit's end the groups hand their sums to the first, which writes the weight (or a part, where chunks of rows are joined by key_weights_join_kernel)
+//   warps 4-19  thread = key and a group of 32 rows of either tile, 16 at a time with the next ones on their way from tensor memory: e^(x - lse) summed up in a register, masked where some
+//               key of the warp is not seen by some of the rows; at the unit's end the groups hand their sums to the first, which writes the weight (or a part, where chunks of rows
+//               are joined by key_weights_join_kernel)
 // (All of that in one kernel, by a planner warp and four that described rows, was slower: such code runs at 10 cycles an instruction, by one warp beside sixteen, and the block waited for it.
 // 32 x 512 candidates over up to 1022 keys, 8 heads of 64: 62 us; 8 x 1022 tokens that see themselves, 16 heads of 128: 66 us.)
 // Waits are bounded; when one runs out the flag is raised, every later wait of any role fails at once, and a role whose wait failed is done.
@@ -52,6 +53,14 @@ __host__ __device__ constexpr long long parts_bytes(long long units, int chunks)
 constexpr uint32_t LAST = 1, FINAL = 2;  // of PairNote.flags: the unit's last pair, the block's
 struct PairNote { int tiles; uint32_t flags; };      // how many tiles it has (0: a unit without rows)
 struct KeyNote { int x, y, place, at; };             // span, place in the window's terms, word of the weights: a new key's as -2 - word, -1: no key
+
+// Wait for the tensor-memory loads in flight; the 16 registers are operands, so that no use of them is scheduled in front of it
+__device__ __forceinline__ void wait_on_16(float* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]),
+                 "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+               :: "memory");
+}
 
 // The tiles of keys that rows may see; all of them where weights fade
 __device__ __forceinline__ TileRange key_tiles(const WeightsView& t, const KeyRange& k) {
@@ -306,52 +315,62 @@ struct KwBlock {
       if (first) { key = key_of(sm.unit[n % NU], in); part = sm.unit[n % NU].part; sum = 0.f; }
       if (!wait(sm.s_full[j % NS], j / NS)) return;
       tc_fence_after();
-#pragma unroll 1
-      for (int i = 0; i < note.tiles; ++i) {
-        const RowNote& rows = sm.rows[j % NR][i];
-        const int4 bound = rows.bound[g];
-        if (!__any_sync(0xffffffffu, key.x <= bound.y && key.y > bound.x && key.place > bound.z)) continue;
-        const bool masked = !__all_sync(0xffffffffu, key.x <= bound.x && key.y > bound.y && key.place > bound.w);
-        float s[32];
-        tmem_ld32_nowait(column + (j % NS) * RT + i * HT, reinterpret_cast<uint32_t*>(s));
-        tmem_ld_wait_on(s);
+      auto load = [&](float* s, int q) { tmem_ld16_nowait(column + (j % NS) * RT + (q >> 1) * HT + (q & 1) * 16, reinterpret_cast<uint32_t*>(s)); };   // half q & 1 of the group, tile q >> 1
+      auto add = [&](float* s, int q, bool masked) {
+        const RowNote& rows = sm.rows[j % NR][q >> 1];
         if (CAP == 1) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) s[k] = cap.form.template of<1>(s[k]);
+          for (int k = 0; k < 16; ++k) s[k] = cap.form.template of<1>(s[k]);
         } else if (CAP == 2) {
           float most = 0.f;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) most = fmaxf(most, fabsf(s[k]));
+          for (int k = 0; k < 16; ++k) most = fmaxf(most, fabsf(s[k]));
           if (__all_sync(0xffffffffu, cap.small(most))) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) cap.of_small(s[k], s[k + 1]);
+            for (int k = 0; k < 16; k += 2) cap.of_small(s[k], s[k + 1]);
           } else {
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) cap.of_any(s[k], s[k + 1]);
+            for (int k = 0; k < 16; k += 2) cap.of_any(s[k], s[k + 1]);
           }
         }
-        const float4* const less = reinterpret_cast<const float4*>(rows.less + g * 32);
+        const int row = g * 32 + (q & 1) * 16;
+        const float4* const less = reinterpret_cast<const float4*>(rows.less + row);
         const float2 scale = make_float2(csc, csc);
         float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        if (!masked) {
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          const float4 l = less[k / 4];
-          const float2 e0 = __ffma2_rn(make_float2(s[k], s[k + 1]), scale, make_float2(l.x, l.y)), e1 = __ffma2_rn(make_float2(s[k + 2], s[k + 3]), scale, make_float2(l.z, l.w));
-          s[k] = tree_ex2(e0.x); s[k + 1] = tree_ex2(e0.y); s[k + 2] = tree_ex2(e1.x); s[k + 3] = tree_ex2(e1.y);
-          if (!masked) {
-            acc[0] = __fadd2_rn(acc[0], make_float2(s[k], s[k + 1]));
-            acc[1] = __fadd2_rn(acc[1], make_float2(s[k + 2], s[k + 3]));
+          for (int k = 0; k < 16; k += 4) {
+            const float4 l = less[k / 4];
+            const float2 e0 = __ffma2_rn(make_float2(s[k], s[k + 1]), scale, make_float2(l.x, l.y)), e1 = __ffma2_rn(make_float2(s[k + 2], s[k + 3]), scale, make_float2(l.z, l.w));
+            acc[0] = __fadd2_rn(acc[0], make_float2(tree_ex2(e0.x), tree_ex2(e0.y)));
+            acc[1] = __fadd2_rn(acc[1], make_float2(tree_ex2(e1.x), tree_ex2(e1.y)));
           }
-        }
-        if (masked) {
-          const int4* const sees = reinterpret_cast<const int4*>(rows.sees + g * 32);
+        } else {
+          const int4* const sees = reinterpret_cast<const int4*>(rows.sees + row);
+          const float2* const less2 = reinterpret_cast<const float2*>(less);
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
+          for (int k = 0; k < 16; k += 2) {
             const int4 see = sees[k / 2];
-            acc[0] = __fadd2_rn(acc[0], make_float2(key.x <= see.x && see.x < key.y && key.place > see.y ? s[k] : 0.f, key.x <= see.z && see.z < key.y && key.place > see.w ? s[k + 1] : 0.f));
+            const float2 e = __ffma2_rn(make_float2(s[k], s[k + 1]), scale, less2[k / 2]);
+            acc[(k / 2) & 1] = __fadd2_rn(acc[(k / 2) & 1], make_float2(key.x <= see.x && see.x < key.y && key.place > see.y ? tree_ex2(e.x) : 0.f,
+                                                                         key.x <= see.z && see.z < key.y && key.place > see.w ? tree_ex2(e.y) : 0.f));
           }
         }
         sum += (acc[0].x + acc[1].x) + (acc[0].y + acc[1].y);
+      };
+      float s0[16], s1[16];
+      if (note.tiles > 0) load(s0, 0);
+#pragma unroll 1
+      for (int i = 0; i < note.tiles; ++i) {
+        const int4 bound = sm.rows[j % NR][i].bound[g];
+        const bool any = __any_sync(0xffffffffu, key.x <= bound.y && key.y > bound.x && key.place > bound.z);
+        const bool masked = !__all_sync(0xffffffffu, key.x <= bound.x && key.y > bound.y && key.place > bound.w);
+        wait_on_16(s0);
+        load(s1, 2 * i + 1);
+        if (any) add(s0, 2 * i, masked);
+        wait_on_16(s1);
+        if (i + 1 < note.tiles) load(s0, 2 * i + 2);
+        if (any) add(s1, 2 * i + 1, masked);
       }
       tc_fence_before();
       const bool last = note.flags & LAST;
