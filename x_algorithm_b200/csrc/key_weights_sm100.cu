@@ -100,14 +100,26 @@ __device__ void plan_unit(const WeightsView& t, int box, int chunks, int pos, co
   uint32_t seen0 = 0xffffffffu, seen1 = 0xffffffffu;
   if (t.a.spans && key0 >= rq.cached && rq.tokens > 0) {
     int x_least = 0x7fffffff, y_most = -1;
-    for (int i = lane; i < KT; i += 32)
-      if (key0 + i < k.keys) { const int2 s = span_of(t, rq, key0 + i - rq.cached); x_least = min(x_least, s.x); y_most = max(y_most, s.y); }
+#pragma unroll
+    for (int i = 0; i < KT; i += 32) {
+      const int2 s = span_of(t, rq, min(key0 + i + lane, k.keys - 1) - rq.cached);   // of the last one again behind it
+      x_least = min(x_least, s.x); y_most = max(y_most, s.y);
+    }
     x_least = __reduce_min_sync(0xffffffffu, x_least); y_most = __reduce_max_sync(0xffffffffu, y_most);
     seen0 = seen1 = 0;
     const int first = begin * per_tile, last = min(min(end, begin + 64) * per_tile, rq.tokens);
-    for (int token = first + lane; token < last; token += 32) {
-      const int pre = t.a.spans[2ll * (rq.row0 + token)], tile = (token - first) / per_tile;
-      if (pre >= x_least && pre < y_most) { if (tile < 32) seen0 |= 1u << tile; else seen1 |= 1u << (tile - 32); }
+    const float inverse = 1.0f / (float)per_tile;            // exact enough for quotients below 64: 8192 tokens at most
+    for (int token0 = first + lane; token0 < last; token0 += 256) {   // eight round trips at once
+      int pre[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) pre[k] = t.a.spans[2ll * (rq.row0 + min(token0 + k * 32, rq.tokens - 1))];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int in_chunk = token0 + k * 32 - first;
+        int tile = (int)((float)in_chunk * inverse);
+        tile += (tile + 1) * per_tile <= in_chunk ? 1 : tile * per_tile > in_chunk ? -1 : 0;
+        if (first + in_chunk < last && pre[k] >= x_least && pre[k] < y_most) { if (tile < 32) seen0 |= 1u << tile; else seen1 |= 1u << (tile - 32); }
+      }
     }
     seen0 = __reduce_or_sync(0xffffffffu, seen0); seen1 = __reduce_or_sync(0xffffffffu, seen1);
   }
@@ -145,6 +157,7 @@ __device__ void plan_rows(const WeightsView& t, int pos, const TreePlan<PLAN_THR
 __global__ void __launch_bounds__(PLAN_THREADS) key_weights_plan_kernel(const WeightsView t, int box) {
   __shared__ TreePlan<PLAN_THREADS> units, tiles;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   units.make_of(t, [&](const KeyRange& k) { return (long long)key_tiles_of(t, k) * t.c.num_kv_heads; });
   tiles.make_of(t, [&](const KeyRange& k) { return (long long)row_tiles_of(t, k) * t.c.num_kv_heads; });
   const long long all_units = units.all(t), all_tiles = tiles.all(t);
@@ -518,8 +531,7 @@ phx_status weights_tc_launch(WeightsView& t, cudaStream_t stream, std::string& e
       t.chunks = (int)((pairs + per - 1) / per);
     }
     const long long notes = units * t.chunks + row_tiles * t.c.num_kv_heads * t.c.batch, plans = (notes + PLAN_THREADS / 32 - 1) / (PLAN_THREADS / 32);
-    key_weights_plan_kernel<<<(unsigned)(plans < 4 * sms ? plans : 4 * sms), PLAN_THREADS, 0, stream>>>(t, box);
-    PHX_CUDA_TRY(cudaGetLastError(), err);
+    PHX_CUDA_TRY(launch_programmatic(key_weights_plan_kernel, dim3((unsigned)(plans < 4 * sms ? plans : 4 * sms)), dim3(PLAN_THREADS), 0, stream, t, box), err);
     const int blocks = (int)(units * t.chunks < sms ? units * t.chunks : sms);
     s = t.c.key_size == 64 ? launch<64>(t, map_q, map_k, box, blocks, stream, err) : launch<128>(t, map_q, map_k, box, blocks, stream, err);
     if (s == PHX_OK && t.chunks > 1) {
