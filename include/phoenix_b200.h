@@ -847,8 +847,7 @@ phx_status phx_tree_attention_device(int32_t device, const phx_cache_batch* cach
  * `sinks` (the first keys of a history keep taking the weight that a softmax has to put somewhere).  A cached key's place is its number in the cache, a new
  * token's positions[token] (a draft's depth behind the cache: lengths[b] + depth), at least lengths[b]; positions NULL: lengths[b] + i for token i of a chain
  * (spans NULL), lengths[b] for tokens with spans.  A window counts the token's own key: 1 leaves a chain's token itself and the first keys.  window 0: none.
- * Tiles of keys that no token of a block's rows sees are not read, nor are the pages in such a gap looked up for a chain or behind the cache: a caller may hand out pages that lie
- * wholly in front of all windows and behind the first keys anew, with -1 in the table.  lse_out [num_tokens][num_q_heads] fp32: ln sum e^x over the keys
+ * Pages that lie behind the first keys and in front of the window of a token at place lengths[b] are not read: a caller may hand them out anew, whatever the table says there.  lse_out [num_tokens][num_q_heads] fp32: ln sum e^x over the keys
  * seen, of the logits x that the softmax takes (scaled, capped); -inf for a token that sees none.  Everything else as above. */
 typedef struct phx_window_args {
   phx_tree_args attention;
@@ -862,8 +861,9 @@ phx_status phx_window_attention_device(int32_t device, const phx_cache_batch* ca
 /* The attention weight that the keys of the cache receive: for every key j of a request and key head, the sum over the new tokens that see it and the
  * head's queries of e^(x_ij - lse[i]), with the logits x of the attention above (same sm_scale, cap, spans, positions, window and sinks) and lse
  * [num_tokens][num_q_heads] as phx_window_attention_device gave it.  A cached key's weights[page][kv head][slot] becomes decay * weight + sum, a new one's
- * (behind lengths[b]) the sum: nothing has to be cleared when a page is handed out.  Places of no key are left as they are.  A row whose lse is infinite adds
- * nothing: -inf is a row that saw nothing, +inf leaves a row out.  With decay 1 the keys that no window reaches keep their weights and are not touched.  The order of
+ * (behind lengths[b]) the sum: nothing has to be cleared when a page is handed out.  Places of no key are left as they are.  A page that receives weights belongs to one
+ * request of the call.  A row whose lse is infinite adds
+ * nothing: -inf is a row that saw nothing, +inf leaves a row out.  With decay 1 the keys that no window reaches keep their weights, and pages that the attention does not read are not touched; any other decay looks all pages up.  The order of
  * every sum follows from the sizes alone.  max_tokens and max_keys choose kernels and launch sizes only, as above.  workspace: phx_tree_workspace_bytes, not shared by
  * calls that may overlap.  Asynchronous on `stream`. */
 typedef struct phx_key_weights_args {

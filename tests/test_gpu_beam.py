@@ -62,3 +62,60 @@ def test_beam_search_scores_are_those_of_its_sequences():
     d.forget(2)
     d.remember([2], [histories[1]])
     assert torch.equal(d.search([2], [6], steps=2, beam=3)[0], d.search([0], [6], steps=2, beam=3)[0])
+
+
+def test_a_shrunk_history_serves_on():
+    """Weights of a history that has entered: each row hands out 1 a query head, so a layer's and key head's weights add up to rows x group.  A search over what a shrink
+    leaves is one over caches that hold the kept keys from the start."""
+    import torch
+    from x_algorithm_b200 import decoding
+    from x_algorithm_b200.beam import BeamConfig, SemanticIdBeam, make_weights
+    cfg = BeamConfig(vocab=256, keep_weights=True, sinks=3)
+    w = make_weights(cfg, seed=4)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    histories = [torch.randn((n, cfg.emb_size), device="cuda", generator=g).to(torch.bfloat16) for n in (150, 33)]
+    d = SemanticIdBeam(cfg, w, max_users=2)
+    d.remember([0, 1], histories)
+    plain = SemanticIdBeam(BeamConfig(vocab=256), w, max_users=2)
+    plain.remember([0, 1], histories)
+    for a, b in zip(d.pages, plain.pages):                    # the same keys, to the rounding of an attention by other splits
+        assert torch.allclose(a.float(), b.float(), atol=0.1)
+    table = torch.tensor([d.owned[0]], device="cuda")
+    at = torch.arange(150, device="cuda")
+    group = cfg.num_q_heads // cfg.num_kv_heads
+    for weights in d.weights:
+        got = weights[table[0, at // 16], :, at % 16].double().sum(0)
+        assert torch.allclose(got, torch.full_like(got, 150.0 * group), rtol=1e-5)
+    kept_pages, copies = [], []
+    lengths, tab = torch.tensor([150], dtype=torch.int32, device="cuda"), table.to(torch.int32)
+    for pages, weights in zip(d.pages, d.weights):
+        p, v = pages.clone(), weights.clone()
+        _, kept = decoding.evict(v, p, lengths, tab, budget=64, sinks=3, recent=10)
+        copies.append(p)
+        for h in range(cfg.num_kv_heads):                     # in place is what a gather of the kept places gives
+            k = kept[0, h].long()
+            assert torch.equal(p[table[0, torch.arange(64, device="cuda") // 16], :, h, torch.arange(64, device="cuda") % 16], pages[table[0, k // 16], :, h, k % 16])
+        kept_pages.append(kept)
+    d.shrink([0, 1], budget=64, recent=10)
+    assert d.length == [64, 33] and d.place == [150, 33] and len(d.owned[0]) == 4
+    for p, c in zip(d.pages, copies):
+        assert torch.equal(p, c)
+    ids, scores = d.search([0, 1], [5, 6], steps=2, beam=4)
+    full, full_scores = plain.search([1], [6], steps=2, beam=4)
+    assert torch.allclose(scores[1], full_scores[0], atol=0.3) and torch.isfinite(scores).all()
+    assert ids.shape == (2, 4, 2)
+
+
+def test_a_window_as_long_as_the_history_changes_nothing():
+    import torch
+    from x_algorithm_b200.beam import BeamConfig, SemanticIdBeam, make_weights
+    w = make_weights(BeamConfig(vocab=256), seed=6)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    history = [torch.randn((90, 256), device="cuda", generator=g).to(torch.bfloat16)]
+    scores = []
+    for window in (0, 200, 20):
+        d = SemanticIdBeam(BeamConfig(vocab=256, window=window, sinks=2 if window else 0), w, max_users=1)
+        d.remember([0], history)
+        scores.append(d.search([0], [9], steps=3, beam=4)[1])
+    assert torch.allclose(scores[0], scores[1], atol=0.3)
+    assert not torch.allclose(scores[0], scores[2], atol=1e-3)

@@ -3,7 +3,8 @@
 A small decoder in the trunk's arithmetic (pre-norm layers, merged QKV, rotation, GELU feed-forward; transformer.py:461-618) keeps the keys and
 values of every user's history in one paged cache a layer.  `remember` sends history rows through the layers once, each
 seeing the whole history; `search` grows a tree of ids behind it: every step sends the tree's tokens through the layers, appended behind the history
-and seeing it and their own branch, and extends the best branches by the best alternatives of the next id.  The projections are the
+and seeing it and their own branch, and extends the best branches by the best alternatives of the next id.  With `keep_weights` the caches also count the attention that their keys
+receive while a history enters, and `shrink` lets the keys that received the least leave; `window` and `sinks` bound what a new token sees of a history.  The projections are the
 engine's GEMM call, which waits for the device each time; norms and the choice of branches are plain torch.  (A new token sees all that is cached, so a tree is not
 cached level by level: each step sends it whole.)"""
 from __future__ import annotations
@@ -32,6 +33,9 @@ class BeamConfig:
     max_positions: int = 4096
     rms_eps: float = 1e-5
     logit_cap: float = 30.0
+    window: int = 0              # cached keys that a new token sees, itself counted; 0: all
+    sinks: int = 0               # first keys that it sees whatever the window
+    keep_weights: bool = False   # count what the keys receive, for `shrink`
 
 
 def make_weights(cfg: BeamConfig, seed: int = 0, device="cuda"):
@@ -59,7 +63,9 @@ class SemanticIdBeam:
         self.cos, self.sin = decoding.rope_tables(cfg.max_positions, cfg.key_size, device=device)
         self.free = list(range(cfg.num_pages))
         self.owned: List[List[int]] = [[] for _ in range(max_users)]
-        self.length = [0] * max_users
+        self.length = [0] * max_users                        # keys in the cache
+        self.place = [0] * max_users                         # positions that the history has taken: its length, as it was before it was shrunk
+        self.weights = [torch.zeros((cfg.num_pages, cfg.num_kv_heads, cfg.page_size), dtype=torch.float32, device=device) for _ in range(cfg.num_layers)] if cfg.keep_weights else []
 
     @staticmethod
     def _distinct(users: List[int]):
@@ -86,8 +92,9 @@ class SemanticIdBeam:
         x = x.float()
         return (x * torch.rsqrt((x * x).mean(-1, keepdim=True) + self.cfg.rms_eps) * gain).to(torch.bfloat16)
 
-    def _layers(self, x, users: List[int], counts: List[int], positions, spans):
-        """Token rows x bf16 [N, D] of the users, counts[i] each, behind what their caches hold; appends their keys, returns the rows."""
+    def _layers(self, x, users: List[int], counts: List[int], positions, spans, depth=None, weigh=False):
+        """Token rows x bf16 [N, D] of the users, counts[i] each, behind what their caches hold; appends their keys, returns the rows.  depth int32 [N]: how far behind the
+        cache a token stands (None: all directly behind it); weigh: their attention is added to the keys' weights."""
         cfg = self.cfg
         self._reserve(users, [self.length[u] + n for u, n in zip(users, counts)])
         cols = max(len(self.owned[u]) for u in users)
@@ -96,11 +103,18 @@ class SemanticIdBeam:
         lengths = torch.tensor([self.length[u] for u in users], **dev)
         q_start = torch.tensor([0] + counts, **dev).cumsum(0).to(torch.int32)
         most = dict(max_tokens=max(counts), max_keys=max(self.length[u] + n for u, n in zip(users, counts)))
-        for w, pages in zip(self.w["layers"], self.pages):
+        stands = None if depth is None or not cfg.window else depth + lengths.repeat_interleave(torch.tensor(counts, device=self.device)).to(torch.int32)
+        seen = dict(spans=spans, positions=stands, window=cfg.window or None, sinks=cfg.sinks, **most)
+        for i, (w, pages) in enumerate(zip(self.w["layers"], self.pages)):
             qkv = self._gemm(self._norm(x, w["pre_attn"]), w["qkv"])
             q = decoding.history_append(qkv, pages, q_start, lengths, table, positions, self.cos, self.sin, num_q_heads=cfg.num_q_heads,
                                         q_gain=w["q_gain"], k_gain=w["k_gain"], eps=cfg.rms_eps)
-            a = decoding.tree_attention(q, pages, q_start, lengths, table, spans, **most)
+            if weigh or cfg.window:
+                a, lse = decoding.window_attention(q, pages, q_start, lengths, table, **seen)
+                if weigh:
+                    decoding.key_weights(q, pages, q_start, lengths, table, lse, self.weights[i], **seen)
+            else:
+                a = decoding.tree_attention(q, pages, q_start, lengths, table, spans, **most)
             x = self._gemm(a.view(a.shape[0], -1), w["out"], x, epilogue=1)
             h = self._gemm(self._norm(x, w["pre_ffn"]), w["up"], epilogue=2)
             x = self._gemm(h, w["down"], x, epilogue=1)
@@ -117,13 +131,33 @@ class SemanticIdBeam:
         positions = torch.cat([torch.arange(n, dtype=torch.int32, device=self.device) for n in counts])
         spans = torch.tensor([[0, 1]], dtype=torch.int32, device=self.device).repeat(sum(counts), 1)
         with torch.cuda.device(self.index):
-            self._layers(torch.cat(rows), users, counts, positions, spans)
+            self._layers(torch.cat(rows), users, counts, positions, spans, weigh=self.cfg.keep_weights)
         for u, n in zip(users, counts):
-            self.length[u] = n
+            self.length[u] = self.place[u] = n
+
+    def shrink(self, users: List[int], budget: int, recent: int = 0):
+        """At most `budget` keys of each user stay in each layer and key head: the first `sinks` of the configuration, the last `recent`, and of the others those that received the
+        most attention.  The pages that come free are other histories'."""
+        self._distinct(users)
+        if not self.weights:
+            raise ValueError("the caches count no weights: keep_weights")
+        users = [u for u in users if self.length[u] > budget]
+        if not users:
+            return
+        cols, dev = max(len(self.owned[u]) for u in users), dict(dtype=torch.int32, device=self.device)
+        table = torch.tensor([self.owned[u] + [-1] * (cols - len(self.owned[u])) for u in users], **dev)
+        lengths = torch.tensor([self.length[u] for u in users], **dev)
+        with torch.cuda.device(self.index):
+            for pages, weights in zip(self.pages, self.weights):
+                decoding.evict(weights, pages, lengths, table, budget=budget, sinks=self.cfg.sinks, recent=recent, max_keys=max(self.length[u] for u in users))
+        for u in users:
+            keep = -(-budget // self.cfg.page_size)
+            self.free += self.owned[u][keep:]
+            self.owned[u], self.length[u] = self.owned[u][:keep], budget
 
     def forget(self, user: int):
         self.free += self.owned[user]
-        self.owned[user], self.length[user] = [], 0
+        self.owned[user], self.length[user], self.place[user] = [], 0, 0
 
     def search(self, users: List[int], first_ids: List[int], steps: int, beam: int):
         """The `beam` best continuations of `steps` ids behind each user's history and first id: (ids int64 [users, beam, steps],
@@ -131,7 +165,7 @@ class SemanticIdBeam:
         self._distinct(users)
         if not 1 <= beam <= min(self.cfg.vocab, 128):
             raise ValueError("beam must be 1 to the vocabulary, at most 128")
-        self._placed(max((self.length[u] for u in users), default=0) + steps)
+        self._placed(max((self.place[u] for u in users), default=0) + steps)
         with torch.cuda.device(self.index):
             return self._search(users, first_ids, steps, beam)
 
@@ -143,9 +177,10 @@ class SemanticIdBeam:
         for step in range(steps):
             counts = [len(t) for t in ids]
             spans = torch.cat([torch.from_numpy(decoding.tree_spans(p)) for p in parents]).to(self.device)
-            positions = torch.tensor([self.length[u] + d for u, ds in zip(users, depth) for d in ds], dtype=torch.int32, device=self.device)
+            depths = torch.tensor([d for ds in depth for d in ds], dtype=torch.int32, device=self.device)
+            positions = torch.tensor([self.place[u] + d for u, ds in zip(users, depth) for d in ds], dtype=torch.int32, device=self.device)
             x = self.w["embed"][torch.tensor([i for t in ids for i in t], device=self.device)]
-            x = self._layers(x, users, counts, positions, spans)
+            x = self._layers(x, users, counts, positions, spans, depths)
             starts = [sum(counts[:i]) for i in range(count)]
             last = torch.tensor([s + leaf for s, ls in zip(starts, leaves) for leaf in ls], device=self.device)
             logits = self._gemm(self._norm(x[last], self.w["final"]), self.w["unembed"])
@@ -175,7 +210,7 @@ class SemanticIdBeam:
 
 
 def main():
-    cfg = BeamConfig()
+    cfg = BeamConfig(sinks=4, keep_weights=True)
     weights = make_weights(cfg)
     decoder = SemanticIdBeam(cfg, weights, max_users=3)
     g = torch.Generator(device="cuda").manual_seed(1)
@@ -184,6 +219,9 @@ def main():
     ids, scores = decoder.search([0, 1, 2], [1, 2, 3], steps=3, beam=8)
     for u in range(3):
         print("user %d: best ids %s, log probability %.3f" % (u, ids[u, 0].tolist(), scores[u, 0].item()))
+    decoder.shrink([0], budget=100, recent=16)
+    ids, scores = decoder.search([0], [1], steps=3, beam=8)
+    print("user 0 with half of its keys: best ids %s, log probability %.3f" % (ids[0, 0].tolist(), scores[0, 0].item()))
 
 
 if __name__ == "__main__":

@@ -361,10 +361,17 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
   if (t.a.max_keys > columns) t.a.max_keys = columns;
   const int e = t.c.page_size / 16;
   t.page_magic = ((1ull << 36) + e - 1) / e;
+  const long long heads = (long long)t.c.batch * t.c.num_kv_heads;
+  t.rows = MOVE_BYTES / (4 * t.c.key_size);                   // 64 to 256
+  t.chunks = (int)(((long long)t.a.budget + t.rows - 1) / t.rows);
+  if (heads * t.chunks > 2147483647ll) return bad("budget x heads x batch is too large");
+  if (t.a.workspace_bytes < 16 + heads * t.chunks * 4) return bad("workspace is smaller than phx_tree_workspace_bytes or too small for this many heads and budget");
+  if (!t.a.workspace || !aligned16(t.a.workspace)) return bad("workspace must be a 16-byte aligned buffer");
+  t.ticket = static_cast<int*>(t.a.workspace);
+  t.read = t.ticket + 4;
   DeviceScope scope(device);
   if (!scope.ok()) { set_global_error("phx_evict_device: cudaSetDevice failed"); return PHX_E_CUDA; }
   cudaStream_t st = (cudaStream_t)stream;
-  const long long heads = (long long)t.c.batch * t.c.num_kv_heads;
 
   // Blocks of a cluster: as long as the heads' clusters fit the device twice over and a block keeps 1024 weights
   int ranks = 1;
@@ -377,13 +384,6 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
   const long long move_bytes = (long long)sizeof(ChunkPlaces) + (long long)t.a.budget * 4 * t.c.key_size;
   t.alone = t.a.budget <= 256 && move_bytes <= 68 * 1024 && (t.a.lengths_out + t.c.batch <= t.c.lengths || t.c.lengths + t.c.batch <= t.a.lengths_out);
   if (t.alone && t.held * 4 < move_bytes) t.held = (int)((move_bytes + 3) / 4);
-  t.rows = MOVE_BYTES / (4 * t.c.key_size);                   // 64 to 256
-  t.chunks = (t.a.budget + t.rows - 1) / t.rows;
-  if (heads * t.chunks > 2147483647ll) return bad("budget x heads x batch is too large");
-  if (t.a.workspace_bytes < 16 + heads * t.chunks * 4) return bad("workspace is smaller than phx_tree_workspace_bytes or too small for this many heads and budget");
-  if (!t.a.workspace || !aligned16(t.a.workspace)) return bad("workspace must be a 16-byte aligned buffer");
-  t.ticket = static_cast<int*>(t.a.workspace);
-  t.read = t.ticket + 4;
   const int select_smem = (int)sizeof(SelectSmem) + t.held * 4;
   static SmemLimit select_limit;
   std::string err;

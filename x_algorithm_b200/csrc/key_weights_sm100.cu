@@ -85,7 +85,8 @@ __device__ void plan_unit(const WeightsView& t, int box, int chunks, int pos, co
   // its boxes: lane i has box i
   const int key = key0 + lane * box, col = key / page_size, slot0 = key - col * page_size;
   int page = -2;
-  if (lane < boxes && key < k.keys) page = k.table[col];
+  // (a box that no window reaches and no first key lies in: its page may be another request's by now)
+  if (lane < boxes && key < k.keys && (t.decay != 1.0f || key + box - 1 > rq.cached - t.window || key < t.sinks)) page = k.table[col];
   const bool there = (unsigned)page < (unsigned)t.c.num_pages;
   if (page != -2 && !there) cache_report(t.c, CACHE_BAD_PAGE);
   if (lane == 0 && key0 == 0 && h == 0 && chunk == 0 && k.keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);

@@ -559,6 +559,7 @@ phx_status attend(int32_t device, const phx_cache_batch* cache, View& t, cudaStr
   if (!t.a.q || !t.a.out || !aligned16(t.a.q) || !aligned16(t.a.out)) return bad("q and out must be 16-byte aligned buffers");
   if ((reinterpret_cast<uintptr_t>(t.a.spans) & 7) != 0) return bad("spans must be 8-byte aligned");
   if (!t.a.workspace || !aligned16(t.a.workspace)) return bad("workspace must be a 16-byte aligned buffer");
+  if (t.c.num_pages == 0) return bad("an empty pool has no keys to attend to");
   t.csc = t.a.sm_scale * TREE_LOG2E;
   t.group = t.a.num_q_heads / t.c.num_kv_heads;
   DeviceScope scope(device);
@@ -595,7 +596,6 @@ phx_status attend(int32_t device, const phx_cache_batch* cache, View& t, cudaStr
   t.part_o = static_cast<float*>(t.a.workspace);
   t.part_ml = reinterpret_cast<float2*>(t.part_o + 2ll * t.split * t.rows * t.c.key_size);
   t.join = reinterpret_cast<TreeJoin*>(t.part_ml + 2ll * t.split * t.rows);
-  if (t.c.num_pages == 0) return bad("an empty pool has no keys to attend to");
   phx_status s = tc ? tree_tc_launch(t, st, err) : t.c.key_size == 32 ? tree_mma_launch<32>(t, st, err) : t.c.key_size == 64 ? tree_mma_launch<64>(t, st, err) : tree_mma_launch<128>(t, st, err);
   if (s == PHX_OK && t.split) {
     const long long rows = (long long)t.a.max_tokens * t.group;

@@ -253,7 +253,10 @@ struct TcBlock {
         return true;
       };
       for (int first = j;; ++j) {                            // K runs a tile ahead of V
-        const bool in_keys = lane < boxes && tile * KT + lane * box < keys, ok = in_keys && (unsigned)page < (unsigned)t.c.num_pages;
+        bool in_keys = lane < boxes && tile * KT + lane * box < keys;
+        // a box that no row's window reaches and no first key lies in: its page may be another request's by now
+        if constexpr (WINDOW) in_keys &= tile * KT + (lane + 1) * box - 1 > min(behind_least, rq.cached - 1) || tile * KT + lane * box < t.sinks;
+        const bool ok = in_keys && (unsigned)page < (unsigned)t.c.num_pages;
         const int row = ok ? page * page_rows + head_row + slot : no_row;
         const uint32_t there = __ballot_sync(0xffffffffu, ok);
         if (in_keys && !ok) cache_report(t.c, CACHE_BAD_PAGE);
