@@ -44,7 +44,8 @@ __device__ __forceinline__ EvictRequest evict_request(const EvictView& t, int b)
 
 // ---- a chunk of a head's places, moved by a block ------------------------------------------------------------------------------
 
-struct ChunkPlaces { int to_page[256], from[256], from_page[256]; float weight[256]; };   // of each place: its page, the slot and page of what it receives (slot -1: nothing)
+// Of each place: its key's row of the pool and that which it receives (-1: none), its word among the weights, the weight that it receives
+struct ChunkPlaces { int to[256], from[256], word[256]; float weight[256]; };
 template <int THREADS>
 struct ChunkMove {
   const EvictView& t;
@@ -56,42 +57,47 @@ struct ChunkMove {
     cache_report(t.c, CACHE_BAD_PAGE);
     return false;
   }
-  __device__ __forceinline__ uint8_t* address(int page, int which, int slot, int piece) const {
-    return reinterpret_cast<uint8_t*>(t.c.pages + cache_row0(t.c, page, which, h) + (long long)slot * t.c.key_size) + piece * 16;
-  }
-  __device__ __forceinline__ const int* table() const { return t.c.block_table + (long long)b * t.c.table_stride; }
-  // place `i` of the chunk, in page `to`, receives place `src`; whether it is another
-  __device__ __forceinline__ bool place(int i, int src, int to) {
-    const int src_col = page_column(t, src), page = table()[src_col], slot = src - src_col * t.c.page_size;
+  // place `i` of the chunk, in page `to`, receives place `src`, in `page`; whether it is another
+  __device__ __forceinline__ bool place(int i, int src, int to, int page) {
+    const int from_slot = src - page_column(t, src) * t.c.page_size, to_slot = first + i - page_column(t, first + i) * t.c.page_size;
     const bool there = good(to), moves = good(page) && there && src != first + i;
-    at.from[i] = moves ? slot : -1;
-    at.from_page[i] = page; at.to_page[i] = to;
+    at.from[i] = moves ? (page * 2 * t.c.num_kv_heads + h) * t.c.page_size + from_slot : -1;   // the pool's rows fit 31 bits
+    at.to[i] = (to * 2 * t.c.num_kv_heads + h) * t.c.page_size + to_slot;
+    at.word[i] = (to * t.c.num_kv_heads + h) * t.c.page_size + to_slot;
     if (moves)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(at.weight + i)), "l"(t.a.weights + ((long long)page * t.c.num_kv_heads + h) * t.c.page_size + slot) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(at.weight + i)), "l"(t.a.weights + ((long long)page * t.c.num_kv_heads + h) * t.c.page_size + from_slot) : "memory");
     return moves;
   }
+  // A thread has one piece of every so many rows, of the key and the value.  (With addresses worked out a piece at a time the move was issue-bound: 64 x 4 heads 82 us, 2 x 4 long ones 62.)
   __device__ __forceinline__ void fetch() {                  // behind a barrier behind place()
-    const int row_of = threadIdx.x / pieces, piece = threadIdx.x - row_of * pieces;
-    for (int r = row_of; r < 2 * count; r += THREADS / pieces) {
-      const int which = r >= count, i = r - which * count;
-      if (at.from[i] < 0) continue;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(data + (r * pieces + piece) * 16)), "l"(address(at.from_page[i], which, at.from[i], piece)) : "memory");
+    const int row_of = threadIdx.x / pieces, piece = threadIdx.x - row_of * pieces, row_bytes = pieces * 16;
+    const uint16_t* const keys = t.c.pages + piece * 8;
+    const uint16_t* const values = keys + (long long)t.c.num_kv_heads * t.c.page_size * t.c.key_size;
+    const uint32_t to = smem_u32(data) + piece * 16;
+#pragma unroll 4
+    for (int i = row_of; i < count; i += THREADS / pieces) {
+      const int row = at.from[i];
+      if (row < 0) continue;
+      const long long from = (long long)row * t.c.key_size;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * row_bytes), "l"(keys + from) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (count + i) * row_bytes), "l"(values + from) : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   __device__ __forceinline__ void store() const {            // once nothing reads what it writes over
-    const int row_of = threadIdx.x / pieces, piece = threadIdx.x - row_of * pieces;
-    for (int r = row_of; r < 2 * count; r += THREADS / pieces) {
-      const int which = r >= count, i = r - which * count;
+    const int row_of = threadIdx.x / pieces, piece = threadIdx.x - row_of * pieces, row_bytes = pieces * 16;
+    uint16_t* const keys = t.c.pages + piece * 8;
+    uint16_t* const values = keys + (long long)t.c.num_kv_heads * t.c.page_size * t.c.key_size;
+    const uint8_t* const from = data + piece * 16;
+#pragma unroll 4
+    for (int i = row_of; i < count; i += THREADS / pieces) {
       if (at.from[i] < 0) continue;
-      const int to = first + i, slot = to - page_column(t, to) * t.c.page_size;
-      *reinterpret_cast<uint4*>(address(at.to_page[i], which, slot, piece)) = *reinterpret_cast<const uint4*>(data + (r * pieces + piece) * 16);
+      const long long to = (long long)at.to[i] * t.c.key_size;
+      *reinterpret_cast<uint4*>(keys + to) = *reinterpret_cast<const uint4*>(from + i * row_bytes);
+      *reinterpret_cast<uint4*>(values + to) = *reinterpret_cast<const uint4*>(from + (count + i) * row_bytes);
     }
     for (int i = threadIdx.x; i < count; i += THREADS)
-      if (at.from[i] >= 0) {
-        const int to = first + i, slot = to - page_column(t, to) * t.c.page_size;
-        t.a.weights[((long long)at.to_page[i] * t.c.num_kv_heads + h) * t.c.page_size + slot] = at.weight[i];
-      }
+      if (at.from[i] >= 0) t.a.weights[at.word[i]] = at.weight[i];
   }
 };
 
@@ -259,7 +265,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   __syncthreads();
   if (kept[t.a.budget - 1] < t.a.budget) return;
   ChunkMove<SEL_THREADS> move{t, *reinterpret_cast<ChunkPlaces*>(held), reinterpret_cast<uint8_t*>(held) + sizeof(ChunkPlaces), b, h, 0, t.a.budget, t.c.key_size / 8};
-  for (int i = tid; i < t.a.budget; i += SEL_THREADS) move.place(i, kept[i], table[page_column(t, i)]);
+  for (int i = tid; i < t.a.budget; i += SEL_THREADS) move.place(i, kept[i], table[page_column(t, i)], table[page_column(t, kept[i])]);
   __syncthreads();
   move.fetch();
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -305,6 +311,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictVie
   // the one reader of this request's length in this launch, so that lengths_out may be lengths
   if (chunk == 0 && h == 0 && tid == 0) t.a.lengths_out[b] = min(evict_request(t, b).length, t.a.budget);
   const int first = chunk * t.rows, count = min(t.rows, t.a.budget - first);
+  const int* const table = t.c.block_table + (long long)b * t.c.table_stride;
   ChunkMove<MOVE_THREADS> move{t, places, data, b, h, first, count, t.c.key_size / 8};
   // Round trips: the place that this thread's place receives and its page at once (the first `budget` places have columns where a request is over its budget), that one's page, its rows.
   const int last = kept[t.a.budget - 1];
@@ -312,11 +319,11 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictVie
   const int col = page_column(t, first + tid);
   if (tid < count) {
     src = kept[first + tid];
-    if (col < t.c.table_cols) to = move.table()[col];
+    if (col < t.c.table_cols) to = table[col];
   }
   if (last < t.a.budget) return;                             // at most `budget` keys: all where they are
   int* const read = t.read + (long long)of * t.chunks;
-  if (!__syncthreads_or(tid < count && move.place(tid, src, to))) {   // all stays where it is
+  if (!__syncthreads_or(tid < count && move.place(tid, src, to, table[page_column(t, src)]))) {   // all stays where it is
     if (tid == 0) asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(read + chunk), "r"(1) : "memory");
     return;
   }
