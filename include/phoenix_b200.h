@@ -861,8 +861,8 @@ phx_status phx_window_attention_device(int32_t device, const phx_cache_batch* ca
 /* The attention weight that the keys of the cache receive: for every key j of a request and key head, the sum over the new tokens that see it and the
  * head's queries of e^(x_ij - lse[i]), with the logits x of the attention above (same sm_scale, cap, spans, positions, window and sinks) and lse
  * [num_tokens][num_q_heads] as phx_window_attention_device gave it.  A cached key's weights[page][kv head][slot] becomes decay * weight + sum, a new one's
- * (behind lengths[b]) the sum: nothing has to be cleared when a page is handed out.  Places of no key are left as they are.  A page that receives weights belongs to one
- * request of the call.  A row whose lse is infinite adds
+ * (behind lengths[b]) the sum: nothing has to be cleared when a page is handed out.  Places of no key are left as they are.  A page that receives weights stands once in the
+ * call's tables.  A row whose lse is infinite adds
  * nothing: -inf is a row that saw nothing, +inf leaves a row out.  With decay 1 the keys that no window reaches keep their weights, and pages that the attention does not read are not touched; any other decay looks all pages up.  The order of
  * every sum follows from the sizes alone.  max_tokens and max_keys choose kernels and launch sizes only, as above.  workspace: phx_tree_workspace_bytes, not shared by
  * calls that may overlap.  Asynchronous on `stream`. */
@@ -891,8 +891,8 @@ phx_status phx_key_weights_device(int32_t device, const phx_cache_batch* cache, 
  * ones with the largest weights (ties: the lower place; NaN counts as largest; a key whose page is outside the pool as lowest).  What stays moves to places 0, 1, ... budget - 1
  * in its order, key, value and weight, in the request's own pages; places behind are left as they are, and the pages behind the budget are the caller's to
  * hand out.  A request with at most `budget` keys stays as it is.  kept_out [batch][num_kv_heads][budget]: the places that the kept keys had, ascending,
- * -1 behind a shorter request's last; lengths_out [batch]: keys per request now (may be `lengths` itself).  A page may belong to one request of the call only.
- * max_keys (the most that a request has) chooses launch sizes only.  workspace: phx_tree_workspace_bytes (of which batch x heads x budget / 16 bytes are used), not
+ * -1 behind a shorter request's last; lengths_out [batch]: keys per request now (may be `lengths` itself).  A page may stand once in the table's columns that hold
+ * keys: it belongs to one request of the call, at one place.  budget is at most 2^30.  max_keys (the most that a request has) chooses launch sizes only.  workspace: phx_tree_workspace_bytes (of which batch x heads x budget / 16 bytes are used), not
  * shared by calls that may overlap; nothing in it is kept.  Of the cache block q_start and num_tokens are not used.  Bad pages and lengths raise
  * status bits as above.  Asynchronous on `stream`. */
 typedef struct phx_evict_args {

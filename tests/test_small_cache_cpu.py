@@ -180,3 +180,9 @@ def test_shrinking_needs_weights(host):
         e.shrink([1, 1], budget=4)
     e.shrink([0, 1], budget=4)                               # nothing cached
     assert not host["evict"]
+
+
+@pytest.mark.parametrize("budget", [2 ** 30 + 1, 2 ** 31 - 1])
+def test_a_budget_that_a_grid_would_count_past_is_refused(budget):
+    f, a = _evict(budget=budget)
+    assert f(0, C.byref(_cache()), C.byref(a), None) == 1 and b"2^30" in _lib.lib.phx_global_error()

@@ -18,6 +18,8 @@ namespace {
 
 using namespace sm100;
 
+constexpr int MOST_BUDGET = 1 << 30;   // the kernels count past it by a grid's threads, in 32 bits
+
 struct EvictView {
   phx_cache_batch c;
   phx_evict_args a;
@@ -360,6 +362,7 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
   if (*what) return bad(what);
   if (t.c.batch > 65535) return bad("at most 65535 requests");
   if (t.a.budget < 1 || t.a.sinks < 0 || t.a.recent < 0 || (long long)t.a.sinks + t.a.recent > t.a.budget) return bad("budget must be at least 1 and hold sinks + recent keys");
+  if (t.a.budget > MOST_BUDGET) return bad("budget must be at most 2^30");
   if (t.a.max_keys < 0) return bad("negative size");
   if (t.c.batch == 0) return PHX_OK;
   if (t.c.num_pages == 0) return bad("an empty pool has no keys");

@@ -345,8 +345,8 @@ def evict(weights, pages, lengths, block_table, *, budget: int, sinks: int = 0, 
           workspace=None, stream: Optional[int] = None):
     """Requests with more than `budget` keys keep, in each key head, the first `sinks`, the last `recent`, and of the others the ones with the largest weights (ties: the
     earlier); keys, values and weights move together in their order, in place, to the front of the request's own pages.  Returns (lengths int32 [B] now, the
-    places that the kept keys had, ascending, int32 [B, kv heads, budget], -1 behind the last of a shorter request).  lengths_out may be `lengths`.  A page may belong
-    to one request of the call only; the pages behind a request's new length are the caller's to hand out."""
+    places that the kept keys had, ascending, int32 [B, kv heads, budget], -1 behind the last of a shorter request).  lengths_out may be `lengths`.  A page may stand
+    once in the rows of the call, as one request's; the pages behind a request's new length are the caller's to hand out."""
     device = _rows(weights, "weights", _F32, 3)
     if _elsewhere(device, stream):
         with _under(device, stream):
@@ -355,8 +355,8 @@ def evict(weights, pages, lengths, block_table, *, budget: int, sinks: int = 0, 
     state, mine = _keep(device, stream), _structs
     kv_heads, page_size, _, cols = _batch(mine.batch, pages, _NO_ROWS, lengths, block_table, 0, device, state)
     _need(weights, "weights", _F32, (pages.shape[0], kv_heads, page_size), device)
-    if not (1 <= budget <= 2**31 - 1 and sinks >= 0 and recent >= 0 and sinks + recent <= budget):
-        raise ValueError("budget must be at least 1 and hold sinks + recent keys")
+    if not (1 <= budget <= 2**30 and sinks >= 0 and recent >= 0 and sinks + recent <= budget):
+        raise ValueError("budget must be 1 to 2^30 and hold sinks + recent keys")
     batch = block_table.shape[0]
     if lengths_out is None:
         lengths_out = torch.empty_strided((batch,), (1,), dtype=_I32, device=weights.device)
