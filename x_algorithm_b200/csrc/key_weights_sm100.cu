@@ -29,7 +29,7 @@ constexpr int KW_FIRST = 4, KW_SETS = 4, KW_SUM = 4 * KW_SETS;   // warps 4 .. 1
 constexpr int KW_THREADS = 32 * (KW_FIRST + KW_SUM);
 constexpr int PLAN_THREADS = 256;
 constexpr int NK = 2, NS = 2, NR = 4;    // K tiles in shared memory, S^T buffers in tensor memory, pairs whose rows are described
-__host__ __device__ constexpr int q_buffers(int dh) { return dh == 64 ? 3 : 2; }      // pairs of Q tiles
+__host__ __device__ constexpr int q_buffers(int dh) { return dh == 128 ? 2 : 3; }      // pairs of Q tiles
 constexpr int NU = 4;                    // units that are worked on
 
 // What is written down in the workspace.  Rows: -lse in the log2 domain (-inf: no weight); (place in the walk, place behind which the window begins); for each 32 of them the least and the last
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) key_weights_plan_kernel(const We
 
 template <int DH>
 struct KwSmem {
-  static constexpr int DCH = DH / 64, NQ = q_buffers(DH);
+  static constexpr int DCH = (DH + 63) / 64, NQ = q_buffers(DH);
   uint8_t k[NK][DCH * KT * 128];
   uint8_t q[NQ][DCH * RT * 128];
   RowNote rows[NR][2];
@@ -197,7 +197,7 @@ struct KwSmem {
 
 template <int DH, int CAP>
 struct KwBlock {
-  static constexpr int DCH = DH / 64, NQ = q_buffers(DH);
+  static constexpr int DCH = (DH + 63) / 64, NQ = q_buffers(DH);
   static constexpr uint32_t BLK = DCH * KT * 128;
   const WeightsView& t;
   const CUtensorMap& map_q;
@@ -286,7 +286,7 @@ struct KwBlock {
       for (int c = 0; c < DCH; ++c) {
         const uint64_t kd = make_smem_desc(smem_u32(sm.k[n % NK]) + c * KT * 128), qd = make_smem_desc(smem_u32(sm.q[j % NQ]) + c * RT * 128);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_bf16(tmem + (j % NS) * RT, kd + (uint64_t)(k * 2), qd + (uint64_t)(k * 2), idesc, (c | k) != 0);
+        for (int k = 0; k < (DH < 64 ? DH / 16 : 4); ++k) umma_bf16(tmem + (j % NS) * RT, kd + (uint64_t)(k * 2), qd + (uint64_t)(k * 2), idesc, (c | k) != 0);
       }
       umma_commit(smem_u32(&sm.q_empty[j % NQ]));
       umma_commit(smem_u32(&sm.s_full[j % NS]));
@@ -494,9 +494,9 @@ long long units_bound(const WeightsView& t) { return ((long long)t.c.table_cols 
 }  // namespace
 
 // Up to 16 rows a key head the mma.sync kernel reads the keys once, as fast as they come.  What is written down about rows (13 bytes each) and one request's keys has to fit three quarters of the
-// workspace, some two million rows and 100 thousand tiles of keys; calls beyond that, and heads of 32, stay with it, too.
+// workspace, some two million rows and 100 thousand tiles of keys; calls beyond that stay with it, too.
 bool weights_tc_supported(const WeightsView& t) {
-  if ((t.c.key_size != 64 && t.c.key_size != 128) || t.group > HT || (long long)t.a.max_tokens * t.group <= 16) return false;
+  if (t.group > HT || (long long)t.a.max_tokens * t.group <= 16) return false;
   return UNITS_AT + row_tiles_bound(t, t.c.batch < TREE_MAX_SPLIT_BATCH ? t.c.batch : TREE_MAX_SPLIT_BATCH) * (long long)sizeof(RowNote) + units_bound(t) * (long long)sizeof(UnitNote) <= t.a.workspace_bytes / 4 * 3;
 }
 
@@ -506,7 +506,7 @@ phx_status weights_tc_launch(WeightsView& t, cudaStream_t stream, std::string& e
   while (t.c.page_size % box != 0) box /= 2;
   CUtensorMap map_q, map_k;
   phx_status s = tree_query_map(&map_q, t, err);
-  if (s == PHX_OK) s = tree_pool_map(&map_k, t, box, err);
+  if (s == PHX_OK) s = tree_pool_map(&map_k, t, box, true, err);
   const WeightsView whole = t;
   const int per_tile = t.rows / t.group, sms = device_sms();
   // as many requests at a time as a block plans and whose notes fit
@@ -534,7 +534,7 @@ phx_status weights_tc_launch(WeightsView& t, cudaStream_t stream, std::string& e
     const long long notes = units * t.chunks + row_tiles * t.c.num_kv_heads * t.c.batch, plans = (notes + PLAN_THREADS / 32 - 1) / (PLAN_THREADS / 32);
     PHX_CUDA_TRY(launch_programmatic(key_weights_plan_kernel, dim3((unsigned)(plans < 4 * sms ? plans : 4 * sms)), dim3(PLAN_THREADS), 0, stream, t, box), err);
     const int blocks = (int)(units * t.chunks < sms ? units * t.chunks : sms);
-    s = t.c.key_size == 64 ? launch<64>(t, map_q, map_k, box, blocks, stream, err) : launch<128>(t, map_q, map_k, box, blocks, stream, err);
+    s = t.c.key_size == 32 ? launch<32>(t, map_q, map_k, box, blocks, stream, err) : t.c.key_size == 64 ? launch<64>(t, map_q, map_k, box, blocks, stream, err) : launch<128>(t, map_q, map_k, box, blocks, stream, err);
     if (s == PHX_OK && t.chunks > 1) {
       const long long joins = (units * KT + 255) / 256;
       const cudaError_t e = launch_programmatic(key_weights_join_kernel, dim3((unsigned)(joins < 4 * sms ? joins : 4 * sms)), dim3(256), 0, stream, t);

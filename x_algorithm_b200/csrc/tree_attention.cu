@@ -483,7 +483,7 @@ phx_status tree_mma_launch(const View& t, cudaStream_t stream, std::string& err)
   static SmemLimit limit;
   PHX_CUDA_TRY(limit.raise(tree_mma_kernel<DH, CAP, View>, smem), err);
   CUtensorMap map;
-  const phx_status st = tree_pool_map(&map, t, KEYS, err);
+  const phx_status st = tree_pool_map(&map, t, KEYS, false, err);
   if (st != PHX_OK) return st;
   const long long rows = (long long)t.a.max_tokens * t.group;
   const unsigned tiles = (unsigned)((rows + ROWS - 1) / ROWS < 65535 ? (rows + ROWS - 1) / ROWS : 65535);
@@ -510,15 +510,16 @@ long long part_bytes(int split, int rows, int dh) { return 2ll * split * rows * 
 }  // namespace
 
 // The pool as rows of key_size; a box is 64 (32) columns of `box_rows` rows, swizzled; rows behind the pool read as zeros
-phx_status tree_pool_map(CUtensorMap* map, const TreeView& t, int box_rows, std::string& err) {
+phx_status tree_pool_map(CUtensorMap* map, const TreeView& t, int box_rows, bool wide, std::string& err) {
   EncodeTiledFn fn = get_encode_fn(err);
   if (!fn) return PHX_E_CUDA;
   const int dh = t.c.key_size;
   cuuint64_t dims[2] = {(cuuint64_t)dh, (cuuint64_t)(2 * t.c.num_pages * t.c.num_kv_heads * t.c.page_size)};
   cuuint64_t strides[1] = {(cuuint64_t)dh * 2};
-  cuuint32_t box[2] = {(cuuint32_t)(dh < 64 ? dh : 64), (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  const bool narrow = dh < 64 && !wide;
+  cuuint32_t box[2] = {(cuuint32_t)(narrow ? dh : 64), (cuuint32_t)box_rows}, estr[2] = {1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, t.c.pages, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        dh < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { err = "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r); return PHX_E_CUDA; }
   return PHX_OK;
 }

@@ -240,10 +240,11 @@ template <int THREADS> struct TreePlan {
   }
 };
 
-phx_status tree_pool_map(CUtensorMap* map, const TreeView& t, int box_rows, std::string& err);
+phx_status tree_pool_map(CUtensorMap* map, const TreeView& t, int box_rows, bool wide, std::string& err);   // wide: boxes of 64 columns for heads of 32 as well, zeros behind them
 phx_status tree_query_map(CUtensorMap* map, const TreeView& t, std::string& err);
 // tcgen05 kernel (tree_attention_sm100.cu): whether it takes the call, its tile shape, its launch
 bool tree_tc_supported(const TreeView& t);
+bool tree_tc_supported(const WindowView& t);
 void tree_tc_shape(TreeView& t);                 // rows and keys of a tile
 int tree_tc_blocks_per_sm();
 phx_status tree_tc_launch(const TreeView& t, cudaStream_t stream, std::string& err);

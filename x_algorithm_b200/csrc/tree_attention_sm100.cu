@@ -30,7 +30,7 @@ constexpr int TC_THREADS = 192;
 constexpr int SLAB = QT * 128;          // bytes of one [128 rows x 64 bf16] swizzled tile
 constexpr int KT = 64;                  // keys of a tile: S of two tiles and O share the block's 256 columns of tensor memory
 // K and V buffers each: 64 KB a block
-__host__ __device__ constexpr int tc_buffers(int dh) { return dh == 64 ? 4 : 2; }
+__host__ __device__ constexpr int tc_buffers(int dh) { return dh == 128 ? 2 : 4; }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -71,7 +71,7 @@ constexpr uint32_t MASKED = 16, LAST = 32, FINAL = 64, PLACES = 128, BOXES = 15;
 
 template <int DH, class View>
 struct TcSmem {
-  static constexpr int DCH = DH / 64, NB = tc_buffers(DH);
+  static constexpr int DCH = (DH + 63) / 64, NB = tc_buffers(DH);
   uint8_t q[DCH * SLAB];
   uint8_t k[NB][DCH * KT * 128];
   uint8_t v[NB][DCH * KT * 128];
@@ -123,7 +123,7 @@ struct PieceWalk {
 template <int DH, int CAP, class View>
 struct TcBlock {
   static constexpr bool WINDOW = has_window<View>;
-  static constexpr int DCH = DH / 64, NB = tc_buffers(DH);
+  static constexpr int DCH = (DH + 63) / 64, NB = tc_buffers(DH);
   static constexpr uint32_t BLK = DCH * KT * 128, TM_S = 0, TM_O = 128;
   const View& t;
   const CUtensorMap& map_q;
@@ -315,7 +315,7 @@ struct TcBlock {
 
   // ---- MMA issuer (one thread) -------------------------------------------------------------------------------------------
   __device__ __forceinline__ void issue() {
-    constexpr uint32_t idesc_s = make_idesc(QT, KT), idesc_o = make_idesc_b_mn(QT, DH);
+    constexpr uint32_t idesc_s = make_idesc(QT, KT), idesc_o = make_idesc_b_mn(QT, DCH * 64);
     int s_pieces = 0;                                       // pieces whose S has been begun
     bool s_first = true;
     uint32_t flags_next = 0;
@@ -329,7 +329,7 @@ struct TcBlock {
       for (int c = 0; c < DCH; ++c) {
         const uint64_t qd = make_smem_desc(smem_u32(sm.q) + c * SLAB), kd = make_smem_desc(smem_u32(sm.k[b]) + c * KT * 128);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_bf16(tmem + TM_S + (j & 1) * KT, qd + (uint64_t)(k * 2), kd + (uint64_t)(k * 2), idesc_s, (c | k) != 0);
+        for (int k = 0; k < (DH < 64 ? DH / 16 : 4); ++k) umma_bf16(tmem + TM_S + (j & 1) * KT, qd + (uint64_t)(k * 2), kd + (uint64_t)(k * 2), idesc_s, (c | k) != 0);
       }
       umma_commit(smem_u32(&sm.k_empty[b]));
       umma_commit(smem_u32(&sm.s_full[j & 1]));
@@ -755,7 +755,7 @@ phx_status launch(const View& t, cudaStream_t stream, std::string& err) {
   while (t.c.page_size % box != 0) box /= 2;
   CUtensorMap map_q, map_kv;
   phx_status s = tree_query_map(&map_q, t, err);
-  if (s == PHX_OK) s = tree_pool_map(&map_kv, t, box, err);
+  if (s == PHX_OK) s = tree_pool_map(&map_kv, t, box, true, err);
   if (s != PHX_OK) return s;
   const long long row_tiles = ((long long)t.a.max_tokens * t.group + t.rows - 1) / t.rows;
   const dim3 grid = t.split || t.turns ? dim3(t.split ? t.split : t.turns) : dim3((unsigned)(row_tiles < 65535 ? row_tiles : 65535), t.c.num_kv_heads, t.c.batch);
@@ -771,12 +771,13 @@ phx_status launch_any(const View& t, cudaStream_t stream, std::string& err) {
     if (t.a.cap_method == 0 && !(t.a.sm_scale > 0.f)) return launch<DH, 3>(t, stream, err);
     return t.a.cap_method == 0 ? launch<DH, 0>(t, stream, err) : t.a.cap_method == 1 ? launch<DH, 1>(t, stream, err) : launch<DH, 2>(t, stream, err);
   };
+  if constexpr (has_window<View>) { if (t.c.key_size == 32) return of(std::integral_constant<int, 32>()); }
   return t.c.key_size == 64 ? of(std::integral_constant<int, 64>()) : of(std::integral_constant<int, 128>());
 }
 
 }  // namespace
 
-// Queries as [token][head][column]; a box is 64 columns of the group's heads of as many tokens as 128 rows hold
+// Queries as [token][head][column]; a box is 64 columns (behind a head of 32: zeros) of the group's heads of as many tokens as 128 rows hold
 phx_status tree_query_map(CUtensorMap* map, const TreeView& t, std::string& err) {
   EncodeTiledFn fn = get_encode_fn(err);
   if (!fn) return PHX_E_CUDA;
@@ -791,6 +792,7 @@ phx_status tree_query_map(CUtensorMap* map, const TreeView& t, std::string& err)
 }
 
 bool tree_tc_supported(const TreeView& t) { return (t.c.key_size == 64 || t.c.key_size == 128) && t.group <= QT; }
+bool tree_tc_supported(const WindowView& t) { return t.group <= QT; }
 void tree_tc_shape(TreeView& t) { t.rows = QT / t.group * t.group; t.keys = KT; t.setup = 6; }
 int tree_tc_blocks_per_sm() { return 2; }
 phx_status tree_tc_launch(const TreeView& t, cudaStream_t stream, std::string& err) { return launch_any(t, stream, err); }
