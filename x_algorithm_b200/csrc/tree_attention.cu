@@ -571,6 +571,7 @@ phx_status attend(int32_t device, const phx_cache_batch* cache, View& t, cudaStr
   const bool tc = tree_tc_supported(t) && (long long)t.a.max_tokens * t.group > ROWS;
   t.rows = ROWS; t.keys = KEYS * TREE_WARPS; t.setup = 2;
   if (tc) tree_tc_shape(t);
+  set_tile_tokens(t);
   const int per_sm = tc ? tree_tc_blocks_per_sm() : t.c.key_size == 128 ? mma_blocks<128>() : mma_blocks<64>();
   // Blocks share the tiles of all units where there are few units for them and long ones among them.  Measured on the tensor cores (us, shared / whole): 2 to 3
   // units a block, heads of 128, with 0.4 of the last round's blocks empty and 16, 64, 128 tiles a unit 108 / 87, 285 / 273, 523 / 523; with 0.84 empty 97 / 82, 245 / 253,

@@ -37,6 +37,7 @@ struct WindowView : TreeView {
   const int* positions;
   float* lse;
   int window, sinks;
+  int tile_tokens, rows_tokens;   // that a tile of rows may touch, that it has where it has whole ones
 };
 template <class View> constexpr bool has_window = std::is_same<View, WindowView>::value;
 // A unit cut by the bound between blocks x - 1 and x, the first that cuts it: block x - 1 has its first tiles, blocks x .. to - 1 the others
@@ -127,6 +128,15 @@ struct TreePiece {
 
 __device__ __forceinline__ int tree_row_tiles(const TreeView& t, int tokens) { return (int)(((long long)tokens * t.group + t.rows - 1) / t.rows); }
 __device__ __forceinline__ int tree_key_tiles(const TreeView& t, int keys) { return keys > 0 ? (keys - 1) / t.keys + 1 : 1; }
+__device__ __forceinline__ int rows_tokens(const TreeView& t) { return t.rows / t.group; }
+__device__ __forceinline__ int rows_tokens(const WindowView& t) { return t.rows_tokens; }
+// (a tile of rows has whole tokens, or a power of two of rows)
+__device__ __forceinline__ int tree_row_tiles(const WindowView& t, int tokens) {
+  if (t.rows == t.rows_tokens * t.group) return (int)((uint32_t)(tokens + t.rows_tokens - 1) / (uint32_t)t.rows_tokens);
+  return (int)(((long long)tokens * t.group + t.rows - 1) >> (31 - __clz(t.rows)));
+}
+__device__ __forceinline__ int key_shift(const WindowView& t) { return 31 - __clz(t.keys); }
+__device__ __forceinline__ int tree_key_tiles(const WindowView& t, int keys) { return keys > 0 ? ((keys - 1) >> key_shift(t)) + 1 : 1; }
 
 // The place of new token j, at which its window ends and which a window has to reach for its key to be seen
 __device__ __forceinline__ int place_of(const WindowView& t, const CacheRequest& rq, int j) {
@@ -138,27 +148,32 @@ __device__ __forceinline__ int key_place(const WindowView& t, const CacheRequest
   return place < t.sinks ? 0x7fffffff : place;
 }
 // The tiles of keys that rows of some tokens may see: [0, sinks) and [first, end).  A unit's tiles are counted without the gap.
+// (t.keys is a power of two, and shifts serve: a unit begins with this in every role, and a division takes the one warp beside the busy ones a quarter of a microsecond.)
 struct TileRange {
   int sinks, first, end;
   __device__ __forceinline__ int at(int i) const { return i < sinks ? i : i - sinks + first; }
 };
 __device__ __forceinline__ bool is_chain(const WindowView& t) { return !t.positions && !t.a.spans; }
 __device__ __forceinline__ TileRange tile_range(const WindowView& t, const KeyRange& k, int token0, int token1) {   // tokens token0 .. token1
+  const int shift = key_shift(t);
   TileRange r;
   r.end = tree_key_tiles(t, k.keys);
-  r.sinks = min(r.end, t.sinks > 0 ? (t.sinks - 1) / t.keys + 1 : 0);
-  r.first = max(r.sinks, max(0, k.rq.cached + (is_chain(t) ? token0 : 0) - t.window + 1) / t.keys);
-  if (is_chain(t)) r.end = max(r.sinks, min(r.end, (k.rq.cached + token1) / t.keys + 1));
+  r.sinks = min(r.end, t.sinks > 0 ? ((t.sinks - 1) >> shift) + 1 : 0);
+  r.first = max(r.sinks, max(0, k.rq.cached + (is_chain(t) ? token0 : 0) - t.window + 1) >> shift);
+  if (is_chain(t)) r.end = max(r.sinks, min(r.end, (int)((uint32_t)(k.rq.cached + token1) >> shift) + 1));
   return r;
 }
+// What TileRange needs of the row tile's tokens is set by the host where t.rows and t.group are
+inline void set_tile_tokens(TreeView&) {}
+inline void set_tile_tokens(WindowView& t) { t.tile_tokens = (t.rows + t.group - 2) / t.group + 1; t.rows_tokens = t.rows / t.group; }
 // Tiles of a unit of this request: the most that a tile of its rows may see
 __device__ __forceinline__ int unit_tiles(const TreeView& t, const KeyRange& k) { return tree_key_tiles(t, k.keys); }
 __device__ __forceinline__ int unit_tiles(const WindowView& t, const KeyRange& k) {
   const TileRange r = tile_range(t, k, 0, k.rq.tokens - 1);
   const int all = r.sinks + max(0, tree_key_tiles(t, k.keys) - r.first);
   if (!is_chain(t)) return max(1, all);
-  const int tokens = (t.rows + t.group - 2) / t.group + 1;   // that a tile of rows may touch: its windows reach over window + tokens - 1 keys
-  return (int)max(1ll, min((long long)all, r.sinks + ((long long)t.window + tokens + t.keys - 3) / t.keys + 1));
+  const uint32_t reach = ((uint32_t)t.window + (uint32_t)(t.tile_tokens + t.keys - 3)) >> key_shift(t);   // its windows reach over window + tile_tokens - 1 keys
+  return (int)max(1u, min((uint32_t)all, r.sinks + reach + 1));
 }
 
 // Places in front of each request, in shared memory; without a split, units

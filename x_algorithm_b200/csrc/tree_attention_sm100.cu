@@ -139,7 +139,7 @@ struct TcBlock {
   // (8192 tokens that see themselves, 16 heads of 128: 716 us before the first, 577 before the second, 502 then.)
   __device__ __forceinline__ void produce(PieceWalk<DH, View> walk) {
     const int lane = threadIdx.x & 31, boxes = KT / box, page_size = t.c.page_size, v_off = t.c.num_kv_heads * page_size, page_rows = 2 * v_off;
-    const int no_row = (int)(t.c.num_pages * page_rows), tokens_per_tile = t.rows / t.group, cols_on = KT / page_size, slots_on = KT % page_size;
+    const int no_row = (int)(t.c.num_pages * page_rows), tokens_per_tile = rows_tokens(t), cols_on = KT / page_size, slots_on = KT % page_size;
     TreePiece pc, after;
     bool more = walk.next(&after);
     int j = 0;                                              // tiles of the block so far
@@ -313,8 +313,45 @@ struct TcBlock {
     }
   }
 
-  // ---- MMA issuer (one thread) -------------------------------------------------------------------------------------------
+  // Infinities and NaN among a masked tile's values: out of the product.  By THREADS threads, of which this is number `r`; piece: what sm.odd notes
+  template <int THREADS> __device__ __forceinline__ void take_out_odd(int buffer, int r, int piece) const {
+    uint4* const v = reinterpret_cast<uint4*>(sm.v[buffer]);
+    bool odd = false;
+    for (int i = r; i < (int)BLK / 16; i += THREADS) {
+      uint4 x = v[i];
+      if (odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w)) {
+        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { if (odd_value(w[k])) w[k] &= 0xffff0000u; if (odd_value(w[k] >> 16)) w[k] &= 0xffffu; }
+        v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        odd = true;
+      }
+    }
+    if (odd) sm.odd[piece & 1] = piece + 1;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  // The same by a warp, which looks first whether there is one: 0 x + 0 is NaN then
+  __device__ __forceinline__ void look_for_odd(int buffer, int piece) const {
+    const uint4* const v = reinterpret_cast<const uint4*>(sm.v[buffer]);
+    const int lane = threadIdx.x & 31;
+    const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
+    __nv_bfloat162 sum[4] = {zero, zero, zero, zero};
+#pragma unroll 8
+    for (int i = 0; i < (int)BLK / 512; ++i) {
+      const uint4 x = v[i * 32 + lane];
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] = __hfma2(zero, *reinterpret_cast<const __nv_bfloat162*>(&w[k]), sum[k]);
+    }
+    sum[0] = __hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3]));
+    if (__any_sync(0xffffffffu, odd_pair(*reinterpret_cast<const uint32_t*>(&sum[0])))) take_out_odd<32>(buffer, lane, piece);
+    __syncwarp();
+  }
+
+  // ---- MMA issuer (one thread; with a window a warp, which searches masked tiles' values while the softmax is at their logits) ---
   __device__ __forceinline__ void issue() {
+    const bool leader = !WINDOW || elect_one();
+    auto wait = [&](const uint64_t& bar, int phase) { const bool there = this->wait(bar, phase); return WINDOW ? __all_sync(0xffffffffu, there) != 0 : there; };
     constexpr uint32_t idesc_s = make_idesc(QT, KT), idesc_o = make_idesc_b_mn(QT, DCH * 64);
     int s_pieces = 0;                                       // pieces whose S has been begun
     bool s_first = true;
@@ -325,6 +362,8 @@ struct TcBlock {
       if (!wait(sm.k_full[b], j / NB)) return false;
       tc_fence_after();
       flags_next = sm.note[j & 7].flags;
+      s_first = flags_next & LAST;
+      if (!leader) return true;
 #pragma unroll
       for (int c = 0; c < DCH; ++c) {
         const uint64_t qd = make_smem_desc(smem_u32(sm.q) + c * SLAB), kd = make_smem_desc(smem_u32(sm.k[b]) + c * KT * 128);
@@ -333,7 +372,6 @@ struct TcBlock {
       }
       umma_commit(smem_u32(&sm.k_empty[b]));
       umma_commit(smem_u32(&sm.s_full[j & 1]));
-      s_first = flags_next & LAST;
       if (s_first) umma_commit(smem_u32(&sm.q_empty));
       return true;
     };
@@ -345,16 +383,21 @@ struct TcBlock {
       // the S buffer of the next tile was last read by the softmax whose P has been awaited below
       if (!(flags & FINAL) && !issue_s(j + 1)) return;
       const int b = j % NB;
-      if (!wait(sm.v_full[b], j / NB) || !wait(sm.p_ready, j)) return;
+      if (!wait(sm.v_full[b], j / NB)) return;
+      if constexpr (WINDOW) { if (flags & MASKED) look_for_odd(b, pieces); }
+      if (!wait(sm.p_ready, j)) return;
+      if (WINDOW && (flags & LAST) && leader) mbar_arrive(smem_u32(&sm.together));   // sm.odd has its piece's answer (the softmax is done with that of the piece before)
       if (first && pieces > 0 && !wait(sm.o_empty, pieces - 1)) return;   // the rows of the piece before have been read
       tc_fence_after();
+      if (leader) {
 #pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk) {
-        const uint64_t vd = make_smem_desc_mn(smem_u32(sm.v[b]) + kk * 16 * 128, KT * 128, 1024);
-        umma_ts(tmem + TM_O, tmem + TM_S + (j & 1) * KT + kk * 8, vd, idesc_o, !first || kk != 0);
+        for (int kk = 0; kk < KT / 16; ++kk) {
+          const uint64_t vd = make_smem_desc_mn(smem_u32(sm.v[b]) + kk * 16 * 128, KT * 128, 1024);
+          umma_ts(tmem + TM_O, tmem + TM_S + (j & 1) * KT + kk * 8, vd, idesc_o, !first || kk != 0);
+        }
+        umma_commit(smem_u32(&sm.v_empty[b]));
+        umma_commit(smem_u32(&sm.o_done));
       }
-      umma_commit(smem_u32(&sm.v_empty[b]));
-      umma_commit(smem_u32(&sm.o_done));
       first = flags & LAST;
       pieces += first;
       if (flags & FINAL) return;
@@ -449,7 +492,7 @@ struct TcBlock {
     bool valid_after = false;
     auto look = [&]() {
       kr_after = key_range(t.c, after.b);
-      const int token = after.row_tile * (t.rows / group) + token_of;
+      const int token = after.row_tile * rows_tokens(t) + token_of;
       valid_after = r < t.rows && token < kr_after.rq.tokens;
       pre_after = valid_after ? span_of(t, kr_after.rq, token).x : -1;
       if constexpr (WINDOW) behind_after = valid_after ? place_of(t, kr_after.rq, token) - t.window : 0;
@@ -460,7 +503,7 @@ struct TcBlock {
       pc = after;
       const KeyRange kr = kr_after;
       const CacheRequest& rq = kr.rq;
-      const int pre = pre_after, behind = behind_after, token = pc.row_tile * (t.rows / group) + token_of;
+      const int pre = pre_after, behind = behind_after, token = pc.row_tile * rows_tokens(t) + token_of;
       const bool valid = valid_after, busy = __any_sync(0xffffffffu, valid);   // a warp without rows only keeps the others company
       float m = valid ? -INFINITY : 0.f, l = 0.f;
       const int first = j;
@@ -475,36 +518,6 @@ struct TcBlock {
         }
         const NoteOf<View> note = sm.note[j & 7];
         const bool masked = note.flags & MASKED;
-        // Infinities and NaN among a masked tile's values: out of the product
-        auto take_out_odd = [&](bool look_first) {
-          if (!wait(sm.v_full[j % NB], j / NB)) return false;
-          uint4* const v = reinterpret_cast<uint4*>(sm.v[j % NB]);
-          if (look_first) {                                  // the largest size of all: neither infinite nor NaN, as a rule
-            __nv_bfloat162 most = __float2bfloat162_rn(0.f);
-#pragma unroll
-            for (int i = 0; i < (int)BLK / 2048; ++i) {
-              const uint4 x = v[i * 128 + r];
-              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) most = __hmax2_nan(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[k])));
-            }
-            if (!odd_pair(*reinterpret_cast<const uint32_t*>(&most))) return true;
-          }
-          bool odd = false;
-          for (int i = r; i < (int)BLK / 16; i += 128) {
-            uint4 x = v[i];
-            if (odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w)) {
-              uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) { if (odd_value(w[k])) w[k] &= 0xffff0000u; if (odd_value(w[k] >> 16)) w[k] &= 0xffffu; }
-              v[i] = make_uint4(w[0], w[1], w[2], w[3]);
-              odd = true;
-            }
-          }
-          if (odd) sm.odd[piece & 1] = piece + 1;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          return true;
-        };
         if (!WINDOW && masked) {                            // the same for all 128 threads
           if (r < KT) {
             const int key = note.tile * KT + r;
@@ -513,7 +526,8 @@ struct TcBlock {
             else if (key >= rq.cached) sp = span_of(t, rq, key - rq.cached);
             sm.span[j & 1][r] = sp;
           }
-          if (!take_out_odd(false)) return;
+          if (!wait(sm.v_full[j % NB], j / NB)) return;
+          take_out_odd<128>(j % NB, r, piece);
           mbar_arrive(smem_u32(&sm.together));              // a barrier of the softmax threads whose wait is bounded, too
           if (!wait(sm.together, together++)) return;
         }
@@ -612,7 +626,6 @@ struct TcBlock {
           tc_fence_before();
           l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
         }
-        if (WINDOW && masked && !take_out_odd(true)) return;    // no other thread's stores are read here: they are there with the arrival below
         // S of this tile did not wait for P V of the one before: its barrier must not run two phases ahead of the issuer
         if (j > first && !wait(sm.o_done, j - 1)) return;
         mbar_arrive(smem_u32(&sm.p_ready));
@@ -656,6 +669,7 @@ struct TcBlock {
       }
       // What the row sees of the infinities and NaN that were taken out of masked tiles, onto what has been stored.  (One of an unmasked tile is in there
       // already: adding it again changes nothing.)
+      if constexpr (WINDOW) { if (!wait(sm.together, piece)) return; }
       if (sm.odd[piece & 1] == piece + 1 && valid && !none) {
         TileRange range{0, 0, 0};
         if constexpr (WINDOW) range = tile_range(t, kr, pc.row_tile * (t.rows / group), min((pc.row_tile + 1) * (t.rows / group), rq.tokens) - 1);
@@ -696,7 +710,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) tree_tc_kernel(const __grid_con
     sm.odd[0] = sm.odd[1] = 0;
     prefetch_map(&map_q); prefetch_map(&map_kv);
     mbar_init(smem_u32(&sm.q_full), 1); mbar_init(smem_u32(&sm.q_empty), 1); mbar_init(smem_u32(&sm.p_ready), 128); mbar_init(smem_u32(&sm.o_done), 1);
-    mbar_init(smem_u32(&sm.o_empty), 128); mbar_init(smem_u32(&sm.together), 128);
+    mbar_init(smem_u32(&sm.o_empty), 128); mbar_init(smem_u32(&sm.together), has_window<View> ? 1 : 128);
     for (int i = 0; i < tc_buffers(DH); ++i) {
       mbar_init(smem_u32(&sm.k_full[i]), 1); mbar_init(smem_u32(&sm.k_empty[i]), 1);
       mbar_init(smem_u32(&sm.v_full[i]), 1); mbar_init(smem_u32(&sm.v_empty[i]), 1);
@@ -733,7 +747,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) tree_tc_kernel(const __grid_con
   } else if (warp == 1) {
     PieceWalk<DH, View> mine = walk;
     TreePiece pc;
-    if (mine.next(&pc) && elect_one()) block.issue();
+    if (mine.next(&pc) && (has_window<View> || elect_one())) block.issue();
   } else {
     block.softmax(walk);
   }
