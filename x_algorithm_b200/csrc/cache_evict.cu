@@ -105,11 +105,11 @@ struct ChunkMove {
 
 // ---- what stays ------------------------------------------------------------------------------------------------------------
 
-constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, SEL_BINS = 2048, SEL_COARSE = SEL_BINS / 32, SEL_RANKS = 8;
+constexpr int SEL_THREADS = 1024, SEL_FEW = 256, SEL_BINS = 2048, SEL_COARSE = SEL_BINS / 32, SEL_RANKS = 8;
 struct alignas(16) SelectSmem {
   uint32_t hist[3][SEL_BINS];
   uint32_t coarse[3][SEL_COARSE];        // sums of 32 bins
-  uint32_t warp_more[SEL_WARPS], warp_same[SEL_WARPS];
+  uint32_t warp_more[SEL_THREADS / 32], warp_same[SEL_THREADS / 32];
   uint32_t taken[2];                     // this block's heavier weights, and those equal to the smallest that stays
   uint32_t bin, above, in_bin;
 };
@@ -128,7 +128,9 @@ __device__ __forceinline__ uint32_t remote_u32(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-__global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictView t) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictView t) {
+  constexpr int WARPS = THREADS / 32;
   extern __shared__ __align__(16) uint8_t smem_bytes[];
   SelectSmem& sm = *reinterpret_cast<SelectSmem*>(smem_bytes);
   uint32_t* const held = reinterpret_cast<uint32_t*>(smem_bytes + sizeof(SelectSmem));
@@ -140,11 +142,11 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   if (t.alone && rank == 0 && h == 0 && tid == 0) t.a.lengths_out[b] = min(rq.length, t.a.budget);
   if (!t.alone && rank == 0) {                               // for the launch behind
     int* const read = t.read + ((long long)b * t.c.num_kv_heads + h) * t.chunks;
-    for (int i = tid; i < t.chunks; i += SEL_THREADS) read[i] = 0;
+    for (int i = tid; i < t.chunks; i += THREADS) read[i] = 0;
     if (b == 0 && h == 0 && tid == 0) *t.ticket = 0;
   }
   if (rq.length <= t.a.budget) {                             // the same for the whole cluster
-    for (int i = rank * SEL_THREADS + tid; i < t.a.budget; i += ranks * SEL_THREADS) kept[i] = i < rq.length ? i : -1;
+    for (int i = rank * THREADS + tid; i < t.a.budget; i += ranks * THREADS) kept[i] = i < rq.length ? i : -1;
     return;
   }
   const int* const table = t.c.block_table + (long long)b * t.c.table_stride;
@@ -155,16 +157,16 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
     return weight_order(t.a.weights[((long long)page * t.c.num_kv_heads + h) * t.c.page_size + key - col * t.c.page_size]);
   };
   const bool in_smem = per <= t.held;
-  for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) (&sm.hist[0][0])[i] = 0;
+  for (int i = tid; i < 3 * SEL_BINS; i += THREADS) (&sm.hist[0][0])[i] = 0;
   if (in_smem) {                                             // loads without a condition: a batch of pages, then of weights, on their way at once
     constexpr int BATCH = 4;
-    for (int i0 = tid; i0 < count; i0 += BATCH * SEL_THREADS) {
+    for (int i0 = tid; i0 < count; i0 += BATCH * THREADS) {
       int page[BATCH], slot[BATCH];
       float w[BATCH];
       bool bad = false;
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
-        const int key = from + min(i0 + k * SEL_THREADS, count - 1), col = page_column(t, key);
+        const int key = from + min(i0 + k * THREADS, count - 1), col = page_column(t, key);
         page[k] = table[col]; slot[k] = key - col * t.c.page_size;
       }
 #pragma unroll
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
         page[k] = good;
       }
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k) if (i0 + k * SEL_THREADS < count) held[i0 + k * SEL_THREADS] = page[k] ? weight_order(w[k]) : 0u;
+      for (int k = 0; k < BATCH; ++k) if (i0 + k * THREADS < count) held[i0 + k * THREADS] = page[k] ? weight_order(w[k]) : 0u;
       if (bad) cache_report(t.c, CACHE_BAD_PAGE);
     }
   }
@@ -189,12 +191,12 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   for (int pass = 0; pass < 3 && want > 0; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     uint32_t* const hist = sm.hist[pass];
-    for (int i = tid; i < count; i += SEL_THREADS) {
+    for (int i = tid; i < count; i += THREADS) {
       const uint32_t v = order_at(i);
       if (pass == 0 || (v >> (shift + bits)) == prefix) atomicAdd(&hist[(v >> shift) & ((1u << bits) - 1)], 1u);
     }
     __syncthreads();
-    for (int c = warp; c < SEL_COARSE; c += SEL_WARPS) {
+    for (int c = warp; c < SEL_COARSE; c += WARPS) {
       const uint32_t sum = __reduce_add_sync(0xffffffffu, hist[c * 32 + lane]);
       if (lane == 0) sm.coarse[pass][c] = sum;
     }
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   }
 
   // numbers of what stays: a warp's keys lie one behind the other, 32 at a time
-  const int seg = ((count + SEL_WARPS - 1) / SEL_WARPS + 31) & ~31, i0 = min(warp * seg, count), i1 = min(i0 + seg, count);
+  const int seg = ((count + WARPS - 1) / WARPS + 31) & ~31, i0 = min(warp * seg, count), i1 = min(i0 + seg, count);
   uint32_t more = 0, same = 0;
   for (int i = i0 + lane; i - lane < i1; i += 32) {
     const uint32_t v = i < i1 ? order_at(i) : 0;
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   __syncthreads();
   uint32_t more_before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_more[lane] : 0), same_before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_same[lane] : 0);
   if (ranks > 1) {
-    if (tid == SEL_THREADS - 32) { sm.taken[0] = more_before + more; sm.taken[1] = same_before + same; }   // the last warp
+    if (tid == THREADS - 32) { sm.taken[0] = more_before + more; sm.taken[1] = same_before + same; }   // the last warp
     cluster_sync_all();
     const bool in_front = lane < rank;
     more_before += __reduce_add_sync(0xffffffffu, in_front ? remote_u32(mapa_shared(smem_u32(&sm.taken[0]), in_front ? lane : 0)) : 0);
@@ -260,14 +262,14 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const EvictVi
   }
   // the first keys and the last ones
   const int recent = rq.length - rq.behind;
-  for (int i = rank * SEL_THREADS + tid; i < rq.sinks; i += ranks * SEL_THREADS) kept[i] = i;
-  for (int i = rank * SEL_THREADS + tid; i < recent; i += ranks * SEL_THREADS) kept[t.a.budget - recent + i] = rq.behind + i;
+  for (int i = rank * THREADS + tid; i < rq.sinks; i += ranks * THREADS) kept[i] = i;
+  for (int i = rank * THREADS + tid; i < recent; i += ranks * THREADS) kept[t.a.budget - recent + i] = rq.behind + i;
   if (ranks > 1) cluster_sync_all();                         // the others may still be reading this block's counts; the places that they wrote are there
   if (!t.alone || rank > 0) return;
   __syncthreads();
   if (kept[t.a.budget - 1] < t.a.budget) return;
-  ChunkMove<SEL_THREADS> move{t, *reinterpret_cast<ChunkPlaces*>(held), reinterpret_cast<uint8_t*>(held) + sizeof(ChunkPlaces), b, h, 0, t.a.budget, t.c.key_size / 8};
-  for (int i = tid; i < t.a.budget; i += SEL_THREADS) move.place(i, kept[i], table[page_column(t, i)], table[page_column(t, kept[i])]);
+  ChunkMove<THREADS> move{t, *reinterpret_cast<ChunkPlaces*>(held), reinterpret_cast<uint8_t*>(held) + sizeof(ChunkPlaces), b, h, 0, t.a.budget, t.c.key_size / 8};
+  for (int i = tid; i < t.a.budget; i += THREADS) move.place(i, kept[i], table[page_column(t, i)], table[page_column(t, kept[i])]);
   __syncthreads();
   move.fetch();
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -394,19 +396,23 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
   const long long move_bytes = (long long)sizeof(ChunkPlaces) + (long long)t.a.budget * 4 * t.c.key_size;
   t.alone = t.a.budget <= 256 && move_bytes <= 68 * 1024 && (t.a.lengths_out + t.c.batch <= t.c.lengths || t.c.lengths + t.c.batch <= t.a.lengths_out);
   if (t.alone && t.held * 4 < move_bytes) t.held = (int)((move_bytes + 3) / 4);
+  // More blocks than SMs, of up to 4096 keys each: small ones, four or five an SM (832 heads of 67 keys: 15 us, 40 by blocks of 1024; 1024 of 3000: 134 and 157, with the
+  // move; 512 of 8000: 246 and 241, of 20 k: 431 and 403; 32 of 300 alike)
+  const bool few = heads * ranks > device_sms() && per <= 4096;
   const int select_smem = (int)sizeof(SelectSmem) + t.held * 4;
-  static SmemLimit select_limit;
+  static SmemLimit select_limit, few_limit;
   std::string err;
   auto launch = [&]() -> phx_status {
-    PHX_CUDA_TRY(select_limit.raise(evict_select_kernel, (int)sizeof(SelectSmem) + MOST_HELD * 4), err);
+    PHX_CUDA_TRY(select_limit.raise(evict_select_kernel<SEL_THREADS>, (int)sizeof(SelectSmem) + MOST_HELD * 4), err);
+    PHX_CUDA_TRY(few_limit.raise(evict_select_kernel<SEL_FEW>, (int)sizeof(SelectSmem) + MOST_HELD * 4), err);
     cudaLaunchConfig_t lc;
     memset(&lc, 0, sizeof(lc));
-    lc.gridDim = dim3(ranks, t.c.num_kv_heads, t.c.batch); lc.blockDim = dim3(SEL_THREADS); lc.dynamicSmemBytes = select_smem; lc.stream = st;
+    lc.gridDim = dim3(ranks, t.c.num_kv_heads, t.c.batch); lc.blockDim = dim3(few ? SEL_FEW : SEL_THREADS); lc.dynamicSmemBytes = select_smem; lc.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = ranks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     lc.attrs = at; lc.numAttrs = 1;
-    PHX_CUDA_TRY(cudaLaunchKernelEx(&lc, evict_select_kernel, t), err);
+    PHX_CUDA_TRY(few ? cudaLaunchKernelEx(&lc, evict_select_kernel<SEL_FEW>, t) : cudaLaunchKernelEx(&lc, evict_select_kernel<SEL_THREADS>, t), err);
     if (!t.alone) PHX_CUDA_TRY(launch_programmatic(evict_move_kernel, dim3((unsigned)(heads * t.chunks)), dim3(MOVE_THREADS), 0, st, t), err);
     dispatch_note(DK_CACHE_EVICT);
     return PHX_OK;
