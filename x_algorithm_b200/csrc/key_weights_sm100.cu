@@ -10,7 +10,9 @@
 //               key of the warp is not seen by some of the rows; at the unit's end the groups hand their sums to the first, which writes the weight (or a part, where chunks of rows
 //               are joined by key_weights_join_kernel)
 // (All of that in one kernel, by a planner warp and four that described rows, was slower: such code runs at 10 cycles an instruction, by one warp beside sixteen, and the block waited for it.
-// 32 x 512 candidates over up to 1022 keys, 8 heads of 64: 62 us; 8 x 1022 tokens that see themselves, 16 heads of 128: 66 us.)
+// 32 x 512 candidates over up to 1022 keys, 8 heads of 64: 62 us; 8 x 1022 tokens that see themselves, 16 heads of 128: 66 us.  Now 60 and 61, the plan, of 9 us, included, of which some
+// lies under the tail of what is in front; without the sums 39.)  Bound by the sums' chains: tensor memory, multiply-add, exponential, add (special-function unit 41 and 64 %, issue 44 and 48 %).
+// Sets of 32 columns for 16, in twice the registers and half the warps: 68; a polynomial for an eighth to a half of the exponentials: 62 to 67; loops unrolled over the tiles: 76 and 88.
 // Waits are bounded; when one runs out the flag is raised, every later wait of any role fails at once, and a role whose wait failed is done.
 #include <string.h>
 

@@ -14,6 +14,10 @@
 // Bound by memory: 16 operations a byte of the cache, padded rows counted.  96 single tokens over up to 4096 keys, 4 key heads of 128 (382 MB), take 75 us = 5.1 TB/s, 138 us =
 // 5.8 TB/s where all have 4096.  Two stages a warp and three blocks an SM against three and two: 75 / 78 us for the first, 138 / 137 for the second, 89 / 104 for
 // 400 tokens over up to 1000 keys.
+//
+// With a window (phx_window_attention_device) j also has to be one of the first keys or to stand behind i's place - window, and ln sum_j e^x_ij is stored; the kernels are the
+// same, compiled for a WindowView.  Tiles are counted without the gap between the first keys and the window (TileRange), so a unit is as long as what its rows see, and pages in the gap
+// are not looked up.  96 single tokens, windows of 2048 behind up to 16384 keys, 4 key heads of 128 (410 MB): 78 us = 5.2 TB/s.
 #include <math.h>
 
 #include <string>

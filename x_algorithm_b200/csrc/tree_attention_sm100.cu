@@ -15,6 +15,12 @@
 // Measured: 8192 tokens that see themselves, 16 heads of 128, 506 us = 1086 TFLOP/s (bound by a tile's chain of load, maximum, exponentials and store, 1800
 // cycles of two blocks in turns, and by the special-function unit, 1024 of them); 24 trees of 32 over up to 8192 keys, 32 heads of 128 (465 MB), 100 us = 4.6 TB/s,
 // with capped logits 106; 74 such trees over 8192 keys each 405 us = 6.2 TB/s.
+// With a window what a row sees of a masked tile is two words: of the cached keys, and of a chain's, a stretch and the first ones, worked out from four numbers; of new keys with
+// spans what the producer has laid beside the tile's note.  No barrier of the softmax threads is needed then, and the values are searched by the issuer's warp while the softmax is at the
+// logits.  Measured (us): 4 x 2048 tokens in a chain, window 1024, 16 heads on 4 of 128: 122; 24 trees of 32, windows of 4096, 32 heads on 8 of 128, capped: 109; 32 x 512 candidates, window 512, 8
+// heads of 64: 82 - with the search by the softmax threads 120, 107, 88 (37 x 512 tokens in a chain, 8 heads of 64: 78, 75 by the issuer's warp); with spans compared key by key behind a barrier 152
+// and 101 for the first and the third.  Divisions by a tile's keys in PieceWalk, which every role does for every unit, cost 6, 7 and 6 us.
+// Heads of 32 (with a window) are tiles of 64 columns whose second half is zeros behind the tensors' edge; products take half the steps.
 #include <string.h>
 
 #include "sm100_ptx.cuh"
