@@ -179,13 +179,20 @@ struct TcBlock {
       auto ask_page = [&]() { page = keys > 0 ? kr.table[min(col, last_col)] : -1; };
       look_up(begin);
       ask_page();
-      if (piece > 0 && !wait(sm.q_empty, piece - 1)) return;
-      __syncwarp();
-      if (elect_one()) {
-        mbar_expect_tx(smem_u32(&sm.q_full), DCH * t.rows * 128);
-        for (int c = 0; c < DCH; ++c) tma_load_3d(smem_u32(sm.q) + c * SLAB, &map_q, smem_u32(&sm.q_full), c * 64, pc.h * t.group, rq.row0 + token0);
-      }
-      __syncwarp();
+      auto queries = [&]() {
+        if (piece > 0 && !wait(sm.q_empty, piece - 1)) return false;
+        __syncwarp();
+        if (elect_one()) {
+          mbar_expect_tx(smem_u32(&sm.q_full), DCH * t.rows * 128);
+          for (int c = 0; c < DCH; ++c) tma_load_3d(smem_u32(sm.q) + c * SLAB, &map_q, smem_u32(&sm.q_full), c * 64, pc.h * t.group, rq.row0 + token0);
+        }
+        __syncwarp();
+        return true;
+      };
+      // With four buffers the producer is here before the last S of the piece before has been multiplied, and looks things up first: 37 x 512 tokens, 8 heads, window 64, 42.5 -> 41.2 us; with two
+      // buffers it is late, and Q goes first (128 columns 58.6, 60.3 the other way).
+      constexpr bool Q_LATE = WINDOW && NB > 2;
+      if (!Q_LATE && !queries()) return;
       // the places that the block's rows take, once a tile of new keys asks for them
       int lo = 0x7fffffff, hi = -2;
       auto places = [&]() {
@@ -258,6 +265,7 @@ struct TcBlock {
         __syncwarp();
         return true;
       };
+      if (Q_LATE && !queries()) return;
       for (int first = j;; ++j) {                            // K runs a tile ahead of V
         bool in_keys = lane < boxes && tile * KT + lane * box < keys;
         // a box that no row's window reaches and no first key lies in: its page may be another request's by now
