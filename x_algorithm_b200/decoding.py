@@ -272,8 +272,8 @@ def _space(workspace, kept, device: int, stream: int):
     return kept.space or _take_space(kept, device)
 
 
-def _queries(q, cache_dh: int, cap: float, cap_method: Optional[str]):
-    if cache_dh != q.shape[2] or (q.shape[1] > 1 and q.stride(1) != cache_dh):
+def _queries(q, heads: int, dh: int, cache_dh: int, cap: float, cap_method: Optional[str]):
+    if cache_dh != dh or (heads > 1 and q.stride(1) != dh):
         raise ValueError("q must have the cache's head dim, its heads side by side")
     if cap_method not in CAP_METHODS:
         raise ValueError(f"cap_method must be one of {list(CAP_METHODS)}")
@@ -289,15 +289,16 @@ def window_attention(q, pages, q_start, lengths, block_table, spans=None, positi
     depth), by default lengths + i in a chain and lengths for tokens with spans.  Pages between the first keys and a window are not read.  Returns (bf16 [N, heads,
     head dim], the logits' ln sum exp fp32 [N, heads], -inf where a token sees nothing)."""
     device = _rows(q, "q", _BF16, 3)
-    if _elsewhere(device, stream):
+    if stream is not None and _elsewhere(device, stream):
         with _under(device, stream):
             return window_attention(q, pages, q_start, lengths, block_table, spans, positions, window=window, sinks=sinks, sm_scale=sm_scale, cap=cap, cap_method=cap_method,
                                     max_tokens=max_tokens, max_keys=max_keys, out=out, lse=lse, workspace=workspace)
     n, heads, dh = shape = q.shape
-    stream = _stream(device, stream)
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(device)
     kept, mine = _keep(device, stream), _structs
     _, page_size, cache_dh, cols = _batch(mine.batch, pages, q_start, lengths, block_table, n, device, kept)
-    _queries(q, cache_dh, cap, cap_method)
+    _queries(q, heads, dh, cache_dh, cap, cap_method)
     spans, positions, window, sinks = _seen(spans, positions, window, sinks, n, device)
     if out is None:
         out = torch.empty_strided(shape, (heads * dh, dh, 1), dtype=_BF16, device=q.device)
@@ -321,15 +322,16 @@ def key_weights(q, pages, q_start, lengths, block_table, lse, weights, spans=Non
     kv heads, page size], in place: decay * weight + sum for cached keys, the sum alone for new ones.  lse fp32 [N, heads] is what `window_attention` gave for the same
     queries, spans, positions, window, sinks, scale and cap (a row with an infinite one adds nothing).  Returns weights."""
     device = _rows(q, "q", _BF16, 3)
-    if _elsewhere(device, stream):
+    if stream is not None and _elsewhere(device, stream):
         with _under(device, stream):
             return key_weights(q, pages, q_start, lengths, block_table, lse, weights, spans, positions, window=window, sinks=sinks, sm_scale=sm_scale, cap=cap,
                                cap_method=cap_method, decay=decay, max_tokens=max_tokens, max_keys=max_keys, workspace=workspace)
     n, heads, dh = q.shape
-    stream = _stream(device, stream)
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(device)
     kept, mine = _keep(device, stream), _structs
     kv_heads, page_size, cache_dh, cols = _batch(mine.batch, pages, q_start, lengths, block_table, n, device, kept)
-    _queries(q, cache_dh, cap, cap_method)
+    _queries(q, heads, dh, cache_dh, cap, cap_method)
     spans, positions, window, sinks = _seen(spans, positions, window, sinks, n, device)
     lse_ptr = _need(lse, "lse", _F32, (n, heads), device)
     weights_ptr = _need(weights, "weights", _F32, (pages.shape[0], kv_heads, page_size), device)
@@ -348,16 +350,17 @@ def evict(weights, pages, lengths, block_table, *, budget: int, sinks: int = 0, 
     places that the kept keys had, ascending, int32 [B, kv heads, budget], -1 behind the last of a shorter request).  lengths_out may be `lengths`.  A page may stand
     once in the rows of the call, as one request's; the pages behind a request's new length are the caller's to hand out."""
     device = _rows(weights, "weights", _F32, 3)
-    if _elsewhere(device, stream):
+    if stream is not None and _elsewhere(device, stream):
         with _under(device, stream):
             return evict(weights, pages, lengths, block_table, budget=budget, sinks=sinks, recent=recent, max_keys=max_keys, lengths_out=lengths_out, kept=kept, workspace=workspace)
-    stream = _stream(device, stream)
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(device)
     state, mine = _keep(device, stream), _structs
     kv_heads, page_size, _, cols = _batch(mine.batch, pages, _NO_ROWS, lengths, block_table, 0, device, state)
     _need(weights, "weights", _F32, (pages.shape[0], kv_heads, page_size), device)
     if not (1 <= budget <= 2**30 and sinks >= 0 and recent >= 0 and sinks + recent <= budget):
         raise ValueError("budget must be 1 to 2^30 and hold sinks + recent keys")
-    batch = block_table.shape[0]
+    batch = lengths.numel()
     if lengths_out is None:
         lengths_out = torch.empty_strided((batch,), (1,), dtype=_I32, device=weights.device)
     else:
