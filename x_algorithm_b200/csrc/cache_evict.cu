@@ -8,7 +8,7 @@
 // places is taken by that chunk or one before it, by two at most: it is no more than fills one.  Chunks are handed out in order, by a counter, so a block only waits for blocks that
 // have begun, and whose reads wait for nothing.
 // Measured (us, keys that leave for the first time): 64 x 4 heads of up to 4096 keys of 128, half of them stay (338 MB read and written): select 19, move 66 = 5.1 TB/s; 2 x 4 heads of 100 k keys, a third
-// stays: 25 and 56 (221 MB, 3.9 TB/s, by 4096 blocks that wait for one another's reads).  With a wait for all chunks in front the second took 73 for its move where 61 were left with two; blocks that went through a head's places from front to
+// stays: 25 and 56 (221 MB, 3.9 TB/s, by 3280 blocks that wait for one another's reads).  With a wait for all chunks in front the second took 73 for its move where 61 were left with two; blocks that went through a head's places from front to
 // back by themselves took 247 for the second and 89 for the first.
 #include <string>
 
@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictView t
 
 // ---- moving together ---------------------------------------------------------------------------------------------------------
 
-constexpr int MOVE_THREADS = 256, MOVE_BYTES = 32 * 1024;   // of a chunk's keys and values
+// Bytes of a chunk's keys and values: 16, 24, 32, 40 KB, of rows of 128, 64 x 4 heads of 4096 keys 90, 82, 80, 80 us, 2 x 4 of 100 k 89, 88, 83, 81 (with the select)
+constexpr int MOVE_THREADS = 256, MOVE_BYTES = 40 * 1024;
 
 // Bounded wait until the n words at p are set, by all threads; false when the limit ran out or another wait's did.  Every thread comes out with the same answer.
 __device__ __forceinline__ bool wait_all_set(const int* p, int n, volatile int* status) {
@@ -376,7 +377,8 @@ extern "C" phx_status phx_evict_device(int32_t device, const phx_cache_batch* ca
   const int e = t.c.page_size / 16;
   t.page_magic = ((1ull << 36) + e - 1) / e;
   const long long heads = (long long)t.c.batch * t.c.num_kv_heads;
-  t.rows = MOVE_BYTES / (4 * t.c.key_size);                   // 64 to 256
+  t.rows = MOVE_BYTES / (4 * t.c.key_size);                   // 80, 160,
+  if (t.rows > MOVE_THREADS) t.rows = MOVE_THREADS;           // and of heads of 32 one a thread
   t.chunks = (int)(((long long)t.a.budget + t.rows - 1) / t.rows);
   if (heads * t.chunks > 2147483647ll) return bad("budget x heads x batch is too large");
   if (t.a.workspace_bytes < 16 + heads * t.chunks * 4) return bad("workspace is smaller than phx_tree_workspace_bytes or too small for this many heads and budget");
