@@ -863,7 +863,8 @@ phx_status phx_window_attention_device(int32_t device, const phx_cache_batch* ca
  * [num_tokens][num_q_heads] as phx_window_attention_device gave it.  A cached key's weights[page][kv head][slot] becomes decay * weight + sum, a new one's
  * (behind lengths[b]) the sum: nothing has to be cleared when a page is handed out.  Places of no key are left as they are.  A page that receives weights stands once in the
  * call's tables.  A row whose lse is infinite adds
- * nothing: -inf is a row that saw nothing, +inf leaves a row out.  With decay 1 the keys that no window reaches keep their weights, and pages that the attention does not read are not touched; any other decay looks all pages up.  The order of
+ * nothing: -inf is a row that saw nothing, +inf leaves a row out.  Cached weights fade whether or not a request, or the whole call, has new tokens (without any, q and lse are not
+ * read; the cache block's arrays are).  With decay 1 the keys that no window reaches keep their weights, and pages that the attention does not read are not touched; any other decay looks all pages up.  The order of
  * every sum follows from the sizes alone.  max_tokens and max_keys choose kernels and launch sizes only, as above.  workspace: phx_tree_workspace_bytes, not shared by
  * calls that may overlap.  Asynchronous on `stream`. */
 typedef struct phx_key_weights_args {

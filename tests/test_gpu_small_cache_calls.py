@@ -1,0 +1,70 @@
+"""Key weights, window attention and eviction in calls that are seldom made: no new token in the whole call, a table that is too short for a request's keys, threads that share a stream.
+Checks and tolerances are those of test_gpu_small_cache."""
+import pytest
+import torch
+
+from test_gpu_small_cache import DEV, close, make_case, plain, plain_weights
+
+pytestmark = pytest.mark.gpu
+IDS = lambda s: "-".join(map(str, s))  # noqa: E731
+
+
+def args_of(c):
+    return c["q"], c["pages"], c["q_start"], c["lengths"], c["table"]
+
+
+@pytest.mark.parametrize("shape", [
+    # batch, cached, heads, kv heads, head dim, page
+    (3, 300, 16, 4, 64, 32),
+    (1, 1, 8, 8, 64, 16),
+    (4, 700, 32, 1, 128, 48),
+    (2, 90, 4, 4, 32, 16),
+], ids=IDS)
+@pytest.mark.parametrize("decay", [0.5, 0.0, 1.0])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (20, 3)])
+def test_weights_fade_without_new_tokens(shape, decay, window, sinks):
+    from x_algorithm_b200 import decoding
+    batch, cached, heads, kv_heads, dh, page = shape
+    c = make_case(batch, 0, cached, heads, kv_heads, dh, page, "chain", seed=81)
+    lse = torch.zeros((0, heads), device=DEV)
+    want, tol = plain_weights(c, lse, window, sinks, decay=decay)
+    for hints in ({}, dict(max_tokens=100, max_keys=1)):
+        got = decoding.key_weights(*args_of(c), lse, c["weights"].clone(), window=window, sinks=sinks, decay=decay, **hints)
+        close(got, want, tol, f"weights, {hints}")
+    decoding.check_status()
+
+
+@pytest.mark.parametrize("tokens", [2, 60])
+def test_weights_fade_alike_beside_a_request_with_tokens(tokens):
+    """The weights of a request without tokens are the same in a call of its own."""
+    from x_algorithm_b200 import decoding
+    c = make_case(2, tokens, 400, 16, 4, 64, 32, "chain", seed=82, ragged=False)
+    c["q"], c["n_new"] = c["q"][tokens:], [0, tokens]
+    c["q_start"] = torch.tensor([0, 0, tokens], dtype=torch.int32, device=DEV)
+    lse = plain(c, None, 0)[1].float()
+    want, tol = plain_weights(c, lse, None, 0, decay=0.75)
+    both = decoding.key_weights(*args_of(c), lse, c["weights"].clone(), decay=0.75)
+    close(both, want, tol, "weights of both")
+    alone = decoding.key_weights(c["q"][:0], c["pages"], c["q_start"][:2], c["lengths"][:1], c["table"][:1], lse[:0], c["weights"].clone(), decay=0.75)
+    mine = c["table"][0, :-(-400 // c["page"])].long()
+    assert torch.equal(alone[mine], both[mine])
+    decoding.check_status()
+
+
+def test_bad_pages_and_lengths_are_reported_without_new_tokens():
+    from x_algorithm_b200 import PhoenixError, decoding
+    c = make_case(2, 0, 200, 8, 4, 64, 16, "chain", seed=83, ragged=False)
+    lse = torch.zeros((0, 8), device=DEV)
+    full, tol = plain_weights(c, lse, None, 0, decay=0.5)
+    bad = c["table"].clone()
+    bad[1, 3] = c["pages"].shape[0]
+    got = decoding.key_weights(c["q"], c["pages"], c["q_start"], c["lengths"], bad, lse, c["weights"].clone(), decay=0.5)
+    with pytest.raises(PhoenixError):
+        decoding.check_status()
+    lost = c["table"][1, 3].long()
+    full[lost] = c["weights"][lost].double()
+    close(got, full, tol, "weights")
+    c["lengths"][0] = -1
+    decoding.key_weights(*args_of(c), lse, c["weights"].clone(), decay=0.5)
+    with pytest.raises(PhoenixError):
+        decoding.check_status()

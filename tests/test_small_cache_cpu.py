@@ -186,3 +186,17 @@ def test_shrinking_needs_weights(host):
 def test_a_budget_that_a_grid_would_count_past_is_refused(budget):
     f, a = _evict(budget=budget)
     assert f(0, C.byref(_cache()), C.byref(a), None) == 1 and b"2^30" in _lib.lib.phx_global_error()
+
+
+def test_fading_weights_are_asked_for_without_new_tokens_too():
+    """With a decay cached weights change in a call without tokens: what such a call reads has to be there, and its queries need not."""
+    f, a = _weights(decay=0.5, q=None, lse=None)
+    for wrong in (dict(lengths=None), dict(q_start=None), dict(block_table=None), dict(table_stride=3), dict(pages=8), dict(table_cols=2 ** 30), dict(num_pages=2 ** 40)):
+        assert f(0, C.byref(_cache(num_tokens=0, **wrong)), C.byref(a), None) == 1, wrong
+        assert b"phx_key_weights_device" in _lib.lib.phx_global_error()
+    for kw in (dict(weights=None), dict(decay=float("nan")), dict(max_keys=-1)):
+        f, a = _weights(**{"decay": 0.5, **kw})
+        assert f(0, C.byref(_cache(num_tokens=0)), C.byref(a), None) == 1, kw
+    f, a = _weights(decay=0.5)
+    for empty in (dict(batch=0), dict(num_pages=0), dict(table_cols=0)):
+        assert f(0, C.byref(_cache(num_tokens=0, **empty)), C.byref(a), None) == 0, empty

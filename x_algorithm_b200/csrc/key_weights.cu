@@ -224,11 +224,15 @@ using namespace phx;
 
 extern "C" phx_status phx_key_weights_device(int32_t device, const phx_cache_batch* cache, const phx_key_weights_args* args, void* stream) {
   auto bad = [](const char* m) { set_global_error(std::string("phx_key_weights_device: ") + m); return PHX_E_ARG; };
-  const char* what = cache_check(cache);
-  if (*what) return bad(what);
-  if (!args) return bad("null argument");
+  if (!cache || !args) return bad("null argument");
   WeightsView t;
   t.c = *cache;
+  // Without new tokens cached weights fade all the same, so such a call is asked for all that it reads, too
+  const bool fades = args->decay != 1.0f;
+  if (fades && t.c.num_tokens == 0) t.c.num_tokens = 1;
+  const char* what = cache_check(&t.c);
+  t.c.num_tokens = cache->num_tokens;
+  if (*what) return bad(what);
   t.a.q = args->q; t.a.q_stride = args->q_stride; t.a.spans = args->spans; t.a.out = nullptr; t.a.workspace = args->workspace; t.a.workspace_bytes = args->workspace_bytes;
   t.a.max_keys = args->max_keys; t.a.max_tokens = args->max_tokens; t.a.num_q_heads = args->num_q_heads;
   t.a.sm_scale = args->sm_scale; t.a.cap = args->cap; t.a.cap_method = args->cap_method;
@@ -243,12 +247,12 @@ extern "C" phx_status phx_key_weights_device(int32_t device, const phx_cache_bat
   if (t.c.batch > 65535) return bad("at most 65535 requests");
   if (t.a.q_stride < (long long)t.a.num_q_heads * t.c.key_size || t.a.q_stride % 8 != 0) return bad("q_stride must be a multiple of 8 and cover a token's heads");
   if (t.a.max_tokens < 0 || t.a.max_keys < 0) return bad("negative size");
-  if (t.c.batch == 0 || t.c.num_tokens == 0) return PHX_OK;
+  if (t.c.batch == 0 || (t.c.num_tokens == 0 && (!fades || t.c.num_pages == 0))) return PHX_OK;
   if (t.a.max_tokens < 1) t.a.max_tokens = 1;
   if (t.a.max_tokens > t.c.num_tokens) t.a.max_tokens = t.c.num_tokens;
   if ((long long)t.c.num_tokens * t.a.num_q_heads > 2147483647ll) return bad("num_tokens x num_q_heads must fit 31 bits");
-  if (!t.a.q || !aligned16(t.a.q)) return bad("q must be a 16-byte aligned buffer");
-  if (!t.lse || !t.weights) return bad("lse and weights are required");
+  if (t.c.num_tokens > 0 && (!t.a.q || !aligned16(t.a.q))) return bad("q must be a 16-byte aligned buffer");
+  if ((t.c.num_tokens > 0 && !t.lse) || !t.weights) return bad("lse and weights are required");
   if (t.a.workspace_bytes < 0 || (t.a.workspace_bytes > 0 && (!t.a.workspace || !aligned16(t.a.workspace)))) return bad("workspace must be a 16-byte aligned buffer");
   if ((reinterpret_cast<uintptr_t>(t.a.spans) & 7) != 0) return bad("spans must be 8-byte aligned");
   if (t.c.num_pages == 0) return bad("an empty pool has no keys");

@@ -496,9 +496,9 @@ long long units_bound(const WeightsView& t) { return ((long long)t.c.table_cols 
 }  // namespace
 
 // Up to 16 rows a key head the mma.sync kernel reads the keys once, as fast as they come.  What is written down about rows (13 bytes each) and one request's keys has to fit three quarters of the
-// workspace, some two million rows and 100 thousand tiles of keys; calls beyond that stay with it, too.
+// workspace, some two million rows and 100 thousand tiles of keys; calls beyond that stay with it, too, as do those without new tokens, which have no queries to copy.
 bool weights_tc_supported(const WeightsView& t) {
-  if (t.group > HT || (long long)t.a.max_tokens * t.group <= 16) return false;
+  if (t.c.num_tokens == 0 || t.group > HT || (long long)t.a.max_tokens * t.group <= 16) return false;
   return UNITS_AT + row_tiles_bound(t, t.c.batch < TREE_MAX_SPLIT_BATCH ? t.c.batch : TREE_MAX_SPLIT_BATCH) * (long long)sizeof(RowNote) + units_bound(t) * (long long)sizeof(UnitNote) <= t.a.workspace_bytes / 4 * 3;
 }
 
