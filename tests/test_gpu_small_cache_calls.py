@@ -68,3 +68,36 @@ def test_bad_pages_and_lengths_are_reported_without_new_tokens():
     decoding.key_weights(*args_of(c), lse, c["weights"].clone(), decay=0.5)
     with pytest.raises(PhoenixError):
         decoding.check_status()
+
+
+@pytest.mark.parametrize("tokens", [3, 70])
+@pytest.mark.parametrize("window,sinks", [(100, 0), (100, 4), (None, 0)])
+@pytest.mark.parametrize("decay", [1.0, 0.5])
+def test_keys_behind_the_table_are_reported_by_the_weights(tokens, window, sinks, decay):
+    """A table without columns for a request's last keys: they get no weight, and the call says so, whichever kernel takes it."""
+    from x_algorithm_b200 import PhoenixError, decoding
+    from x_algorithm_b200.engine import dispatch_counts
+    c = make_case(2, tokens, 512, 16, 4, 128, 16, "chain", seed=84, ragged=False, extra_cols=0)
+    lse = plain(c, window, sinks)[1].float()
+    want, tol = plain_weights(c, lse, window, sinks, decay=decay)
+    cols = 512 // 16
+    for b in range(2):                                        # pages behind the last column: as they were
+        lost = c["table"][b, cols:].long()
+        want[lost] = c["weights"][lost].double()
+    before = dispatch_counts()["key_weights.tcgen05"]
+    got = decoding.key_weights(*args_of(c)[:4], c["table"][:, :cols], lse, c["weights"].clone(), window=window, sinks=sinks, decay=decay, max_tokens=tokens)
+    assert (dispatch_counts()["key_weights.tcgen05"] > before) == (tokens == 70)
+    with pytest.raises(PhoenixError):
+        decoding.check_status()
+    close(got, want, tol, "weights")
+
+
+@pytest.mark.parametrize("tokens", [3, 70])
+def test_a_table_without_columns_is_reported_by_the_weights(tokens):
+    from x_algorithm_b200 import PhoenixError, decoding
+    c = make_case(2, tokens, 0, 16, 4, 64, 16, "chain", seed=85, ragged=False)
+    lse, before = torch.zeros((2 * tokens, 16), device=DEV), c["weights"].clone()
+    decoding.key_weights(*args_of(c)[:4], c["table"][:, :0], lse, c["weights"], decay=0.5)
+    with pytest.raises(PhoenixError):
+        decoding.check_status()
+    assert torch.equal(c["weights"], before)

@@ -257,9 +257,9 @@ extern "C" phx_status phx_key_weights_device(int32_t device, const phx_cache_bat
   if ((reinterpret_cast<uintptr_t>(t.a.spans) & 7) != 0) return bad("spans must be 8-byte aligned");
   if (t.c.num_pages == 0) return bad("an empty pool has no keys");
   const long long columns = (long long)t.c.table_cols * t.c.page_size;
-  if (columns == 0) return PHX_OK;
-  if (t.a.max_keys < 1) t.a.max_keys = 1;
+  if (columns == 0 && t.c.num_tokens == 0) return PHX_OK;
   if (t.a.max_keys > columns) t.a.max_keys = columns;
+  if (t.a.max_keys < 1) t.a.max_keys = 1;                      // no column at all: a block that reports it
   t.csc = t.a.sm_scale * TREE_LOG2E;
   t.group = t.a.num_q_heads / t.c.num_kv_heads;
   DeviceScope scope(device);

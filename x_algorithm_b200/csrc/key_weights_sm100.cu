@@ -91,7 +91,6 @@ __device__ void plan_unit(const WeightsView& t, int box, int chunks, int pos, co
   if (lane < boxes && key < k.keys && (t.decay != 1.0f || key + box - 1 > rq.cached - t.window || key < t.sinks)) page = k.table[col];
   const bool there = (unsigned)page < (unsigned)t.c.num_pages;
   if (page != -2 && !there) cache_report(t.c, CACHE_BAD_PAGE);
-  if (lane == 0 && key0 == 0 && h == 0 && chunk == 0 && k.keys < (long long)rq.cached + rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);
   // its tiles of rows.  In a chain those in front of the keys, and those whose windows lie behind them, are not looked at.
   const int tiles = row_tiles_of(t, k), per = ((tiles + chunks - 1) / chunks + 1) & ~1;
   int begin = min(chunk * per, tiles), end = min(begin + per, tiles);
@@ -175,8 +174,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) key_weights_plan_kernel(const We
   const long long rows_at = UNITS_AT + all_units * chunks * (long long)sizeof(UnitNote), notes = all_units * chunks + all_tiles;
   if (blockIdx.x == 0) {
     if (threadIdx.x == 0) *reinterpret_cast<Head*>(space) = Head{all_units, rows_at, rows_at + all_tiles * (long long)sizeof(RowNote), chunks, 0};
-    for (int b = threadIdx.x; b < t.c.batch; b += PLAN_THREADS)
-      if (!cache_request(t.c, b).ok) cache_report(t.c, CACHE_BAD_OFFSETS);
+    for (int b = threadIdx.x; b < t.c.batch; b += PLAN_THREADS) {
+      const KeyRange k = key_range(t.c, b);
+      if (!k.rq.ok) cache_report(t.c, CACHE_BAD_OFFSETS);
+      if (k.keys < (long long)k.rq.cached + k.rq.tokens) cache_report(t.c, CACHE_BAD_PAGE);   // of a request, not of a unit: no unit need hold its first key
+    }
   }
   for (long long i = blockIdx.x * (PLAN_THREADS / 32) + (threadIdx.x >> 5); i < notes; i += (long long)gridDim.x * (PLAN_THREADS / 32)) {
     if (i < all_tiles) plan_rows(t, (int)i, tiles, reinterpret_cast<RowNote*>(space + rows_at) + i);
@@ -496,9 +498,10 @@ long long units_bound(const WeightsView& t) { return ((long long)t.c.table_cols 
 }  // namespace
 
 // Up to 16 rows a key head the mma.sync kernel reads the keys once, as fast as they come.  What is written down about rows (13 bytes each) and one request's keys has to fit three quarters of the
-// workspace, some two million rows and 100 thousand tiles of keys; calls beyond that stay with it, too, as do those without new tokens, which have no queries to copy.
+// workspace, some two million rows and 100 thousand tiles of keys; calls beyond that stay with it, too, as do those without new tokens, which have no queries to copy, and
+// those without a column in their tables, which only have that to report.
 bool weights_tc_supported(const WeightsView& t) {
-  if (t.c.num_tokens == 0 || t.group > HT || (long long)t.a.max_tokens * t.group <= 16) return false;
+  if (t.c.num_tokens == 0 || t.c.table_cols == 0 || t.group > HT || (long long)t.a.max_tokens * t.group <= 16) return false;
   return UNITS_AT + row_tiles_bound(t, t.c.batch < TREE_MAX_SPLIT_BATCH ? t.c.batch : TREE_MAX_SPLIT_BATCH) * (long long)sizeof(RowNote) + units_bound(t) * (long long)sizeof(UnitNote) <= t.a.workspace_bytes / 4 * 3;
 }
 
