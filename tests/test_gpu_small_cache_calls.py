@@ -101,3 +101,34 @@ def test_a_table_without_columns_is_reported_by_the_weights(tokens):
     with pytest.raises(PhoenixError):
         decoding.check_status()
     assert torch.equal(c["weights"], before)
+
+
+@pytest.mark.parametrize("name", ["window_attention", "tree_attention", "key_weights", "evict"])
+@pytest.mark.parametrize("tokens", [2, 60])
+def test_a_threads_first_call(name, tokens):
+    """A thread that has made no CUDA call before has no context; its outputs are there, so that torch makes none for it either."""
+    import threading
+    from x_algorithm_b200 import decoding
+    c = make_case(2, tokens, 300, 16, 4, 64, 32, "chain", seed=95, ragged=False)
+    n = 2 * tokens
+    out, lse = torch.zeros((n, 16, 64), dtype=torch.bfloat16, device=DEV), torch.zeros((n, 16), device=DEV)
+    decoding.window_attention(*args_of(c), window=90, out=out, lse=lse)
+    lengths, kept = torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros((2, 4, 280), dtype=torch.int32, device=DEV)
+    call = dict(window_attention=lambda: decoding.window_attention(*args_of(c), window=90, out=out, lse=lse), tree_attention=lambda: decoding.tree_attention(*args_of(c), out=out),
+                key_weights=lambda: decoding.key_weights(*args_of(c), lse, c["weights"], window=90),
+                evict=lambda: decoding.evict(c["weights"], c["pages"], c["lengths"], c["table"], budget=280, lengths_out=lengths, kept=kept))[name]
+    torch.cuda.synchronize()
+    raised = []
+
+    def body():
+        try:
+            call()
+        except Exception as e:  # noqa: BLE001
+            raised.append(e)
+
+    t = threading.Thread(target=body)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert not raised, raised
+    decoding.check_status()

@@ -50,11 +50,12 @@ inline cudaError_t taken_back(cudaError_t e) {
   return e;
 }
 
-// makes `device` current for the calls of one entry point and puts the caller's back
+// Makes `device` current for the calls of one entry point and puts the caller's back.  It is set whether or not it is current already: a thread that has made no call yet is on
+// device 0 by name but has no context, which tensor maps are refused without.
 class DeviceScope {
  public:
   explicit DeviceScope(int device) {
-    ok_ = taken_back(cudaGetDevice(&before_)) == cudaSuccess && (before_ == device || taken_back(cudaSetDevice(device)) == cudaSuccess);
+    ok_ = taken_back(cudaGetDevice(&before_)) == cudaSuccess && taken_back(cudaSetDevice(device)) == cudaSuccess;
     changed_ = ok_ && before_ != device;
   }
   ~DeviceScope() { if (changed_) cudaSetDevice(before_); }
