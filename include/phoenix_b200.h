@@ -823,7 +823,8 @@ phx_status phx_history_append_device(int32_t device, const phx_cache_batch* cach
  * output, whatever its key and value rows hold (infinities, NaN).  cap > 0: logits go through cap_method (1 soft sign, 2 tanh).
  * max_tokens and max_keys (cached + new) say how large a request may be; they choose kernels and splits only: larger
  * requests are computed all the same.  workspace: phx_tree_workspace_bytes of device memory, not shared by calls that may
- * overlap; nothing in it has to be kept or cleared between calls.  The order of every sum follows from the sizes alone: equal calls
+ * overlap; nothing in it has to be kept or cleared between calls.  A call may launch several kernels that talk through it, so threads that share a workspace and its stream
+ * make their calls one after the other (x_algorithm_b200.decoding sees to that).  The order of every sum follows from the sizes alone: equal calls
  * give equal bits.  Asynchronous on `stream`. */
 typedef struct phx_tree_args {
   const uint16_t* q;           /* [num_tokens][num_q_heads][key_size], rows q_stride apart */

@@ -132,3 +132,41 @@ def test_a_threads_first_call(name, tokens):
     torch.cuda.synchronize()
     assert not raised, raised
     decoding.check_status()
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_threads_that_share_a_stream(own_stream):
+    """Calls of several kernels (parts and their join; plan, product and join; select and move) from threads at once, on the default stream and on one of their own, are what they are
+    one after the other."""
+    import threading
+    from x_algorithm_b200 import decoding
+    cases = [make_case(*shape, seed=91 + i, ragged=False) for i, shape in enumerate([
+        (2, 40, 3000, 16, 2, 64, 64, "chain"), (4, 200, 700, 16, 4, 128, 64, "whole"), (1, 900, 1500, 32, 1, 64, 32, "chain"), (6, 30, 2000, 8, 4, 128, 16, "chain")])]
+
+    def step(c):
+        out, lse = decoding.window_attention(*args_of(c), c["spans"], window=1200, sinks=4)
+        tree = decoding.tree_attention(*args_of(c), c["spans"])
+        weights = decoding.key_weights(*args_of(c), lse, c["weights"].clone(), c["spans"], window=1200, sinks=4, decay=0.9)
+        heavy, pages = weights.clone(), c["pages"].clone()
+        return out, lse, tree, weights, heavy, pages, *decoding.evict(heavy, pages, c["lengths"], c["table"], budget=600, sinks=4, recent=50)
+
+    want = [step(c) for c in cases]
+    torch.cuda.synchronize()
+    stream, wrong = torch.cuda.Stream() if own_stream else torch.cuda.current_stream(), []
+
+    def body(c, expected):
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(15):
+                    wrong.extend(i for i, (x, y) in enumerate(zip(step(c), expected)) if not torch.equal(x, y))
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=body, args=pair) for pair in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong, wrong[:5]
+    decoding.check_status(stream=stream.cuda_stream)

@@ -200,3 +200,104 @@ def test_fading_weights_are_asked_for_without_new_tokens_too():
     f, a = _weights(decay=0.5)
     for empty in (dict(batch=0), dict(num_pages=0), dict(table_cols=0)):
         assert f(0, C.byref(_cache(num_tokens=0, **empty)), C.byref(a), None) == 0, empty
+
+
+# ---- threads ---------------------------------------------------------------------------------------------------------------------
+
+
+class _OnDevice:
+    """A host tensor that says it is on device 0."""
+    is_cuda = True
+
+    def __init__(self, t):
+        self._t = t
+
+    def __getattr__(self, name):
+        return getattr(self._t, name)
+
+    def get_device(self):
+        return 0
+
+
+def _calls_of(kept_args):
+    z = lambda *s, dtype=torch.int32: _OnDevice(torch.zeros(s, dtype=dtype))  # noqa: E731
+    q, pages, w = z(1, 4, 64, dtype=torch.bfloat16), z(2, 2, 2, 16, 64, dtype=torch.bfloat16), z(2, 2, 16, dtype=torch.float32)
+    q_start, lengths, table, lse = z(2), z(1), z(1, 2), z(1, 4, dtype=torch.float32)
+    return [lambda: decoding.tree_attention(q, pages, q_start, lengths, table, **kept_args), lambda: decoding.window_attention(q, pages, q_start, lengths, table, window=4, **kept_args),
+            lambda: decoding.key_weights(q, pages, q_start, lengths, table, lse, w, **kept_args), lambda: decoding.evict(w, pages, lengths, table, budget=4, **kept_args)]
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The entry points as functions that take a while: [stream, calls in them, the most at once, workspaces seen] of each stream; `current` is a thread's stream."""
+    import threading
+    import time
+    import types
+    seen, guard, current = {}, threading.Lock(), threading.local()
+
+    def entry(device, batch, args, stream):
+        with guard:
+            s = seen.setdefault(stream, dict(now=0, most=0, calls=0, freed=False))
+            s["now"] += 1
+            s["calls"] += 1
+            s["most"] = max(s["most"], s["now"])
+            kept = decoding._kept[(0, stream)]
+            had = kept.space
+        time.sleep(0.002)
+        with guard:
+            s["now"] -= 1
+            s["freed"] |= kept.space is not had
+        return 0
+
+    names = ("phx_tree_attention_device", "phx_window_attention_device", "phx_key_weights_device", "phx_evict_device")
+    monkeypatch.setattr(decoding, "lib", types.SimpleNamespace(phx_global_error=lambda: b"", **{n: entry for n in names}))
+    monkeypatch.setattr(decoding, "_kept", {})
+    monkeypatch.setattr(decoding, "_status_block", lambda device: torch.zeros(4, dtype=torch.int32))
+    monkeypatch.setattr(decoding, "_workspace", lambda device: torch.zeros(64, dtype=torch.uint8))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: getattr(current, "stream", 0), raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False, raising=False)
+    return seen, current
+
+
+def _at_once(current, streams, work):
+    import threading
+    errors = []
+
+    def body(stream):
+        current.stream = stream
+        try:
+            for _ in range(3):
+                for f in work:
+                    f()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=body, args=(s,)) for s in streams]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+@pytest.mark.parametrize("workspace", [False, True])
+def test_calls_of_threads_on_one_stream_do_not_interleave(launches, workspace):
+    """A call's kernels talk through its workspace, so no other call's launches may come between them, whoever owns it; other streams' may."""
+    seen, current = launches
+    work = _calls_of(dict(workspace=_OnDevice(torch.zeros(64, dtype=torch.uint8))) if workspace else {})
+    _at_once(current, [0, 0, 0, 7], work)
+    assert seen[0]["most"] == 1 and seen[7]["most"] == 1 and seen[0]["calls"] == 36 and seen[7]["calls"] == 12
+
+
+def test_a_workspace_is_not_given_back_under_a_call(launches):
+    seen, current = launches
+    _at_once(current, [0, 0], _calls_of({}) + [lambda: decoding.release(0, 0)])
+    assert not seen[0]["freed"]
+
+
+def test_a_refused_call_lets_the_next_one_in(launches, monkeypatch):
+    monkeypatch.setattr(decoding.lib, "phx_evict_device", lambda *a: 1)
+    tree, _, _, evict = _calls_of({})
+    with pytest.raises(PhoenixError):
+        evict()
+    tree()

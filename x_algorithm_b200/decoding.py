@@ -3,7 +3,7 @@
 (`token_logprobs`).  What the keys of a cache receive of the attention is added up (`key_weights`), and the keys that received the least leave it (`evict`).  torch CUDA tensors in
 and out, asynchronous on torch's current stream; nothing here waits for what is queued but `check_status`.  `stream`, a raw handle, names another
 as `with torch.cuda.stream(...)` around the call would: what the call allocates is that stream's, and what it reads has to be there and stay until it
-has run.
+has run.  Threads may make calls at once, on one stream, too; a workspace that the caller passes belongs to the calls of one stream at a time.
 
 The cache is a tensor `pages` bf16 [num_pages, 2 (key, value), kv heads, page size, head dim] that the caller owns and hands out page by
 page; `block_table` int32 [B, columns] names a request's pages in order, `lengths` int32 [B] counts its cached keys, and the new tokens of
@@ -28,11 +28,13 @@ _NO_ROWS = object()
 
 
 class _Kept:
-    """What one stream of one device keeps between calls: the status block and, from its first attention on, that one's workspace."""
+    """What one stream of one device keeps between calls: the status block and, from its first attention on, that one's workspace.  `calls` is held around a call
+    that uses a workspace: its kernels talk through it, and those of another thread's call must not come between them."""
 
     def __init__(self, device: int):
         self.status = _status_block(device)
         self.status_ptr, self.workspace, self.space = self.status.data_ptr(), None, None
+        self.calls = threading.Lock()
 
 
 def _take_space(kept, device: int):
@@ -243,11 +245,12 @@ def tree_attention(q, pages, q_start, lengths, block_table, spans=None, *, sm_sc
         out = torch.empty_strided(shape, (heads * dh, dh, 1), dtype=_BF16, device=q.device)
     else:
         _need(out, "out", _BF16, shape, device)
-    space, size = _space(workspace, kept, device, stream)
-    _TREE(mine.tree, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, 0 if spans is None else _need(spans, "spans", _I32, (n, 2), device),
-          out.data_ptr(), space, size, cols * page_size if max_keys is None else max_keys, n if max_tokens is None else max_tokens, heads,
-          math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], 0)
-    _ok(lib.phx_tree_attention_device(device, mine.batch_ref, mine.tree_ref, stream))
+    spans = 0 if spans is None else _need(spans, "spans", _I32, (n, 2), device)
+    with kept.calls:
+        space, size = _space(workspace, kept, device, stream)
+        _TREE(mine.tree, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, spans, out.data_ptr(), space, size, cols * page_size if max_keys is None else max_keys,
+              n if max_tokens is None else max_tokens, heads, math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], 0)
+        _ok(lib.phx_tree_attention_device(device, mine.batch_ref, mine.tree_ref, stream))
     return out
 
 
@@ -308,10 +311,11 @@ def window_attention(q, pages, q_start, lengths, block_table, spans=None, positi
         lse = torch.empty_strided((n, heads), (heads, 1), dtype=_F32, device=q.device)
     else:
         _need(lse, "lse", _F32, (n, heads), device)
-    space, size = _space(workspace, kept, device, stream)
-    _WINDOW(mine.window, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, spans, out.data_ptr(), space, size, cols * page_size if max_keys is None else max_keys,
-            n if max_tokens is None else max_tokens, heads, math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], 0, positions, lse.data_ptr(), window, sinks)
-    _ok(lib.phx_window_attention_device(device, mine.batch_ref, mine.window_ref, stream))
+    with kept.calls:
+        space, size = _space(workspace, kept, device, stream)
+        _WINDOW(mine.window, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, spans, out.data_ptr(), space, size, cols * page_size if max_keys is None else max_keys,
+                n if max_tokens is None else max_tokens, heads, math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], 0, positions, lse.data_ptr(), window, sinks)
+        _ok(lib.phx_window_attention_device(device, mine.batch_ref, mine.window_ref, stream))
     return out, lse
 
 
@@ -335,11 +339,12 @@ def key_weights(q, pages, q_start, lengths, block_table, lse, weights, spans=Non
     spans, positions, window, sinks = _seen(spans, positions, window, sinks, n, device)
     lse_ptr = _need(lse, "lse", _F32, (n, heads), device)
     weights_ptr = _need(weights, "weights", _F32, (pages.shape[0], kv_heads, page_size), device)
-    space, size = _space(workspace, kept, device, stream)
-    _WEIGHTS(mine.weights, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, spans, positions, lse_ptr, weights_ptr, space, size,
-             cols * page_size if max_keys is None else max_keys, n if max_tokens is None else max_tokens, heads, window, sinks,
-             math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], decay)
-    _ok(lib.phx_key_weights_device(device, mine.batch_ref, mine.weights_ref, stream))
+    with kept.calls:
+        space, size = _space(workspace, kept, device, stream)
+        _WEIGHTS(mine.weights, 0, q.data_ptr(), q.stride(0) if n > 1 else heads * dh, spans, positions, lse_ptr, weights_ptr, space, size,
+                 cols * page_size if max_keys is None else max_keys, n if max_tokens is None else max_tokens, heads, window, sinks,
+                 math.sqrt(128.0) / dh if sm_scale is None else sm_scale, cap, CAP_METHODS[cap_method], decay)
+        _ok(lib.phx_key_weights_device(device, mine.batch_ref, mine.weights_ref, stream))
     return weights
 
 
@@ -370,9 +375,10 @@ def evict(weights, pages, lengths, block_table, *, budget: int, sinks: int = 0, 
         kept = torch.empty_strided(shape, (kv_heads * budget, budget, 1), dtype=_I32, device=weights.device)
     else:
         _need(kept, "kept", _I32, shape, device)
-    space, size = _space(workspace, state, device, stream)
-    _EVICT(mine.evict, 0, weights.data_ptr(), lengths_out.data_ptr(), kept.data_ptr(), space, size, cols * page_size if max_keys is None else max_keys, budget, sinks, recent, 0)
-    _ok(lib.phx_evict_device(device, mine.batch_ref, mine.evict_ref, stream))
+    with state.calls:
+        space, size = _space(workspace, state, device, stream)
+        _EVICT(mine.evict, 0, weights.data_ptr(), lengths_out.data_ptr(), kept.data_ptr(), space, size, cols * page_size if max_keys is None else max_keys, budget, sinks, recent, 0)
+        _ok(lib.phx_evict_device(device, mine.batch_ref, mine.evict_ref, stream))
     return lengths_out, kept
 
 
@@ -411,7 +417,8 @@ def release(device: Optional[int] = None, stream: Optional[int] = None) -> None:
     device = torch.cuda.current_device() if device is None else device
     kept = _kept.get((device, _stream(device, stream)))
     if kept is not None:
-        kept.workspace = kept.space = None
+        with kept.calls:                                     # not between a call's look at it and its launches
+            kept.workspace = kept.space = None
 
 
 def check_status(device: Optional[int] = None, stream: Optional[int] = None) -> None:
