@@ -222,7 +222,7 @@ void phx_engine_destroy(phx_engine* e);
 /* Text of the last error on this engine (never NULL).  Replaces the string errors of the plugin
  * seam (candidate-pipeline/scorer.rs:29-44). */
 const char* phx_last_error(const phx_engine* e);
-/* Library-level message for failures before an engine exists. */
+/* Library-level message for failures before an engine exists, and of the calls that take none: the last one of the calling thread, until its next. */
 const char* phx_global_error(void);
 
 /* ---- parameters ------------------------------------------------------------------------------ */

@@ -301,3 +301,25 @@ def test_a_refused_call_lets_the_next_one_in(launches, monkeypatch):
     with pytest.raises(PhoenixError):
         evict()
     tree()
+
+
+def test_an_error_is_the_calling_threads():
+    """The message of a refused call is still there, and the caller's, after another thread's call was refused."""
+    import threading
+    first, second, seen = threading.Event(), threading.Event(), {}
+
+    def body(call, mine, other, name):
+        f, a = call(**({"budget": 0} if call is _evict else {"window": -1}))
+        if other is first:
+            first.wait(10)
+        f(0, C.byref(_cache()), C.byref(a), None)
+        mine.set()
+        other.wait(10)
+        seen[name] = _lib.lib.phx_global_error()
+
+    threads = [threading.Thread(target=body, args=(_evict, first, second, "evict")), threading.Thread(target=body, args=(_window, second, first, "window"))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert b"phx_evict_device" in seen["evict"] and b"phx_window_attention_device" in seen["window"]

@@ -19,12 +19,8 @@
 
 namespace phx {
 
-static std::mutex g_err_mu;
-static std::string g_err = "";
-void set_global_error(const std::string& msg) {
-  std::lock_guard<std::mutex> lk(g_err_mu);
-  g_err = msg;
-}
+static thread_local std::string g_err;   // a thread's own: another one's error neither replaces the text nor frees it while it is read
+void set_global_error(const std::string& msg) { g_err = msg; }
 
 static std::atomic<long long> g_dispatch[DK_COUNT];
 void dispatch_note(int kind) {
