@@ -7,8 +7,8 @@
 // keys, values and weights, into shared memory, says so, and writes it once what it writes over has been read.  A row only ever moves to the front, so what lies in a chunk's
 // places is taken by that chunk or one before it, by two at most: it is no more than fills one.  Chunks are handed out in order, by a counter, so a block only waits for blocks that
 // have begun, and whose reads wait for nothing.
-// Measured (us, keys that leave for the first time): 64 x 4 heads of up to 4096 keys of 128, half of them stay (338 MB read and written): select 19, move 66 = 5.1 TB/s; 2 x 4 heads of 100 k keys, a third
-// stays: 25 and 56 (221 MB, 3.9 TB/s, by 3280 blocks that wait for one another's reads).  With a wait for all chunks in front the second took 73 for its move where 61 were left with two; blocks that went through a head's places from front to
+// Measured (us, keys that leave for the first time, cold caches): 64 x 4 heads of up to 4096 keys of 128, half of them stay (375 k rows change their place, 387 MB read and written): select 19, move 66 =
+// 5.9 TB/s, the call 88; 2 x 4 heads of 100 k keys, a third stays: 25 and 55 (262 k rows, 270 MB, 4.9 TB/s, by 3280 blocks that wait for one another's reads), the call 84.  With a wait for all chunks in front the second took 73 for its move where 61 were left with two; blocks that went through a head's places from front to
 // back by themselves took 247 for the second and 89 for the first.
 #include <string>
 

@@ -10,6 +10,8 @@
 // share.  K goes from memory to registers, two tiles of a warp on their way; nothing is shared between warps.
 // Bound by memory and by a tile's round trips: pages, keys and old weights.  96 single tokens over up to 4096 keys, 4 key heads of 128 (273 MB): 56 us = 4.9 TB/s.  A warp's pages are asked for
 // at once and old weights with the keys: 66 us without.  Tiles of a warp 4, 8, 16: 66, 55, 59 us; four warps a block for eight 55.0 and 55.7, but one token over 128 keys 3.7 and 3.1.
+// That cut, 1024 keys a block, is for many users.  One token of a single user pays a warp's eight tiles in a row, eight and two tiles of a warp: over 1 k, 4 k, 16 k, 100 k keys 9.9, 10.2, 10.4, 27.9 and 4.3, 4.6,
+// 5.5, 27.7 us (4 key heads of 128), 9.1, 9.2, 9.6, 33.7 and 4.1, 4.2, 7.9, 40.4 (8 of 64); 16 and 96 users of 4 k keys each 16.1, 80.7 and 20.5, 95.9 (23.6, 118.6 and 28.7, 155.4).
 #include <math.h>
 
 #include <string>

@@ -324,7 +324,8 @@ def key_weights(q, pages, q_start, lengths, block_table, lse, weights, spans=Non
                 max_keys: Optional[int] = None, workspace=None, stream: Optional[int] = None):
     """The attention weight that every key of the requests receives from the new tokens, summed over them and the queries of the key's head, joins weights fp32 [num_pages,
     kv heads, page size], in place: decay * weight + sum for cached keys, with new tokens or without, the sum alone for new ones.  lse fp32 [N, heads] is what `window_attention` gave for the same
-    queries, spans, positions, window, sinks, scale and cap (a row with an infinite one adds nothing).  Returns weights."""
+    queries, spans, positions, window, sinks, scale and cap (a row with an infinite one adds nothing).  A page that receives weights may stand once in the tables of a call: what two
+    requests share is attended to, not weighed.  Returns weights."""
     device = _rows(q, "q", _BF16, 3)
     if stream is not None and _elsewhere(device, stream):
         with _under(device, stream):
